@@ -48,6 +48,9 @@ extern "C" {
 #define HMOE_DT_I64 4
 #define HMOE_DT_I8 5
 
+#define HMOE_SCORE_SOFTMAX 0
+#define HMOE_SCORE_SIGMOID 1
+
 typedef void* hmoe_stream_t; /* a hipStream_t (0 = the null stream) */
 
 int hmoe_abi_version(void);
@@ -85,6 +88,24 @@ int hmoe_route_topk(const void* x, int64_t ldx, const void* wr, const float* bia
 int hmoe_route_sigmoid_group(const void* x, int64_t ldx, const void* wr, const float* expert_bias, int64_t T,
                              int64_t d, int E, int k, int n_group, int topk_group, float scaling, float* scores,
                              int32_t* topk_ids, float* topk_w, hmoe_stream_t stream);
+
+/* Routing from given logits: softmax or sigmoid scores, a selection bias (for balance), groups, top-k, renormalised
+ * weights (the routing of aurora/hf_pipeline.py:352-359 with either score).  logits (T, E) bf16, fp16 or fp32 (dtype),
+ * row stride ld >= E.  Scores s = softmax(l) over all E experts or 1 / (1 + exp(-l)) (score: HMOE_SCORE_*); selection
+ * value = s + bias (bias (E,) fp32, NULL = none; for selection only).  With topk_group < n_group the experts form n_group
+ * groups of E / n_group; a group's value is the sum of its group_top (1 or 2) largest selection values, and only the
+ * topk_group best groups (ties to the lower one) are kept.  topk_ids (T, k) int32: the k experts of largest selection value,
+ * descending, ties to the lower expert; topk_w (T, k) fp32 = their scores, divided by (their sum + 1e-20) with renorm,
+ * times scaling.  Selection values are taken in fp64 (of which 43 mantissa bits take part in the last selection; a
+ * selection without bias and groups compares the logits exactly); weights in fp32.
+ * An expert with the logit or the bias -inf or NaN, or outside the kept groups, is chosen only where no other is left (the
+ * lowest such expert first) and has the weight 0; a NaN or +inf logit makes every softmax weight of its row NaN.
+ * live (T,) bytes or NULL: a token with live = 0 (padding) gets ids -1 and weights 0 -- it routes nowhere
+ * (hmoe_dispatch).  E <= 512, k <= 16, k <= E; with groups n_group <= 64, E / n_group >= group_top, k <= topk_group *
+ * E / n_group. */
+int hmoe_route_scores(const void* logits, int64_t ld, int dtype, const float* bias, const uint8_t* live, int64_t T,
+                      int E, int k, int score, int n_group, int topk_group, int group_top, int renorm, float scaling,
+                      int32_t* topk_ids, float* topk_w, hmoe_stream_t stream);
 
 /* Workspace bytes for hmoe_dispatch. */
 size_t hmoe_dispatch_workspace_size(int64_t T, int k, int E);
@@ -345,6 +366,87 @@ int hmoe_unpermute_bwd(const void* dxs, int dxs_dtype, const int32_t* inv_pos, c
 /* The same from the parts of hmoe_gate_up_dgrad_split: dxs (parts, T k, d) fp32, added in order. */
 int hmoe_unpermute_bwd_split(const float* dxs, int parts, const int32_t* inv_pos, const float* dlogits, const void* wr,
                              int64_t T, int k, int64_t d, int E, void* dx, hmoe_stream_t stream);
+
+/* Backward of hmoe_route_scores: dlogits (T, E), contiguous, of the logits' type, from dtopk_w (T, k) fp32; topk_ids and
+ * topk_w as the forward wrote them.  The selection is constant; the gradient goes through the chosen scores and the
+ * renormalisation, for softmax on to every logit.  Slots with an id outside [0, E) or the weight 0 have none; an expert
+ * that several slots name gets their sum. */
+int hmoe_route_scores_bwd(const float* dtopk_w, const float* topk_w, const void* logits, int64_t ld, int dtype,
+                          const int32_t* topk_ids, int64_t T, int E, int k, int score, int renorm, float scaling,
+                          void* dlogits, hmoe_stream_t stream);
+
+/* The router weight's gradient from given logit gradients: dwr (E, d) = dlogits^T @ x (fp32 or bf16), the second half of
+ * hmoe_router_bwd with its sizes, types and workspace. */
+int hmoe_router_wgrad(const float* dlogits, const void* x, int64_t ldx, int64_t T, int E, int64_t d, void* dwr,
+                      int dwr_dtype, void* workspace, size_t workspace_bytes, hmoe_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------------------------------
+ * Norms around the block (the normed, modulated input and the gated residual of a transformer block whose mlp is the
+ * routed layer, aurora/model.py:191-210)
+ *
+ * Rows T x d in a stream type (x, the residual stream) and a block type (the routed layer's input and output): equal, or
+ * an fp32 stream around a 16-bit block.  Per-sample parameters (B, d): without starts, T / B consecutive rows belong to
+ * each sample (B = 1: one set for all rows); with starts (B + 1,) int32, ascending, rows starts[b] .. starts[b + 1] - 1
+ * belong to sample b (which may be empty) and rows outside [starts[0], starts[B]) are padding.  Parameters are bf16, fp16 or
+ * fp32, each with its own type.  Statistics, sums and products are fp32, every output is rounded once.  d % 8 == 0,
+ * d <= 16384, ldx % 8 == 0, 16-byte aligned pointers.
+ * ------------------------------------------------------------------------------------------------------------- */
+
+/* h = n * weight * (1 + scale_b) + shift_b with n = x / sqrt(mean(x^2) + eps); each of the three optional (NULL); 0 on
+ * padding rows.  h (T, d) contiguous. */
+int hmoe_norm_modulate(const void* x, int64_t ldx, int x_dtype, const void* weight, int weight_dtype,
+                       const void* scale, const void* shift, int mod_dtype, const int32_t* starts, int64_t B, int64_t T,
+                       int64_t d, float eps, void* h, int h_dtype, hmoe_stream_t stream);
+
+/* Its backward: dx (T, d) of x's type = the gradient through h plus dres_scale * dres (dres (T, d) of x's type, the
+ * gradient that reaches x past the block; NULL for none; the only term on padding rows); dweight (d,), dscale and dshift
+ * (B, d) of their parameters' types (NULL to skip).  Sums over rows are taken in a fixed order.  workspace:
+ * hmoe_norm_modulate_bwd_workspace_size bytes, 16-byte aligned (unused, may be NULL, without a parameter gradient). */
+size_t hmoe_norm_modulate_bwd_workspace_size(int64_t T, int64_t d, int64_t B);
+int hmoe_norm_modulate_bwd(const void* dh, int h_dtype, const void* x, int64_t ldx, int x_dtype, const void* weight,
+                           int weight_dtype, const void* scale, const void* shift, int mod_dtype, const int32_t* starts,
+                           int64_t B, int64_t T, int64_t d, float eps, const void* dres, float dres_scale, void* dx,
+                           void* dweight, void* dscale, void* dshift, void* workspace, size_t workspace_bytes,
+                           hmoe_stream_t stream);
+
+/* out = alpha * x + gate_b * weight * n, n = s / sqrt(mean(s^2) + eps) (norm = 0: n = s), s = the sum over the k slots of y
+ * (T * k, d) in (token, slot) order, as hmoe_combine sums them but not rounded, plus add (T, d) (NULL for none).  inv_pos as
+ * in hmoe_combine.  weight (d,), gate (B, d) or NULL.  alpha * x on padding rows, whose y is not used.  x (T, d) with row
+ * stride ldx; out (T, d) contiguous, of x's type (it may be x itself where ldx == d). */
+int hmoe_norm_residual(const void* y, const int32_t* inv_pos, int k, const void* add, int y_dtype, const void* x,
+                       int64_t ldx, int x_dtype, const void* weight, int weight_dtype, const void* gate, int gate_dtype,
+                       const int32_t* starts, int64_t B, int64_t T, int64_t d, int norm, float eps, float alpha,
+                       void* out, hmoe_stream_t stream);
+
+/* Its backward but for x (dx = alpha * dout): dy (T, d) of y's type, the gradient of the slots' sum and so of every slot
+ * and of add (0 on padding rows); dweight (d,), dgate (B, d) of their parameters' types (NULL to skip).  dout (T, d)
+ * contiguous, of x's type (out_dtype).  Workspace as above. */
+size_t hmoe_norm_residual_bwd_workspace_size(int64_t T, int64_t d, int64_t B);
+int hmoe_norm_residual_bwd(const void* dout, int out_dtype, const void* y, const int32_t* inv_pos, int k,
+                           const void* add, int y_dtype, const void* weight, int weight_dtype, const void* gate,
+                           int gate_dtype, const int32_t* starts, int64_t B, int64_t T, int64_t d, int norm, float eps,
+                           void* dy, void* dweight, void* dgate, void* workspace, size_t workspace_bytes,
+                           hmoe_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------------------------------
+ * Gradient clipping by the global norm (of the layer's gradients and any others)
+ * n tensors: host arrays of their addresses, element counts and types (bf16, fp16, fp32; contiguous; aligned to an element
+ * only), read during the call.  Any number of tensors: 128 travel in the arguments of a launch.
+ * ------------------------------------------------------------------------------------------------------------- */
+
+/* sq_norm (1,) fp64 = the sum of the squares of every element, in fp64 and a fixed order.  workspace:
+ * hmoe_grad_sq_norm_workspace_size(n) bytes, 8-byte aligned. */
+size_t hmoe_grad_sq_norm_workspace_size(int n);
+int hmoe_grad_sq_norm(const void* const* grads, const int64_t* numel, const int* dtypes, int n, double* sq_norm,
+                      void* workspace, size_t workspace_bytes, hmoe_stream_t stream);
+
+/* out[i] = grads[i] * min(1, max_norm / (norm + 1e-6)) with norm = sqrt(sq_norm): the product in fp32, rounded once.  out[i]
+ * has grads[i]'s type or is fp32 (out_dtypes) and may be grads[i] itself (left as it is where the factor is 1).  A NaN
+ * sq_norm makes every output NaN, an infinite one zeros (NaN where a gradient is infinite).  norm (1,) fp32 or NULL.  sq_norm
+ * is read on the device, so gradients spread over several processes can sum it between the two calls.  max_norm >= 0. */
+int hmoe_grad_clip(const void* const* grads, void* const* out, const int64_t* numel, const int* dtypes,
+                   const int* out_dtypes, int n, const double* sq_norm, float max_norm, float* norm,
+                   hmoe_stream_t stream);
 
 #ifdef __cplusplus
 }

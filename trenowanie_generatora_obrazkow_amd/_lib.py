@@ -71,6 +71,22 @@ SIGNATURES = {
                                _P]),
     "hmoe_unpermute_bwd": (_I32, [_P, _I32, _P, _P, _P, _I64, _I32, _I64, _I32, _P, _P]),
     "hmoe_unpermute_bwd_split": (_I32, [_P, _I32, _P, _P, _P, _I64, _I32, _I64, _I32, _P, _P]),
+    "hmoe_route_scores": (_I32, [_P, _I64, _I32, _P, _P, _I64, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _F32, _P, _P,
+                                 _P]),
+    "hmoe_route_scores_bwd": (_I32, [_P, _P, _P, _I64, _I32, _P, _I64, _I32, _I32, _I32, _I32, _F32, _P, _P]),
+    "hmoe_router_wgrad": (_I32, [_P, _P, _I64, _I64, _I32, _I64, _P, _I32, _P, _SZ, _P]),
+    "hmoe_norm_modulate": (_I32, [_P, _I64, _I32, _P, _I32, _P, _P, _I32, _P, _I64, _I64, _I64, _F32, _P, _I32, _P]),
+    "hmoe_norm_modulate_bwd_workspace_size": (_SZ, [_I64, _I64, _I64]),
+    "hmoe_norm_modulate_bwd": (_I32, [_P, _I32, _P, _I64, _I32, _P, _I32, _P, _P, _I32, _P, _I64, _I64, _I64, _F32, _P,
+                                      _F32, _P, _P, _P, _P, _P, _SZ, _P]),
+    "hmoe_norm_residual": (_I32, [_P, _P, _I32, _P, _I32, _P, _I64, _I32, _P, _I32, _P, _I32, _P, _I64, _I64, _I64, _I32,
+                                  _F32, _F32, _P, _P]),
+    "hmoe_norm_residual_bwd_workspace_size": (_SZ, [_I64, _I64, _I64]),
+    "hmoe_norm_residual_bwd": (_I32, [_P, _I32, _P, _P, _I32, _P, _I32, _P, _I32, _P, _I32, _P, _I64, _I64, _I64, _I32,
+                                      _F32, _P, _P, _P, _P, _SZ, _P]),
+    "hmoe_grad_sq_norm_workspace_size": (_SZ, [_I32]),
+    "hmoe_grad_sq_norm": (_I32, [_P, _P, _P, _I32, _P, _P, _SZ, _P]),
+    "hmoe_grad_clip": (_I32, [_P, _P, _P, _P, _P, _I32, _P, _F32, _P, _P]),
 }
 
 _lib = None

@@ -2263,6 +2263,26 @@ size_t hmoe_router_bwd_workspace_size(int64_t T, int E, int64_t d) {
   return (size_t)(nchunk > 0 ? nchunk : 1) * (size_t)E * (size_t)d * 4;
 }
 
+// dwr (E, d) = dlogits^T @ x: chunk partials in the workspace, then their fixed-order sum (T = 0: zeros)
+static int router_wgrad(const float* dlogits, const uint16_t* x, int64_t ldx, int64_t T, int E, int64_t d, void* dwr,
+                        int dwr_dtype, void* workspace, hipStream_t s) {
+  const int nchunk = (int)((T + kDwrChunk - 1) / kDwrChunk);
+  float* part = static_cast<float*>(workspace);
+  if (nchunk > 0) {
+    if (E <= 16)
+      hipLaunchKernelGGL(router_dwr_mfma_kernel, dim3(nchunk, (unsigned)((d + 511) / 512)), dim3(256), 0, s, dlogits, x,
+                         ldx, T, E, d, part);
+    else
+      hipLaunchKernelGGL(router_dwr_partial_kernel, dim3(nchunk, (unsigned)((d + 511) / 512)), dim3(256), 0, s, dlogits,
+                         x, ldx, T, E, d, part);
+    HMOE_CHECK_LAUNCH();
+  }
+  hipLaunchKernelGGL(router_dwr_reduce_kernel, dim3(grid_for((int64_t)E * d, 64, 4096)), dim3(1024), 0, s, part, nchunk,
+                     E, d, dwr, dwr_dtype == HMOE_DT_BF16);
+  HMOE_CHECK_LAUNCH();
+  return HMOE_OK;
+}
+
 int hmoe_router_bwd(const float* logits, const int32_t* topk_ids, const float* dtopk_w, int64_t T, int E, int k,
                     int renorm, float scaling, const void* x, int64_t ldx, int64_t d, float* dlogits, void* dwr,
                     int dwr_dtype, void* workspace, size_t workspace_bytes, hmoe_stream_t stream) {
@@ -2283,23 +2303,18 @@ int hmoe_router_bwd(const float* logits, const int32_t* topk_ids, const float* d
                          dtopk_w, T, E, k, renorm, scaling, dlogits);
     HMOE_CHECK_LAUNCH();
   }
-  if (dwr) {
-    const int nchunk = (int)((T + kDwrChunk - 1) / kDwrChunk);
-    float* part = static_cast<float*>(workspace);
-    if (nchunk > 0) {
-      if (E <= 16)
-        hipLaunchKernelGGL(router_dwr_mfma_kernel, dim3(nchunk, (unsigned)((d + 511) / 512)), dim3(256), 0, s,
-                           dlogits, static_cast<const uint16_t*>(x), ldx, T, E, d, part);
-      else
-        hipLaunchKernelGGL(router_dwr_partial_kernel, dim3(nchunk, (unsigned)((d + 511) / 512)), dim3(256), 0, s,
-                           dlogits, static_cast<const uint16_t*>(x), ldx, T, E, d, part);
-      HMOE_CHECK_LAUNCH();
-    }
-    hipLaunchKernelGGL(router_dwr_reduce_kernel, dim3(grid_for((int64_t)E * d, 64, 4096)), dim3(1024), 0, s, part,
-                       nchunk, E, d, dwr, dwr_dtype == HMOE_DT_BF16);
-    HMOE_CHECK_LAUNCH();
-  }
-  return HMOE_OK;
+  return dwr ? router_wgrad(dlogits, static_cast<const uint16_t*>(x), ldx, T, E, d, dwr, dwr_dtype, workspace, s) : HMOE_OK;
+}
+
+int hmoe_router_wgrad(const float* dlogits, const void* x, int64_t ldx, int64_t T, int E, int64_t d, void* dwr,
+                      int dwr_dtype, void* workspace, size_t workspace_bytes, hmoe_stream_t stream) {
+  if (T < 0 || E <= 0 || d <= 0) return HMOE_ERR_ARG;
+  if (E > kRouteMaxE) return HMOE_ERR_SHAPE;
+  if (dwr_dtype != HMOE_DT_F32 && dwr_dtype != HMOE_DT_BF16) return HMOE_ERR_DTYPE;
+  if (!dwr || (T > 0 && (!x || !dlogits)) || d % 8 || ldx % 8 || ldx < d || !al16(x)) return HMOE_ERR_ARG;
+  if (!workspace || workspace_bytes < hmoe_router_bwd_workspace_size(T, E, d)) return HMOE_ERR_WORKSPACE;
+  return router_wgrad(dlogits, static_cast<const uint16_t*>(x), ldx, T, E, d, dwr, dwr_dtype, workspace,
+                      reinterpret_cast<hipStream_t>(stream));
 }
 
 static int unpermute_bwd(const void* dxs, int dxs_dtype, int parts, const int32_t* inv_pos, const float* dlogits,

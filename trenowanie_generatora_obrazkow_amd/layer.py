@@ -239,3 +239,21 @@ def moe_param_groups(module: nn.Module, lr: float, weight_decay: float, router_l
               dict(params=routers, lr=rlr, base_lr=rlr, weight_decay=0.0, name="moe_router")]
     groups = [g for g in groups if g["params"]]
     return groups, {id(p) for g in groups for p in g["params"]}
+
+
+def clip_grad_norm(grads, max_norm, out=None):
+    """Clips a list of gradient tensors by their global norm: each becomes itself times min(1, max_norm / (norm + 1e-6)), in
+    place, or in `out` (tensors of the same shapes and strides, of the gradients' types or fp32, such as an optimizer's fp32
+    gradients; the gradients then stay as they are).  bf16, fp16 and fp32 tensors of any size and alignment may be mixed,
+    None entries are skipped.  Returns the norm before clipping, a () fp32 tensor on the device; nothing waits for the GPU.
+    A gradient spread over several processes: all-reduce ops.grad_sq_norm's sum before ops.grad_clip."""
+    grads = list(grads)
+    outs = None if out is None else list(out)
+    if outs is not None and len(outs) != len(grads):
+        raise ValueError(f"{len(outs)} outputs for {len(grads)} gradients")
+    if any(g is None for g in grads):
+        if outs is not None:
+            outs = [o for g, o in zip(grads, outs) if g is not None]
+        grads = [g for g in grads if g is not None]
+    gl = ops.GradList(grads, outs)
+    return ops.grad_clip(gl, ops.grad_sq_norm(gl), max_norm)

@@ -2,6 +2,7 @@
 validates layouts, and launches on the current stream of the tensors' device.  GPU tensors only."""
 from __future__ import annotations
 
+from array import array
 from dataclasses import dataclass
 
 import torch
@@ -703,3 +704,323 @@ def unpermute_bwd(dxs, inv_pos, T, k, dlogits=None, wr=None):
             L.call("hmoe_unpermute_bwd", L.ptr(dxs), L.dt(dxs), L.ptr(inv_pos), L.ptr(dlogits), L.ptr(wr), T, k, d, E,
                    L.ptr(dx), _dev_stream(dxs))
     return dx
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# Routing from logits, the norms around the block, gradient clipping
+# ---------------------------------------------------------------------------------------------------------------
+_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
+_SCORES = {"softmax": 0, "sigmoid": 1}
+
+
+def _call_on(dev, name, *args):
+    """A C call with its stream, launched on `dev` also where another device is the current one."""
+    if dev.index == torch.cuda.current_device():
+        L.call(name, *args, L.stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            L.call(name, *args, L.stream(dev))
+
+
+def _on(t, name, dev, shape, dtypes):
+    """A contiguous operand of a call whose first tensor lives on `dev`; None passes."""
+    if t is None:
+        return None
+    if t.device != dev:
+        raise ValueError(f"{name} is on {t.device}, the call's other tensors on {dev}")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name}: dtype {t.dtype} not in {dtypes}")
+    if t.shape != shape:
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    return t
+
+
+def _rows(t, name, dtypes=_FLOATS):
+    """(T, d, row stride) of a matrix whose rows are contiguous."""
+    L.require_gpu(t, name)
+    if t.dim() != 2:
+        raise ValueError(f"{name} must be a (rows, width) matrix (got {tuple(t.shape)})")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name}: dtype {t.dtype} not in {dtypes}")
+    T, d = t.shape
+    if d % 8 or d == 0:
+        raise ValueError(f"{name}: width {d} must be a positive multiple of 8")
+    ld = t.stride(0) if T > 1 else d
+    if (d > 1 and t.stride(1) != 1) or ld < d or ld % 8:
+        raise ValueError(f"{name}: rows must be contiguous, with a row stride of a multiple of 8 (strides {t.stride()})")
+    return T, d, ld
+
+
+def _routing(logits, k, score, n_group, topk_group, group_top):
+    L.require_gpu(logits, "logits")
+    if logits.dim() != 2 or logits.dtype not in _FLOATS:
+        raise TypeError(f"logits must be a (T, E) matrix of bf16, fp16 or fp32 (got {tuple(logits.shape)} {logits.dtype})")
+    if score not in _SCORES:
+        raise ValueError(f"score must be 'softmax' or 'sigmoid' (got {score!r})")
+    T, E = logits.shape
+    if E < 1 or not 1 <= k <= min(E, 16) or E > 512:
+        raise ValueError(f"routing takes up to 512 experts and 1 to min(16, E) slots (got E = {E}, k = {k})")
+    if (E > 1 and logits.stride(1) != 1) or (T > 1 and logits.stride(0) < E):
+        raise ValueError(f"logits rows must be contiguous (strides {logits.stride()})")
+    if n_group < 1 or not 1 <= topk_group <= n_group or E % n_group or group_top not in (1, 2):
+        raise ValueError(f"groups: E = {E} must divide into n_group = {n_group}, 1 <= topk_group = {topk_group} <= n_group, "
+                         f"group_top = {group_top} 1 or 2")
+    if topk_group < n_group and (n_group > 64 or E // n_group < group_top or k > topk_group * (E // n_group)):
+        raise ValueError(f"{topk_group} of {n_group} groups of {E // n_group} experts cannot give k = {k} (at most 64 groups)")
+    return T, E, logits.stride(0) if T > 1 else E
+
+
+def route_scores(logits, k, score="softmax", bias=None, n_group=1, topk_group=1, group_top=2, renorm=True, scaling=1.0,
+                 live=None):
+    """The k experts of each token from given logits (T, E), bf16, fp16 or fp32 -> (topk_ids (T, k) int32, topk_w (T, k)
+    fp32).  score "softmax" or "sigmoid"; bias (E,) fp32 joins the scores for the selection only; topk_group < n_group keeps
+    the groups with the largest sums of their group_top best values; renorm divides the weights by their sum; live (T,)
+    bool: padding tokens (False) get ids -1 and weights 0, which dispatch and moe_experts route nowhere."""
+    T, E, ld = _routing(logits, k, score, n_group, topk_group, group_top)
+    dev = logits.device
+    _on(bias, "bias", dev, (E,), (torch.float32,))
+    _on(live, "live", dev, (T,), (torch.bool, torch.uint8))
+    ids = torch.empty(T, k, device=dev, dtype=torch.int32)
+    w = torch.empty(T, k, device=dev, dtype=torch.float32)
+    _call_on(dev, "hmoe_route_scores", logits.data_ptr(), ld, L.dt(logits), L.ptr(bias), L.ptr(live), T, E, k,
+             _SCORES[score], n_group, topk_group, group_top, int(bool(renorm)), float(scaling), ids.data_ptr(), w.data_ptr())
+    return ids, w
+
+
+def route_scores_bwd(dtw, tw, logits, ids, score="softmax", renorm=True, scaling=1.0):
+    """dlogits (T, E) of the logits' type from dtw (T, k) fp32, the gradient of route_scores' weights tw; ids as it gave
+    them."""
+    T, k = ids.shape
+    _, E, ld = _routing(logits, k, score, 1, 1, 1)
+    dev = logits.device
+    if logits.shape[0] != T:
+        raise ValueError(f"topk_ids for {T} tokens, logits for {logits.shape[0]}")
+    _on(ids, "topk_ids", dev, (T, k), _I32)
+    _on(tw, "topk_w", dev, (T, k), (torch.float32,))
+    _on(dtw, "dtopk_w", dev, (T, k), (torch.float32,))
+    dl = torch.empty(T, E, device=dev, dtype=logits.dtype)
+    _call_on(dev, "hmoe_route_scores_bwd", dtw.data_ptr(), tw.data_ptr(), logits.data_ptr(), ld, L.dt(logits),
+             ids.data_ptr(), T, E, k, _SCORES[score], int(bool(renorm)), float(scaling), dl.data_ptr())
+    return dl
+
+
+def router_wgrad(dlogits, x, dtype=torch.float32):
+    """dwr (E, d) = dlogits^T @ x from the logits' gradient (T, E) fp32 and x (T, d) bf16; fp32 or bf16."""
+    T, E = dlogits.shape
+    d = x.shape[1]
+    _need(dlogits, "dlogits", (T, E), (torch.float32,))
+    _need(x, "x", (T, d), _BF16, contig=False)
+    dwr = torch.empty(E, d, device=x.device, dtype=dtype)
+    ws_bytes = L.lib().hmoe_router_bwd_workspace_size(T, E, d)
+    ws = torch.empty(ws_bytes, device=x.device, dtype=torch.uint8)
+    L.call("hmoe_router_wgrad", L.ptr(dlogits), L.ptr(x), x.stride(0), T, E, d, L.ptr(dwr), L.dt(dwr), L.ptr(ws), ws_bytes,
+           _dev_stream(x))
+    return dwr
+
+
+def _sample_params(T, d, dev, starts, **mods):
+    """The number of samples B of per-sample parameters: (B, d) each, or (d,) for one set; with starts (B + 1,)."""
+    B = None
+    for name, t in mods.items():
+        if t is None:
+            continue
+        b = 1 if t.dim() == 1 else t.shape[0]
+        _on(t, name, dev, (d,) if t.dim() == 1 else (b, d), _FLOATS)
+        if B is not None and b != B:
+            raise ValueError(f"{name} has {b} samples, another parameter {B}")
+        B = b
+    if starts is not None:
+        n = starts.numel() - 1
+        _on(starts, "starts", dev, (n + 1,), _I32)
+        if n < 1 or (B is not None and B != n):
+            raise ValueError(f"starts names {n} samples" + ("" if B is None else f", the parameters hold {B}"))
+        return n
+    if B is None:
+        return 1
+    if B < 1 or T % B:
+        raise ValueError(f"{T} rows do not divide into {B} samples (pass starts for samples of unequal lengths)")
+    return B
+
+
+def _block_dtype(stream, dtype):
+    dtype = stream if dtype is None else dtype
+    if dtype not in _FLOATS or (dtype != stream and stream != torch.float32):
+        raise TypeError(f"a block type of {dtype} does not go with a stream of {stream} (equal, or an fp32 stream)")
+    return dtype
+
+
+def _dt0(t):
+    return 0 if t is None else L._DT[t.dtype]
+
+
+def norm_modulate(x, weight=None, scale=None, shift=None, starts=None, eps=1e-6, dtype=None):
+    """h (T, d) = n * weight * (1 + scale_b) + shift_b, n = x / sqrt(mean(x^2) + eps): the input of a block from the
+    residual stream x (T, d).  weight (d,); scale and shift (B, d) per sample of T / B rows each, or with starts (B + 1,)
+    int32 of rows starts[b] .. starts[b + 1] - 1 (rows outside are padding: h = 0); (d,) for one set.  dtype: h's type, x's
+    by default; an fp32 stream may have a 16-bit block."""
+    T, d, ldx = _rows(x, "x")
+    dev = x.device
+    dtype = _block_dtype(x.dtype, dtype)
+    _on(weight, "weight", dev, (d,), _FLOATS)
+    B = _sample_params(T, d, dev, starts, scale=scale, shift=shift)
+    if scale is not None and shift is not None and scale.dtype != shift.dtype:
+        raise TypeError(f"scale and shift must have one type (got {scale.dtype}, {shift.dtype})")
+    h = torch.empty(T, d, device=dev, dtype=dtype)
+    _call_on(dev, "hmoe_norm_modulate", x.data_ptr(), ldx, L._DT[x.dtype], L.ptr(weight), _dt0(weight), L.ptr(scale),
+             L.ptr(shift), _dt0(shift if scale is None else scale), L.ptr(starts), B, T, d, float(eps), h.data_ptr(),
+             L._DT[dtype])
+    return h
+
+
+def norm_modulate_bwd(dh, x, weight=None, scale=None, shift=None, starts=None, eps=1e-6, dres=None, dres_scale=1.0,
+                      want=("weight", "scale", "shift")):
+    """(dx, dweight, dscale, dshift) of norm_modulate, None for parameters that are absent or not in `want`; dres (T, d) of
+    x's type, the gradient of x past the block, joins dx as dres_scale * dres.  dx has x's type, the others their
+    parameters'."""
+    T, d, ldx = _rows(x, "x")
+    dev = x.device
+    _on(dh, "dh", dev, (T, d), (_block_dtype(x.dtype, dh.dtype),))
+    _on(weight, "weight", dev, (d,), _FLOATS)
+    _on(dres, "dres", dev, (T, d), (x.dtype,))
+    B = _sample_params(T, d, dev, starts, scale=scale, shift=shift)
+    if scale is not None and shift is not None and scale.dtype != shift.dtype:
+        raise TypeError(f"scale and shift must have one type (got {scale.dtype}, {shift.dtype})")
+    dx = torch.empty(T, d, device=dev, dtype=x.dtype)
+    dw = torch.empty_like(weight) if weight is not None and "weight" in want else None
+    dsc = torch.empty_like(scale) if scale is not None and "scale" in want else None
+    dsh = torch.empty_like(shift) if shift is not None and "shift" in want else None
+    ws, ws_bytes = None, 0
+    if dw is not None or dsc is not None or dsh is not None:
+        ws_bytes = L.lib().hmoe_norm_modulate_bwd_workspace_size(T, d, B)
+        ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
+    _call_on(dev, "hmoe_norm_modulate_bwd", dh.data_ptr(), L._DT[dh.dtype], x.data_ptr(), ldx, L._DT[x.dtype],
+             L.ptr(weight), _dt0(weight), L.ptr(scale), L.ptr(shift), _dt0(shift if scale is None else scale),
+             L.ptr(starts), B, T, d, float(eps), L.ptr(dres), float(dres_scale), dx.data_ptr(), L.ptr(dw), L.ptr(dsc),
+             L.ptr(dsh), L.ptr(ws), ws_bytes)
+    return dx, dw, dsc, dsh
+
+
+def _slots(y, k, T, d, dev, inv_pos, add):
+    if k < 1:
+        raise ValueError(f"k = {k} slots")
+    _on(y, "y", dev, (T * k, d), _FLOATS)
+    _on(inv_pos, "inv_pos", dev, (T * k,), _I32)
+    _on(add, "add", dev, (T, d), (y.dtype,))
+
+
+def norm_residual(y, x, gate=None, weight=None, norm=True, starts=None, eps=1e-6, alpha=1.0, k=1, inv_pos=None, add=None):
+    """out (T, d) = alpha * x + gate_b * weight * n, n = s / sqrt(mean(s^2) + eps) (s itself without norm): the gated
+    residual behind a block.  s is the sum over the k slots of y (T*k, d) (plus add (T, d), the shared expert's output), what
+    combine gives without its rounding; with inv_pos from the dispatch, slots routed nowhere add nothing.  gate (B, d) per
+    sample as in norm_modulate, or (d,); padding rows get alpha * x.  out has the type of the stream x."""
+    T, d, ldx = _rows(x, "x")
+    dev = x.device
+    _block_dtype(x.dtype, y.dtype)
+    _slots(y, k, T, d, dev, inv_pos, add)
+    _on(weight, "weight", dev, (d,), _FLOATS)
+    B = _sample_params(T, d, dev, starts, gate=gate)
+    out = torch.empty(T, d, device=dev, dtype=x.dtype)
+    _call_on(dev, "hmoe_norm_residual", y.data_ptr(), L.ptr(inv_pos), k, L.ptr(add), L._DT[y.dtype], x.data_ptr(), ldx,
+             L._DT[x.dtype], L.ptr(weight), _dt0(weight), L.ptr(gate), _dt0(gate), L.ptr(starts), B, T, d, int(bool(norm)),
+             float(eps), float(alpha), out.data_ptr())
+    return out
+
+
+def norm_residual_bwd(dout, y, gate=None, weight=None, norm=True, starts=None, eps=1e-6, k=1, inv_pos=None, add=None,
+                      want=("weight", "gate")):
+    """(dy, dgate, dweight) of norm_residual, None for parameters that are absent or not in `want`: dy (T, d) of y's type is
+    the gradient of the slots' sum (of every slot and of add); x's is alpha * dout."""
+    _, d, ld = _rows(dout, "dout")
+    T = dout.shape[0]
+    dev = dout.device
+    _on(dout, "dout", dev, (T, d), _FLOATS)
+    _block_dtype(dout.dtype, y.dtype)
+    _slots(y, k, T, d, dev, inv_pos, add)
+    _on(weight, "weight", dev, (d,), _FLOATS)
+    B = _sample_params(T, d, dev, starts, gate=gate)
+    dy = torch.empty(T, d, device=dev, dtype=y.dtype)
+    dw = torch.empty_like(weight) if weight is not None and "weight" in want else None
+    dg = torch.empty_like(gate) if gate is not None and "gate" in want else None
+    ws, ws_bytes = None, 0
+    if dw is not None or dg is not None:
+        ws_bytes = L.lib().hmoe_norm_residual_bwd_workspace_size(T, d, B)
+        ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
+    _call_on(dev, "hmoe_norm_residual_bwd", dout.data_ptr(), L._DT[dout.dtype], y.data_ptr(), L.ptr(inv_pos), k,
+             L.ptr(add), L._DT[y.dtype], L.ptr(weight), _dt0(weight), L.ptr(gate), _dt0(gate), L.ptr(starts), B, T, d,
+             int(bool(norm)), float(eps), dy.data_ptr(), L.ptr(dw), L.ptr(dg), L.ptr(ws), ws_bytes)
+    return dy, dg, dw
+
+
+def _dense(t):
+    """Whether t's elements fill one stretch of memory (contiguous in some order of its dimensions)."""
+    return t.is_contiguous() or t.permute(sorted(range(t.dim()), key=t.stride, reverse=True)).is_contiguous()
+
+
+class GradList:
+    """The tensors of a clipping call as the C entry points take them: addresses, element counts and types."""
+
+    def __init__(self, grads, out=None):
+        grads = list(grads)
+        out = grads if out is None else list(out)
+        if len(out) != len(grads):
+            raise ValueError(f"{len(out)} outputs for {len(grads)} gradients")
+        dev = None
+        for g, o in zip(grads, out):
+            if not g.is_cuda or g.layout is not torch.strided:
+                raise RuntimeError("gradients must be dense ROCm GPU tensors: the hmoe kernels have no CPU path")
+            if g.dtype not in _FLOATS:
+                raise TypeError(f"gradient: dtype {g.dtype} not in {_FLOATS}")
+            if dev is None:
+                dev = g.device
+            if g.device != dev or o.device != dev:
+                raise ValueError("the gradients of a call live on one device")
+            if not _dense(g):
+                raise ValueError(f"a gradient's elements must be contiguous (strides {g.stride()})")
+            if o is not g and (o.shape != g.shape or (o.stride() != g.stride() and g.numel() > 1)
+                               or o.dtype not in (g.dtype, torch.float32)):
+                raise ValueError("an output has its gradient's shape and strides, and its type or fp32")
+        self.n = len(grads)
+        self.device = dev
+        self.keep = (grads, out)
+        self.ptr = array("Q", [g.data_ptr() for g in grads])
+        self.out = array("Q", [o.data_ptr() for o in out])
+        self.numel = array("q", [g.numel() for g in grads])
+        self.dt = array("i", [L._DT[g.dtype] for g in grads])
+        self.odt = array("i", [L._DT[o.dtype] for o in out])
+        used = [p for p, n in zip(self.out, self.numel) if n]
+        if len(set(used)) != len(used):
+            raise ValueError("a tensor is listed twice")
+
+
+def _addr(a):
+    return a.buffer_info()[0] if len(a) else None
+
+
+def grad_sq_norm(grads):
+    """(1,) fp64 on the device: the sum of the squares of every element of a list of gradients (or a GradList)."""
+    gl = grads if isinstance(grads, GradList) else GradList(grads)
+    dev = gl.device if gl.device is not None else torch.device("cuda", torch.cuda.current_device())
+    sq = torch.empty(1, device=dev, dtype=torch.float64)
+    ws_bytes = L.lib().hmoe_grad_sq_norm_workspace_size(gl.n)
+    ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
+    _call_on(dev, "hmoe_grad_sq_norm", _addr(gl.ptr), _addr(gl.numel), _addr(gl.dt), gl.n, sq.data_ptr(), ws.data_ptr(),
+             ws_bytes)
+    return sq
+
+
+def grad_clip(grads, sq_norm, max_norm, out=None):
+    """Scales a list of gradients (or a GradList) by min(1, max_norm / (norm + 1e-6)), norm = sqrt(sq_norm) -- in place, or
+    into `out` (tensors of the gradients' shapes, of their types or fp32).  Returns the norm, () fp32 on the device."""
+    gl = grads if isinstance(grads, GradList) else GradList(grads, out)
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError(f"max_norm = {max_norm}")
+    dev = sq_norm.device
+    _on(sq_norm, "sq_norm", dev if gl.device is None else gl.device, (1,), (torch.float64,))
+    L.require_gpu(sq_norm, "sq_norm")
+    norm = torch.empty((), device=dev, dtype=torch.float32)
+    _call_on(dev, "hmoe_grad_clip", _addr(gl.ptr), _addr(gl.out), _addr(gl.numel), _addr(gl.dt), _addr(gl.odt), gl.n,
+             sq_norm.data_ptr(), max_norm, norm.data_ptr())
+    return norm
