@@ -6,13 +6,25 @@
 namespace hmoe {
 
 // ---------------------------------------------------------------------------------------------------------------
-// Eight consecutive elements as fp32, of a type known at compile time (rows) or at run time (parameters: a branch that
+// Eight consecutive elements, 16 bytes aligned, at column col of the row that starts at element `row` of p: the row is the
+// same for the whole wave, so it stays in scalar registers.  As fp32, of a type known at compile time (rows) or at run time (parameters: a branch that
 // is uniform over the grid).
 // ---------------------------------------------------------------------------------------------------------------
 template <int DT>
-__device__ __forceinline__ void load8(const void* p, int64_t off, float (&v)[8]) {
+constexpr int kSize = DT == HMOE_DT_F32 ? 4 : 2;
+template <int DT>
+__device__ __forceinline__ const void* at(const void* p, int64_t row, uint32_t col) {
+  return static_cast<const char*>(p) + row * kSize<DT> + col * kSize<DT>;
+}
+template <int DT>
+__device__ __forceinline__ void* at(void* p, int64_t row, uint32_t col) {
+  return static_cast<char*>(p) + row * kSize<DT> + col * kSize<DT>;
+}
+
+template <int DT>
+__device__ __forceinline__ void load8(const void* p, int64_t row, uint32_t col, float (&v)[8]) {
   if constexpr (DT == HMOE_DT_F32) {
-    const f32x4* q = reinterpret_cast<const f32x4*>(static_cast<const float*>(p) + off);
+    const f32x4* q = static_cast<const f32x4*>(at<DT>(p, row, col));
     const f32x4 a = q[0], b = q[1];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -21,7 +33,7 @@ __device__ __forceinline__ void load8(const void* p, int64_t off, float (&v)[8])
     }
   } else {
     using X = Elt<DT == HMOE_DT_F16>;
-    const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + off);
+    const uint4 u = *static_cast<const uint4*>(at<DT>(p, row, col));
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -31,35 +43,70 @@ __device__ __forceinline__ void load8(const void* p, int64_t off, float (&v)[8])
   }
 }
 
+// The same eight elements as they lie in memory: a row waits for its sums in this form (half the registers of fp32 for
+// 16-bit types) and is widened at each use.
 template <int DT>
-__device__ __forceinline__ void store8(void* p, int64_t off, const float (&v)[8]) {
+struct Raw8 {
+  static constexpr int kRegs = DT == HMOE_DT_F32 ? 8 : 4;
+  uint32_t w[kRegs];
+  __device__ __forceinline__ void load(const void* p, int64_t row, uint32_t col) {
+    const uint4* q = static_cast<const uint4*>(at<DT>(p, row, col));
+#pragma unroll
+    for (int i = 0; i < kRegs / 4; ++i) {
+      const uint4 u = q[i];
+      w[4 * i] = u.x;
+      w[4 * i + 1] = u.y;
+      w[4 * i + 2] = u.z;
+      w[4 * i + 3] = u.w;
+    }
+  }
+  __device__ __forceinline__ float operator[](int e) const {
+    if constexpr (DT == HMOE_DT_F32) return __uint_as_float(w[e]);
+    else {
+      using X = Elt<DT == HMOE_DT_F16>;
+      return e & 1 ? X::hi(w[e >> 1]) : X::lo(w[e >> 1]);
+    }
+  }
+  __device__ __forceinline__ void keep(bool on) {
+#pragma unroll
+    for (int i = 0; i < kRegs; ++i) w[i] = on ? w[i] : 0;
+  }
+  // the compiler must not keep the widened elements across this point
+  __device__ __forceinline__ void hold() {
+#pragma unroll
+    for (int i = 0; i < kRegs; ++i) asm volatile("" : "+v"(w[i]));
+  }
+};
+
+template <int DT>
+__device__ __forceinline__ void store8(void* p, int64_t row, uint32_t col, const float (&v)[8]) {
   if constexpr (DT == HMOE_DT_F32) {
-    f32x4* q = reinterpret_cast<f32x4*>(static_cast<float*>(p) + off);
+    f32x4* q = static_cast<f32x4*>(at<DT>(p, row, col));
     q[0] = f32x4{v[0], v[1], v[2], v[3]};
     q[1] = f32x4{v[4], v[5], v[6], v[7]};
   } else {
     using X = Elt<DT == HMOE_DT_F16>;
-    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + off) =
+    *static_cast<uint4*>(at<DT>(p, row, col)) =
         make_uint4(X::pack2(v[0], v[1]), X::pack2(v[2], v[3]), X::pack2(v[4], v[5]), X::pack2(v[6], v[7]));
   }
 }
 
-__device__ __forceinline__ void load8_rt(const void* p, int dt, int64_t off, float (&v)[8]) {
+__device__ __forceinline__ void load8_rt(const void* p, int dt, int64_t row, uint32_t col, float (&v)[8]) {
   if (dt == HMOE_DT_F32)
-    load8<HMOE_DT_F32>(p, off, v);
+    load8<HMOE_DT_F32>(p, row, col, v);
   else if (dt == HMOE_DT_F16)
-    load8<HMOE_DT_F16>(p, off, v);
+    load8<HMOE_DT_F16>(p, row, col, v);
   else
-    load8<HMOE_DT_BF16>(p, off, v);
+    load8<HMOE_DT_BF16>(p, row, col, v);
 }
 
-__device__ __forceinline__ void store8_rt(void* p, int dt, int64_t off, const float (&v)[8]) {
+__device__ __forceinline__ void store8_rt(void* p, int dt, int64_t row, uint32_t col, const float (&v)[8]) {
   if (dt == HMOE_DT_F32)
-    store8<HMOE_DT_F32>(p, off, v);
+    store8<HMOE_DT_F32>(p, row, col, v);
   else if (dt == HMOE_DT_F16)
-    store8<HMOE_DT_F16>(p, off, v);
+    store8<HMOE_DT_F16>(p, row, col, v);
   else
-    store8<HMOE_DT_BF16>(p, off, v);
+    store8<HMOE_DT_BF16>(p, row, col, v);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -72,50 +119,74 @@ struct Samples {
   int B, L, T;
 };
 
-// the sample of row r (-1 or B: a padding row before the first / behind the last) and the end of its run of rows
+// The sample of row r (-1 or B: a padding row before the first / behind the last) and the end of its run of rows.  r is
+// the same for the whole wave: a search down to 64 entries, which the lanes then read at once.
 __device__ __forceinline__ int sample_of(const Samples& s, int r, int& end) {
   if (!s.starts) {
     const int b = (uint32_t)r / (uint32_t)s.L;
     end = (b + 1) * s.L;
     return b;
   }
-  int lo = -1, hi = s.B + 1;  // starts[lo] <= r < starts[hi]
-  while (hi - lo > 1) {
+  int lo = -1, hi = s.B + 1;  // starts[lo] <= r < starts[hi], with starts[-1] = 0 and starts[B + 1] = T
+  while (hi - lo > 64) {
     const int m = (lo + hi) >> 1;
     if (s.starts[m] <= r)
       lo = m;
     else
       hi = m;
   }
-  end = hi <= s.B ? s.starts[hi] : s.T;
+  const int i = lo + 1 + wave_lane();
+  const int v = i <= s.B && i <= hi ? s.starts[i] : INT32_MAX;
+  const uint64_t past = ~__ballot(v <= r);
+  const int n = past ? __builtin_ctzll(past) : 63;
+  end = min(__builtin_amdgcn_readlane(v, n), s.T);
   end = end > r ? end : r + 1;
-  return lo;
+  return lo + n;
 }
 
 // ---------------------------------------------------------------------------------------------------------------
 // A row is held by WPR waves, each lane VPL vectors of eight columns: vector i of lane l of the row's 64 WPR is
-// l + 64 WPR i.
+// l + 64 WPR i.  The backward's workgroups have eight waves (16 for WPR = 16) and hold several rows at once.  At most three
+// vectors a lane: it keeps two column sums and the row's parameters in registers beside the rows.  by_width picks VPL and WPR
+// so that only a lane's last vector can lie past the row (vec_in).  Loads are not predicated, which would make them wait for
+// each other: such a vector reads the row's last one and a row past the end the last row, and both are dropped after.
 // ---------------------------------------------------------------------------------------------------------------
-constexpr int64_t kNormMaxD = 16 * 64 * 2 * 8;  // the widest: 16 waves, 64 lanes, two vectors of eight columns
-
-// sums of two values over a row's waves; every lane of the row ends with both
+constexpr int64_t kNormMaxD = 16 * 64 * 2 * 8;
 template <int WPR>
-__device__ __forceinline__ void row_sum2(float& a, float& b, float* red) {
+constexpr int kNormThreads = WPR == 16 ? 1024 : 512;
+template <int WPR>
+constexpr int kNormGroups = kNormThreads<WPR> / 64 / WPR;
+template <int WPR>
+constexpr int kFwdThreads = WPR <= 2 ? 128 : 64 * WPR;  // the forward's: small, for an even share of the rows
+template <int WPR>
+constexpr int kFwdGroups = kFwdThreads<WPR> / 64 / WPR;
+
+// whether vector c, a lane's i-th, lies in a row of nv vectors
+template <int VPL>
+__device__ __forceinline__ bool vec_in(int i, int c, int nv) {
+  return i < VPL - 1 || c < nv;
+}
+
+// sums of two values over a row's waves; every lane of the row ends with both.  Successive calls alternate between the two
+// halves of red (2 x 32 floats): one barrier each, since a wave comes back to a half only past the other half's barrier.
+template <int WPR>
+__device__ __forceinline__ void row_sum2(float& a, float& b, float* red, int& half) {
   a = wave_sum_butterfly(a);
   b = wave_sum_butterfly(b);
   if constexpr (WPR > 1) {
     const int wave = threadIdx.x >> 6, row = wave / WPR * WPR;
-    __syncthreads();  // the last use of red is over
+    float* r = red + 32 * half;
+    half ^= 1;
     if ((threadIdx.x & 63) == 0) {
-      red[2 * wave] = a;
-      red[2 * wave + 1] = b;
+      r[2 * wave] = a;
+      r[2 * wave + 1] = b;
     }
     __syncthreads();
     a = b = 0.0f;
 #pragma unroll
     for (int i = 0; i < WPR; ++i) {
-      a += red[2 * (row + i)];
-      b += red[2 * (row + i) + 1];
+      a += r[2 * (row + i)];
+      b += r[2 * (row + i) + 1];
     }
   }
 }
@@ -133,61 +204,78 @@ struct NormInArgs {
   void* h;
   NormParams p;
   Samples s;
-  int d;
+  int d, R;
   float eps;
 };
 
-// h = x r w (1 + scale_b) + shift_b, r = (mean(x^2) + eps)^-1/2, 0 on padding rows.  Waves walk rows grid-strided.
+// h = x r w (1 + scale_b) + shift_b, r = (mean(x^2) + eps)^-1/2, 0 on padding rows.  A workgroup takes R rows, each of its
+// row groups every kNormGroups-th; the parameters of a sample are read once, beside its first row, and the next row is
+// on its way while a row is summed.
 template <int ST, int HT, int VPL, int WPR>
-__global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void norm_in_kernel(NormInArgs a) {
-  __shared__ float red[2 * 16];
-  const int nv = a.d / 8, rpb = (int)(blockDim.x >> 6) / WPR;
-  const int lane = threadIdx.x % (64 * WPR);
-  for (int r0 = blockIdx.x * rpb; r0 < a.s.T; r0 += gridDim.x * rpb) {
-    const int r = r0 + threadIdx.x / (64 * WPR);
-    const bool row = r < a.s.T;
-    float x[VPL][8];
-    float sq = 0.0f, unused = 0.0f;
+__global__ __launch_bounds__(kFwdThreads<WPR>) void norm_in_kernel(NormInArgs a) {
+  __shared__ float red[2 * 32];
+  constexpr int G = kFwdGroups<WPR>;
+  const int nv = a.d / 8, lane = threadIdx.x % (64 * WPR);
+  const int grp = __builtin_amdgcn_readfirstlane(threadIdx.x / (64 * WPR));
+  const int r_end = min(a.s.T, (int)(blockIdx.x + 1) * a.R);
+  int half = 0, b = 0, end = -1;
+  bool live = false;
+  Raw8<ST> x[VPL], nx[VPL];
+  auto fetch = [&](int r, Raw8<ST> (&v)[VPL]) {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      v[i].load(a.x, (int64_t)min(r, r_end - 1) * a.ldx, 8 * min(lane + 64 * WPR * i, nv - 1));
+  };
+  float m[VPL][8], sh[VPL][8];
+  const int r0 = blockIdx.x * a.R;
+  fetch(r0 + grp, nx);
+  for (int rg = r0; rg < r_end; rg += G) {  // (the same count for every wave: row_sum2 may hold a barrier)
+    const int r = rg + grp;
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
-      const int c = lane + 64 * WPR * i;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[i][e] = 0.0f;
-      if (row && c < nv) load8<ST>(a.x, (int64_t)r * a.ldx + 8 * c, x[i]);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sq += x[i][e] * x[i][e];
+      x[i] = nx[i];
+      x[i].keep(vec_in<VPL>(i, lane + 64 * WPR * i, nv));
     }
-    row_sum2<WPR>(sq, unused, red);
-    const float rms = inv_rms(sq, a.d, a.eps);
-    if (!row) continue;
-    int end;
-    const int b = sample_of(a.s, r, end);
-    const bool live = b >= 0 && b < a.s.B;
+    if (rg + G < r_end) fetch(r + G, nx);
+    if (r < r_end && r >= end) {
+      b = sample_of(a.s, r, end);
+      live = b >= 0 && b < a.s.B;
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      const int c = lane + 64 * WPR * i;
-      if (c >= nv) continue;
-      float h[8], t[8];
+      for (int i = 0; i < VPL; ++i) {
+        const int c = lane + 64 * WPR * i;
+        float t[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) h[e] = live ? x[i][e] * rms : 0.0f;
-      if (live) {
-        if (a.p.weight) {
-          load8_rt(a.p.weight, a.p.weight_dt, 8 * c, t);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) h[e] *= t[e];
+        for (int e = 0; e < 8; ++e) {
+          m[i][e] = 1.0f;
+          sh[i][e] = 0.0f;
         }
-        if (a.p.scale) {
-          load8_rt(a.p.scale, a.p.scale_dt, (int64_t)b * a.d + 8 * c, t);
+        if (live && vec_in<VPL>(i, c, nv)) {
+          if (a.p.weight) load8_rt(a.p.weight, a.p.weight_dt, 0, 8 * c, m[i]);
+          if (a.p.scale) {
+            load8_rt(a.p.scale, a.p.scale_dt, (int64_t)b * a.d, 8 * c, t);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) h[e] *= 1.0f + t[e];
-        }
-        if (a.p.shift) {
-          load8_rt(a.p.shift, a.p.shift_dt, (int64_t)b * a.d + 8 * c, t);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) h[e] += t[e];
+            for (int e = 0; e < 8; ++e) m[i][e] *= 1.0f + t[e];
+          }
+          if (a.p.shift) load8_rt(a.p.shift, a.p.shift_dt, (int64_t)b * a.d, 8 * c, sh[i]);
         }
       }
-      store8<HT>(a.h, (int64_t)r * a.d + 8 * c, h);
+    }
+    float sq = 0.0f, unused = 0.0f;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sq += x[i][e] * x[i][e];
+    row_sum2<WPR>(sq, unused, red, half);
+    const float rms = inv_rms(sq, a.d, a.eps);
+    if (r >= r_end) continue;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      const int c = lane + 64 * WPR * i;
+      if (!vec_in<VPL>(i, c, nv)) continue;
+      float h[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) h[e] = live ? x[i][e] * rms * m[i][e] + sh[i][e] : 0.0f;
+      store8<HT>(a.h, (int64_t)r * a.d, 8 * c, h);
     }
   }
 }
@@ -200,82 +288,116 @@ struct NormOutArgs {
   void* out;
   NormParams p;
   Samples s;
-  int d, k, norm;
+  int d, k, norm, R;
   float eps, alpha;
 };
 
-// the k slots of row r, columns 8 c .. 8 c + 7, summed in slot order in fp32, then the addend; a slot routed nowhere
-// adds nothing (its row of y was never written)
-template <int HT>
+// s = the sum over the k slots of row r in slot order in fp32, then the addend; a slot routed nowhere adds nothing (its row of
+// y was never written).  KB slots are on their way at once.
+template <int HT, int VPL, int WPR, int KB>
 __device__ __forceinline__ void load_slots(const void* y, const int32_t* inv_pos, const void* add, int k, int d, int r,
-                                           int c, float (&v)[8]) {
+                                           int lane, float (&s)[VPL][8]) {
+  const int nv = d / 8;
+  uint32_t col[VPL];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-  float t[8];
-  for (int j = 0; j < k; ++j) {
-    const int64_t f = (int64_t)r * k + j;
-    load8<HT>(y, f * d + 8 * c, t);
-    const bool on = !inv_pos || inv_pos[f] >= 0;
+  for (int i = 0; i < VPL; ++i) {
+    col[i] = 8 * min(lane + 64 * WPR * i, nv - 1);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] += on ? t[e] : 0.0f;
+    for (int e = 0; e < 8; ++e) s[i][e] = 0.0f;
+  }
+  Raw8<HT> ad[VPL];
+  if (add) {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) ad[i].load(add, (int64_t)r * d, col[i]);
+  }
+  for (int j0 = 0; j0 < k; j0 += KB) {
+    Raw8<HT> t[KB][VPL];
+    bool on[KB];
+#pragma unroll
+    for (int j = 0; j < KB; ++j) {
+      const int64_t f = (int64_t)r * k + min(j0 + j, k - 1);
+      on[j] = j0 + j < k && (!inv_pos || inv_pos[f] >= 0);
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) t[j][i].load(y, f * d, col[i]);
+    }
+#pragma unroll
+    for (int j = 0; j < KB; ++j)
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) {
+        t[j][i].keep(on[j] && vec_in<VPL>(i, lane + 64 * WPR * i, nv));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[i][e] += t[j][i][e];
+      }
   }
   if (add) {
-    load8<HT>(add, (int64_t)r * d + 8 * c, t);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] += t[e];
+    for (int i = 0; i < VPL; ++i) {
+      ad[i].keep(vec_in<VPL>(i, lane + 64 * WPR * i, nv));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[i][e] += ad[i][e];
+    }
   }
 }
 
-// out = alpha x + gate_b w s r(s), s the sum over the row's slots; alpha x on padding rows (whose y is not used)
-template <int ST, int HT, int VPL, int WPR>
-__global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void norm_out_kernel(NormOutArgs a) {
-  __shared__ float red[2 * 16];
-  const int nv = a.d / 8, rpb = (int)(blockDim.x >> 6) / WPR;
-  const int lane = threadIdx.x % (64 * WPR);
-  for (int r0 = blockIdx.x * rpb; r0 < a.s.T; r0 += gridDim.x * rpb) {
-    const int r = r0 + threadIdx.x / (64 * WPR);
-    const bool row = r < a.s.T;
+// out = alpha x + gate_b w s r(s), s the sum over the row's slots; alpha x on padding rows (whose y is not used).  Rows are
+// dealt as in norm_in_kernel.
+template <int ST, int HT, int VPL, int WPR, int KB>
+__global__ __launch_bounds__(kFwdThreads<WPR>, ST == HMOE_DT_F32 || KB == 4 ? 2 : 4) void norm_out_kernel(NormOutArgs a) {
+  __shared__ float red[2 * 32];
+  constexpr int G = kFwdGroups<WPR>;
+  const int nv = a.d / 8, lane = threadIdx.x % (64 * WPR);
+  const int grp = __builtin_amdgcn_readfirstlane(threadIdx.x / (64 * WPR));
+  const int r_end = min(a.s.T, (int)(blockIdx.x + 1) * a.R);
+  int half = 0, b = 0, end = -1;
+  bool live = false;
+  float m[VPL][8];
+  for (int rg = blockIdx.x * a.R; rg < r_end; rg += G) {
+    const int r = rg + grp;
+    const bool row = r < r_end;
+    Raw8<ST> x[VPL];
     float y[VPL][8];
-    float sq = 0.0f, unused = 0.0f;
+    const int rc = min(r, r_end - 1);
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      const int c = lane + 64 * WPR * i;
+    for (int i = 0; i < VPL; ++i) x[i].load(a.x, (int64_t)rc * a.ldx, 8 * min(lane + 64 * WPR * i, nv - 1));
+    load_slots<HT, VPL, WPR, KB>(a.y, a.inv_pos, a.add, a.k, a.d, rc, lane, y);
+    if (row && r >= end) {
+      b = sample_of(a.s, r, end);
+      live = b >= 0 && b < a.s.B;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[i][e] = 0.0f;
-      if (row && c < nv) load_slots<HT>(a.y, a.inv_pos, a.add, a.k, a.d, r, c, y[i]);
+      for (int i = 0; i < VPL; ++i) {
+        const int c = lane + 64 * WPR * i;
+        float t[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sq += y[i][e] * y[i][e];
+        for (int e = 0; e < 8; ++e) m[i][e] = 1.0f;
+        if (live && vec_in<VPL>(i, c, nv)) {
+          if (a.p.weight) load8_rt(a.p.weight, a.p.weight_dt, 0, 8 * c, m[i]);
+          if (a.p.scale) {
+            load8_rt(a.p.scale, a.p.scale_dt, (int64_t)b * a.d, 8 * c, t);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) m[i][e] *= t[e];
+          }
+        }
+      }
     }
     float rms = 1.0f;
     if (a.norm) {
-      row_sum2<WPR>(sq, unused, red);
+      float sq = 0.0f, unused = 0.0f;
+#pragma unroll
+      for (int i = 0; i < VPL; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sq += y[i][e] * y[i][e];
+      row_sum2<WPR>(sq, unused, red, half);
       rms = inv_rms(sq, a.d, a.eps);
     }
     if (!row) continue;
-    int end;
-    const int b = sample_of(a.s, r, end);
-    const bool live = b >= 0 && b < a.s.B;
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
       const int c = lane + 64 * WPR * i;
-      if (c >= nv) continue;
-      float x[8], t[8], z[8];
-      load8<ST>(a.x, (int64_t)r * a.ldx + 8 * c, x);
+      if (!vec_in<VPL>(i, c, nv)) continue;
+      float z[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) z[e] = live ? y[i][e] * rms : 0.0f;
-      if (live && a.p.weight) {
-        load8_rt(a.p.weight, a.p.weight_dt, 8 * c, t);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) z[e] *= t[e];
-      }
-      if (live && a.p.scale) {
-        load8_rt(a.p.scale, a.p.scale_dt, (int64_t)b * a.d + 8 * c, t);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) z[e] *= t[e];
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) z[e] = a.alpha * x[e] + z[e];
-      store8<ST>(a.out, (int64_t)r * a.d + 8 * c, z);
+      for (int e = 0; e < 8; ++e) z[e] = a.alpha * x[i][e] + (live ? y[i][e] * rms * m[i][e] : 0.0f);
+      store8<ST>(a.out, (int64_t)r * a.d, 8 * c, z);
     }
   }
 }
@@ -311,39 +433,69 @@ struct NormBwdArgs {
   float eps;
 };
 
-template <bool OUT, int ST, int HT, int VPL, int WPR>
-__global__ __launch_bounds__(WPR == 16 ? 1024 : 512) void norm_bwd_kernel(NormBwdArgs a) {
-  constexpr int UT = OUT ? ST : HT;  // upstream type
-  __shared__ float red[2 * 16];
-  extern __shared__ float colsum[];  // (row groups) x d
-  const int nv = a.d / 8, ngrp = (int)(blockDim.x >> 6) / WPR;
-  const int lane = threadIdx.x % (64 * WPR), grp = threadIdx.x / (64 * WPR);
+// KB: 0 for norm_in, else the slots loaded at once for norm_out.
+template <int KB, int ST, int HT, int VPL, int WPR>
+__global__ __launch_bounds__(kNormThreads<WPR>) void norm_bwd_kernel(NormBwdArgs a) {
+  constexpr bool OUT = KB > 0;
+  constexpr int UT = OUT ? ST : HT, DT = OUT ? HT : ST;  // types of u and of dv
+  constexpr int G = kNormGroups<WPR>;
+  // column vectors a thread adds up over the row groups: tid, tid + threads, ...
+  constexpr int NC = (64 * WPR * VPL + kNormThreads<WPR> - 1) / kNormThreads<WPR>;
+  __shared__ float red[2 * 32];
+  extern __shared__ float colsum[];  // G x d
+  const int nv = a.d / 8, lane = threadIdx.x % (64 * WPR);
+  const int grp = __builtin_amdgcn_readfirstlane(threadIdx.x / (64 * WPR));
   const int r_begin = blockIdx.x * a.R, r_end = min(a.s.T, r_begin + a.R);
-  const bool sums = a.dscale || a.dshift;
   const int nsum = (a.dscale != nullptr) + (a.dshift != nullptr);
-  float wacc[VPL][8];
+  int half = 0;
+  float wacc[NC][8];
 #pragma unroll
-  for (int i = 0; i < VPL; ++i)
+  for (int i = 0; i < NC; ++i)
 #pragma unroll
     for (int e = 0; e < 8; ++e) wacc[i][e] = 0.0f;
-  // adds a column sum over the row groups and hands eight columns at a time to fin(column vector, sums)
+  // adds a column sum over the row groups and hands eight columns at a time to fin(i, column vector, sums)
   auto over_groups = [&](const float (&acc)[VPL][8], auto&& fin) {
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
       const int c = lane + 64 * WPR * i;
-      if (c < nv) store8<HMOE_DT_F32>(colsum, (int64_t)grp * a.d + 8 * c, acc[i]);
+      if (c < nv) store8<HMOE_DT_F32>(colsum, (int64_t)grp * a.d, 8 * c, acc[i]);
     }
     __syncthreads();
-    for (int c = threadIdx.x; c < nv; c += blockDim.x) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = threadIdx.x + kNormThreads<WPR> * i;
+      if (c >= nv) continue;
       float t[8], q[8];
-      load8<HMOE_DT_F32>(colsum, 8 * c, t);
-      for (int g = 1; g < ngrp; ++g) {
-        load8<HMOE_DT_F32>(colsum, (int64_t)g * a.d + 8 * c, q);
+      load8<HMOE_DT_F32>(colsum, 0, 8 * c, t);
+#pragma unroll
+      for (int g = 1; g < G; ++g) {
+        load8<HMOE_DT_F32>(colsum, (int64_t)g * a.d, 8 * c, q);
 #pragma unroll
         for (int e = 0; e < 8; ++e) t[e] += q[e];
       }
-      fin(c, t);
+      fin(i, c, t);
+    }
+  };
+  using VRaw = Raw8<OUT ? HMOE_DT_F32 : ST>;  // (the slots' sum stays fp32)
+  auto load_rows = [&](int r, auto& ru, auto& rv, auto& rd) {
+    r = min(r, r_end - 1);
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      const uint32_t col = 8 * min(lane + 64 * WPR * i, nv - 1);
+      ru[i].load(a.u, (int64_t)r * a.d, col);
+      if constexpr (!OUT) {
+        rv[i].load(a.v, (int64_t)r * a.ldv, col);
+        if (a.dres) rd[i].load(a.dres, (int64_t)r * a.d, col);
+      }
+    }
+    if constexpr (OUT) {
+      float t[VPL][8];
+      load_slots<HT, VPL, WPR, KB>(a.v, a.inv_pos, a.add, a.k, a.d, r, lane, t);
+#pragma unroll
+      for (int i = 0; i < VPL; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) rv[i].w[e] = __float_as_uint(t[i][e]);
     }
   };
   for (int r0 = r_begin; r0 < r_end;) {
@@ -352,17 +504,17 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 512) void norm_bwd_kernel(NormBw
     const int piece_end = min(end, r_end);
     const bool live = b >= 0 && b < a.s.B;
     if (!live) {  // padding rows: no gradient from the norm
-      for (int r = r0 + grp; r < piece_end; r += ngrp)
+      for (int r = r0 + grp; r < piece_end; r += G)
         for (int c = lane; c < nv; c += 64 * WPR) {
           float t[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) t[e] = 0.0f;
           if (a.dres) {
-            load8<ST>(a.dres, (int64_t)r * a.d + 8 * c, t);
+            load8<ST>(a.dres, (int64_t)r * a.d, 8 * c, t);
 #pragma unroll
             for (int e = 0; e < 8; ++e) t[e] *= a.dres_scale;
           }
-          store8<OUT ? HT : ST>(a.dv, (int64_t)r * a.d + 8 * c, t);
+          store8<DT>(a.dv, (int64_t)r * a.d, 8 * c, t);
         }
       r0 = piece_end;
       continue;
@@ -376,33 +528,28 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 512) void norm_bwd_kernel(NormBw
         aacc[i][e] = sacc[i][e] = 0.0f;
         wm[i][e] = 1.0f;
       }
-      if (c < nv) {
+      if (vec_in<VPL>(i, c, nv)) {
         float t[8];
-        if (a.p.weight) load8_rt(a.p.weight, a.p.weight_dt, 8 * c, wm[i]);
+        if (a.p.weight) load8_rt(a.p.weight, a.p.weight_dt, 0, 8 * c, wm[i]);
         if (a.p.scale) {
-          load8_rt(a.p.scale, a.p.scale_dt, (int64_t)b * a.d + 8 * c, t);
+          load8_rt(a.p.scale, a.p.scale_dt, (int64_t)b * a.d, 8 * c, t);
 #pragma unroll
           for (int e = 0; e < 8; ++e) wm[i][e] *= OUT ? t[e] : 1.0f + t[e];
         }
       }
     }
-    for (int rg = r0; rg < piece_end; rg += ngrp) {
+    for (int rg = r0; rg < piece_end; rg += G) {
       const int r = rg + grp;
-      const bool row = r < piece_end;
-      float u[VPL][8], v[VPL][8];
+      Raw8<UT> u[VPL];
+      VRaw v[VPL];
+      Raw8<ST> dr[OUT ? 1 : VPL];
+      load_rows(r, u, v, dr);
       float sq = 0.0f, dot = 0.0f;
 #pragma unroll
       for (int i = 0; i < VPL; ++i) {
-        const int c = lane + 64 * WPR * i;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) u[i][e] = v[i][e] = 0.0f;
-        if (row && c < nv) {
-          load8<UT>(a.u, (int64_t)r * a.d + 8 * c, u[i]);
-          if constexpr (OUT)
-            load_slots<HT>(a.v, a.inv_pos, a.add, a.k, a.d, r, c, v[i]);
-          else
-            load8<ST>(a.v, (int64_t)r * a.ldv + 8 * c, v[i]);
-        }
+        const bool in = vec_in<VPL>(i, lane + 64 * WPR * i, nv);
+        u[i].keep(in);
+        v[i].keep(in);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           sq += v[i][e] * v[i][e];
@@ -411,138 +558,152 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 512) void norm_bwd_kernel(NormBw
       }
       float rms = 1.0f, proj = 0.0f;  // proj = r^3 mean(g v): dv = r g - v proj
       if (a.norm) {
-        row_sum2<WPR>(sq, dot, red);
+        row_sum2<WPR>(sq, dot, red, half);
         rms = inv_rms(sq, a.d, a.eps);
         proj = rms * rms * rms * (dot / (float)a.d);
       }
-      if (!row) continue;
+      if (r >= piece_end) continue;
 #pragma unroll
       for (int i = 0; i < VPL; ++i) {
         const int c = lane + 64 * WPR * i;
-        if (c >= nv) continue;
-        float t[8], dr[8];
+        if (!vec_in<VPL>(i, c, nv)) continue;
+        float t[8];
+        u[i].hold();
+        v[i].hold();
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float n = v[i][e] * rms;
-          aacc[i][e] += u[i][e] * n;
-          sacc[i][e] += u[i][e];
-          t[e] = rms * (u[i][e] * wm[i][e]) - v[i][e] * proj;
+          const float ue = u[i][e], ve = v[i][e];
+          aacc[i][e] += ue * (ve * rms);
+          if constexpr (!OUT) sacc[i][e] += ue;
+          t[e] = rms * (ue * wm[i][e]) - ve * proj;
         }
-        if (a.dres) {
-          load8<ST>(a.dres, (int64_t)r * a.d + 8 * c, dr);
+        if constexpr (!OUT)
+          if (a.dres) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) t[e] += a.dres_scale * dr[e];
-        }
-        store8<OUT ? HT : ST>(a.dv, (int64_t)r * a.d + 8 * c, t);
+            for (int e = 0; e < 8; ++e) t[e] += a.dres_scale * dr[i][e];
+          }
+        store8<DT>(a.dv, (int64_t)r * a.d, 8 * c, t);
       }
     }
-    if (a.dweight) {  // the weight's sum: A_b (1 + scale_b), or A_b gate_b
+    // (whole: this block holds every row of the sample)
+    const int first = a.s.starts ? a.s.starts[b] : b * a.s.L;
+    const bool whole = first >= r_begin && end <= r_end;
+    float* slot = a.part + (int64_t)(blockIdx.x + b) * nsum * a.d;
+    if (a.dscale || a.dweight)
+      over_groups(aacc, [&](int i, int c, float (&t)[8]) {
+        float q[8];
+        if (a.dweight) {  // A_b (1 + scale_b), or A_b gate_b
 #pragma unroll
-      for (int i = 0; i < VPL; ++i) {
-        const int c = lane + 64 * WPR * i;
-        float t[8];
+          for (int e = 0; e < 8; ++e) q[e] = OUT ? 1.0f : 0.0f;
+          if (a.p.scale) load8_rt(a.p.scale, a.p.scale_dt, (int64_t)b * a.d, 8 * c, q);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) t[e] = OUT ? 1.0f : 0.0f;
-        if (a.p.scale && c < nv) load8_rt(a.p.scale, a.p.scale_dt, (int64_t)b * a.d + 8 * c, t);
+          for (int e = 0; e < 8; ++e) wacc[i][e] += (OUT ? q[e] : 1.0f + q[e]) * t[e];
+        }
+        if (!a.dscale) return;
+        if (!whole) {
+          store8<HMOE_DT_F32>(slot, 0, 8 * c, t);
+          return;
+        }
+        if (a.p.weight) {
+          load8_rt(a.p.weight, a.p.weight_dt, 0, 8 * c, q);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) wacc[i][e] += (OUT ? t[e] : 1.0f + t[e]) * aacc[i][e];
-      }
-    }
-    if (sums) {
-      // (whole: this block holds every row of the sample)
-      const int first = a.s.starts ? a.s.starts[b] : b * a.s.L;
-      const bool whole = first >= r_begin && end <= r_end;
-      float* slot = a.part + (int64_t)(blockIdx.x + b) * nsum * a.d;
-      if (a.dscale)
-        over_groups(aacc, [&](int c, float (&t)[8]) {
-          if (!whole) {
-            store8<HMOE_DT_F32>(slot, 8 * c, t);
-            return;
-          }
-          if (a.p.weight) {
-            float q[8];
-            load8_rt(a.p.weight, a.p.weight_dt, 8 * c, q);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) t[e] *= q[e];
-          }
-          store8_rt(a.dscale, a.p.scale_dt, (int64_t)b * a.d + 8 * c, t);
-        });
+          for (int e = 0; e < 8; ++e) t[e] *= q[e];
+        }
+        store8_rt(a.dscale, a.p.scale_dt, (int64_t)b * a.d, 8 * c, t);
+      });
+    if constexpr (!OUT) {
       if (a.dshift)
-        over_groups(sacc, [&](int c, float (&t)[8]) {
+        over_groups(sacc, [&](int, int c, float (&t)[8]) {
           if (whole)
-            store8_rt(a.dshift, a.p.shift_dt, (int64_t)b * a.d + 8 * c, t);
+            store8_rt(a.dshift, a.p.shift_dt, (int64_t)b * a.d, 8 * c, t);
           else
-            store8<HMOE_DT_F32>(slot, (int64_t)(nsum - 1) * a.d + 8 * c, t);
+            store8<HMOE_DT_F32>(slot, (int64_t)(nsum - 1) * a.d, 8 * c, t);
         });
     }
     r0 = piece_end;
   }
-  if (a.dweight)
-    over_groups(wacc, [&](int c, float (&t)[8]) {
-      store8<HMOE_DT_F32>(a.wpart, (int64_t)blockIdx.x * a.d + 8 * c, t);
-    });
-}
-
-// The column sums left in the workspace: block (item, 64-column slab), item < B: sample item's sums, unless one chunk
-// finished it (an empty sample gets zeros); item B: the weight's over all chunks.  16 waves take every 16th slot.
-__global__ __launch_bounds__(1024) void norm_sums_kernel(NormBwdArgs a, int nchunk) {
-  __shared__ float lds[2][16][64];
-  const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6, b = blockIdx.x;
-  const int col = blockIdx.y * 64 + tx;
-  const int nsum = (a.dscale != nullptr) + (a.dshift != nullptr);
-  const bool weight = b == a.s.B;
-  int c0 = 0, c1 = nchunk - 1;
-  if (!weight) {
-    int s = a.s.starts ? a.s.starts[b] : b * a.s.L, e = a.s.starts ? a.s.starts[b + 1] : (b + 1) * a.s.L;
-    s = max(0, min(s, a.s.T));
-    e = max(0, min(e, a.s.T));
-    c0 = s / a.R;
-    c1 = (e - 1) / a.R;
-    if (e <= s)
-      c1 = c0 - 1;  // empty: zeros
-    else if (c0 == c1)
-      return;
-  }
-  float t0 = 0.0f, t1 = 0.0f;
-  if (col < a.d) {
-    for (int c = c0 + ty; c <= c1; c += 16) {
-      if (weight) {
-        t0 += a.wpart[(int64_t)c * a.d + col];
-      } else {
-        const float* slot = a.part + (int64_t)(c + b) * nsum * a.d + col;
-        t0 += slot[0];
-        if (nsum == 2) t1 += slot[a.d];
-      }
+  if (a.dweight) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = threadIdx.x + kNormThreads<WPR> * i;
+      if (c < nv) store8<HMOE_DT_F32>(a.wpart, (int64_t)blockIdx.x * a.d, 8 * c, wacc[i]);
     }
   }
-  lds[0][ty][tx] = t0;
-  lds[1][ty][tx] = t1;
-  __syncthreads();
-  if (ty != 0 || col >= a.d) return;
-  for (int i = 1; i < 16; ++i) {
-    t0 += lds[0][i][tx];
-    t1 += lds[1][i][tx];
-  }
+}
+
+// The column sums left in the workspace.  Workgroups walk the items: item b < B is sample b's sums, unless one chunk
+// finished it (an empty sample gets zeros), item B the weight's over all chunks.  32 columns by SPLIT parts of the slots, each
+// part reading every SPLIT-th with eight loads on their way, added in part order.
+template <int SPLIT>
+__global__ __launch_bounds__(32 * SPLIT) void norm_sums_kernel(NormBwdArgs a, int nchunk, int items) {
+  __shared__ float lds[2][SPLIT][32];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, col = blockIdx.y * 32 + tx;
+  const int nsum = (a.dscale != nullptr) + (a.dshift != nullptr);
+  const bool in = col < a.d;
   auto put = [&](void* p, int dt, int64_t off, float v) {
     if (dt == HMOE_DT_F32)
       static_cast<float*>(p)[off] = v;
     else
       static_cast<uint16_t*>(p)[off] = (uint16_t)(dt == HMOE_DT_F16 ? cvt_h2(v, v) : cvt_bf2(v, v));
   };
-  if (weight) {
-    put(a.dweight, a.p.weight_dt, col, t0);
-    return;
+  for (int b = blockIdx.x; b < items; b += gridDim.x) {
+    const bool weight = b == a.s.B;
+    int c0 = 0, c1 = nchunk - 1;
+    if (!weight) {
+      int s = a.s.starts ? a.s.starts[b] : b * a.s.L, e = a.s.starts ? a.s.starts[b + 1] : (b + 1) * a.s.L;
+      s = max(0, min(s, a.s.T));
+      e = max(0, min(e, a.s.T));
+      c0 = s / a.R;
+      c1 = (e - 1) / a.R;
+      if (e <= s)
+        c1 = c0 - 1;  // empty: zeros
+      else if (c0 == c1)
+        continue;
+    }
+    const int64_t pitch = weight ? a.d : (int64_t)nsum * a.d;
+    const float* src = weight ? a.wpart + col : a.part + (int64_t)b * pitch + col;
+    const bool two = !weight && nsum == 2;
+    float t0 = 0.0f, t1 = 0.0f;
+    for (int c = c0 + ty; c <= c1; c += 8 * SPLIT) {
+      float v[8], w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int k = c + i * SPLIT;
+        const bool on = in && k <= c1;
+        v[i] = on ? src[k * pitch] : 0.0f;
+        w[i] = on && two ? src[k * pitch + a.d] : 0.0f;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        t0 += v[i];
+        t1 += w[i];
+      }
+    }
+    __syncthreads();
+    lds[0][ty][tx] = t0;
+    lds[1][ty][tx] = t1;
+    __syncthreads();
+    if (ty != 0 || !in) continue;
+#pragma unroll
+    for (int i = 1; i < SPLIT; ++i) {
+      t0 += lds[0][i][tx];
+      t1 += lds[1][i][tx];
+    }
+    if (weight) {
+      put(a.dweight, a.p.weight_dt, col, t0);
+      continue;
+    }
+    const int64_t off = (int64_t)b * a.d + col;
+    if (a.dscale) {
+      float w = 1.0f;
+      if (a.p.weight)
+        w = a.p.weight_dt == HMOE_DT_F32 ? static_cast<const float*>(a.p.weight)[col]
+            : a.p.weight_dt == HMOE_DT_F16 ? Elt<true>::one(static_cast<const uint16_t*>(a.p.weight)[col])
+                                           : Elt<false>::one(static_cast<const uint16_t*>(a.p.weight)[col]);
+      put(a.dscale, a.p.scale_dt, off, w * t0);
+    }
+    if (a.dshift) put(a.dshift, a.p.shift_dt, off, a.dscale ? t1 : t0);
   }
-  const int64_t off = (int64_t)b * a.d + col;
-  if (a.dscale) {
-    float w = 1.0f;
-    if (a.p.weight)
-      w = a.p.weight_dt == HMOE_DT_F32 ? static_cast<const float*>(a.p.weight)[col]
-          : a.p.weight_dt == HMOE_DT_F16 ? Elt<true>::one(static_cast<const uint16_t*>(a.p.weight)[col])
-                                         : Elt<false>::one(static_cast<const uint16_t*>(a.p.weight)[col]);
-    put(a.dscale, a.p.scale_dt, off, w * t0);
-  }
-  if (a.dshift) put(a.dshift, a.p.shift_dt, off, a.dscale ? t1 : t0);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -570,7 +731,7 @@ static int norm_params(const NormParams& p) {
   return al16(p.weight) && al16(p.scale) && al16(p.shift) ? HMOE_OK : HMOE_ERR_ARG;
 }
 
-// calls f(VPL, WPR) as integral constants for width d: one wave per row up to 2048 columns, four up to 8192, else 16
+// calls f(VPL, WPR) as integral constants for width d
 template <class F>
 static void by_width(int64_t d, F&& f) {
   const int64_t nv = d / 8;
@@ -578,12 +739,32 @@ static void by_width(int64_t d, F&& f) {
   if (nv <= 64) HMOE_W(1, 1);
   else if (nv <= 128) HMOE_W(2, 1);
   else if (nv <= 192) HMOE_W(3, 1);
-  else if (nv <= 256) HMOE_W(4, 1);
+  else if (nv <= 256) HMOE_W(2, 2);
+  else if (nv <= 384) HMOE_W(3, 2);
   else if (nv <= 512) HMOE_W(2, 4);
   else if (nv <= 768) HMOE_W(3, 4);
-  else if (nv <= 1024) HMOE_W(4, 4);
+  else if (nv <= 1024) HMOE_W(2, 8);
+  else if (nv <= 1536) HMOE_W(3, 8);
   else HMOE_W(2, 16);
 #undef HMOE_W
+}
+
+// row groups of a workgroup for width d
+static int norm_groups(int64_t d) {
+  int g = 0;
+  by_width(d, [&](auto, auto w) { g = kNormGroups<decltype(w)::value>; });
+  return g;
+}
+
+// calls f(KB) as an integral constant for k slots: how many are loaded at once, as far as the registers hold them
+template <int HT, int WPR, class F>
+static void by_slots_at_once(int k, F&& f) {
+  if constexpr (WPR < 16) {
+    if constexpr (HT != HMOE_DT_F32)
+      if (k >= 4) return f(std::integral_constant<int, 4>());
+    if (k >= 2) return f(std::integral_constant<int, 2>());
+  }
+  f(std::integral_constant<int, 1>());
 }
 
 // calls f(ST, HT) as integral constants
@@ -598,31 +779,39 @@ static void by_types(int sdt, int hdt, F&& f) {
 #undef HMOE_T
 }
 
-// blocks of a forward launch: a row per wave (or per WPR waves), at most eight blocks per CU of 256
-static unsigned norm_grid(int64_t T, int rows_per_block) {
-  const int64_t g = (T + rows_per_block - 1) / rows_per_block;
-  return (unsigned)(g < 2048 ? g : 2048);
+// Rows per workgroup of the forward: a row for each of its row groups, or several (up to eight) where 16 waves on each of
+// the 256 CUs have more than one.  16384 x 1536: 22 us (norm_in) and 41 us (norm_out, two slots) with workgroups of two
+// waves, against 24 and 47 with four, 23 and 42 with eight; four rows a wave (16 waves a CU) against two or eight: within 5%.
+static int fwd_rows(int64_t T, int64_t d) {
+  int g = 1, wpr = 1;
+  by_width(d, [&](auto, auto w) {
+    g = kFwdGroups<decltype(w)::value>;
+    wpr = decltype(w)::value;
+  });
+  const int64_t q = T * wpr / (256 * 16);
+  return g * (int)(q < 1 ? 1 : q > 8 ? 8 : q);
 }
 
-// rows per block of the backward: about 512 blocks
-static int bwd_rows(int64_t T, int groups) {
-  int64_t r = (T + 511) / 512;
+// Rows per workgroup of the backward: what gives about 256 workgroups (one per CU: the registers of a row's sums leave room for
+// eight waves), a multiple of the row groups.  16384 x 1536: 41 us against 47 with 512 workgroups and 60 with 1024, whose
+// column sums are also more to write and add.
+static int norm_rows(int64_t T, int groups) {
+  int64_t r = (T + 255) / 256;
   r = (r + groups - 1) / groups * groups;
   return (int)(r > 0 ? r : groups);
 }
-static int bwd_groups(int64_t d) { return d <= 2048 ? 8 : d <= 8192 ? 2 : 1; }
 
 static size_t norm_bwd_ws(int64_t T, int64_t d, int64_t B, int nsum, bool weight) {
   if (T < 0 || d <= 0 || B < 1) return 0;
-  const int64_t R = bwd_rows(T, bwd_groups(d)), nchunk = (T + R - 1) / R;
+  const int64_t R = norm_rows(T, norm_groups(d)), nchunk = (T + R - 1) / R;
   return (size_t)((nchunk + B) * nsum + (weight ? nchunk : 0)) * (size_t)d * 4 + 16;
 }
 
 template <bool OUT>
 static int norm_bwd_run(NormBwdArgs& a, int sdt, int hdt, void* workspace, size_t workspace_bytes, hipStream_t s) {
   const int nsum = (a.dscale != nullptr) + (a.dshift != nullptr);
-  const int groups = bwd_groups(a.d);
-  a.R = bwd_rows(a.s.T, groups);
+  const int groups = norm_groups(a.d);
+  a.R = norm_rows(a.s.T, groups);
   const int nchunk = (a.s.T + a.R - 1) / a.R;
   const bool final = nsum || a.dweight;
   if (final) {
@@ -636,9 +825,14 @@ static int norm_bwd_run(NormBwdArgs& a, int sdt, int hdt, void* workspace, size_
     const size_t lds = final ? (size_t)groups * a.d * 4 : 0;
     by_types(sdt, hdt, [&](auto st, auto ht) {
       by_width(a.d, [&](auto v, auto w) {
-        constexpr int W = decltype(w)::value;
-        hipLaunchKernelGGL((norm_bwd_kernel<OUT, decltype(st)::value, decltype(ht)::value, decltype(v)::value, W>),
-                           dim3(nchunk), dim3(W == 16 ? 1024 : 512), lds, s, a);
+        constexpr int S = decltype(st)::value, H = decltype(ht)::value, V = decltype(v)::value, W = decltype(w)::value;
+        if constexpr (OUT)
+          by_slots_at_once<H, W>(a.k, [&](auto kb) {
+            hipLaunchKernelGGL((norm_bwd_kernel<decltype(kb)::value, S, H, V, W>), dim3(nchunk), dim3(kNormThreads<W>), lds,
+                               s, a);
+          });
+        else
+          hipLaunchKernelGGL((norm_bwd_kernel<0, S, H, V, W>), dim3(nchunk), dim3(kNormThreads<W>), lds, s, a);
       });
     });
     HMOE_CHECK_LAUNCH();
@@ -648,7 +842,12 @@ static int norm_bwd_run(NormBwdArgs& a, int sdt, int hdt, void* workspace, size_
     // without sample sums the weight's item comes first
     NormBwdArgs f = a;
     if (!nsum) f.s.B = 0;
-    hipLaunchKernelGGL(norm_sums_kernel, dim3(items, (a.d + 63) / 64), dim3(1024), 0, s, f, nchunk);
+    const dim3 grid(items < 128 ? items : 128, (a.d + 31) / 32);
+    // many parts for long sums, few where the samples span a few chunks each
+    if (nchunk > 16 * a.s.B)
+      hipLaunchKernelGGL(norm_sums_kernel<32>, grid, dim3(32 * 32), 0, s, f, nchunk, items);
+    else
+      hipLaunchKernelGGL(norm_sums_kernel<8>, grid, dim3(32 * 8), 0, s, f, nchunk, items);
     HMOE_CHECK_LAUNCH();
   }
   return HMOE_OK;
@@ -669,12 +868,13 @@ int hmoe_norm_modulate(const void* x, int64_t ldx, int x_dtype, const void* weig
   if (rc == HMOE_OK) rc = norm_params(p);
   if (rc || T == 0) return rc;
   if (!x || !h || ldx < d || ldx % 8 || !al16(x) || !al16(h)) return HMOE_ERR_ARG;
-  const NormInArgs a = {x, ldx, h, p, {starts, (int)B, starts ? 0 : (int)(T / B), (int)T}, (int)d, eps};
+  const NormInArgs a = {x, ldx, h, p, {starts, (int)B, starts ? 0 : (int)(T / B), (int)T}, (int)d,
+                        fwd_rows(T, d), eps};
   by_types(x_dtype, h_dtype, [&](auto st, auto ht) {
     by_width(d, [&](auto v, auto w) {
       constexpr int W = decltype(w)::value;
       hipLaunchKernelGGL((norm_in_kernel<decltype(st)::value, decltype(ht)::value, decltype(v)::value, W>),
-                         dim3(norm_grid(T, W == 1 ? 4 : 1)), dim3(W == 16 ? 1024 : 256), 0,
+                         dim3((unsigned)((T + a.R - 1) / a.R)), dim3(kFwdThreads<W>), 0,
                          reinterpret_cast<hipStream_t>(stream), a);
     });
   });
@@ -694,13 +894,16 @@ int hmoe_norm_residual(const void* y, const int32_t* inv_pos, int k, const void*
   if (rc || T == 0) return rc;
   if (!y || !x || !out || ldx < d || ldx % 8 || !al16(y) || !al16(x) || !al16(out) || !al16(add)) return HMOE_ERR_ARG;
   const NormOutArgs a = {y, inv_pos, add, x, ldx, out, p, {starts, (int)B, starts ? 0 : (int)(T / B), (int)T}, (int)d,
-                         k, norm, eps, alpha};
+                         k, norm, fwd_rows(T, d), eps, alpha};
   by_types(x_dtype, y_dtype, [&](auto st, auto ht) {
     by_width(d, [&](auto v, auto w) {
       constexpr int W = decltype(w)::value;
-      hipLaunchKernelGGL((norm_out_kernel<decltype(st)::value, decltype(ht)::value, decltype(v)::value, W>),
-                         dim3(norm_grid(T, W == 1 ? 4 : 1)), dim3(W == 16 ? 1024 : 256), 0,
-                         reinterpret_cast<hipStream_t>(stream), a);
+      by_slots_at_once<decltype(ht)::value, W>(k, [&](auto kb) {
+        hipLaunchKernelGGL((norm_out_kernel<decltype(st)::value, decltype(ht)::value, decltype(v)::value, W,
+                                            decltype(kb)::value>),
+                           dim3((unsigned)((T + a.R - 1) / a.R)), dim3(kFwdThreads<W>), 0,
+                           reinterpret_cast<hipStream_t>(stream), a);
+      });
     });
   });
   HMOE_CHECK_LAUNCH();
