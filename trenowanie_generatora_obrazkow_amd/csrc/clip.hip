@@ -9,6 +9,7 @@ namespace hmoe {
 // The tensors of a launch travel in its arguments (no device table to copy, and a captured launch keeps its list).
 constexpr int kClipTensors = 128;   // per launch: 3.8 KB of the 4 KB of arguments
 constexpr int kClipChunk = 16384;   // elements a workgroup takes at a time
+constexpr int kClipAhead = 8;       // vectors of eight elements a thread of the scaling kernel has on their way
 constexpr int kClipBlocks = 2048;   // workgroups per launch: eight per CU
 
 struct ClipList {
@@ -101,7 +102,8 @@ __device__ __forceinline__ void clip_by_type(int dt, F&& f) {
 }
 
 // part[block] = the sum of the squares of the block's chunks, in fp64: fp32 squares would overflow from 1.8e19 on and
-// vanish below 2e-23, and the fp64 fma keeps up with the loads
+// vanish below 2e-23, and the fp64 fma keeps up with the loads: 302M bf16 elements in 118 us, 5.1 TB/s, the rate of a
+// large copy.
 __global__ __launch_bounds__(256) void clip_norm_kernel(ClipList l, double* part) {
   __shared__ double lds[4];
   double acc = 0.0;
@@ -142,12 +144,16 @@ __device__ __forceinline__ float clip_coef(double norm, float max_norm) {
   return c < 1.0 ? (float)c : norm == norm ? 1.0f : __builtin_nanf("");
 }
 
+// out = grad * factor, from the back of the list: what the norm read last may still lie in the 256 MB cache (98.6M fp32
+// elements 137.5 us against 142).  Eight vectors a thread on their way: 302M bf16 elements into fp32 338 us (5.3 TB/s) against
+// 361 with four and 369 with one.
 __global__ __launch_bounds__(256) void clip_scale_kernel(ClipList l, const double* sq, float max_norm, float* norm_out) {
   const double norm = sqrt(*sq);
   if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
   const float coef = clip_coef(norm, max_norm);
   const uint32_t chunks = l.first[l.count];
-  for (uint32_t c = blockIdx.x; c < chunks; c += gridDim.x) {
+  for (uint32_t cc = blockIdx.x; cc < chunks; cc += gridDim.x) {
+    const uint32_t c = chunks - 1 - cc;
     const int ti = clip_tensor(l, c);
     const void* p = l.p[ti];
     void* o = l.o[ti];
@@ -158,6 +164,17 @@ __global__ __launch_bounds__(256) void clip_scale_kernel(ClipList l, const doubl
       auto walk = [&](auto odt) {
         constexpr int OT = decltype(odt)::value;
         int64_t i = i0 + threadIdx.x * 8;
+        for (; i + (kClipAhead - 1) * 256 * 8 + 8 <= i1; i += kClipAhead * 256 * 8) {
+          float v[kClipAhead][8];
+#pragma unroll
+          for (int k = 0; k < kClipAhead; ++k) clip_load8<DT>(p, i + k * 256 * 8, v[k]);
+#pragma unroll
+          for (int k = 0; k < kClipAhead; ++k) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[k][e] *= coef;
+            clip_store8<OT>(o, i + k * 256 * 8, v[k]);
+          }
+        }
         for (; i + 8 <= i1; i += 256 * 8) {
           float v[8];
           clip_load8<DT>(p, i, v);
@@ -175,12 +192,13 @@ __global__ __launch_bounds__(256) void clip_scale_kernel(ClipList l, const doubl
   }
 }
 
-// Fills a list from the tensors at i on (empty ones are left out) and moves i behind them.
+// Fills a list from the tensors at i on (empty ones are left out) and moves i behind them.  Tensors that follow each other in
+// memory, as the views of a gradient bucket do, and whose outputs do so too are walked as one: fewer entries and launches.
 static int clip_list(const void* const* grads, void* const* out, const int64_t* numel, const int* dtypes,
                      const int* out_dtypes, int n, int& i, ClipList& l) {
   l.count = 0;
   uint64_t chunks = 0;
-  for (; i < n && l.count < kClipTensors; ++i) {
+  for (; i < n; ++i) {
     const int64_t m = numel[i];
     const int dt = dtypes[i];
     if (m < 0) return HMOE_ERR_ARG;
@@ -192,14 +210,27 @@ static int clip_list(const void* const* grads, void* const* out, const int64_t* 
     void* o = out ? out[i] : nullptr;
     if (!grads[i] || (reinterpret_cast<uintptr_t>(grads[i]) & al) || (out && !o) || (reinterpret_cast<uintptr_t>(o) & ao))
       return HMOE_ERR_ARG;
-    const uint64_t mine = ((uint64_t)m + kClipChunk - 1) / kClipChunk;
-    if (chunks + mine > 0x7fffffffu) return HMOE_ERR_SHAPE;
+    const int64_t sz = dt == HMOE_DT_F32 ? 4 : 2, so = ot == HMOE_DT_F32 ? 4 : 2;
+    const uint8_t kind = (uint8_t)(dt | ot << 4);
+    if (m > INT64_MAX / 8) return HMOE_ERR_SHAPE;
+    if (l.count) {
+      const int b = l.count - 1;
+      if (kind == l.dt[b] && static_cast<const char*>(l.p[b]) + l.n[b] * sz == grads[i] &&
+          (!out || static_cast<char*>(l.o[b]) + l.n[b] * so == o)) {
+        l.n[b] += m;
+        continue;
+      }
+      if (l.count == kClipTensors) break;
+    }
     l.p[l.count] = grads[i];
     l.o[l.count] = o;
     l.n[l.count] = m;
-    l.dt[l.count] = (uint8_t)(dt | ot << 4);
-    l.first[l.count++] = (uint32_t)chunks;
-    chunks += mine;
+    l.dt[l.count++] = kind;
+  }
+  for (int b = 0; b < l.count; ++b) {
+    l.first[b] = (uint32_t)chunks;
+    chunks += ((uint64_t)l.n[b] + kClipChunk - 1) / kClipChunk;
+    if (chunks > 0x7fffffffu) return HMOE_ERR_SHAPE;
   }
   l.first[l.count] = (uint32_t)chunks;
   return HMOE_OK;

@@ -248,12 +248,13 @@ def clip_grad_norm(grads, max_norm, out=None):
     None entries are skipped.  Returns the norm before clipping, a () fp32 tensor on the device; nothing waits for the GPU.
     A gradient spread over several processes: all-reduce ops.grad_sq_norm's sum before ops.grad_clip."""
     grads = list(grads)
-    outs = None if out is None else list(out)
-    if outs is not None and len(outs) != len(grads):
-        raise ValueError(f"{len(outs)} outputs for {len(grads)} gradients")
-    if any(g is None for g in grads):
-        if outs is not None:
-            outs = [o for g, o in zip(grads, outs) if g is not None]
+    if out is not None:
+        out = list(out)
+        if len(out) != len(grads):
+            raise ValueError(f"{len(out)} outputs for {len(grads)} gradients")
+    if not all([g is not None for g in grads]):
+        if out is not None:
+            out = [o for g, o in zip(grads, out) if g is not None]
         grads = [g for g in grads if g is not None]
-    gl = ops.GradList(grads, outs)
+    gl = ops.GradList(grads, out)
     return ops.grad_clip(gl, ops.grad_sq_norm(gl), max_norm)

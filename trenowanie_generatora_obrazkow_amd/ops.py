@@ -713,9 +713,12 @@ _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 _SCORES = {"softmax": 0, "sigmoid": 1}
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def _call_on(dev, name, *args):
     """A C call with its stream, launched on `dev` also where another device is the current one."""
-    if dev.index == torch.cuda.current_device():
+    if dev.index == _current_device():
         L.call(name, *args, L.stream(dev))
     else:
         with torch.cuda.device(dev):
@@ -959,39 +962,60 @@ def _dense(t):
 
 
 class GradList:
-    """The tensors of a clipping call as the C entry points take them: addresses, element counts and types."""
+    """The tensors of a clipping call as the C entry points take them: addresses, element counts and types.  A program whose
+    gradients stay in place (flat buckets, zero_grad(set_to_none=False)) may keep one from step to step."""
 
     def __init__(self, grads, out=None):
         grads = list(grads)
-        out = grads if out is None else list(out)
-        if len(out) != len(grads):
-            raise ValueError(f"{len(out)} outputs for {len(grads)} gradients")
-        dev = None
-        for g, o in zip(grads, out):
-            if not g.is_cuda or g.layout is not torch.strided:
-                raise RuntimeError("gradients must be dense ROCm GPU tensors: the hmoe kernels have no CPU path")
-            if g.dtype not in _FLOATS:
-                raise TypeError(f"gradient: dtype {g.dtype} not in {_FLOATS}")
-            if dev is None:
-                dev = g.device
-            if g.device != dev or o.device != dev:
-                raise ValueError("the gradients of a call live on one device")
-            if not _dense(g):
-                raise ValueError(f"a gradient's elements must be contiguous (strides {g.stride()})")
-            if o is not g and (o.shape != g.shape or (o.stride() != g.stride() and g.numel() > 1)
-                               or o.dtype not in (g.dtype, torch.float32)):
-                raise ValueError("an output has its gradient's shape and strides, and its type or fp32")
         self.n = len(grads)
-        self.device = dev
-        self.keep = (grads, out)
-        self.ptr = array("Q", [g.data_ptr() for g in grads])
-        self.out = array("Q", [o.data_ptr() for o in out])
+        self.device = self._check(grads, "gradient")
+        self.ptr = self._ptrs(grads)
         self.numel = array("q", [g.numel() for g in grads])
-        self.dt = array("i", [L._DT[g.dtype] for g in grads])
-        self.odt = array("i", [L._DT[o.dtype] for o in out])
-        used = [p for p, n in zip(self.out, self.numel) if n]
-        if len(set(used)) != len(used):
-            raise ValueError("a tensor is listed twice")
+        self.dt = self._types(grads)
+        if out is None:
+            out = grads
+            self.out, self.odt = self.ptr, self.dt
+        else:
+            out = list(out)
+            if len(out) != self.n:
+                raise ValueError(f"{len(out)} outputs for {self.n} gradients")
+            if self._check(out, "output") != self.device:
+                raise ValueError("the gradients and outputs of a call live on one device")
+            for g, o in zip(grads, out):
+                if o is not g and (o.shape != g.shape or (o.stride() != g.stride() and g.numel() > 1)
+                                   or o.dtype not in (g.dtype, torch.float32)):
+                    raise ValueError("an output has its gradient's shape and strides, and its type or fp32")
+            self.out, self.odt = self._ptrs(out), self._types(out)
+        self.keep = (grads, out)
+        if len(set(self.out)) != self.n:  # (tensors without elements may share the address 0)
+            used = [p for p, n in zip(self.out, self.numel) if n]
+            if len(set(used)) != len(used):
+                raise ValueError("a tensor is listed twice")
+
+    # one pass per property: a program clips hundreds of tensors, and the time of this is the host's
+    @staticmethod
+    def _check(ts, name):
+        devs = {t.device for t in ts}
+        if len(devs) > 1:
+            raise ValueError(f"the {name}s of a call live on one device (got {sorted(map(str, devs))})")
+        dev = devs.pop() if devs else None
+        if dev is not None and dev.type != "cuda":
+            raise RuntimeError(f"a {name} must be a ROCm GPU tensor: the hmoe kernels have no CPU path")
+        if not all([t.is_contiguous() for t in ts]) and not all(_dense(t) for t in ts):
+            raise ValueError(f"a {name}'s elements must be contiguous")
+        return dev
+
+    @staticmethod
+    def _ptrs(ts):
+        return array("Q", [t.data_ptr() for t in ts])
+
+    @staticmethod
+    def _types(ts):
+        kinds = [t.dtype for t in ts]
+        bad = set(kinds) - set(_FLOATS)
+        if bad:
+            raise TypeError(f"gradients and outputs are bf16, fp16 or fp32 (got {bad})")
+        return array("i", [L._DT[k] for k in kinds])
 
 
 def _addr(a):
