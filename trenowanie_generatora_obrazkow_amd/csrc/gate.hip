@@ -5,6 +5,12 @@
 namespace hmoe {
 
 // Four tokens per wave: the 16 lanes of segment q take one token, lane j of it experts 16 i + j (i < EPL).
+// What bounds it: the selection's instructions (an fp64 score per expert, the sorting network) and their latency; the logits
+// are read once, 8 MB at 8192 x 256, 2 us at the rate of a large copy.  Sixteen lanes a token: a wave's exchanges stay inside
+// rows of 16 lanes (DPP), and four tokens share every instruction.  8192 tokens, 256 experts in 8 groups, top-8, sigmoid with
+// bias: 10.9 us; with the library's exp and division and the options branched on per element 15.1.  The best k of E by a
+// sorting network and four merges of lists across the lanes, not by k rounds of arg-max: those cost about 110 instructions
+// each, the network 38 and a merge 55 for lists of eight.
 constexpr int kGateMaxE = 512, kGateMaxK = 16, kGateMaxGroups = 64;
 constexpr double kGateDead = -1e300;    // an expert that cannot be chosen while another is left
 constexpr double kGateNone = -1.5e308;  // no expert
@@ -27,6 +33,24 @@ __device__ __forceinline__ float gate_logit(const GateArgs& a, int64_t t, int e)
   if (a.dt == HMOE_DT_F32) return static_cast<const float*>(a.logits)[i];
   const uint16_t b = static_cast<const uint16_t*>(a.logits)[i];
   return a.dt == HMOE_DT_F16 ? Elt<true>::one(b) : bf2f(b);
+}
+// a lane's logits: experts 16 i + j, -inf past E.  All loads first (the index is held inside the row), the type once.
+template <int EPL>
+__device__ __forceinline__ void gate_logits(const GateArgs& a, int64_t t, int j, float (&lg)[EPL]) {
+  if (a.dt == HMOE_DT_F32) {
+    const float* p = static_cast<const float*>(a.logits) + t * a.ld;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) lg[i] = p[min(16 * i + j, a.E - 1)];
+  } else {
+    const uint16_t* p = static_cast<const uint16_t*>(a.logits) + t * a.ld;
+    uint16_t w[EPL];
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) w[i] = p[min(16 * i + j, a.E - 1)];
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) lg[i] = a.dt == HMOE_DT_F16 ? Elt<true>::one(w[i]) : bf2f(w[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) lg[i] = 16 * i + j < a.E ? lg[i] : -__builtin_inff();
 }
 
 // max / min without the quieting of NaN that fmax does (no operand is a NaN)
@@ -66,6 +90,42 @@ __device__ __forceinline__ double seg_sum_d(double v) {
   v += lane_xor_d<4>(v);
   v += lane_xor_d<2>(v);
   return v + lane_xor_d<1>(v);
+}
+
+// a b + c with c in scalar registers (the compiler would copy such a constant into vector registers for every element)
+__device__ __forceinline__ double fma_sc(double a, double b, double c) {
+  double r;
+  asm("v_fma_f64 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "s"(c));
+  return r;
+}
+
+// exp in fp64 to about 1e-14: x = n ln 2 + r (one fma: the product is exact, and ln 2 itself is off by 2e-17 n), then the
+// Taylor polynomial of degree 11 on |r| <= ln 2 / 2, whose first dropped term is below 7e-15, and the scaling by 2^n.  Finer than the 43 bits a sort key keeps, and a third of the library function's
+// instructions.  Inputs up to 1e4 in absolute value (fp32 logits beyond are clamped there: the results are 0 or inf either way).
+__device__ __forceinline__ double gate_exp(double x) {
+  x = dmin(dmax(x, -1e4), 1e4);
+  const double n = __builtin_rint(x * 1.4426950408889634074);
+  const double r = __builtin_fma(n, -0.69314718055994530942, x);
+  double p = 1.0 / 39916800.0;
+  p = fma_sc(p, r, 1.0 / 3628800.0);
+  p = fma_sc(p, r, 1.0 / 362880.0);
+  p = fma_sc(p, r, 1.0 / 40320.0);
+  p = fma_sc(p, r, 1.0 / 5040.0);
+  p = fma_sc(p, r, 1.0 / 720.0);
+  p = fma_sc(p, r, 1.0 / 120.0);
+  p = fma_sc(p, r, 1.0 / 24.0);
+  p = fma_sc(p, r, 1.0 / 6.0);
+  p = __builtin_fma(p, r, 0.5);
+  p = __builtin_fma(p, r, 1.0);
+  p = __builtin_fma(p, r, 1.0);
+  return __builtin_ldexp(p, (int)n);
+}
+// 1 / x for 1 <= x: the hardware's estimate and two Newton steps (x = inf: 0)
+__device__ __forceinline__ double gate_rcp(double x) {
+  double r = __builtin_amdgcn_rcp(x);
+  r = __builtin_fma(__builtin_fma(-x, r, 1.0), r, r);
+  r = __builtin_fma(__builtin_fma(-x, r, 1.0), r, r);
+  return x < 1e300 ? r : 0.0;
 }
 
 // Sort keys.  The selection value in fp64, its lowest nine mantissa bits replaced by the expert's index so that equal
@@ -125,7 +185,7 @@ __device__ __forceinline__ void wave_lds_sync() {
 }
 
 // L: list length, the power of two at or above k.
-template <int EPL, int L, bool GROUPS>
+template <int EPL, int L, bool GROUPS, bool SIG>
 __global__ __launch_bounds__(256) void route_scores_kernel(GateArgs a) {
   constexpr int W = 4;
   __shared__ double s_key[GROUPS ? W * 4 : 1][GROUPS ? EPL * 16 : 1];
@@ -134,41 +194,49 @@ __global__ __launch_bounds__(256) void route_scores_kernel(GateArgs a) {
   const int64_t tw = ((int64_t)blockIdx.x * W + wave) * 4;
   if (tw >= a.T) return;
   const int64_t t = tw + seg < a.T ? tw + seg : a.T - 1;  // (the lanes past T redo the last token and store nothing)
-  float lg[EPL];
-  float m = -__builtin_inff();
+  float lg[EPL], bias[EPL];
+  gate_logits(a, t, j, lg);
+  if (a.bias) {
 #pragma unroll
-  for (int i = 0; i < EPL; ++i) {
-    const int e = 16 * i + j;
-    lg[i] = e < a.E ? gate_logit(a, t, e) : -__builtin_inff();
-    m = fmaxf(m, lg[i]);
+    for (int i = 0; i < EPL; ++i) bias[i] = a.bias[min(16 * i + j, a.E - 1)];
+  } else {
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) bias[i] = 0.0f;
   }
-  m = seg_max(m);
-  // softmax: the sum of exp(l - m); a row without a finite logit has the sum 0 and scores 0
-  float S = 1.0f;
-  if (!a.sigmoid) {
-    float p = 0.0f;
+  // softmax: the row's largest logit and the sum of exp(l - m); a row without a logit above -inf has the sum 0 and scores 0
+  float m = -__builtin_inff(), S = 1.0f;
+  if constexpr (!SIG) {
 #pragma unroll
-    for (int i = 0; i < EPL; ++i)
-      if (16 * i + j < a.E && lg[i] != -__builtin_inff()) p += hexp(lg[i] - m);
-    S = seg_sum(p);
+    for (int i = 0; i < EPL; ++i) m = fmaxf(m, lg[i]);
+    m = seg_max(m);
+    S = 0.0f;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) {
+      const float x = hexp(lg[i] - m);
+      S += lg[i] != -__builtin_inff() ? x : 0.0f;
+    }
+    S = seg_sum(S);
   }
   // selection values
   double v[EPL];
   if (GROUPS || a.bias) {
-    double ex[EPL], sum = 0.0;
+    double sum = 0.0;
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
-      const bool on = lg[i] > -__builtin_inff();
-      ex[i] = a.sigmoid ? 1.0 / (1.0 + exp(-(double)lg[i])) : on ? exp((double)lg[i] - (double)m) : 0.0;
-      sum += ex[i];
+      if constexpr (SIG) {
+        v[i] = gate_rcp(1.0 + gate_exp(-(double)lg[i]));
+      } else {
+        const double x = gate_exp((double)lg[i] - (double)m);
+        v[i] = lg[i] > -__builtin_inff() ? x : 0.0;
+        sum += v[i];
+      }
     }
-    const double inv = a.sigmoid ? 1.0 : 1.0 / seg_sum_d(sum);
+    const double inv = SIG ? 1.0 : 1.0 / seg_sum_d(sum);
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
-      const int e = 16 * i + j;
-      const float b = a.bias && e < a.E ? a.bias[e] : 0.0f;
-      const bool on = lg[i] > -__builtin_inff() && b > -__builtin_inff();
-      v[i] = on ? ex[i] * inv + (double)b : -__builtin_inf();
+      const bool on = lg[i] > -__builtin_inff() && bias[i] > -__builtin_inff();
+      const double x = v[i] * inv + (double)bias[i];
+      v[i] = on ? x : -__builtin_inf();
     }
   } else {
 #pragma unroll
@@ -181,29 +249,43 @@ __global__ __launch_bounds__(256) void route_scores_kernel(GateArgs a) {
 #pragma unroll
     for (int i = 0; i < EPL; ++i) key[16 * i + j] = v[i] == v[i] ? v[i] : -__builtin_inf();
     wave_lds_sync();
+    // groups 16 q + j, or with at most eight of them lanes j and j + 8 half of group j each
+    const int parts = a.n_group <= 8 ? 2 : 1, part = parts == 2 ? j >> 3 : 0;
     double mine[kGateMaxGroups / 16];
 #pragma unroll
     for (int q = 0; q < kGateMaxGroups / 16; ++q) {
-      const int g = 16 * q + j;
       mine[q] = -__builtin_inf();
-      if (g < a.n_group) {
-        double m1 = -__builtin_inf(), m2 = -__builtin_inf();
-        for (int i = 0; i < eg; ++i) {
-          const double x = key[g * eg + i];
-          m2 = dmax(m2, dmin(m1, x));
-          m1 = dmax(m1, x);
+      if (16 * q >= a.n_group) break;
+      const int g = parts == 2 ? j & 7 : 16 * q + j;
+      const bool have = g < a.n_group;
+      double m1 = -__builtin_inf(), m2 = -__builtin_inf();
+      const double* gk = key + (have ? g * eg : 0);
+      for (int i0 = part; i0 < eg; i0 += 4 * parts) {
+        double x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = gk[min(i0 + i * parts, eg - 1)];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const double y = i0 + i * parts < eg ? x[i] : -__builtin_inf();
+          m2 = dmax(m2, dmin(m1, y));
+          m1 = dmax(m1, y);
         }
-        const double val = a.group_top == 2 ? m1 + m2 : m1;
-        mine[q] = val == val ? val : -__builtin_inf();
-        grp[g] = mine[q];
       }
+      if (parts == 2) {
+        const double o1 = lane_xor_d<8>(m1), o2 = lane_xor_d<8>(m2);
+        m2 = dmax(dmin(m1, o1), dmax(m2, o2));
+        m1 = dmax(m1, o1);
+      }
+      const double val = a.group_top == 2 ? m1 + m2 : m1;
+      mine[q] = have && val == val ? val : -__builtin_inf();
+      if (have) grp[g] = mine[q];
     }
     wave_lds_sync();
     uint64_t kept = 0;
 #pragma unroll
     for (int q = 0; q < kGateMaxGroups / 16; ++q) {
       if (16 * q >= a.n_group) break;
-      const int g = 16 * q + j;
+      const int g = parts == 2 ? j & 7 : 16 * q + j;
       int before = 0;  // groups ahead of mine
       for (int o = 0; o < a.n_group; ++o) {
         const double x = grp[o];
@@ -215,7 +297,7 @@ __global__ __launch_bounds__(256) void route_scores_kernel(GateArgs a) {
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
       const uint32_t g = ((uint32_t)(16 * i + j) * a.inv_eg) >> 20;
-      if (!(kept >> (g & 63) & 1)) v[i] = -__builtin_inf();
+      v[i] = kept >> (g & 63) & 1 ? v[i] : -__builtin_inf();
     }
   }
   // top L of the lane's own, then of pairs of lanes
@@ -227,7 +309,12 @@ __global__ __launch_bounds__(256) void route_scores_kernel(GateArgs a) {
 #pragma unroll
     for (int i = 0; i < L; ++i) {
       const int ii = c * L + i, e = 16 * ii + j;
-      x[i] = ii < EPL && e < a.E ? gate_key(v[ii < EPL ? ii : 0], e) : kGateNone;
+      if (ii < EPL) {
+        const double key = gate_key(v[ii < EPL ? ii : 0], e);
+        x[i] = e < a.E ? key : kGateNone;
+      } else {
+        x[i] = kGateNone;
+      }
     }
     bitonic_sort(x);
     if (c == 0) {
@@ -251,7 +338,7 @@ __global__ __launch_bounds__(256) void route_scores_kernel(GateArgs a) {
   float s = 0.0f;
   if (slot) {
     const float l = gate_logit(a, t, e);
-    if (a.sigmoid)
+    if constexpr (SIG)
       s = dead ? 0.0f : 1.0f / (1.0f + hexp(-l));
     else
       s = dead || S == 0.0f ? (S == S ? 0.0f : S) : hexp(l - m) / S;
@@ -275,7 +362,7 @@ struct GateBwdArgs {
 // ds_j = (u_j - (sum u s) / den) / den or u_j; sigmoid dl_e = ds s (1 - s) at the chosen experts, softmax
 // dl_e = p_e (ds_e - sum_j p_j ds_j) at every expert.  A slot with an id outside [0, E) or the weight 0 (no expert was
 // left for it) has no gradient; an expert named by several slots gets their sum.
-template <int EPL>
+template <int EPL, bool SIG>
 __global__ __launch_bounds__(256) void route_scores_bwd_kernel(GateBwdArgs b) {
   constexpr int W = 4;
   __shared__ float s_dp[W * 4][EPL * 16];
@@ -288,34 +375,34 @@ __global__ __launch_bounds__(256) void route_scores_bwd_kernel(GateBwdArgs b) {
   float* dp = s_dp[wave * 4 + seg];
   float lg[EPL];
   float m = -__builtin_inff(), S = 0.0f;
-  if (!a.sigmoid) {
+  if constexpr (!SIG) gate_logits(a, t, j, lg);
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) {
-      const int e = 16 * i + j;
-      lg[i] = e < a.E ? gate_logit(a, t, e) : -__builtin_inff();
-      m = fmaxf(m, lg[i]);
-    }
+  for (int i = 0; i < EPL; ++i) dp[16 * i + j] = 0.0f;
+  // lane j takes slot j
+  int e = -1;
+  float l = 0.0f, u = 0.0f;
+  if (j < a.k) {
+    e = a.ids[t * a.k + j];
+    const float w = a.w[t * a.k + j];
+    u = b.dw[t * a.k + j] * a.scaling;
+    l = gate_logit(a, t, min(max(e, 0), a.E - 1));
+    if (e < 0 || e >= a.E || w == 0.0f) e = -1;
+  }
+  if constexpr (!SIG) {
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) m = fmaxf(m, lg[i]);
     m = seg_max(m);
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
-      lg[i] = lg[i] != -__builtin_inff() ? hexp(lg[i] - m) : 0.0f;
+      const float x = hexp(lg[i] - m);
+      lg[i] = lg[i] != -__builtin_inff() ? x : 0.0f;
       S += lg[i];
     }
     S = seg_sum(S);
   }
-#pragma unroll
-  for (int i = 0; i < EPL; ++i) dp[16 * i + j] = 0.0f;
-  int e = -1;
-  float s = 0.0f, u = 0.0f;
-  if (j < a.k) {
-    e = a.ids[t * a.k + j];
-    if (e < 0 || e >= a.E || a.w[t * a.k + j] == 0.0f) e = -1;
-    if (e >= 0) {
-      const float l = gate_logit(a, t, e);
-      s = a.sigmoid ? 1.0f / (1.0f + hexp(-l)) : S == 0.0f ? 0.0f : hexp(l - m) / S;
-      u = b.dw[t * a.k + j] * a.scaling;
-    }
-  }
+  float s = 0.0f;
+  if (e >= 0) s = SIG ? 1.0f / (1.0f + hexp(-l)) : S == 0.0f ? 0.0f : hexp(l - m) / S;
+  if (e < 0) u = 0.0f;
   float ds = u;
   if (a.renorm) {
     const float den = seg_sum(s) + 1e-20f;
@@ -324,19 +411,26 @@ __global__ __launch_bounds__(256) void route_scores_bwd_kernel(GateBwdArgs b) {
   if (e < 0) ds = 0.0f;
   const float pdp = seg_sum(s * ds);
   wave_lds_sync();
-  if (e >= 0) atomicAdd(&dp[e], a.sigmoid ? ds * s * (1.0f - s) : ds);
+  if (e >= 0) atomicAdd(&dp[e], SIG ? ds * s * (1.0f - s) : ds);
   wave_lds_sync();
   const float inv = S == 0.0f ? 0.0f : 1.0f / S;
+  float d[EPL];
 #pragma unroll
   for (int i = 0; i < EPL; ++i) {
-    const int o = 16 * i + j;
-    if (o >= a.E || !real) continue;
-    const float d = a.sigmoid ? dp[o] : lg[i] * inv * (dp[o] - pdp);
-    const int64_t at = t * a.E + o;
-    if (a.dt == HMOE_DT_F32)
-      static_cast<float*>(b.dlogits)[at] = d;
-    else
-      static_cast<uint16_t*>(b.dlogits)[at] = (uint16_t)(a.dt == HMOE_DT_F16 ? cvt_h2(d, d) : cvt_bf2(d, d));
+    d[i] = dp[16 * i + j];
+    if constexpr (!SIG) d[i] = lg[i] * inv * (d[i] - pdp);
+  }
+  if (!real) return;
+  if (a.dt == HMOE_DT_F32) {
+    float* p = static_cast<float*>(b.dlogits) + t * a.E;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i)
+      if (16 * i + j < a.E) p[16 * i + j] = d[i];
+  } else {
+    uint16_t* p = static_cast<uint16_t*>(b.dlogits) + t * a.E;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i)
+      if (16 * i + j < a.E) p[16 * i + j] = (uint16_t)(a.dt == HMOE_DT_F16 ? cvt_h2(d[i], d[i]) : cvt_bf2(d[i], d[i]));
   }
 }
 
@@ -348,15 +442,12 @@ static void by_experts(int E, F&& f) {
   else if (n <= 2) f(std::integral_constant<int, 2>());
   else if (n <= 4) f(std::integral_constant<int, 4>());
   else if (n <= 8) f(std::integral_constant<int, 8>());
-  else if (n <= 12) f(std::integral_constant<int, 12>());
   else if (n <= 16) f(std::integral_constant<int, 16>());
-  else if (n <= 24) f(std::integral_constant<int, 24>());
   else f(std::integral_constant<int, 32>());
 }
 template <class F>
 static void by_slots(int k, F&& f) {
-  if (k <= 1) f(std::integral_constant<int, 1>());
-  else if (k <= 2) f(std::integral_constant<int, 2>());
+  if (k <= 2) f(std::integral_constant<int, 2>());
   else if (k <= 4) f(std::integral_constant<int, 4>());
   else if (k <= 8) f(std::integral_constant<int, 8>());
   else f(std::integral_constant<int, 16>());
@@ -395,10 +486,15 @@ int hmoe_route_scores(const void* logits, int64_t ld, int dtype, const float* bi
   by_experts(E, [&](auto epl) {
     by_slots(k, [&](auto l) {
       constexpr int EPL = decltype(epl)::value, L = decltype(l)::value;
-      if (groups)
-        hipLaunchKernelGGL((route_scores_kernel<EPL, L, true>), grid, dim3(256), 0, s, a);
-      else
-        hipLaunchKernelGGL((route_scores_kernel<EPL, L, false>), grid, dim3(256), 0, s, a);
+#define HMOE_GATE(G, S) hipLaunchKernelGGL((route_scores_kernel<EPL, L, G, S>), grid, dim3(256), 0, s, a)
+      if (groups) {
+        if (a.sigmoid) HMOE_GATE(true, true);
+        else HMOE_GATE(true, false);
+      } else {
+        if (a.sigmoid) HMOE_GATE(false, true);
+        else HMOE_GATE(false, false);
+      }
+#undef HMOE_GATE
     });
   });
   HMOE_CHECK_LAUNCH();
@@ -426,8 +522,12 @@ int hmoe_route_scores_bwd(const float* dtopk_w, const float* topk_w, const void*
   b.dw = dtopk_w;
   b.dlogits = dlogits;
   by_experts(E, [&](auto epl) {
-    hipLaunchKernelGGL((route_scores_bwd_kernel<decltype(epl)::value>), dim3((unsigned)((T + 15) / 16)), dim3(256), 0,
-                       reinterpret_cast<hipStream_t>(stream), b);
+    constexpr int EPL = decltype(epl)::value;
+    const dim3 grid((unsigned)((T + 15) / 16));
+    if (b.f.sigmoid)
+      hipLaunchKernelGGL((route_scores_bwd_kernel<EPL, true>), grid, dim3(256), 0, reinterpret_cast<hipStream_t>(stream), b);
+    else
+      hipLaunchKernelGGL((route_scores_bwd_kernel<EPL, false>), grid, dim3(256), 0, reinterpret_cast<hipStream_t>(stream), b);
   });
   HMOE_CHECK_LAUNCH();
   return HMOE_OK;
