@@ -17,6 +17,10 @@ Usage (the tensors the step reads must stay the same objects; their contents may
     g = StepGraph(step)
     grads = [p.grad for p in params]       # the captured backward's gradient tensors
     out = g.replay()                       # same tensors every replay, now holding this replay's values
+
+No autograd graph of the same parameters may outlive an eager step into the capture: return detached tensors, and where a
+step runs a module that keeps its routing weights (MoESwiGLU.last_topk_weight carries a gradient), set that to None at the
+step's end.
 """
 from __future__ import annotations
 

@@ -18,6 +18,8 @@ are rounded to bf16 the same way and receive their fp32 gradients rounded once t
 """
 from __future__ import annotations
 
+from dataclasses import dataclass, replace
+
 import torch
 import torch.nn as nn
 
@@ -61,81 +63,155 @@ def _bf16(t):
     return t if t.dtype == torch.bfloat16 else t.to(torch.bfloat16)
 
 
+@dataclass(frozen=True)
+class Gate:
+    """How a layer's gate scores and selects experts (ops.route_scores): softmax over all experts or a sigmoid each, the
+    experts in n_group groups of which the topk_group with the largest sums of their group_top best values are kept, and the
+    factor on the weights.  The default is the plain softmax top-k, which the layer's own router serves in one kernel."""
+
+    score: str = "softmax"
+    n_group: int = 1
+    topk_group: int = 1
+    group_top: int = 2
+    scaling: float = 1.0
+
+
+def _route(x, wr, bias, k, renorm, gate, select_bias):
+    """(logits, topk_ids, topk_weight) of x's rows."""
+    if gate is None and select_bias is None:
+        return ops.route_topk(x, wr, k, bias=bias, renorm=renorm)
+    g = gate or Gate()
+    logits, _, _ = ops.route_topk(x, wr, 1, bias=bias)
+    ids, tw = ops.route_scores(logits, k, g.score, select_bias, g.n_group, g.topk_group, g.group_top, renorm, g.scaling)
+    return logits, ids, tw
+
+
+@dataclass
+class _Experts:
+    """What the backward of a routed layer needs of its forward, besides the tensors in `saved`."""
+
+    saved: tuple
+    k: int
+    renorm: bool
+    gate: Gate | None
+    select: bool  # the routing took a selection bias
+    w_dtypes: tuple
+
+
+def _experts_forward(x, wr, wgu, wd, bias, k, renorm, gate, select_bias, need_grad):
+    """Routing, dispatch and both projections of x (T, d) bf16 -> (y (T*k, d) in (token, slot) order, ids, weights, state)."""
+    _check_layer_args(x, wr, wgu, wd, bias, k)
+    if select_bias is not None and tuple(select_bias.shape) != (wgu.shape[0],):
+        raise ValueError(f"select_bias: shape {tuple(select_bias.shape)}, expected ({wgu.shape[0]},)")
+    M = x.shape[0] * k
+    w_dtypes = (wr.dtype, wgu.dtype, wd.dtype)
+    wr, wgu, wd = _bf16(wr), _bf16(wgu), _bf16(wd)
+    logits, ids, tw = _route(x, wr, bias, k, renorm, gate, select_bias)
+    # The dispatch writes the routed rows as row-group tiles for the gate/up GEMM; with a backward to follow,
+    # also the row-major permuted copy xs (the gate/up weight gradient reads it).
+    disp, act, gu = ops.routed_gate_up(x, ids, wgu.shape[0], wgu, topk_w=tw, keep_gu=need_grad, want_xs=need_grad,
+                                       want_inv=need_grad)
+    y, _ = ops.down_scatter(act, wd, disp.counts, M, disp.w_sorted, disp.order)
+    state = None
+    if need_grad:
+        state = _Experts((x, wr, wgu, wd, logits, ids, disp.counts, disp.order, disp.a_idx, disp.inv_pos, disp.w_sorted,
+                          disp.xs, gu, act, tw), k, renorm, gate, select_bias is not None, w_dtypes)
+    return y, ids, tw, state
+
+
+def _experts_backward(state, dout, dtw_out, need_x, need_wr, need_wgu, need_wd):
+    """(dx, dwr, dwgu, dwd), None where not needed, from dout (T, d) bf16, the gradient of every slot of y, and dtw_out
+    (T, k), that of the returned weights, or None."""
+    x, wr, wgu, wd, logits, ids, counts, order, a_idx, inv_pos, w_sorted, xs, gu, act, tw = state.saved
+    k = state.k
+    T = x.shape[0]
+    E = wgu.shape[0]
+    M = T * k
+    wr_dt, wgu_dt, wd_dt = state.w_dtypes
+    disp = ops.Dispatch(counts, None, None, order, a_idx, inv_pos, w_sorted, xs)
+    # One stream: every GEMM is a persistent launch sized to own all CUs, so two of them side by side only
+    # queue each other's workgroups behind long-running tiles.
+    dys, _ = ops.combine_bwd(dout, None, disp, k)
+    dwd = dwgu = None
+    if need_wd:
+        dwd = _to_param(ops.grouped_wgrad(act, dys, counts, E, dtype=_grad_dtype(wd_dt)), wd_dt)
+    # dgu, and the routing-weight gradient <dout[t], act[r] @ wd[e]> from the same fp32 product
+    dgu, dtw = ops.down_dgrad_swiglu_dw(dout, wd, counts, M, gu, order, k, a_idx=a_idx, w_sorted=w_sorted)
+    if dtw_out is not None:  # the returned routing weights are outputs too: their gradient joins the combine's
+        dtw = dtw + dtw_out.to(torch.float32)
+    if need_wgu:
+        dwgu = _to_param(ops.grouped_wgrad(xs, dgu, counts, E, dtype=_grad_dtype(wgu_dt)), wgu_dt)
+    # (for a few thousand rows its reduction is split, and the un-permute adds the parts)
+    dxs = ops.gate_up_dgrad(dgu, wgu, counts, M, parts=ops.dgrad_parts(M, wgu))
+    if state.gate is None and not state.select:
+        dl, dwr = ops.router_bwd(logits, ids, dtw, x, renorm=state.renorm, dwr_dtype=_grad_dtype(wr_dt), want_dwr=need_wr)
+    else:
+        g = state.gate or Gate()
+        dl = ops.route_scores_bwd(dtw, tw, logits, ids, g.score, state.renorm, g.scaling)
+        dwr = ops.router_wgrad(dl, x, dtype=_grad_dtype(wr_dt)) if need_wr else None
+    dwr = _to_param(dwr, wr_dt)
+    dx = ops.unpermute_bwd(dxs, inv_pos, T, k, dlogits=dl, wr=wr) if need_x else None
+    return dx, dwr, dwgu, dwd
+
+
 class _MoEFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, wr, wgu, wd, bias, k, renorm):
-        _check_layer_args(x, wr, wgu, wd, bias, k)
-        T, d = x.shape
-        E = wgu.shape[0]
-        M = T * k
-        ctx.w_dtypes = (wr.dtype, wgu.dtype, wd.dtype)
-        wr, wgu, wd = _bf16(wr), _bf16(wgu), _bf16(wd)
+    def forward(ctx, x, wr, wgu, wd, bias, k, renorm, gate=None, select_bias=None):
         need_grad = any(ctx.needs_input_grad[:4])
-        logits, ids, tw = ops.route_topk(x, wr, k, bias=bias, renorm=renorm)
-        # The dispatch writes the routed rows as row-group tiles for the gate/up GEMM; with a backward to follow,
-        # also the row-major permuted copy xs (the gate/up weight gradient reads it).
-        disp, act, gu = ops.routed_gate_up(x, ids, E, wgu, topk_w=tw, keep_gu=need_grad, want_xs=need_grad,
-                                           want_inv=need_grad)
-        y, _ = ops.down_scatter(act, wd, disp.counts, M, disp.w_sorted, disp.order)
-        out = ops.combine(y, T, k)
+        y, ids, tw, state = _experts_forward(x, wr, wgu, wd, bias, k, renorm, gate, select_bias, need_grad)
+        out = ops.combine(y, x.shape[0], k)
         if need_grad:
-            ctx.save_for_backward(x, wr, wgu, wd, logits, ids, disp.counts, disp.order, disp.a_idx, disp.inv_pos,
-                                  disp.w_sorted, disp.xs, gu, act)
-        ctx.k, ctx.renorm = k, renorm
+            ctx.save_for_backward(*state.saved)
+            state.saved = None
+        ctx.state = state
         ctx.mark_non_differentiable(ids)
         ctx.set_materialize_grads(False)  # absent output gradients stay None (no zero-filled tensors)
         return out, ids, tw
 
     @staticmethod
     def backward(ctx, dout, _dids, dtw_out):
+        none = (None,) * 5
         if dout is None and dtw_out is None:
-            return None, None, None, None, None, None, None
-        x, wr, wgu, wd, logits, ids, counts, order, a_idx, inv_pos, w_sorted, xs, gu, act = ctx.saved_tensors
-        k = ctx.k
-        T, d = x.shape
-        E = wgu.shape[0]
-        M = T * k
-        wr_dt, wgu_dt, wd_dt = ctx.w_dtypes
-        disp = ops.Dispatch(counts, None, None, order, a_idx, inv_pos, w_sorted, xs)
+            return (None,) * 4 + none
+        state = replace(ctx.state, saved=ctx.saved_tensors)
+        x = state.saved[0]
         if dout is None:  # a loss on the routing weights alone: the expert path carries no gradient
-            dout = torch.zeros(T, d, device=x.device, dtype=torch.bfloat16)
+            dout = torch.zeros(x.shape, device=x.device, dtype=torch.bfloat16)
         dout = dout.contiguous().to(torch.bfloat16)
-        # One stream: every GEMM is a persistent launch sized to own all CUs, so two of them side by side only
-        # queue each other's workgroups behind long-running tiles.
-        dys, _ = ops.combine_bwd(dout, None, disp, k)
-        dwd = dwgu = None
-        if ctx.needs_input_grad[3]:
-            dwd = _to_param(ops.grouped_wgrad(act, dys, counts, E, dtype=_grad_dtype(wd_dt)), wd_dt)
-        # dgu, and the routing-weight gradient <dout[t], act[r] @ wd[e]> from the same fp32 product
-        dgu, dtw = ops.down_dgrad_swiglu_dw(dout, wd, counts, M, gu, order, k, a_idx=a_idx, w_sorted=w_sorted)
-        if dtw_out is not None:  # the returned routing weights are outputs too: their gradient joins the combine's
-            dtw = dtw + dtw_out.to(torch.float32)
-        if ctx.needs_input_grad[2]:
-            dwgu = _to_param(ops.grouped_wgrad(xs, dgu, counts, E, dtype=_grad_dtype(wgu_dt)), wgu_dt)
-        # (for a few thousand rows its reduction is split, and the un-permute adds the parts)
-        dxs = ops.gate_up_dgrad(dgu, wgu, counts, M, parts=ops.dgrad_parts(M, wgu))
-        dl, dwr = ops.router_bwd(logits, ids, dtw, x, renorm=ctx.renorm, dwr_dtype=_grad_dtype(wr_dt),
-                                 want_dwr=ctx.needs_input_grad[1])
-        dwr = _to_param(dwr, wr_dt)
-        dx = ops.unpermute_bwd(dxs, inv_pos, T, k, dlogits=dl, wr=wr) if ctx.needs_input_grad[0] else None
-        return dx, dwr, dwgu, dwd, None, None, None
+        return _experts_backward(state, dout, dtw_out, *ctx.needs_input_grad[:4]) + none
 
 
-def moe_swiglu(x, router_weight, w_gu, w_d, top_k, logit_bias=None, renorm=True):
+def moe_swiglu(x, router_weight, w_gu, w_d, top_k, logit_bias=None, renorm=True, gate=None, select_bias=None):
     """Functional form: x (T, d) bf16 -> (out (T, d) bf16, topk_ids (T, k) int32, topk_weight (T, k) fp32).
 
     router_weight (E, d), w_gu (E, d, 2h) = [gate | up], w_d (E, h, d): bf16, or fp32 / fp16 (rounded to bf16 for
     the products, gradients in the weights' dtype).  logit_bias (E,) fp32 is added to the router logits (no gradient).  Gradients reach
-    x and the three weights from `out` and from `topk_weight` (softmax + renormalisation Jacobian).  Without a
+    x and the three weights from `out` and from `topk_weight` (softmax + renormalisation Jacobian).  gate: a Gate for sigmoid
+    scores, groups or a factor on the weights; select_bias (E,) fp32 joins the scores for the selection only (a bias for
+    balance; no gradient).  Without a
     gradient to record (grad mode off, or no input requiring one) the forward runs as one C call
-    (ops.moe_forward): the same kernels and outputs, a fraction of the host time."""
+    (ops.moe_forward; with a gate or a selection bias, the routing and ops.moe_experts): the same kernels and outputs, a
+    fraction of the host time."""
     if not (torch.is_grad_enabled() and (x.requires_grad or router_weight.requires_grad or w_gu.requires_grad
                                          or w_d.requires_grad)):
-        _check_layer_args(x, router_weight, w_gu, w_d, logit_bias, top_k)
-        out, ids, tw, _ = ops.moe_forward(x, _bf16(router_weight), _bf16(w_gu), _bf16(w_d), top_k, bias=logit_bias,
-                                          renorm=renorm)
-        return out, ids, tw
-    return _MoEFunction.apply(x, router_weight, w_gu, w_d, logit_bias, top_k, renorm)
+        if gate is None and select_bias is None:
+            _check_layer_args(x, router_weight, w_gu, w_d, logit_bias, top_k)
+            out, ids, tw, _ = ops.moe_forward(x, _bf16(router_weight), _bf16(w_gu), _bf16(w_d), top_k, bias=logit_bias,
+                                              renorm=renorm)
+            return out, ids, tw
+        y, ids, tw, inv = _experts_infer(x, router_weight, w_gu, w_d, logit_bias, top_k, renorm, gate, select_bias)
+        return ops.combine(y, x.shape[0], top_k, inv_pos=inv), ids, tw
+    return _MoEFunction.apply(x, router_weight, w_gu, w_d, logit_bias, top_k, renorm, gate, select_bias)
+
+
+def _experts_infer(x, wr, wgu, wd, bias, k, renorm, gate, select_bias):
+    """_experts_forward without anything kept for a backward, the experts in one C call -> (y, ids, weights, inv_pos)."""
+    _check_layer_args(x, wr, wgu, wd, bias, k)
+    if select_bias is not None and tuple(select_bias.shape) != (wgu.shape[0],):
+        raise ValueError(f"select_bias: shape {tuple(select_bias.shape)}, expected ({wgu.shape[0]},)")
+    _, ids, tw = _route(x, _bf16(wr), bias, k, renorm, gate, select_bias)
+    y, inv, _ = ops.moe_experts(x, ids, tw, _bf16(wgu), _bf16(wd))
+    return y, ids, tw, inv
 
 
 class _ExpertStackProj:
@@ -171,19 +247,29 @@ class MoESwiGLU(nn.Module):
     default initialisation is theirs: N(0, in_features ** -0.5) per projection (dim for w_gu and the router, hidden
     for w_d); `init_std` overrides it with one std for all three.
 
+    `gate` (a Gate) chooses sigmoid scores, groups or a factor on the weights; `balance` adds the buffer select_bias (E,)
+    fp32, which joins the scores for the selection only: a training script that balances its experts without a loss raises
+    it for experts that got too few tokens and lowers it for the others.
+
     The products run in bf16 (any other input dtype is rounded to bf16 first); the output has the dtype the
     reference's SwiGLU would return: the autocast dtype inside autocast, else the input's dtype.  The routing of the
     last call is kept in `last_topk_ids` / `last_topk_weight` (the weights carry gradient)."""
 
     def __init__(self, dim: int, hidden: int, experts: int, top_k: int = 2, renorm: bool = True,
-                 init_std: float | None = None, device=None, dtype=torch.bfloat16):
+                 init_std: float | None = None, device=None, dtype=torch.bfloat16, gate: Gate | None = None,
+                 balance: bool = False):
         super().__init__()
         self.dim, self.hidden, self.experts, self.top_k, self.renorm = dim, hidden, experts, top_k, renorm
+        self.gate = gate
         f = dict(device=device, dtype=dtype)
         self.router_weight = nn.Parameter(torch.empty(experts, dim, **f))
         self.w_gu = nn.Parameter(torch.empty(experts, dim, 2 * hidden, **f))
         self.w_d = nn.Parameter(torch.empty(experts, hidden, dim, **f))
         self.register_buffer("logit_bias", torch.zeros(experts, device=device, dtype=torch.float32))
+        if balance:
+            self.register_buffer("select_bias", torch.zeros(experts, device=device, dtype=torch.float32))
+        else:
+            self.select_bias = None
         self.init_std = init_std
         self.reset_parameters()
         self.last_topk_ids = None
@@ -209,7 +295,7 @@ class MoESwiGLU(nn.Module):
         if x.dtype != torch.bfloat16:
             x = x.to(torch.bfloat16)
         out, ids, tw = moe_swiglu(x, self.router_weight, self.w_gu, self.w_d, self.top_k, self.logit_bias,
-                                  self.renorm)
+                                  self.renorm, self.gate, self.select_bias)
         self.last_topk_ids, self.last_topk_weight = ids, tw
         out = out.view(shape)
         return out if out.dtype == out_dtype else out.to(out_dtype)
