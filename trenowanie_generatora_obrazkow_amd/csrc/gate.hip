@@ -400,9 +400,16 @@ __global__ __launch_bounds__(256) void route_scores_bwd_kernel(GateBwdArgs b) {
     }
     S = seg_sum(S);
   }
-  float s = 0.0f;
-  if (e >= 0) s = SIG ? 1.0f / (1.0f + hexp(-l)) : S == 0.0f ? 0.0f : hexp(l - m) / S;
-  if (e < 0) u = 0.0f;
+  // s, and for the sigmoid its derivative s (1 - s) = x / (1 + x)^2 with x = exp(-|l|), without the cancellation in 1 - s
+  float s = 0.0f, slope = 1.0f;
+  if (SIG) {
+    const float x = hexp(-fabsf(l)), r = 1.0f / (1.0f + x);
+    s = l >= 0.0f ? r : x * r;
+    slope = x * r * r;
+  } else {
+    s = S == 0.0f ? 0.0f : hexp(l - m) / S;
+  }
+  if (e < 0) s = u = 0.0f;
   float ds = u;
   if (a.renorm) {
     const float den = seg_sum(s) + 1e-20f;
@@ -411,7 +418,7 @@ __global__ __launch_bounds__(256) void route_scores_bwd_kernel(GateBwdArgs b) {
   if (e < 0) ds = 0.0f;
   const float pdp = seg_sum(s * ds);
   wave_lds_sync();
-  if (e >= 0) atomicAdd(&dp[e], SIG ? ds * s * (1.0f - s) : ds);
+  if (e >= 0) atomicAdd(&dp[e], ds * slope);
   wave_lds_sync();
   const float inv = S == 0.0f ? 0.0f : 1.0f / S;
   float d[EPL];

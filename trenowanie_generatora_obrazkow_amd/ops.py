@@ -718,17 +718,20 @@ _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device
 
 def _call_on(dev, name, *args):
     """A C call with its stream, launched on `dev` also where another device is the current one."""
-    if dev.index == _current_device():
-        L.call(name, *args, L.stream(dev))
+    i = dev.index
+    if i == _current_device():
+        rc = getattr(L.lib(), name)(*args, L.stream(i))
     else:
         with torch.cuda.device(dev):
-            L.call(name, *args, L.stream(dev))
+            rc = getattr(L.lib(), name)(*args, L.stream(i))
+    if rc != 0:
+        raise L.HmoeError(name, rc)
 
 
 def _on(t, name, dev, shape, dtypes):
     """A contiguous operand of a call whose first tensor lives on `dev`; None passes."""
-    if t is None:
-        return None
+    if t is None or (t.dtype in dtypes and t.shape == shape and t.is_contiguous() and t.device == dev):
+        return t
     if t.device != dev:
         raise ValueError(f"{name} is on {t.device}, the call's other tensors on {dev}")
     if t.dtype not in dtypes:
@@ -742,37 +745,45 @@ def _on(t, name, dev, shape, dtypes):
 
 def _rows(t, name, dtypes=_FLOATS):
     """(T, d, row stride) of a matrix whose rows are contiguous."""
-    L.require_gpu(t, name)
-    if t.dim() != 2:
+    if t.dim() != 2 or not t.is_cuda:
+        L.require_gpu(t, name)
         raise ValueError(f"{name} must be a (rows, width) matrix (got {tuple(t.shape)})")
     if t.dtype not in dtypes:
         raise TypeError(f"{name}: dtype {t.dtype} not in {dtypes}")
     T, d = t.shape
     if d % 8 or d == 0:
         raise ValueError(f"{name}: width {d} must be a positive multiple of 8")
+    if t.is_contiguous():
+        return T, d, d
     ld = t.stride(0) if T > 1 else d
-    if (d > 1 and t.stride(1) != 1) or ld < d or ld % 8:
+    if t.stride(1) != 1 or ld < d or ld % 8:
         raise ValueError(f"{name}: rows must be contiguous, with a row stride of a multiple of 8 (strides {t.stride()})")
     return T, d, ld
 
 
 def _routing(logits, k, score, n_group, topk_group, group_top):
-    L.require_gpu(logits, "logits")
-    if logits.dim() != 2 or logits.dtype not in _FLOATS:
+    """(T, E, row stride) of logits, and every condition on the sizes."""
+    if logits.dim() != 2 or not logits.is_cuda or logits.dtype not in _FLOATS:
+        L.require_gpu(logits, "logits")
         raise TypeError(f"logits must be a (T, E) matrix of bf16, fp16 or fp32 (got {tuple(logits.shape)} {logits.dtype})")
     if score not in _SCORES:
         raise ValueError(f"score must be 'softmax' or 'sigmoid' (got {score!r})")
     T, E = logits.shape
-    if E < 1 or not 1 <= k <= min(E, 16) or E > 512:
+    if not 1 <= k <= E or k > 16 or E > 512:
         raise ValueError(f"routing takes up to 512 experts and 1 to min(16, E) slots (got E = {E}, k = {k})")
-    if (E > 1 and logits.stride(1) != 1) or (T > 1 and logits.stride(0) < E):
-        raise ValueError(f"logits rows must be contiguous (strides {logits.stride()})")
-    if n_group < 1 or not 1 <= topk_group <= n_group or E % n_group or group_top not in (1, 2):
-        raise ValueError(f"groups: E = {E} must divide into n_group = {n_group}, 1 <= topk_group = {topk_group} <= n_group, "
-                         f"group_top = {group_top} 1 or 2")
-    if topk_group < n_group and (n_group > 64 or E // n_group < group_top or k > topk_group * (E // n_group)):
-        raise ValueError(f"{topk_group} of {n_group} groups of {E // n_group} experts cannot give k = {k} (at most 64 groups)")
-    return T, E, logits.stride(0) if T > 1 else E
+    ld = E
+    if not logits.is_contiguous():
+        ld = logits.stride(0) if T > 1 else E
+        if (E > 1 and logits.stride(1) != 1) or ld < E:
+            raise ValueError(f"logits rows must be contiguous (strides {logits.stride()})")
+    if n_group != 1 or topk_group != 1 or group_top not in (1, 2):
+        if n_group < 1 or not 1 <= topk_group <= n_group or E % n_group or group_top not in (1, 2):
+            raise ValueError(f"groups: E = {E} must divide into n_group = {n_group}, 1 <= topk_group = {topk_group} <= "
+                             f"n_group, group_top = {group_top} 1 or 2")
+        if topk_group < n_group and (n_group > 64 or E // n_group < group_top or k > topk_group * (E // n_group)):
+            raise ValueError(f"{topk_group} of {n_group} groups of {E // n_group} experts cannot give k = {k} (at most 64 "
+                             f"groups)")
+    return T, E, ld
 
 
 def route_scores(logits, k, score="softmax", bias=None, n_group=1, topk_group=1, group_top=2, renorm=True, scaling=1.0,
@@ -970,7 +981,7 @@ class GradList:
         self.n = len(grads)
         self.device = self._check(grads, "gradient")
         self.ptr = self._ptrs(grads)
-        self.numel = array("q", [g.numel() for g in grads])
+        self.numel = array("q", list(map(torch.Tensor.numel, grads)))
         self.dt = self._types(grads)
         if out is None:
             out = grads
@@ -992,29 +1003,32 @@ class GradList:
             if len(set(used)) != len(used):
                 raise ValueError("a tensor is listed twice")
 
-    # one pass per property: a program clips hundreds of tensors, and the time of this is the host's
+    # one pass per property, mapped over the tensors by the descriptor itself: a program clips hundreds of them, and the time
+    # of this is the host's
     @staticmethod
     def _check(ts, name):
-        devs = {t.device for t in ts}
+        devs = set(map(torch.Tensor.get_device, ts))
         if len(devs) > 1:
-            raise ValueError(f"the {name}s of a call live on one device (got {sorted(map(str, devs))})")
-        dev = devs.pop() if devs else None
+            raise ValueError(f"the {name}s of a call live on one device (got {sorted({str(t.device) for t in ts})})")
+        dev = ts[0].device if ts else None
         if dev is not None and dev.type != "cuda":
             raise RuntimeError(f"a {name} must be a ROCm GPU tensor: the hmoe kernels have no CPU path")
-        if not all([t.is_contiguous() for t in ts]) and not all(_dense(t) for t in ts):
+        if not all(map(torch.Tensor.is_contiguous, ts)) and not all(map(_dense, ts)):
             raise ValueError(f"a {name}'s elements must be contiguous")
         return dev
 
     @staticmethod
     def _ptrs(ts):
-        return array("Q", [t.data_ptr() for t in ts])
+        return array("Q", list(map(torch.Tensor.data_ptr, ts)))
 
     @staticmethod
     def _types(ts):
-        kinds = [t.dtype for t in ts]
-        bad = set(kinds) - set(_FLOATS)
-        if bad:
-            raise TypeError(f"gradients and outputs are bf16, fp16 or fp32 (got {bad})")
+        kinds = list(map(torch.Tensor.dtype.__get__, ts))
+        found = set(kinds)
+        if not found.issubset(_FLOATS):
+            raise TypeError(f"gradients and outputs are bf16, fp16 or fp32 (got {found})")
+        if len(found) == 1:
+            return array("i", [L._DT[kinds[0]]]) * len(kinds)
         return array("i", [L._DT[k] for k in kinds])
 
 
