@@ -86,6 +86,9 @@ CASES = [
     (6, 16384, 2, True, FP, HF, FP, FP, (1, 1)),
     (5000, 64, 611, True, BF, BF, BF, BF, (0, 9)),       # many samples inside one chunk of rows
     (2048, 136, 2048, False, BF, BF, BF, FP, (0, 0)),
+    # equal samples of few rows, finished by the row groups themselves: a part of a workgroup's samples, one row each
+    (20, 1536, 20, False, BF, BF, BF, BF, (0, 0)), (4500, 200, 1500, False, FP, BF, FP, FP, (0, 0)),
+    (66, 4096, 33, False, HF, HF, HF, FP, (0, 0)), (5, 9000, 5, False, BF, BF, FP, BF, (0, 0)),
 ]
 ids = [f"{c[0]}x{c[1]}_{c[2]}{'r' if c[3] else ''}" for c in CASES]
 

@@ -411,8 +411,8 @@ __global__ __launch_bounds__(kFwdThreads<WPR>, ST == HMOE_DT_F32 || KB == 4 ? 2 
 //   norm_out: g = u w gate_b,        dy = r (g - n mean(g n)),          A_b = sum u n,
 //             dgate_b = w A_b,  dw = sum_rows u gate_b n
 // mean(g n) = r sum(g v) / d, so both row sums (v^2 and g v) are taken in one exchange.
-// A sample inside one block's rows is finished by that block; pieces of longer ones go to slot c + b of the workspace
-// (c and b never fall along the rows and one of them grows from piece to piece, so slots are distinct) and
+// A sample inside one block's rows is finished by that block.  Of the others' pieces a block holds at most two: the end or
+// middle of one that began before (slot 2 c of the workspace) and the beginning of one that goes on (slot 2 c + 1);
 // norm_sums_kernel adds them in chunk order.
 // ---------------------------------------------------------------------------------------------------------------
 struct NormBwdArgs {
@@ -426,7 +426,7 @@ struct NormBwdArgs {
   void* dv;
   NormParams p;
   void *dweight, *dscale, *dshift;  // of the parameters' types; NULL to skip
-  float* part;    // (chunks + B) x nsum x d
+  float* part;    // 2 chunks x nsum x d
   float* wpart;   // chunks x d
   Samples s;
   int d, k, norm, R;
@@ -434,13 +434,15 @@ struct NormBwdArgs {
 };
 
 // KB: 0 for norm_in, else the slots loaded at once for norm_out.
-template <int KB, int ST, int HT, int VPL, int WPR>
+// SHORT (equal samples of few rows): each row group takes whole samples, every 8th of the R / L of its block, and writes
+// their sums itself; in the other form the groups share a piece's rows, and with fewer rows than groups most would wait.
+template <int KB, int ST, int HT, int VPL, int WPR, bool SHORT>
 __global__ __launch_bounds__(kNormThreads<WPR>) void norm_bwd_kernel(NormBwdArgs a) {
   constexpr bool OUT = KB > 0;
   constexpr int UT = OUT ? ST : HT, DT = OUT ? HT : ST;  // types of u and of dv
-  constexpr int G = kNormGroups<WPR>;
   // column vectors a thread adds up over the row groups: tid, tid + threads, ...
-  constexpr int NC = (64 * WPR * VPL + kNormThreads<WPR> - 1) / kNormThreads<WPR>;
+  constexpr int G = kNormGroups<WPR>, THREADS = kNormThreads<WPR>;
+  constexpr int NC = (64 * WPR * VPL + THREADS - 1) / THREADS;
   __shared__ float red[2 * 32];
   extern __shared__ float colsum[];  // G x d
   const int nv = a.d / 8, lane = threadIdx.x % (64 * WPR);
@@ -464,7 +466,7 @@ __global__ __launch_bounds__(kNormThreads<WPR>) void norm_bwd_kernel(NormBwdArgs
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const int c = threadIdx.x + kNormThreads<WPR> * i;
+      const int c = threadIdx.x + THREADS * i;
       if (c >= nv) continue;
       float t[8], q[8];
       load8<HMOE_DT_F32>(colsum, 0, 8 * c, t);
@@ -479,7 +481,7 @@ __global__ __launch_bounds__(kNormThreads<WPR>) void norm_bwd_kernel(NormBwdArgs
   };
   using VRaw = Raw8<OUT ? HMOE_DT_F32 : ST>;  // (the slots' sum stays fp32)
   auto load_rows = [&](int r, auto& ru, auto& rv, auto& rd) {
-    r = min(r, r_end - 1);
+    r = min(r, a.s.T - 1);
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
       const uint32_t col = 8 * min(lane + 64 * WPR * i, nv - 1);
@@ -498,28 +500,9 @@ __global__ __launch_bounds__(kNormThreads<WPR>) void norm_bwd_kernel(NormBwdArgs
         for (int e = 0; e < 8; ++e) rv[i].w[e] = __float_as_uint(t[i][e]);
     }
   };
-  for (int r0 = r_begin; r0 < r_end;) {
-    int end;
-    const int b = sample_of(a.s, r0, end);
-    const int piece_end = min(end, r_end);
-    const bool live = b >= 0 && b < a.s.B;
-    if (!live) {  // padding rows: no gradient from the norm
-      for (int r = r0 + grp; r < piece_end; r += G)
-        for (int c = lane; c < nv; c += 64 * WPR) {
-          float t[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) t[e] = 0.0f;
-          if (a.dres) {
-            load8<ST>(a.dres, (int64_t)r * a.d, 8 * c, t);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) t[e] *= a.dres_scale;
-          }
-          store8<DT>(a.dv, (int64_t)r * a.d, 8 * c, t);
-        }
-      r0 = piece_end;
-      continue;
-    }
-    float aacc[VPL][8], sacc[VPL][8], wm[VPL][8];
+  float aacc[VPL][8], sacc[VPL][8], wm[VPL][8];
+  // the parameters of sample b, and its sums from zero
+  auto begin = [&](int b) {
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
       const int c = lane + 64 * WPR * i;
@@ -538,94 +521,162 @@ __global__ __launch_bounds__(kNormThreads<WPR>) void norm_bwd_kernel(NormBwdArgs
         }
       }
     }
-    for (int rg = r0; rg < piece_end; rg += G) {
-      const int r = rg + grp;
-      Raw8<UT> u[VPL];
-      VRaw v[VPL];
-      Raw8<ST> dr[OUT ? 1 : VPL];
-      load_rows(r, u, v, dr);
-      float sq = 0.0f, dot = 0.0f;
+  };
+  // one row of every row group (the row sums may hold a barrier: every wave comes here)
+  auto one_row = [&](int r, bool row) {
+    Raw8<UT> u[VPL];
+    VRaw v[VPL];
+    Raw8<ST> dr[OUT ? 1 : VPL];
+    load_rows(r, u, v, dr);
+    float sq = 0.0f, dot = 0.0f;
 #pragma unroll
-      for (int i = 0; i < VPL; ++i) {
-        const bool in = vec_in<VPL>(i, lane + 64 * WPR * i, nv);
-        u[i].keep(in);
-        v[i].keep(in);
+    for (int i = 0; i < VPL; ++i) {
+      const bool in = vec_in<VPL>(i, lane + 64 * WPR * i, nv);
+      u[i].keep(in);
+      v[i].keep(in);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          sq += v[i][e] * v[i][e];
-          dot += u[i][e] * wm[i][e] * v[i][e];
+      for (int e = 0; e < 8; ++e) {
+        sq += v[i][e] * v[i][e];
+        dot += u[i][e] * wm[i][e] * v[i][e];
+      }
+    }
+    float rms = 1.0f, proj = 0.0f;  // proj = r^3 mean(g v): dv = r g - v proj
+    if (a.norm) {
+      row_sum2<WPR>(sq, dot, red, half);
+      rms = inv_rms(sq, a.d, a.eps);
+      proj = rms * rms * rms * (dot / (float)a.d);
+    }
+    if (!row) return;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      const int c = lane + 64 * WPR * i;
+      if (!vec_in<VPL>(i, c, nv)) continue;
+      float t[8];
+      u[i].hold();
+      v[i].hold();
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float ue = u[i][e], ve = v[i][e];
+        aacc[i][e] += ue * (ve * rms);
+        if constexpr (!OUT) sacc[i][e] += ue;
+        t[e] = rms * (ue * wm[i][e]) - ve * proj;
+      }
+      if constexpr (!OUT)
+        if (a.dres) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) t[e] += a.dres_scale * dr[i][e];
         }
-      }
-      float rms = 1.0f, proj = 0.0f;  // proj = r^3 mean(g v): dv = r g - v proj
-      if (a.norm) {
-        row_sum2<WPR>(sq, dot, red, half);
-        rms = inv_rms(sq, a.d, a.eps);
-        proj = rms * rms * rms * (dot / (float)a.d);
-      }
-      if (r >= piece_end) continue;
+      store8<DT>(a.dv, (int64_t)r * a.d, 8 * c, t);
+    }
+  };
+  if constexpr (SHORT) {
+    const int L = a.s.L, S = a.R / L;  // samples of this block
+    float wsum[VPL][8];
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) wsum[i][e] = 0.0f;
+    for (int s0 = 0; s0 < S; s0 += G) {
+      const int b = blockIdx.x * S + s0 + grp;
+      const bool on = s0 + grp < S && b < a.s.B;
+      const int bc = min(b, a.s.B - 1);
+      begin(bc);
+      for (int l = 0; l < L; ++l) one_row(bc * L + l, on);
+      if (!on) continue;
 #pragma unroll
       for (int i = 0; i < VPL; ++i) {
         const int c = lane + 64 * WPR * i;
         if (!vec_in<VPL>(i, c, nv)) continue;
-        float t[8];
-        u[i].hold();
-        v[i].hold();
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float ue = u[i][e], ve = v[i][e];
-          aacc[i][e] += ue * (ve * rms);
-          if constexpr (!OUT) sacc[i][e] += ue;
-          t[e] = rms * (ue * wm[i][e]) - ve * proj;
-        }
-        if constexpr (!OUT)
-          if (a.dres) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) t[e] += a.dres_scale * dr[i][e];
-          }
-        store8<DT>(a.dv, (int64_t)r * a.d, 8 * c, t);
-      }
-    }
-    // (whole: this block holds every row of the sample)
-    const int first = a.s.starts ? a.s.starts[b] : b * a.s.L;
-    const bool whole = first >= r_begin && end <= r_end;
-    float* slot = a.part + (int64_t)(blockIdx.x + b) * nsum * a.d;
-    if (a.dscale || a.dweight)
-      over_groups(aacc, [&](int i, int c, float (&t)[8]) {
         float q[8];
-        if (a.dweight) {  // A_b (1 + scale_b), or A_b gate_b
+        if (a.dweight) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) q[e] = OUT ? 1.0f : 0.0f;
           if (a.p.scale) load8_rt(a.p.scale, a.p.scale_dt, (int64_t)b * a.d, 8 * c, q);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) wacc[i][e] += (OUT ? q[e] : 1.0f + q[e]) * t[e];
+          for (int e = 0; e < 8; ++e) wsum[i][e] += (OUT ? q[e] : 1.0f + q[e]) * aacc[i][e];
         }
-        if (!a.dscale) return;
-        if (!whole) {
-          store8<HMOE_DT_F32>(slot, 0, 8 * c, t);
-          return;
-        }
-        if (a.p.weight) {
-          load8_rt(a.p.weight, a.p.weight_dt, 0, 8 * c, q);
+        if (a.dscale) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) t[e] *= q[e];
+          for (int e = 0; e < 8; ++e) q[e] = 1.0f;
+          if (a.p.weight) load8_rt(a.p.weight, a.p.weight_dt, 0, 8 * c, q);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) q[e] *= aacc[i][e];
+          store8_rt(a.dscale, a.p.scale_dt, (int64_t)b * a.d, 8 * c, q);
         }
-        store8_rt(a.dscale, a.p.scale_dt, (int64_t)b * a.d, 8 * c, t);
-      });
-    if constexpr (!OUT) {
-      if (a.dshift)
-        over_groups(sacc, [&](int, int c, float (&t)[8]) {
-          if (whole)
-            store8_rt(a.dshift, a.p.shift_dt, (int64_t)b * a.d, 8 * c, t);
-          else
-            store8<HMOE_DT_F32>(slot, (int64_t)(nsum - 1) * a.d, 8 * c, t);
-        });
+        if (!OUT && a.dshift) store8_rt(a.dshift, a.p.shift_dt, (int64_t)b * a.d, 8 * c, sacc[i]);
+      }
     }
-    r0 = piece_end;
+    if (a.dweight)
+      over_groups(wsum, [&](int i, int, float (&t)[8]) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) wacc[i][e] = t[e];
+      });
+  } else {
+    for (int r0 = r_begin; r0 < r_end;) {
+      int end;
+      const int b = sample_of(a.s, r0, end);
+      const int piece_end = min(end, r_end);
+      const bool live = b >= 0 && b < a.s.B;
+      if (!live) {  // padding rows: no gradient from the norm
+        for (int r = r0 + grp; r < piece_end; r += G)
+          for (int c = lane; c < nv; c += 64 * WPR) {
+            float t[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) t[e] = 0.0f;
+            if (a.dres) {
+              load8<ST>(a.dres, (int64_t)r * a.d, 8 * c, t);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) t[e] *= a.dres_scale;
+            }
+            store8<DT>(a.dv, (int64_t)r * a.d, 8 * c, t);
+          }
+        r0 = piece_end;
+        continue;
+      }
+      begin(b);
+      for (int rg = r0; rg < piece_end; rg += G) one_row(rg + grp, rg + grp < piece_end);
+      // (whole: this block holds every row of the sample)
+      const int first = a.s.starts ? a.s.starts[b] : b * a.s.L;
+      const bool whole = first >= r_begin && end <= r_end;
+      float* slot = a.part + (2 * (int64_t)blockIdx.x + (first >= r_begin)) * nsum * a.d;
+      if (a.dscale || a.dweight)
+        over_groups(aacc, [&](int i, int c, float (&t)[8]) {
+          float q[8];
+          if (a.dweight) {  // A_b (1 + scale_b), or A_b gate_b
+#pragma unroll
+            for (int e = 0; e < 8; ++e) q[e] = OUT ? 1.0f : 0.0f;
+            if (a.p.scale) load8_rt(a.p.scale, a.p.scale_dt, (int64_t)b * a.d, 8 * c, q);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) wacc[i][e] += (OUT ? q[e] : 1.0f + q[e]) * t[e];
+          }
+          if (!a.dscale) return;
+          if (!whole) {
+            store8<HMOE_DT_F32>(slot, 0, 8 * c, t);
+            return;
+          }
+          if (a.p.weight) {
+            load8_rt(a.p.weight, a.p.weight_dt, 0, 8 * c, q);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) t[e] *= q[e];
+          }
+          store8_rt(a.dscale, a.p.scale_dt, (int64_t)b * a.d, 8 * c, t);
+        });
+      if constexpr (!OUT) {
+        if (a.dshift)
+          over_groups(sacc, [&](int, int c, float (&t)[8]) {
+            if (whole)
+              store8_rt(a.dshift, a.p.shift_dt, (int64_t)b * a.d, 8 * c, t);
+            else
+              store8<HMOE_DT_F32>(slot, (int64_t)(nsum - 1) * a.d, 8 * c, t);
+          });
+      }
+      r0 = piece_end;
+    }
   }
   if (a.dweight) {
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const int c = threadIdx.x + kNormThreads<WPR> * i;
+      const int c = threadIdx.x + THREADS * i;
       if (c < nv) store8<HMOE_DT_F32>(a.wpart, (int64_t)blockIdx.x * a.d, 8 * c, wacc[i]);
     }
   }
@@ -661,8 +712,9 @@ __global__ __launch_bounds__(32 * SPLIT) void norm_sums_kernel(NormBwdArgs a, in
         continue;
     }
     const int64_t pitch = weight ? a.d : (int64_t)nsum * a.d;
-    const float* src = weight ? a.wpart + col : a.part + (int64_t)b * pitch + col;
+    const float* src = weight ? a.wpart + col : a.part + col;
     const bool two = !weight && nsum == 2;
+    auto slot = [&](int k) { return weight ? k : 2 * k + (k == c0); };
     float t0 = 0.0f, t1 = 0.0f;
     for (int c = c0 + ty; c <= c1; c += 8 * SPLIT) {
       float v[8], w[8];
@@ -670,8 +722,8 @@ __global__ __launch_bounds__(32 * SPLIT) void norm_sums_kernel(NormBwdArgs a, in
       for (int i = 0; i < 8; ++i) {
         const int k = c + i * SPLIT;
         const bool on = in && k <= c1;
-        v[i] = on ? src[k * pitch] : 0.0f;
-        w[i] = on && two ? src[k * pitch + a.d] : 0.0f;
+        v[i] = on ? src[slot(k) * pitch] : 0.0f;
+        w[i] = on && two ? src[slot(k) * pitch + a.d] : 0.0f;
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -801,17 +853,31 @@ static int norm_rows(int64_t T, int groups) {
   return (int)(r > 0 ? r : groups);
 }
 
+// Whether the backward's row groups take whole samples (SHORT, equal samples only): where that leaves fewer steps one after the
+// other.  A workgroup of R rows and G groups takes R / G batches of rows and R / L pieces, whose sums over the groups cost as
+// much as six batches; SHORT takes L rows for each sample of a group.  16384 x 1536, norm_in, SHORT against the other, us: L = 1
+// 158, 702; 2 85, 367; 4 60, 187; 8 47, 103; 16 44, 73; 32 68, 57; 64 121, 50.  4096 x 4096: 8 35, 71; 32 62, 56.  300 x 1536
+// in 30 samples: 27, 21.
+static bool norm_short(int64_t T, int64_t B, bool starts, int64_t R, int G) {
+  if (starts || T == 0 || B < 2) return false;
+  const int64_t L = T / B, pieces = R > L ? R / L : 1;
+  return 6 * pieces + R / G > L * ((R + G * L - 1) / (G * L));
+}
+
 static size_t norm_bwd_ws(int64_t T, int64_t d, int64_t B, int nsum, bool weight) {
   if (T < 0 || d <= 0 || B < 1) return 0;
   const int64_t R = norm_rows(T, norm_groups(d)), nchunk = (T + R - 1) / R;
-  return (size_t)((nchunk + B) * nsum + (weight ? nchunk : 0)) * (size_t)d * 4 + 16;
+  return (size_t)(2 * nchunk * nsum + (weight ? nchunk : 0)) * (size_t)d * 4 + 16;
 }
 
 template <bool OUT>
 static int norm_bwd_run(NormBwdArgs& a, int sdt, int hdt, void* workspace, size_t workspace_bytes, hipStream_t s) {
   const int nsum = (a.dscale != nullptr) + (a.dshift != nullptr);
   const int groups = norm_groups(a.d);
+  // (SHORT: whole samples, and so never more workgroups than the other form has)
   a.R = norm_rows(a.s.T, groups);
+  const bool brief = norm_short(a.s.T, a.s.B, a.s.starts != nullptr, a.R, groups);
+  if (brief) a.R = (a.R + groups * a.s.L - 1) / (groups * a.s.L) * (groups * a.s.L);
   const int nchunk = (a.s.T + a.R - 1) / a.R;
   const bool final = nsum || a.dweight;
   if (final) {
@@ -819,29 +885,34 @@ static int norm_bwd_run(NormBwdArgs& a, int sdt, int hdt, void* workspace, size_
       return HMOE_ERR_WORKSPACE;
     if (!al16(workspace)) return HMOE_ERR_ARG;
     a.part = static_cast<float*>(workspace);
-    a.wpart = a.part + (int64_t)(nchunk + a.s.B) * nsum * a.d;
+    a.wpart = a.part + (int64_t)2 * nchunk * nsum * a.d;
   }
   if (nchunk) {
     const size_t lds = final ? (size_t)groups * a.d * 4 : 0;
     by_types(sdt, hdt, [&](auto st, auto ht) {
       by_width(a.d, [&](auto v, auto w) {
         constexpr int S = decltype(st)::value, H = decltype(ht)::value, V = decltype(v)::value, W = decltype(w)::value;
+        auto launch = [&](auto kb) {
+          constexpr int KB = decltype(kb)::value;
+          if (brief)
+            hipLaunchKernelGGL((norm_bwd_kernel<KB, S, H, V, W, true>), dim3(nchunk), dim3(kNormThreads<W>), lds, s, a);
+          else
+            hipLaunchKernelGGL((norm_bwd_kernel<KB, S, H, V, W, false>), dim3(nchunk), dim3(kNormThreads<W>), lds, s, a);
+        };
         if constexpr (OUT)
-          by_slots_at_once<H, W>(a.k, [&](auto kb) {
-            hipLaunchKernelGGL((norm_bwd_kernel<decltype(kb)::value, S, H, V, W>), dim3(nchunk), dim3(kNormThreads<W>), lds,
-                               s, a);
-          });
+          by_slots_at_once<H, W>(a.k, launch);
         else
-          hipLaunchKernelGGL((norm_bwd_kernel<0, S, H, V, W>), dim3(nchunk), dim3(kNormThreads<W>), lds, s, a);
+          launch(std::integral_constant<int, 0>());
       });
     });
     HMOE_CHECK_LAUNCH();
   }
   if (final) {
-    const int items = (nsum ? a.s.B : 0) + (a.dweight ? 1 : 0);
-    // without sample sums the weight's item comes first
+    // (without sample sums to add, the weight's item comes first)
     NormBwdArgs f = a;
-    if (!nsum) f.s.B = 0;
+    if (!nsum || brief) f.s.B = 0;
+    const int items = f.s.B + (a.dweight ? 1 : 0);
+    if (items == 0) return HMOE_OK;
     const dim3 grid(items < 128 ? items : 128, (a.d + 31) / 32);
     // many parts for long sums, few where the samples span a few chunks each
     if (nchunk > 16 * a.s.B)
