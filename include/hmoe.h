@@ -101,7 +101,8 @@ int hmoe_route_sigmoid_group(const void* x, int64_t ldx, const void* wr, const f
  * An expert with the logit or the bias -inf or NaN, or outside the kept groups, is chosen only where no other is left (the
  * lowest such expert first) and has the weight 0; a NaN or +inf logit makes every softmax weight of its row NaN.
  * live (T,) bytes or NULL: a token with live = 0 (padding) gets ids -1 and weights 0 -- it routes nowhere
- * (hmoe_dispatch).  E <= 512, k <= 16, k <= E; with groups n_group <= 64, E / n_group >= group_top, k <= topk_group *
+ * (hmoe_dispatch).  For inference: hmoe_combine_bwd and hmoe_down_dgrad_swiglu_dw take the index arrays of a dispatch in
+ * which every slot named an expert (the sorted rows past the valid ones are not written).  E <= 512, k <= 16, k <= E; with groups n_group <= 64, E / n_group >= group_top, k <= topk_group *
  * E / n_group. */
 int hmoe_route_scores(const void* logits, int64_t ld, int dtype, const float* bias, const uint8_t* live, int64_t T,
                       int E, int k, int score, int n_group, int topk_group, int group_top, int renorm, float scaling,
@@ -430,8 +431,8 @@ int hmoe_norm_residual_bwd(const void* dout, int out_dtype, const void* y, const
 
 /* ---------------------------------------------------------------------------------------------------------------
  * Gradient clipping by the global norm (of the layer's gradients and any others)
- * n tensors: host arrays of their addresses, element counts and types (bf16, fp16, fp32; contiguous; aligned to an element
- * only), read during the call.  Any number of tensors: 128 travel in the arguments of a launch.
+ * n tensors that do not overlap: host arrays of their addresses, element counts and types (bf16, fp16, fp32; contiguous;
+ * aligned to an element only), read during the call.  Any number of tensors: 128 travel in the arguments of a launch.
  * ------------------------------------------------------------------------------------------------------------- */
 
 /* sq_norm (1,) fp64 = the sum of the squares of every element, in fp64 and a fixed order.  workspace:

@@ -457,6 +457,16 @@ __global__ __launch_bounds__(kNormThreads<WPR>) void norm_bwd_kernel(NormBwdArgs
     for (int e = 0; e < 8; ++e) wacc[i][e] = 0.0f;
   // adds a column sum over the row groups and hands eight columns at a time to fin(i, column vector, sums)
   auto over_groups = [&](const float (&acc)[VPL][8], auto&& fin) {
+    if constexpr (G == 1) {  // a thread's columns are its own sums
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        float t[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t[e] = acc[i][e];
+        if (lane + THREADS * i < nv) fin(i, lane + THREADS * i, t);
+      }
+      return;
+    }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
@@ -888,7 +898,7 @@ static int norm_bwd_run(NormBwdArgs& a, int sdt, int hdt, void* workspace, size_
     a.wpart = a.part + (int64_t)2 * nchunk * nsum * a.d;
   }
   if (nchunk) {
-    const size_t lds = final ? (size_t)groups * a.d * 4 : 0;
+    const size_t lds = final && groups > 1 ? (size_t)groups * a.d * 4 : 0;  // at most 48 KB
     by_types(sdt, hdt, [&](auto st, auto ht) {
       by_width(a.d, [&](auto v, auto w) {
         constexpr int S = decltype(st)::value, H = decltype(ht)::value, V = decltype(v)::value, W = decltype(w)::value;

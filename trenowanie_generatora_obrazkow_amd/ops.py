@@ -791,7 +791,9 @@ def route_scores(logits, k, score="softmax", bias=None, n_group=1, topk_group=1,
     """The k experts of each token from given logits (T, E), bf16, fp16 or fp32 -> (topk_ids (T, k) int32, topk_w (T, k)
     fp32).  score "softmax" or "sigmoid"; bias (E,) fp32 joins the scores for the selection only; topk_group < n_group keeps
     the groups with the largest sums of their group_top best values; renorm divides the weights by their sum; live (T,)
-    bool: padding tokens (False) get ids -1 and weights 0, which dispatch and moe_experts route nowhere."""
+    bool: padding tokens (False) get ids -1 and weights 0, which dispatch and moe_experts route nowhere -- for inference: the
+    experts' backward (combine_bwd, down_dgrad_swiglu_dw) takes routings that name an expert for every slot, so a training
+    step routes its padding too and gives it a zero gradient."""
     T, E, ld = _routing(logits, k, score, n_group, topk_group, group_top)
     dev = logits.device
     _on(bias, "bias", dev, (E,), (torch.float32,))
