@@ -719,13 +719,17 @@ _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device
 def _call_on(dev, name, *args):
     """A C call with its stream, launched on `dev` also where another device is the current one."""
     i = dev.index
+    f = _entry.get(name) or _entry.setdefault(name, getattr(L.lib(), name))
     if i == _current_device():
-        rc = getattr(L.lib(), name)(*args, L.stream(i))
+        rc = f(*args, L.stream(i))
     else:
         with torch.cuda.device(dev):
-            rc = getattr(L.lib(), name)(*args, L.stream(i))
+            rc = f(*args, L.stream(i))
     if rc != 0:
         raise L.HmoeError(name, rc)
+
+
+_entry = {}  # C entry points by name
 
 
 def _on(t, name, dev, shape, dtypes):
@@ -836,33 +840,34 @@ def router_wgrad(dlogits, x, dtype=torch.float32):
     return dwr
 
 
-def _sample_params(T, d, dev, starts, **mods):
-    """The number of samples B of per-sample parameters: (B, d) each, or (d,) for one set; with starts (B + 1,)."""
+def _sample_params(T, d, dev, starts, a, a_name, b=None, b_name=""):
+    """The number of samples B of per-sample parameters a and b: (B, d) each, or (d,) for one set; with starts (B + 1,)."""
+    if a is None and b is None and starts is None:
+        return 1
     B = None
-    for name, t in mods.items():
+    for t, name in ((a, a_name), (b, b_name)):
         if t is None:
             continue
-        b = 1 if t.dim() == 1 else t.shape[0]
-        _on(t, name, dev, (d,) if t.dim() == 1 else (b, d), _FLOATS)
-        if B is not None and b != B:
-            raise ValueError(f"{name} has {b} samples, another parameter {B}")
-        B = b
+        n = 1 if t.dim() == 1 else t.shape[0]
+        _on(t, name, dev, (d,) if t.dim() == 1 else (n, d), _FLOATS)
+        if B is not None and n != B:
+            raise ValueError(f"{name} has {n} samples, another parameter {B}")
+        B = n
     if starts is not None:
         n = starts.numel() - 1
         _on(starts, "starts", dev, (n + 1,), _I32)
         if n < 1 or (B is not None and B != n):
             raise ValueError(f"starts names {n} samples" + ("" if B is None else f", the parameters hold {B}"))
         return n
-    if B is None:
-        return 1
     if B < 1 or T % B:
         raise ValueError(f"{T} rows do not divide into {B} samples (pass starts for samples of unequal lengths)")
     return B
 
 
 def _block_dtype(stream, dtype):
-    dtype = stream if dtype is None else dtype
-    if dtype not in _FLOATS or (dtype != stream and stream != torch.float32):
+    if dtype is None or dtype is stream:
+        return stream
+    if dtype not in _FLOATS or stream is not torch.float32:
         raise TypeError(f"a block type of {dtype} does not go with a stream of {stream} (equal, or an fp32 stream)")
     return dtype
 
@@ -880,7 +885,7 @@ def norm_modulate(x, weight=None, scale=None, shift=None, starts=None, eps=1e-6,
     dev = x.device
     dtype = _block_dtype(x.dtype, dtype)
     _on(weight, "weight", dev, (d,), _FLOATS)
-    B = _sample_params(T, d, dev, starts, scale=scale, shift=shift)
+    B = _sample_params(T, d, dev, starts, scale, "scale", shift, "shift")
     if scale is not None and shift is not None and scale.dtype != shift.dtype:
         raise TypeError(f"scale and shift must have one type (got {scale.dtype}, {shift.dtype})")
     h = torch.empty(T, d, device=dev, dtype=dtype)
@@ -900,7 +905,7 @@ def norm_modulate_bwd(dh, x, weight=None, scale=None, shift=None, starts=None, e
     _on(dh, "dh", dev, (T, d), (_block_dtype(x.dtype, dh.dtype),))
     _on(weight, "weight", dev, (d,), _FLOATS)
     _on(dres, "dres", dev, (T, d), (x.dtype,))
-    B = _sample_params(T, d, dev, starts, scale=scale, shift=shift)
+    B = _sample_params(T, d, dev, starts, scale, "scale", shift, "shift")
     if scale is not None and shift is not None and scale.dtype != shift.dtype:
         raise TypeError(f"scale and shift must have one type (got {scale.dtype}, {shift.dtype})")
     dx = torch.empty(T, d, device=dev, dtype=x.dtype)
@@ -936,7 +941,7 @@ def norm_residual(y, x, gate=None, weight=None, norm=True, starts=None, eps=1e-6
     _block_dtype(x.dtype, y.dtype)
     _slots(y, k, T, d, dev, inv_pos, add)
     _on(weight, "weight", dev, (d,), _FLOATS)
-    B = _sample_params(T, d, dev, starts, gate=gate)
+    B = _sample_params(T, d, dev, starts, gate, "gate")
     out = torch.empty(T, d, device=dev, dtype=x.dtype)
     _call_on(dev, "hmoe_norm_residual", y.data_ptr(), L.ptr(inv_pos), k, L.ptr(add), L._DT[y.dtype], x.data_ptr(), ldx,
              L._DT[x.dtype], L.ptr(weight), _dt0(weight), L.ptr(gate), _dt0(gate), L.ptr(starts), B, T, d, int(bool(norm)),
@@ -955,7 +960,7 @@ def norm_residual_bwd(dout, y, gate=None, weight=None, norm=True, starts=None, e
     _block_dtype(dout.dtype, y.dtype)
     _slots(y, k, T, d, dev, inv_pos, add)
     _on(weight, "weight", dev, (d,), _FLOATS)
-    B = _sample_params(T, d, dev, starts, gate=gate)
+    B = _sample_params(T, d, dev, starts, gate, "gate")
     dy = torch.empty(T, d, device=dev, dtype=y.dtype)
     dw = torch.empty_like(weight) if weight is not None and "weight" in want else None
     dg = torch.empty_like(gate) if gate is not None and "gate" in want else None
