@@ -264,3 +264,18 @@ def test_step_with_clipping_eager_and_captured(kw, packed):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip([y2, n2] + gg, want)), rep
         torch.ones(64, device="cuda").sum().item()
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("T", [0, 1])
+def test_no_token_and_one(T, gated):
+    from trenowanie_generatora_obrazkow_amd import Gate
+    m = _module(4, post_norm=True, gate=Gate("sigmoid", 4, 2) if gated else None)
+    x = torch.randn(T, 128, device="cuda").requires_grad_(True)
+    y = m(x)
+    y.sum().backward()
+    assert y.shape == x.shape and x.grad.shape == x.shape
+    for p in m.parameters():
+        assert p.grad.shape == p.shape and torch.isfinite(p.grad).all() and (T > 0 or not p.grad.any())
+    with torch.no_grad():
+        assert torch.equal(m(x), y)

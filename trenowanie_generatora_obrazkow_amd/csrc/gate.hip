@@ -100,8 +100,9 @@ __device__ __forceinline__ double fma_sc(double a, double b, double c) {
 }
 
 // exp in fp64 to about 1e-14: x = n ln 2 + r (one fma: the product is exact, and ln 2 itself is off by 2e-17 n), then the
-// Taylor polynomial of degree 11 on |r| <= ln 2 / 2, whose first dropped term is below 7e-15, and the scaling by 2^n.  Finer than the 43 bits a sort key keeps, and a third of the library function's
-// instructions.  Inputs up to 1e4 in absolute value (fp32 logits beyond are clamped there: the results are 0 or inf either way).
+// Taylor polynomial of degree 11 on |r| <= ln 2 / 2, whose first dropped term is below 7e-15, and the scaling by 2^n.  Finer
+// than the 43 bits a sort key keeps, and a third of the library function's instructions.  Inputs beyond 1e4 in absolute value
+// are clamped there: the results are 0 or inf either way.
 __device__ __forceinline__ double gate_exp(double x) {
   x = dmin(dmax(x, -1e4), 1e4);
   const double n = __builtin_rint(x * 1.4426950408889634074);
