@@ -1,0 +1,20 @@
+"""Calls that the block's functions and gradient clipping have to answer or refuse and that no size or mask brings up: a single
+row whose elements are strided, clipping outputs given twice or laid over another gradient, parameters for another number of
+samples than the input holds."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def test_one_row_with_strided_elements():
+    from trenowanie_generatora_obrazkow_amd import MoEResidual, norm_modulate, norm_residual
+    g = torch.Generator().manual_seed(61)
+    x = torch.randn(1, 256, generator=g).cuda()[:, ::2]
+    y = torch.randn(1, 256, generator=g).cuda()[:, 1::2]
+    assert torch.equal(norm_modulate(x), norm_modulate(x.contiguous()))
+    assert torch.equal(norm_residual(x, y), norm_residual(x.contiguous(), y.contiguous()))
+    m = MoEResidual(128, 192, 16, 2, device="cuda")
+    for grad in (True, False):
+        with torch.set_grad_enabled(grad):
+            assert torch.equal(m(x), m(x.contiguous()))

@@ -24,7 +24,7 @@ from .layer import MoESwiGLU, _Experts, _experts_backward, _experts_forward, _ex
 def _flat(x):
     """x's rows as a matrix the kernels take: a view where its rows lie in one stride of a multiple of 8, else a copy."""
     x2 = x.reshape(-1, x.shape[-1])
-    if x2.shape[0] > 1 and (x2.stride(1) != 1 or x2.stride(0) < x2.shape[1] or x2.stride(0) % 8 or x2.data_ptr() % 16):
+    if x2.stride(1) != 1 or x2.shape[0] > 1 and (x2.stride(0) < x2.shape[1] or x2.stride(0) % 8):
         x2 = x2.contiguous()
     return x2 if x2.data_ptr() % 16 == 0 else x2.clone(memory_format=torch.contiguous_format)
 
