@@ -18,3 +18,16 @@ def test_one_row_with_strided_elements():
     for grad in (True, False):
         with torch.set_grad_enabled(grad):
             assert torch.equal(m(x), m(x.contiguous()))
+
+
+def test_outputs_beside_a_list_that_has_its_own():
+    from trenowanie_generatora_obrazkow_amd import ops
+    a, o = torch.ones(64, device="cuda"), torch.zeros(64, device="cuda")
+    gl = ops.GradList([a])
+    with pytest.raises(ValueError, match="GradList"):
+        ops.grad_clip(gl, ops.grad_sq_norm(gl), 1.0, out=[o])
+    assert (a == 1).all() and (o == 0).all()
+    gl = ops.GradList([a], [o])
+    ops.grad_clip(gl, ops.grad_sq_norm(gl), 1.0)
+    # norm 8, factor 1 / (8 + 1e-6): two fp32 roundings
+    assert (a == 1).all() and (o - 0.125).abs().max() <= 0.125 * 2.5e-7

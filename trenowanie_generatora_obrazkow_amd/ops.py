@@ -1057,7 +1057,10 @@ def grad_sq_norm(grads):
 
 def grad_clip(grads, sq_norm, max_norm, out=None):
     """Scales a list of gradients (or a GradList) by min(1, max_norm / (norm + 1e-6)), norm = sqrt(sq_norm) -- in place, or
-    into `out` (tensors of the gradients' shapes, of their types or fp32).  Returns the norm, () fp32 on the device."""
+    into `out` (tensors of the gradients' shapes, of their types or fp32; a GradList has its own).  Returns the norm, () fp32
+    on the device."""
+    if out is not None and isinstance(grads, GradList):
+        raise ValueError("a GradList holds its outputs already: pass them to GradList")
     gl = grads if isinstance(grads, GradList) else GradList(grads, out)
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
