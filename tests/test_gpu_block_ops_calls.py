@@ -29,5 +29,19 @@ def test_outputs_beside_a_list_that_has_its_own():
     assert (a == 1).all() and (o == 0).all()
     gl = ops.GradList([a], [o])
     ops.grad_clip(gl, ops.grad_sq_norm(gl), 1.0)
-    # norm 8, factor 1 / (8 + 1e-6): two fp32 roundings
+    # norm 8, factor 1 / (8 + 1e-6): 1.25e-7 below 1 / 8, and two fp32 roundings of 6e-8
     assert (a == 1).all() and (o - 0.125).abs().max() <= 0.125 * 2.5e-7
+
+
+def test_an_output_laid_over_another_gradient():
+    from trenowanie_generatora_obrazkow_amd import clip_grad_norm
+    a, b, c = (torch.full((64,), v, device="cuda") for v in (1.0, 2.0, 3.0))
+    for out in ([b, c], [c, a], [b, a]):
+        with pytest.raises(ValueError, match="another gradient"):
+            clip_grad_norm([a, b], 1.0, out=out)
+    assert (a == 1).all() and (b == 2).all() and (c == 3).all()
+    e = torch.empty(0, device="cuda")  # (no element, no overlap)
+    clip_grad_norm([a, e, e], 1e9, out=[c, e, e])
+    assert (c == 1).all()
+    clip_grad_norm([a, b], 1.0, out=[a, c])  # its own is in place
+    assert (a < 1).all() and (b == 2).all() and (c < 2).all()

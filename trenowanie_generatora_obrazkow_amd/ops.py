@@ -1004,8 +1004,12 @@ class GradList:
                                    or o.dtype not in (g.dtype, torch.float32)):
                     raise ValueError("an output has its gradient's shape and strides, and its type or fp32")
             self.out, self.odt = self._ptrs(out), self._types(out)
+            if not set(self.out).isdisjoint(self.ptr):  # (tensors without elements may share the address 0)
+                held = {p for p, n in zip(self.ptr, self.numel) if n}
+                if any(o != p and n and o in held for p, o, n in zip(self.ptr, self.out, self.numel)):
+                    raise ValueError("an output lies over another gradient")
         self.keep = (grads, out)
-        if len(set(self.out)) != self.n:  # (tensors without elements may share the address 0)
+        if len(set(self.out)) != self.n:
             used = [p for p, n in zip(self.out, self.numel) if n]
             if len(set(used)) != len(used):
                 raise ValueError("a tensor is listed twice")
