@@ -45,3 +45,23 @@ def test_an_output_laid_over_another_gradient():
     assert (c == 1).all()
     clip_grad_norm([a, b], 1.0, out=[a, c])  # its own is in place
     assert (a < 1).all() and (b == 2).all() and (c < 2).all()
+
+
+def test_parameters_of_other_samples():
+    from trenowanie_generatora_obrazkow_amd import MoEResidual, norm_modulate, norm_residual
+    r = lambda *s: torch.randn(*s, device="cuda")
+    x, m = r(2, 6, 128), MoEResidual(128, 192, 16, 2, device="cuda")
+    for n in (3, 4, 6):  # they divide the 12 rows, but not along the samples
+        for f in (lambda: norm_modulate(x, None, r(n, 128)), lambda: norm_modulate(x, None, None, r(n, 128)),
+                  lambda: norm_residual(x, x, r(n, 128)), lambda: m(x, r(n, 128)), lambda: m(x, None, None, r(n, 128))):
+            with pytest.raises(ValueError, match="leading dimensions"):
+                f()
+    for n in (1, 2, 12):  # one set, a set per sample, a set per row
+        s = r(n, 128)
+        want = norm_modulate(x.view(12, 128), None, s.repeat_interleave(12 // n, 0).contiguous()).view(2, 6, 128)
+        assert torch.equal(norm_modulate(x, None, s), want)
+    frames = r(2, 3, 2, 128)
+    for n in (1, 2, 6, 12):
+        assert norm_residual(frames, frames, r(n, 128)).shape == frames.shape
+    with pytest.raises(ValueError, match="leading dimensions"):
+        norm_residual(frames, frames, r(3, 128))

@@ -9,7 +9,8 @@ reference's denoiser block (aurora/model.py:191-210) with MoESwiGLU as its mlp.
   MoEResidual     the module
 
 Rows come as (T, d), or (..., d) with leading dimensions that are flattened; per-sample parameters are (B, d) for equal runs
-of rows -- (B, L, d) inputs -- or with starts (B + 1,) int32 for packed samples of unequal lengths, (d,) for all rows.
+of rows -- (B, L, d) inputs, whose first dimensions they have to match -- or with starts (B + 1,) int32 for packed samples of
+unequal lengths, (d,) for all rows.
 Rows outside the samples are padding: their residual passes through and nothing else does."""
 from __future__ import annotations
 
@@ -37,6 +38,20 @@ def _dense(t):
 
 def _par(t):
     return None if t is None else _dense(t.detach())
+
+
+def _check_samples(x, starts, **params):
+    """Refuses parameters whose samples are not x's: for (B, L, d) one set, B, or one for each of the B * L rows."""
+    if starts is not None or x.dim() < 3:
+        return
+    for name, p in params.items():
+        if p is not None and p.dim() == 2 and p.shape[0] != x.shape[0]:
+            n, runs = 1, {1}
+            for s in x.shape[:-1]:
+                n *= s
+                runs.add(n)
+            if p.shape[0] not in runs:
+                raise ValueError(f"{name} {tuple(p.shape)} does not go with the leading dimensions of x {tuple(x.shape)}")
 
 
 def _want(*flags):
@@ -88,6 +103,7 @@ class _NormResidual(torch.autograd.Function):
 def norm_modulate(x, weight=None, scale=None, shift=None, starts=None, eps=1e-6, dtype=None):
     """h = n * weight * (1 + scale_b) + shift_b with n = x / sqrt(mean(x^2) + eps), of x's shape: ops.norm_modulate with
     gradients to x, weight, scale and shift."""
+    _check_samples(x, starts, scale=scale, shift=shift)
     return _NormModulate.apply(x, weight, scale, shift, starts, eps, dtype)
 
 
@@ -96,6 +112,7 @@ def norm_residual(x, y, gate=None, weight=None, norm=True, starts=None, eps=1e-6
     ops.norm_residual for one slot with gradients to x, y, gate and weight."""
     if x.shape != y.shape:
         raise ValueError(f"x {tuple(x.shape)} and y {tuple(y.shape)} must have one shape")
+    _check_samples(x, starts, gate=gate)
     return _NormResidual.apply(x, y, gate, weight, norm, starts, eps, alpha)
 
 
@@ -177,6 +194,7 @@ class MoEResidual(nn.Module):
         self.post_weight = nn.Parameter(torch.ones(dim, **f)) if affine and post_norm else None
 
     def forward(self, x, scale=None, shift=None, gate=None, starts=None):
+        _check_samples(x, starts, scale=scale, shift=shift, gate=gate)
         m = self.mlp
         out, ids, tw = moe_residual(x.reshape(-1, x.shape[-1]), m.router_weight, m.w_gu, m.w_d, m.top_k, self.norm_weight,
                                     scale, shift, self.post_weight, gate, self.post_norm, starts, self.eps, self.alpha,
