@@ -389,8 +389,9 @@ int hmoe_router_wgrad(const float* dlogits, const void* x, int64_t ldx, int64_t 
  * an fp32 stream around a 16-bit block.  Per-sample parameters (B, d): without starts, T / B consecutive rows belong to
  * each sample (B = 1: one set for all rows); with starts (B + 1,) int32, ascending, rows starts[b] .. starts[b + 1] - 1
  * belong to sample b (which may be empty) and rows outside [starts[0], starts[B]) are padding.  Parameters are bf16, fp16 or
- * fp32, each with its own type.  Statistics, sums and products are fp32, every output is rounded once.  d % 8 == 0,
- * d <= 16384, ldx % 8 == 0, 16-byte aligned pointers.
+ * fp32, each with its own type.  Statistics, sums and products are fp32, every output is rounded once: a row's sum of squares
+ * and, in the backward, sum of upstream times row have to lie in fp32's range.  d % 8 == 0, d <= 16384, ldx % 8 == 0, 16-byte
+ * aligned pointers.
  * ------------------------------------------------------------------------------------------------------------- */
 
 /* h = n * weight * (1 + scale_b) + shift_b with n = x / sqrt(mean(x^2) + eps); each of the three optional (NULL); 0 on

@@ -552,11 +552,12 @@ __global__ __launch_bounds__(kNormThreads<WPR>) void norm_bwd_kernel(NormBwdArgs
         dot += u[i][e] * wm[i][e] * v[i][e];
       }
     }
-    float rms = 1.0f, proj = 0.0f;  // proj = r^3 mean(g v): dv = r g - v proj
+    // (n = v r and mean(g n) before r again: r^3 and v r^3 would leave fp32's range for rows past 1e13 or rms below 1e-13)
+    float rms = 1.0f, mean = 0.0f;  // mean(g n): dv = r (g - n mean)
     if (a.norm) {
       row_sum2<WPR>(sq, dot, red, half);
       rms = inv_rms(sq, a.d, a.eps);
-      proj = rms * rms * rms * (dot / (float)a.d);
+      mean = dot * rms / (float)a.d;
     }
     if (!row) return;
 #pragma unroll
@@ -568,10 +569,10 @@ __global__ __launch_bounds__(kNormThreads<WPR>) void norm_bwd_kernel(NormBwdArgs
       v[i].hold();
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float ue = u[i][e], ve = v[i][e];
-        aacc[i][e] += ue * (ve * rms);
+        const float ue = u[i][e], n = v[i][e] * rms;
+        aacc[i][e] += ue * n;
         if constexpr (!OUT) sacc[i][e] += ue;
-        t[e] = rms * (ue * wm[i][e]) - ve * proj;
+        t[e] = rms * (ue * wm[i][e] - n * mean);
       }
       if constexpr (!OUT)
         if (a.dres) {
