@@ -572,7 +572,8 @@ __global__ __launch_bounds__(kNormThreads<WPR>) void norm_bwd_kernel(NormBwdArgs
         const float ue = u[i][e], n = v[i][e] * rms;
         aacc[i][e] += ue * n;
         if constexpr (!OUT) sacc[i][e] += ue;
-        t[e] = rms * (ue * wm[i][e] - n * mean);
+        const float ge = ue * wm[i][e];
+        t[e] = a.norm ? rms * (ge - n * mean) : ge;  // (without the norm the row, which may be inf or NaN, has no part)
       }
       if constexpr (!OUT)
         if (a.dres) {
