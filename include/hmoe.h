@@ -370,8 +370,8 @@ int hmoe_unpermute_bwd_split(const float* dxs, int parts, const int32_t* inv_pos
 
 /* Backward of hmoe_route_scores: dlogits (T, E), contiguous, of the logits' type, from dtopk_w (T, k) fp32; topk_ids and
  * topk_w as the forward wrote them.  The selection is constant; the gradient goes through the chosen scores and the
- * renormalisation, for softmax on to every logit.  Slots with an id outside [0, E) or the weight 0 have none; an expert
- * that several slots name gets their sum. */
+ * renormalisation, for softmax on to every logit.  Slots with an id outside [0, E) or the weight 0 have none; a token with no
+ * other slot (padding) gets zeros, whatever its logits and dtopk_w hold; an expert that several slots name gets their sum. */
 int hmoe_route_scores_bwd(const float* dtopk_w, const float* topk_w, const void* logits, int64_t ld, int dtype,
                           const int32_t* topk_ids, int64_t T, int E, int k, int score, int renorm, float scaling,
                           void* dlogits, hmoe_stream_t stream);

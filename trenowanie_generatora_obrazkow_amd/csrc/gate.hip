@@ -362,7 +362,7 @@ struct GateBwdArgs {
 // dlogits of the slots' weights w_j = c s_j / (sum s + 1e-20) (renorm) or c s_j: with u_j = c dw_j,
 // ds_j = (u_j - (sum u s) / den) / den or u_j; sigmoid dl_e = ds s (1 - s) at the chosen experts, softmax
 // dl_e = p_e (ds_e - sum_j p_j ds_j) at every expert.  A slot with an id outside [0, E) or the weight 0 (no expert was
-// left for it) has no gradient; an expert named by several slots gets their sum.
+// left for it) has no gradient, a token without any other slot zeros; an expert named by several slots gets their sum.
 template <int EPL, bool SIG>
 __global__ __launch_bounds__(256) void route_scores_bwd_kernel(GateBwdArgs b) {
   constexpr int W = 4;
@@ -422,11 +422,13 @@ __global__ __launch_bounds__(256) void route_scores_bwd_kernel(GateBwdArgs b) {
   if (e >= 0) atomicAdd(&dp[e], ds * slope);
   wave_lds_sync();
   const float inv = S == 0.0f ? 0.0f : 1.0f / S;
+  // (a token none of whose slots counts, as padding does, has a zero gradient whatever its logits are)
+  const bool any = __ballot(e >= 0) >> (16 * seg) & 0xffff;
   float d[EPL];
 #pragma unroll
   for (int i = 0; i < EPL; ++i) {
     d[i] = dp[16 * i + j];
-    if constexpr (!SIG) d[i] = lg[i] * inv * (d[i] - pdp);
+    if constexpr (!SIG) d[i] = any ? lg[i] * inv * (d[i] - pdp) : 0.0f;
   }
   if (!real) return;
   if (a.dt == HMOE_DT_F32) {
