@@ -12,6 +12,7 @@ import torch
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "libhmoe.so")
 
+ERR_OVERLAP = -8
 DT_BF16, DT_F16, DT_F32, DT_I32, DT_I64, DT_I8 = 0, 1, 2, 3, 4, 5
 _DT = {torch.bfloat16: DT_BF16, torch.float16: DT_F16, torch.float32: DT_F32, torch.int32: DT_I32,
        torch.int64: DT_I64, torch.int8: DT_I8}

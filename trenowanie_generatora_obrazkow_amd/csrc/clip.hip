@@ -2,7 +2,9 @@
 // and are bound by that.
 #include "hmoe_common.h"
 
+#include <algorithm>
 #include <cmath>
+#include <cstdlib>
 
 namespace hmoe {
 
@@ -157,7 +159,7 @@ __global__ __launch_bounds__(256) void clip_scale_kernel(ClipList l, const doubl
     const int ti = clip_tensor(l, c);
     const void* p = l.p[ti];
     void* o = l.o[ti];
-    if (p == o && coef == 1.0f) continue;  // nothing to change in place
+    if (p == o && coef == 1.0f) continue;  // nothing to change in place (one address: one type, clip_overlap)
     const int64_t i0 = (int64_t)(c - l.first[ti]) * kClipChunk, i1 = min(l.n[ti], i0 + kClipChunk);
     clip_by_type(l.dt[ti] & 15, [&](auto dt) {
       constexpr int DT = decltype(dt)::value;
@@ -236,6 +238,43 @@ static int clip_list(const void* const* grads, void* const* out, const int64_t* 
   return HMOE_OK;
 }
 
+// Whether a tensor that is written lies over any other of the call (its own gradient at the same address and of the same type
+// is in place).  Workgroups walk the chunks in any order, so such a call would race.  Listed in the order of their addresses,
+// as views of a bucket are, the tensors need no sorting; 300 of them take 1 us then.  -1: no host memory to look.
+struct ClipSpan {
+  uintptr_t first, end;
+  bool written;
+};
+static int clip_overlap(const void* const* grads, void* const* out, const int64_t* numel, const int* dtypes,
+                        const int* out_dtypes, int n) {
+  ClipSpan few[1024];
+  ClipSpan* s = n <= 512 ? few : static_cast<ClipSpan*>(std::malloc(2 * (size_t)n * sizeof(ClipSpan)));
+  if (!s) return -1;
+  int m = 0;
+  bool sorted = true;
+  auto put = [&](const void* p, int64_t bytes, bool written) {
+    const uintptr_t first = reinterpret_cast<uintptr_t>(p);
+    sorted = sorted && (m == 0 || s[m - 1].first <= first);
+    s[m++] = {first, first + (uintptr_t)bytes, written};
+  };
+  for (int i = 0; i < n; ++i) {
+    if (numel[i] == 0) continue;
+    const bool own = grads[i] == out[i] && dtypes[i] == out_dtypes[i];
+    if (!own) put(grads[i], numel[i] * (dtypes[i] == HMOE_DT_F32 ? 4 : 2), false);
+    put(out[i], numel[i] * (out_dtypes[i] == HMOE_DT_F32 ? 4 : 2), true);
+  }
+  if (!sorted) std::sort(s, s + m, [](const ClipSpan& a, const ClipSpan& b) { return a.first < b.first; });
+  uintptr_t any = 0, written = 0;  // ends of what came before
+  int over = 0;
+  for (int i = 0; i < m && !over; ++i) {
+    over = s[i].first < (s[i].written ? any : written);
+    any = std::max(any, s[i].end);
+    if (s[i].written) written = std::max(written, s[i].end);
+  }
+  if (s != few) std::free(s);
+  return over;
+}
+
 static unsigned clip_grid(const ClipList& l) {
   const uint32_t c = l.first[l.count];
   return c < kClipBlocks ? c : kClipBlocks;
@@ -295,6 +334,10 @@ int hmoe_grad_clip(const void* const* grads, void* const* out, const int64_t* nu
   for (int i = 0; i < n;) {
     rc = clip_list(grads, out, numel, dtypes, out_dtypes, n, i, l);
     if (rc) return rc;
+  }
+  if (n > 0) {
+    const int over = clip_overlap(grads, out, numel, dtypes, out_dtypes, n);
+    if (over) return over < 0 ? HMOE_ERR_WORKSPACE : HMOE_ERR_OVERLAP;
   }
   bool first = true;
   int i = 0;

@@ -2101,6 +2101,7 @@ const char* hmoe_error_string(int code) {
     case HMOE_ERR_DEVICE: return "device query failed";
     case HMOE_ERR_TOO_LARGE:
       return "input too large for the fixed device scratch of an allocation-free entry point (use the workspace form)";
+    case HMOE_ERR_OVERLAP: return "a tensor to be written lies over another tensor of the call";
     default: return "unknown error";
   }
 }

@@ -332,7 +332,7 @@ def moe_param_groups(module: nn.Module, lr: float, weight_decay: float, router_l
 def clip_grad_norm(grads, max_norm, out=None):
     """Clips a list of gradient tensors by their global norm: each becomes itself times min(1, max_norm / (norm + 1e-6)), in
     place, or in `out` (tensors of the same shapes and strides, of the gradients' types or fp32, such as an optimizer's fp32
-    gradients; the gradients then stay as they are).  The tensors of a call do not overlap.  bf16, fp16 and fp32 tensors of
+    gradients; the gradients then stay as they are).  Tensors written by a call that overlap others of it are refused.  bf16, fp16 and fp32 tensors of
     any size and alignment may be mixed, None entries are skipped.  Returns the norm before clipping, a () fp32 tensor on the
     device; nothing waits for the GPU.
     A gradient spread over several processes: all-reduce ops.grad_sq_norm's sum before ops.grad_clip."""

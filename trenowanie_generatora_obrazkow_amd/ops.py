@@ -1061,8 +1061,8 @@ def grad_sq_norm(grads):
 
 def grad_clip(grads, sq_norm, max_norm, out=None):
     """Scales a list of gradients (or a GradList) by min(1, max_norm / (norm + 1e-6)), norm = sqrt(sq_norm) -- in place, or
-    into `out` (tensors of the gradients' shapes, of their types or fp32; a GradList has its own).  Returns the norm, () fp32
-    on the device."""
+    into `out` (tensors of the gradients' shapes, of their types or fp32; a GradList has its own).  Outputs that overlap each
+    other, another gradient or their own in another type are refused.  Returns the norm, () fp32 on the device."""
     if out is not None and isinstance(grads, GradList):
         raise ValueError("a GradList holds its outputs already: pass them to GradList")
     gl = grads if isinstance(grads, GradList) else GradList(grads, out)
@@ -1073,6 +1073,12 @@ def grad_clip(grads, sq_norm, max_norm, out=None):
     _on(sq_norm, "sq_norm", dev if gl.device is None else gl.device, (1,), (torch.float64,))
     L.require_gpu(sq_norm, "sq_norm")
     norm = torch.empty((), device=dev, dtype=torch.float32)
-    _call_on(dev, "hmoe_grad_clip", _addr(gl.ptr), _addr(gl.out), _addr(gl.numel), _addr(gl.dt), _addr(gl.odt), gl.n,
-             sq_norm.data_ptr(), max_norm, norm.data_ptr())
+    try:
+        _call_on(dev, "hmoe_grad_clip", _addr(gl.ptr), _addr(gl.out), _addr(gl.numel), _addr(gl.dt), _addr(gl.odt), gl.n,
+                 sq_norm.data_ptr(), max_norm, norm.data_ptr())
+    except L.HmoeError as e:
+        if e.code != L.ERR_OVERLAP:
+            raise
+        raise ValueError("a tensor to be written lies over another gradient or output of the call, or over its own gradient "
+                         "in another type") from e
     return norm
