@@ -116,15 +116,17 @@ def _experts_forward(x, wr, wgu, wd, bias, k, renorm, gate, select_bias, need_gr
     y, _ = ops.down_scatter(act, wd, disp.counts, M, disp.w_sorted, disp.order)
     state = None
     if need_grad:
-        state = _Experts((x, wr, wgu, wd, logits, ids, disp.counts, disp.order, disp.a_idx, disp.inv_pos, disp.w_sorted,
-                          disp.xs, gu, act, tw), k, renorm, gate, select_bias is not None, w_dtypes)
+        saved = (x, wr, wgu, wd, logits, ids, disp.counts, disp.order, disp.a_idx, disp.inv_pos, disp.w_sorted, disp.xs, gu, act)
+        if gate is not None or select_bias is not None:  # (else not kept: a program may change the weights in place)
+            saved += (tw,)
+        state = _Experts(saved, k, renorm, gate, select_bias is not None, w_dtypes)
     return y, ids, tw, state
 
 
 def _experts_backward(state, dout, dtw_out, need_x, need_wr, need_wgu, need_wd):
     """(dx, dwr, dwgu, dwd), None where not needed, from dout (T, d) bf16, the gradient of every slot of y, and dtw_out
     (T, k), that of the returned weights, or None."""
-    x, wr, wgu, wd, logits, ids, counts, order, a_idx, inv_pos, w_sorted, xs, gu, act, tw = state.saved
+    x, wr, wgu, wd, logits, ids, counts, order, a_idx, inv_pos, w_sorted, xs, gu, act, *tw = state.saved
     k = state.k
     T = x.shape[0]
     E = wgu.shape[0]
@@ -149,7 +151,7 @@ def _experts_backward(state, dout, dtw_out, need_x, need_wr, need_wgu, need_wd):
         dl, dwr = ops.router_bwd(logits, ids, dtw, x, renorm=state.renorm, dwr_dtype=_grad_dtype(wr_dt), want_dwr=need_wr)
     else:
         g = state.gate or Gate()
-        dl = ops.route_scores_bwd(dtw, tw, logits, ids, g.score, state.renorm, g.scaling)
+        dl = ops.route_scores_bwd(dtw, tw[0], logits, ids, g.score, state.renorm, g.scaling)
         dwr = ops.router_wgrad(dl, x, dtype=_grad_dtype(wr_dt)) if need_wr else None
     dwr = _to_param(dwr, wr_dt)
     dx = ops.unpermute_bwd(dxs, inv_pos, T, k, dlogits=dl, wr=wr) if need_x else None
