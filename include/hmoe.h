@@ -445,7 +445,8 @@ int hmoe_grad_sq_norm(const void* const* grads, const int64_t* numel, const int*
 
 /* out[i] = grads[i] * min(1, max_norm / (norm + 1e-6)) with norm = sqrt(sq_norm): the product in fp32, rounded once.  out[i]
  * has grads[i]'s type or is fp32 (out_dtypes) and may be grads[i] itself (left as it is where the factor is 1).  A NaN
- * sq_norm makes every output NaN, an infinite one zeros (NaN where a gradient is infinite).  norm (1,) fp32 or NULL.  sq_norm
+ * sq_norm makes every output NaN, an infinite one zeros (NaN where a gradient is infinite) unless max_norm is
+ * infinite too, which leaves the factor 1.  norm (1,) fp32 or NULL.  sq_norm
  * is read on the device, so gradients spread over several processes can sum it between the two calls.  max_norm >= 0.
  * An output that lies over another output, over another gradient or otherwise than in place over its own (another start or
  * type) is refused with HMOE_ERR_OVERLAP before anything is launched (host memory for the check beyond 512 tensors:
@@ -453,6 +454,10 @@ int hmoe_grad_sq_norm(const void* const* grads, const int64_t* numel, const int*
 int hmoe_grad_clip(const void* const* grads, void* const* out, const int64_t* numel, const int* dtypes,
                    const int* out_dtypes, int n, const double* sq_norm, float max_norm, float* norm,
                    hmoe_stream_t stream);
+/* The same with an fp64 bound: the factor is formed from it in fp64 and rounded once to fp32. */
+int hmoe_grad_clip_f64(const void* const* grads, void* const* out, const int64_t* numel, const int* dtypes,
+                       const int* out_dtypes, int n, const double* sq_norm, double max_norm, float* norm,
+                       hmoe_stream_t stream);
 
 #ifdef __cplusplus
 }

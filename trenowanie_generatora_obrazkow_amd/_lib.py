@@ -21,6 +21,7 @@ _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I32 = ctypes.c_int
 _F32 = ctypes.c_float
+_F64 = ctypes.c_double
 _SZ = ctypes.c_size_t
 
 # name -> (restype, argtypes); mirrors include/hmoe.h
@@ -88,6 +89,7 @@ SIGNATURES = {
     "hmoe_grad_sq_norm_workspace_size": (_SZ, [_I32]),
     "hmoe_grad_sq_norm": (_I32, [_P, _P, _P, _I32, _P, _P, _SZ, _P]),
     "hmoe_grad_clip": (_I32, [_P, _P, _P, _P, _P, _I32, _P, _F32, _P, _P]),
+    "hmoe_grad_clip_f64": (_I32, [_P, _P, _P, _P, _P, _I32, _P, _F64, _P, _P]),
 }
 
 _lib = None

@@ -141,15 +141,15 @@ __global__ __launch_bounds__(256) void clip_total_kernel(const double* part, int
   if (threadIdx.x == 0) *sq = acc;
 }
 
-__device__ __forceinline__ float clip_coef(double norm, float max_norm) {
-  const double c = (double)max_norm / (norm + 1e-6);
+__device__ __forceinline__ float clip_coef(double norm, double max_norm) {
+  const double c = max_norm / (norm + 1e-6);
   return c < 1.0 ? (float)c : norm == norm ? 1.0f : __builtin_nanf("");
 }
 
 // out = grad * factor, from the back of the list: what the norm read last may still lie in the 256 MB cache (98.6M fp32
 // elements 137.5 us against 142).  Eight vectors a thread on their way: 302M bf16 elements into fp32 338 us (5.3 TB/s) against
 // 361 with four and 369 with one.
-__global__ __launch_bounds__(256) void clip_scale_kernel(ClipList l, const double* sq, float max_norm, float* norm_out) {
+__global__ __launch_bounds__(256) void clip_scale_kernel(ClipList l, const double* sq, double max_norm, float* norm_out) {
   const double norm = sqrt(*sq);
   if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
   const float coef = clip_coef(norm, max_norm);
@@ -323,12 +323,12 @@ int hmoe_grad_sq_norm(const void* const* grads, const int64_t* numel, const int*
   return HMOE_OK;
 }
 
-int hmoe_grad_clip(const void* const* grads, void* const* out, const int64_t* numel, const int* dtypes,
-                   const int* out_dtypes, int n, const double* sq_norm, float max_norm, float* norm,
-                   hmoe_stream_t stream) {
+int hmoe_grad_clip_f64(const void* const* grads, void* const* out, const int64_t* numel, const int* dtypes,
+                       const int* out_dtypes, int n, const double* sq_norm, double max_norm, float* norm,
+                       hmoe_stream_t stream) {
   int rc = clip_check(grads, numel, dtypes, n);
   if (rc) return rc;
-  if (!sq_norm || (n > 0 && (!out || !out_dtypes)) || !(max_norm >= 0.0f)) return HMOE_ERR_ARG;
+  if (!sq_norm || (n > 0 && (!out || !out_dtypes)) || !(max_norm >= 0.0)) return HMOE_ERR_ARG;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   ClipList l;
   for (int i = 0; i < n;) {
@@ -351,6 +351,12 @@ int hmoe_grad_clip(const void* const* grads, void* const* out, const int64_t* nu
     first = false;
   } while (i < n);
   return HMOE_OK;
+}
+
+int hmoe_grad_clip(const void* const* grads, void* const* out, const int64_t* numel, const int* dtypes,
+                   const int* out_dtypes, int n, const double* sq_norm, float max_norm, float* norm,
+                   hmoe_stream_t stream) {
+  return hmoe_grad_clip_f64(grads, out, numel, dtypes, out_dtypes, n, sq_norm, (double)max_norm, norm, stream);
 }
 
 }  // extern "C"

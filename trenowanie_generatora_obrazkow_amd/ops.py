@@ -1074,8 +1074,8 @@ def grad_clip(grads, sq_norm, max_norm, out=None):
     L.require_gpu(sq_norm, "sq_norm")
     norm = torch.empty((), device=dev, dtype=torch.float32)
     try:
-        _call_on(dev, "hmoe_grad_clip", _addr(gl.ptr), _addr(gl.out), _addr(gl.numel), _addr(gl.dt), _addr(gl.odt), gl.n,
-                 sq_norm.data_ptr(), max_norm, norm.data_ptr())
+        _call_on(dev, "hmoe_grad_clip_f64", _addr(gl.ptr), _addr(gl.out), _addr(gl.numel), _addr(gl.dt), _addr(gl.odt),
+                 gl.n, sq_norm.data_ptr(), max_norm, norm.data_ptr())
     except L.HmoeError as e:
         if e.code != L.ERR_OVERLAP:
             raise
