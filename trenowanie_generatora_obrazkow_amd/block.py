@@ -19,7 +19,7 @@ import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
 from . import ops
-from .layer import MoESwiGLU, _Experts, _experts_backward, _experts_forward, _experts_infer
+from .layer import MoESwiGLU, _Experts, _experts_backward, _experts_forward, _experts_infer, _recorded
 
 
 def _flat(x):
@@ -166,8 +166,7 @@ def moe_residual(x, router_weight, w_gu, w_d, top_k, pre_weight=None, scale=None
     norm_modulate's and norm_residual's."""
     if x.dim() != 2 or x.dtype not in (torch.bfloat16, torch.float32):
         raise TypeError(f"x must be a (T, d) matrix in bf16 or fp32 (got {tuple(x.shape)} {x.dtype})")
-    tensors = (x, router_weight, w_gu, w_d, pre_weight, scale, shift, post_weight, gate)
-    if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)):
+    if not _recorded(x, router_weight, w_gu, w_d, pre_weight, scale, shift, post_weight, gate):
         x2 = _flat(x)
         h = ops.norm_modulate(x2, _par(pre_weight), _par(scale), _par(shift), starts, eps, torch.bfloat16)
         y, ids, tw, inv = _experts_infer(h, router_weight, w_gu, w_d, logit_bias, top_k, renorm, router, select_bias)

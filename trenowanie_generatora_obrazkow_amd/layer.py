@@ -21,6 +21,7 @@ from __future__ import annotations
 from dataclasses import dataclass, replace
 
 import torch
+import torch.autograd.forward_ad as fwd
 import torch.nn as nn
 
 from . import ops
@@ -61,6 +62,14 @@ def _check_layer_args(x, wr, wgu, wd, bias, k):
 
 def _bf16(t):
     return t if t.dtype == torch.bfloat16 else t.to(torch.bfloat16)
+
+
+def _recorded(*tensors):
+    """Whether a call has to go through its autograd node: it has a gradient to record, or an input with a forward-mode
+    tangent, which the nodes refuse (the one-call forms would drop it)."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return True
+    return fwd._current_level >= 0 and any(t is not None and fwd.unpack_dual(t).tangent is not None for t in tensors)
 
 
 @dataclass(frozen=True)
@@ -196,8 +205,7 @@ def moe_swiglu(x, router_weight, w_gu, w_d, top_k, logit_bias=None, renorm=True,
     gradient to record (grad mode off, or no input requiring one) the forward runs as one C call
     (ops.moe_forward; with a gate or a selection bias, the routing and ops.moe_experts): the same kernels and outputs, a
     fraction of the host time."""
-    if not (torch.is_grad_enabled() and (x.requires_grad or router_weight.requires_grad or w_gu.requires_grad
-                                         or w_d.requires_grad)):
+    if not _recorded(x, router_weight, w_gu, w_d):
         if gate is None and select_bias is None:
             _check_layer_args(x, router_weight, w_gu, w_d, logit_bias, top_k)
             out, ids, tw, _ = ops.moe_forward(x, _bf16(router_weight), _bf16(w_gu), _bf16(w_d), top_k, bias=logit_bias,
