@@ -830,13 +830,14 @@ def router_wgrad(dlogits, x, dtype=torch.float32):
     """dwr (E, d) = dlogits^T @ x from the logits' gradient (T, E) fp32 and x (T, d) bf16; fp32 or bf16."""
     T, E = dlogits.shape
     d = x.shape[1]
-    _need(dlogits, "dlogits", (T, E), (torch.float32,))
     _need(x, "x", (T, d), _BF16, contig=False)
-    dwr = torch.empty(E, d, device=x.device, dtype=dtype)
+    dev = x.device
+    _on(dlogits, "dlogits", dev, (T, E), (torch.float32,))
+    dwr = torch.empty(E, d, device=dev, dtype=dtype)
     ws_bytes = L.lib().hmoe_router_bwd_workspace_size(T, E, d)
-    ws = torch.empty(ws_bytes, device=x.device, dtype=torch.uint8)
-    L.call("hmoe_router_wgrad", L.ptr(dlogits), L.ptr(x), x.stride(0), T, E, d, L.ptr(dwr), L.dt(dwr), L.ptr(ws), ws_bytes,
-           _dev_stream(x))
+    ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
+    _call_on(dev, "hmoe_router_wgrad", L.ptr(dlogits), L.ptr(x), x.stride(0), T, E, d, L.ptr(dwr), L.dt(dwr), L.ptr(ws),
+             ws_bytes)
     return dwr
 
 
