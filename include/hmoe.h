@@ -433,21 +433,23 @@ int hmoe_norm_residual_bwd(const void* dout, int out_dtype, const void* y, const
 
 /* ---------------------------------------------------------------------------------------------------------------
  * Gradient clipping by the global norm (of the layer's gradients and any others)
- * n tensors that do not overlap: host arrays of their addresses, element counts and types (bf16, fp16, fp32; contiguous;
+ * n tensors: host arrays of their addresses, element counts and types (bf16, fp16, fp32; contiguous;
  * aligned to an element only), read during the call.  Any number of tensors: 128 travel in the arguments of a launch.
  * ------------------------------------------------------------------------------------------------------------- */
 
-/* sq_norm (1,) fp64 = the sum of the squares of every element, in fp64 and a fixed order.  workspace:
- * hmoe_grad_sq_norm_workspace_size(n) bytes, 8-byte aligned. */
+/* sq_norm (1,) fp64 = the sum of the squares of every element, in fp64, in an order that is fixed for one list at one set of
+ * addresses (tensors that follow each other in memory are walked as one): at other addresses the last bits may differ, so
+ * processes that hold copies of the same gradients and have to stay equal share one sq_norm.  Only read: tensors may overlap
+ * here.  workspace: hmoe_grad_sq_norm_workspace_size(n) bytes, 8-byte aligned. */
 size_t hmoe_grad_sq_norm_workspace_size(int n);
 int hmoe_grad_sq_norm(const void* const* grads, const int64_t* numel, const int* dtypes, int n, double* sq_norm,
                       void* workspace, size_t workspace_bytes, hmoe_stream_t stream);
 
 /* out[i] = grads[i] * min(1, max_norm / (norm + 1e-6)) with norm = sqrt(sq_norm): the product in fp32, rounded once.  out[i]
  * has grads[i]'s type or is fp32 (out_dtypes) and may be grads[i] itself (left as it is where the factor is 1).  A NaN
- * sq_norm makes every output NaN, an infinite one zeros (NaN where a gradient is infinite) unless max_norm is
- * infinite too, which leaves the factor 1.  norm (1,) fp32 or NULL.  sq_norm
- * is read on the device, so gradients spread over several processes can sum it between the two calls.  max_norm >= 0.
+ * sq_norm makes every output NaN, an infinite one zeros (NaN where a gradient is infinite) unless max_norm is infinite
+ * too, which leaves the factor 1.  norm (1,) fp32 or NULL.  sq_norm is read on the device, so gradients spread over several
+ * processes can sum it between the two calls.  max_norm >= 0.
  * An output that lies over another output, over another gradient or otherwise than in place over its own (another start or
  * type) is refused with HMOE_ERR_OVERLAP before anything is launched (host memory for the check beyond 512 tensors:
  * HMOE_ERR_WORKSPACE without it). */

@@ -109,7 +109,8 @@ def norm_modulate(x, weight=None, scale=None, shift=None, starts=None, eps=1e-6,
 
 def norm_residual(x, y, gate=None, weight=None, norm=True, starts=None, eps=1e-6, alpha=1.0):
     """alpha * x + gate_b * weight * n with n = y / sqrt(mean(y^2) + eps) (y itself without norm), of x's shape and type:
-    ops.norm_residual for one slot with gradients to x, y, gate and weight."""
+    ops.norm_residual for one slot with gradients to x, y, gate and weight.  (The stream x comes first here, the block's output
+    y in ops.norm_residual.)"""
     if x.shape != y.shape:
         raise ValueError(f"x {tuple(x.shape)} and y {tuple(y.shape)} must have one shape")
     _check_samples(x, starts, gate=gate)
@@ -181,7 +182,8 @@ class MoEResidual(nn.Module):
     second half of a denoiser block, its modulation (scale, shift, gate: (B, d) each) from outside.  norm_weight and, with
     post_norm, post_weight are learned (ones at first; affine=False: none).  x (B, L, d), or packed rows (T, d) with starts, in
     bf16 or fp32; the output has its shape and type.  The routing of the last call is kept in mlp.last_topk_ids /
-    mlp.last_topk_weight."""
+    mlp.last_topk_weight, padding rows included: all of them have h = 0 and so the same experts.  mlp holds the parameters and is
+    not called: hooks on it do not run, and what gathers sharded weights wraps this module, not mlp."""
 
     def __init__(self, dim: int, hidden: int, experts: int, top_k: int = 2, post_norm: bool = False, affine: bool = True,
                  eps: float = 1e-6, alpha: float = 1.0, device=None, norm_dtype=torch.float32, **mlp):

@@ -8,7 +8,7 @@ namespace hmoe {
 // What bounds it: the selection's instructions (an fp64 score per expert, the sorting network) and their latency; the logits
 // are read once, 8 MB at 8192 x 256, 2 us at the rate of a large copy.  Sixteen lanes a token: a wave's exchanges stay inside
 // rows of 16 lanes (DPP), and four tokens share every instruction.  8192 tokens, 256 experts in 8 groups, top-8, sigmoid with
-// bias: 10.9 us; with the library's exp and division and the options branched on per element 15.1.  The best k of E by a
+// bias: 11.0 us; with the library's exp and division and the options branched on per element 15.1.  The best k of E by a
 // sorting network and four merges of lists across the lanes, not by k rounds of arg-max: those cost about 110 instructions
 // each, the network 38 and a merge 55 for lists of eight.
 constexpr int kGateMaxE = 512, kGateMaxK = 16, kGateMaxGroups = 64;

@@ -1,8 +1,8 @@
 // The norms around the routed block, with their C entry points: the RMS norm before it with weight and per-sample
 // scale / shift, and the sum over the routed slots, RMS norm, gate and scaled residual after it; both with backward.
 // A few operations per element: every kernel here is bound by the rows it reads and writes.  16384 x 1536 bf16, 4 samples:
-// norm_in 23.1 us forward (101 MB, 4.4 TB/s), 36.8 backward (201 MB, 5.5 TB/s) and 4.6 for the sums; norm_out with two slots
-// 43.9 (201 MB, 4.6 TB/s), 36.1 (201 MB, 5.6 TB/s) and 5.2.  A copy of 2 GB runs at 5.1 TB/s.
+// norm_in 22.9 us forward (101 MB, 4.4 TB/s), 36.4 backward (201 MB, 5.5 TB/s) and 4.7 for the sums; norm_out with two slots
+// 44.2 (201 MB, 4.6 TB/s), 36.6 (201 MB, 5.5 TB/s) and 5.2.  A copy of 2 GB runs at 5.1 TB/s.
 #include "hmoe_common.h"
 
 namespace hmoe {
@@ -927,8 +927,13 @@ static int norm_bwd_run(NormBwdArgs& a, int sdt, int hdt, void* workspace, size_
     if (!nsum || brief) f.s.B = 0;
     const int items = f.s.B + (a.dweight ? 1 : 0);
     if (items == 0) return HMOE_OK;
+    // Up to 128 workgroups of a column block walk the items: with many samples most items are a chunk's own and left at once.
+    // 128 against 1024, us: 16384 x 1536, 128 samples 15.2, 10.6; 1000 36, 40; 4000 97, 100; 16000 334, 326; 100000 x 64, 50000
+    // samples 162, 53.
     const dim3 grid(items < 128 ? items : 128, (a.d + 31) / 32);
-    // many parts for long sums, few where the samples span a few chunks each
+    // Many parts for long sums, few where the samples span a few chunks each.  32 against 8, us (256 chunks): 16384 x 1536, 1
+    // sample 4.4, 6.4; 4 4.1, 5.1; 12 6.1, 5.5; 16 6.6, 5.6; 64 16.5, 7.8; 30000 x 512, 1 4.2, 6.2; 16 4.1, 5.1; 100 9.3, 5.8;
+    // 4096 x 8192, 4 11.1, 7.5 (the side the rule does not take, as at 12 samples).
     if (nchunk > 16 * a.s.B)
       hipLaunchKernelGGL(norm_sums_kernel<32>, grid, dim3(32 * 32), 0, s, f, nchunk, items);
     else

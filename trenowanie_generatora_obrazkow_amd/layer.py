@@ -345,7 +345,8 @@ def clip_grad_norm(grads, max_norm, out=None):
     gradients; the gradients then stay as they are).  Tensors written by a call that overlap others of it are refused.  bf16, fp16 and fp32 tensors of
     any size and alignment may be mixed, None entries are skipped.  Returns the norm before clipping, a () fp32 tensor on the
     device; nothing waits for the GPU.
-    A gradient spread over several processes: all-reduce ops.grad_sq_norm's sum before ops.grad_clip."""
+    A gradient spread over several processes: all-reduce ops.grad_sq_norm's sum before ops.grad_clip.  Autograd does not see
+    the change in place: where gradients are themselves part of a graph (create_graph=True), clip after its last backward."""
     grads = list(grads)
     if out is not None:
         out = list(out)

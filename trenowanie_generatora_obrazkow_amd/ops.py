@@ -936,7 +936,8 @@ def norm_residual(y, x, gate=None, weight=None, norm=True, starts=None, eps=1e-6
     """out (T, d) = alpha * x + gate_b * weight * n, n = s / sqrt(mean(s^2) + eps) (s itself without norm): the gated
     residual behind a block.  s is the sum over the k slots of y (T*k, d) (plus add (T, d), the shared expert's output), what
     combine gives without its rounding; with inv_pos from the dispatch, slots routed nowhere add nothing.  gate (B, d) per
-    sample as in norm_modulate, or (d,); padding rows get alpha * x.  out has the type of the stream x."""
+    sample as in norm_modulate, or (d,); padding rows get alpha * x.  out has the type of the stream x.  (The block's output
+    comes first here; the differentiable norm_residual of the package takes the stream first.)"""
     T, d, ldx = _rows(x, "x")
     dev = x.device
     _block_dtype(x.dtype, y.dtype)
@@ -1049,7 +1050,8 @@ def _addr(a):
 
 
 def grad_sq_norm(grads):
-    """(1,) fp64 on the device: the sum of the squares of every element of a list of gradients (or a GradList)."""
+    """(1,) fp64 on the device: the sum of the squares of every element of a list of gradients (or a GradList).  The order of the
+    sum, and so its last bits, goes by the list and its tensors' addresses."""
     gl = grads if isinstance(grads, GradList) else GradList(grads)
     dev = gl.device if gl.device is not None else torch.device("cuda", torch.cuda.current_device())
     sq = torch.empty(1, device=dev, dtype=torch.float64)
