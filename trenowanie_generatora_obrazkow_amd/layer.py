@@ -287,6 +287,12 @@ class MoESwiGLU(nn.Module):
         self.last_topk_ids = None
         self.last_topk_weight = None
 
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self.__dict__.setdefault("gate", None)  # (pickled before the layer had gates)
+        if "select_bias" not in self._buffers:
+            self.__dict__.setdefault("select_bias", None)
+
     @property
     def in_proj(self) -> _ExpertStackProj:
         return _ExpertStackProj(self.w_gu, self.dim, 2 * self.hidden)
