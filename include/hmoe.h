@@ -461,6 +461,50 @@ int hmoe_grad_clip_f64(const void* const* grads, void* const* out, const int64_t
                        const int* out_dtypes, int n, const double* sq_norm, double max_norm, float* norm,
                        hmoe_stream_t stream);
 
+/* ---------------------------------------------------------------------------------------------------------------
+ * Experts in 8-bit floating point with a scale per block of 128
+ * Values are e4m3 (bytes), scales e8m0 (bytes: the exponent e of 2^e plus 127).  A block's scale is the least 2^e, e >= -126,
+ * with its largest finite value at most 448 * 2^e; its values are x * 2^-e rounded to nearest even, infinities and NaNs
+ * become NaN.  Rows (M, K): a scale per 1 x 128 columns.  Stacks (E, K, N): a scale per 128 x 128.  Scale rows are
+ * hmoe_f8_scale_ld(columns) bytes apart (one per 128 columns, in whole 16 bytes; 16-byte aligned, the rest unused).
+ * ------------------------------------------------------------------------------------------------------------- */
+size_t hmoe_f8_scale_ld(int64_t K);
+
+/* x (M, K) bf16, fp16 or fp32 (row stride ldx, a multiple of 8) -> q (M, K) with row stride ldq, s (M, lds).  K % 16 == 0. */
+int hmoe_f8_quant_rows(const void* x, int64_t ldx, int dtype, int64_t M, int64_t K, void* q, int64_t ldq, uint8_t* s,
+                       int64_t lds, hmoe_stream_t stream);
+/* The values of quantised rows, a scale per `block` columns (128, or 32: hmoe_swiglu_pack): x (M, K) bf16, fp16 or fp32,
+ * rounded to that type where it cannot hold them.  K % 8 == 0. */
+int hmoe_f8_dequant_rows(const void* q, int64_t ldq, const uint8_t* s, int64_t lds, int64_t M, int64_t K, int block, void* x,
+                         int64_t ldx, int dtype, hmoe_stream_t stream);
+/* A stack w (E, K, N), N contiguous, bf16, fp16 or fp32, to 8 bits; the `halves` (1 or 2: [gate | up]) equal column ranges
+ * have their blocks from their own first column on.  transpose = 1, the operand of a product that sums over K: q (E, N, K),
+ * s (E, halves * ceil(N / halves / 128), scale_ld(K)).  transpose = 0, that of one that sums over N (the gradient of the rows;
+ * halves = 1): q (E, K, N), s (E, ceil(K / 128), scale_ld(N)).  K and N / halves multiples of 16. */
+int hmoe_f8_quant_stack(const void* w, int dtype, int64_t E, int64_t K, int64_t N, int64_t stride_we, int64_t stride_wk,
+                        int halves, int transpose, void* q, uint8_t* s, hmoe_stream_t stream);
+
+/* hmoe_grouped_mm on quantised rows and stacks (aurora/moe_triton.py:22-56 with 8-bit operands): y[y_idx[r] or r] =
+ * scale * a[a_idx[r] or r] @ w[e(r)], summed in fp32 and rounded once to y_dtype (bf16, fp16 or fp32).  w (E, N, K) and w_s from
+ * hmoe_f8_quant_stack.  scale (M,) fp32, bf16 or fp16 or NULL, by sorted row or, with scale_by_y, by y_idx[r].  Rows that no
+ * expert counts are zeros (without y_idx; with it nothing is written for them). */
+int hmoe_f8_grouped_mm(const void* a, int64_t lda, const uint8_t* a_s, int64_t lda_s, const void* w, const uint8_t* w_s,
+                       int64_t E, int64_t K, int64_t N, int halves, const void* counts, int counts_dtype, int64_t M,
+                       const int32_t* a_idx, const int32_t* y_idx, const void* scale, int scale_dtype, int scale_by_y, void* y,
+                       int64_t ldy, int y_dtype, hmoe_stream_t stream);
+/* act = silu(g) * u of [g | u] = x[a_idx] @ wgu[e], all in fp32, quantised: act (M, h) e4m3, act_s (M, scale_ld(h)).  wgu
+ * (E, 2h, d) with halves = 2. */
+int hmoe_f8_gate_up_swiglu(const void* x, int64_t ldx, const uint8_t* x_s, int64_t ldx_s, const int32_t* a_idx, const void* wgu,
+                           const uint8_t* wgu_s, int64_t E, int64_t d, int64_t h, const void* counts, int counts_dtype,
+                           int64_t M, void* act, uint8_t* act_s, hmoe_stream_t stream);
+/* hmoe_moe_experts with such stacks: x (T, d) bf16 or fp16 is quantised, y (T * k, d) of its type; the routing weights enter
+ * as given (not rounded). */
+size_t hmoe_f8_moe_experts_workspace_size(int64_t T, int64_t d, int E, int k, int64_t h);
+int hmoe_f8_moe_experts(const void* x, int64_t ldx, int dtype, const void* topk_ids, int ids_dtype, const void* topk_w,
+                        int topk_w_dtype, const void* wgu, const uint8_t* wgu_s, const void* wd, const uint8_t* wd_s, int64_t T,
+                        int64_t d, int E, int k, int64_t h, void* y, int32_t* inv_pos, int32_t* n_invalid, void* workspace,
+                        size_t workspace_bytes, hmoe_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

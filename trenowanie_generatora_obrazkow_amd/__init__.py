@@ -12,6 +12,7 @@
 from . import _lib  # noqa: F401
 from .block import MoEResidual, moe_residual, norm_modulate, norm_residual  # noqa: F401
 from .layer import Gate, MoESwiGLU, clip_grad_norm, moe_param_groups, moe_swiglu  # noqa: F401
+from .ops import F8Stack  # noqa: F401
 
 __all__ = ["MoESwiGLU", "Gate", "moe_swiglu", "moe_param_groups", "clip_grad_norm", "MoEResidual", "moe_residual",
-           "norm_modulate", "norm_residual"]
+           "norm_modulate", "norm_residual", "F8Stack"]

@@ -1,0 +1,813 @@
+// Products in 8-bit floating point with a scale per block of 128: quantisation of rows and of expert stacks, the grouped
+// GEMM over them (plain, with row scale and scatter; SwiGLU with the activation quantised again), and the experts of a
+// routed layer in one call.
+//
+//   y[r, n] = scale[r] * sum_k (a8[r, k] 2^ea[r, k / 128]) (w8[n, k] 2^ew[n / 128, k / 128])
+//
+// Both operands lie with k contiguous, so a k-slice of 128 is one 128-byte line of every row, and one slice has one scale
+// per row of a and one per 128 columns of w.
+#include <algorithm>
+#include <atomic>
+
+#include "f8_common.h"
+#include "gemm_common.h"
+
+namespace hmoe {
+
+// ----------------------------------------------------------------------------------------------------------------
+// Quantisation
+// ----------------------------------------------------------------------------------------------------------------
+// eight consecutive values of a row as floats
+template <int DT>
+__device__ __forceinline__ void load8(const void* p, int64_t at, float* v) {
+  if constexpr (DT == HMOE_DT_F32) {
+    const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
+    const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + at + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  } else {
+    using X = Elt<DT == HMOE_DT_F16>;
+    const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + at);
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = X::lo(u[i]);
+      v[2 * i + 1] = X::hi(u[i]);
+    }
+  }
+}
+
+// Rows: 16 lanes hold a block of 128 columns, eight each, so a wave reads four blocks in 256-byte (16-bit input) pieces, and
+// the block's largest value takes four exchanges within 16 lanes.  Memory-bound: M K (bytes + 1) bytes.
+template <int DT>
+__global__ __launch_bounds__(256) void quant_rows_kernel(const void* __restrict__ x, int64_t ldx, int64_t M, int K, int nb,
+                                                         uint8_t* __restrict__ q, int64_t ldq, uint8_t* __restrict__ s,
+                                                         int64_t lds) {
+  const int sub = threadIdx.x & 15;
+  const int64_t blocks = M * nb, step = (int64_t)gridDim.x * 16;
+  for (int64_t i = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); i < blocks; i += step) {
+    const int64_t r = i / nb;
+    const int b = (int)(i - r * nb), col = b * kF8Block + sub * 8;
+    float v[8];
+    float m = 0.0f;
+    const bool in = col < K;
+    if (in) {
+      load8<DT>(x, r * ldx + col, v);
+#pragma unroll
+      for (int t = 0; t < 8; ++t) m = fmaxf(m, f8_abs(v[t]));
+    }
+    m = bfly_max<8>(bfly_max<4>(bfly_max<2>(bfly_max<1>(m))));
+    const int e = f8_exp(m);
+    if (in) {
+      const float inv = f8_inv(e);
+      *reinterpret_cast<uint2*>(q + r * ldq + col) =
+          make_uint2(f8_pack4(v[0], v[1], v[2], v[3], inv), f8_pack4(v[4], v[5], v[6], v[7], inv));
+    }
+    if (sub == 0) s[r * lds + b] = (uint8_t)(e + 127);
+  }
+}
+
+// A stack (K, N) per expert, N contiguous, in blocks of 128 x 128: a workgroup holds one block in registers (thread t: column
+// piece t % 16, rows t / 16 + 16 i), finds its scale, and writes it as it lies (TR = false) or with k contiguous (TR = true,
+// through LDS).  Done once for the weights' lifetime.
+template <int DT, bool TR>
+__global__ __launch_bounds__(256) void quant_stack_kernel(const void* __restrict__ w, int64_t stride_we, int64_t stride_wk,
+                                                          int K, int Nh, int halves, uint8_t* __restrict__ q,
+                                                          uint8_t* __restrict__ s, int64_t lds, int kb_n, int nb_h) {
+  __shared__ __attribute__((aligned(16))) uint8_t tile[128 * 144];  // [n][k], rows 16 bytes apart from a power of two
+  __shared__ float wave_max[4];
+  const int t = threadIdx.x;
+  const int kb = (int)(blockIdx.x % kb_n), nb = (int)(blockIdx.x / kb_n), half = nb / nb_h;
+  const int64_t e = blockIdx.y;
+  const int c0 = (nb - half * nb_h) * kF8Block + (t & 15) * 8, k0 = kb * kF8Block + (t >> 4);
+  const bool cin = c0 < Nh;
+  float v[8][8];
+  float m = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int k = k0 + 16 * i;
+    if (cin && k < K) {
+      load8<DT>(w, e * stride_we + k * stride_wk + half * Nh + c0, v[i]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = fmaxf(m, f8_abs(v[i][j]));
+  }
+  m = wave_max_butterfly(m);
+  if ((t & 63) == 0) wave_max[t >> 6] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(wave_max[0], wave_max[1]), fmaxf(wave_max[2], wave_max[3]));
+  const int ex = f8_exp(m);
+  const float inv = f8_inv(ex);
+  const int N = halves * Nh;
+  if (t == 0) {
+    const int rows = TR ? halves * nb_h : kb_n;
+    s[(e * rows + (TR ? nb : kb)) * lds + (TR ? kb : nb)] = (uint8_t)(ex + 127);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t lo = f8_pack4(v[i][0], v[i][1], v[i][2], v[i][3], inv);
+    const uint32_t hi = f8_pack4(v[i][4], v[i][5], v[i][6], v[i][7], inv);
+    const int k = k0 + 16 * i;
+    if constexpr (!TR) {
+      if (cin && k < K) *reinterpret_cast<uint2*>(q + (e * K + k) * (int64_t)N + c0) = make_uint2(lo, hi);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        tile[((t & 15) * 8 + j) * 144 + (t >> 4) + 16 * i] = (uint8_t)(lo >> (8 * j));
+        tile[((t & 15) * 8 + 4 + j) * 144 + (t >> 4) + 16 * i] = (uint8_t)(hi >> (8 * j));
+      }
+    }
+  }
+  if constexpr (TR) {
+    __syncthreads();
+    for (int i = t; i < 128 * 8; i += 256) {
+      const int n = i >> 3, c = i & 7;
+      const int col = (nb - half * nb_h) * kF8Block + n, k = kb * kF8Block + c * 16;
+      if (col < Nh && k < K)
+        *reinterpret_cast<uint4*>(q + (e * N + half * Nh + col) * (int64_t)K + k) =
+            *reinterpret_cast<const uint4*>(tile + n * 144 + c * 16);
+    }
+  }
+}
+
+// The values of a quantised matrix, a scale per `block` columns (a power of two, at least 8).
+template <int DT>
+__global__ __launch_bounds__(256) void dequant_rows_kernel(const uint8_t* __restrict__ q, int64_t ldq,
+                                                           const uint8_t* __restrict__ s, int64_t lds, int64_t M, int K8,
+                                                           int shift, void* __restrict__ x, int64_t ldx) {
+  const int64_t n = M * K8, step = (int64_t)gridDim.x * 256;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += step) {
+    const int64_t r = i / K8;
+    const int col = (int)(i - r * K8) * 8;
+    const uint2 w = *reinterpret_cast<const uint2*>(q + r * ldq + col);
+    const float sc = f8_pow((int)s[r * lds + (col >> shift)] - 127);
+    float v[8];
+    f8_unpack2<0>(w.x, v[0], v[1]);
+    f8_unpack2<1>(w.x, v[2], v[3]);
+    f8_unpack2<0>(w.y, v[4], v[5]);
+    f8_unpack2<1>(w.y, v[6], v[7]);
+#pragma unroll
+    for (int t = 0; t < 8; ++t) v[t] *= sc;
+    if constexpr (DT == HMOE_DT_F32) {
+      float4* o = reinterpret_cast<float4*>(static_cast<float*>(x) + r * ldx + col);
+      o[0] = make_float4(v[0], v[1], v[2], v[3]);
+      o[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+      using X = Elt<DT == HMOE_DT_F16>;
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(x) + r * ldx + col) =
+          make_uint4(X::pack2(v[0], v[1]), X::pack2(v[2], v[3]), X::pack2(v[4], v[5]), X::pack2(v[6], v[7]));
+    }
+  }
+}
+
+// ----------------------------------------------------------------------------------------------------------------
+// Grouped GEMM
+// ----------------------------------------------------------------------------------------------------------------
+struct F8Params {
+  const uint8_t* A;        // rows of a8 (sorted row r, or a_idx[r]), K bytes, row stride lda
+  int64_t lda;
+  const uint8_t* As;       // their scales, row stride ldas
+  int64_t ldas;
+  const int32_t* a_idx;
+  const uint8_t* B;        // (E, halves N, K)
+  const uint8_t* Bs;       // (E, halves nbs, ldbs): rows of 128 columns of one half
+  int64_t ldbs;
+  const void* counts;
+  int counts64, E;
+  int64_t M;
+  int K, N, halves, nbs;   // N: columns of a half
+  int nb;                  // n-tiles: of all halves (store), of act columns (SwiGLU)
+  void* C;                 // store: y; SwiGLU: act as e4m3
+  int64_t ldc;
+  const int32_t* y_idx;
+  const void* scale;       // per row, or NULL
+  int scale_dt, scale_by_y;  // indexed by the sorted row, or by the row's place in y
+  uint8_t* Cs;             // SwiGLU: act's scales
+  int64_t ldcs;
+};
+
+constexpr int kF8Slice = 128;  // k per slice: one line of a row, one scale
+constexpr int kF8BandM = 4;    // m-tiles of an expert that are walked together over the n-tiles (L2 reuse of the weights)
+
+enum F8Epi { F8_STORE = 0, F8_SWIGLU = 1 };
+
+template <int BM_, int BN_, int WM_, int WN_, int NS_>
+struct F8Cfg {
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NS = NS_;
+  static constexpr int NW = WM * WN, NT = 64 * NW, TM = BM / WM, TN = BN / WN, FM = TM / 32, FN = TN / 32;
+  static constexpr int A_BYTES = BM * kF8Slice, B_BYTES = BN * kF8Slice, STAGE = A_BYTES + B_BYTES;
+  static constexpr int LDS_BYTES = NS * STAGE;
+  static constexpr int PA = BM / 8 / NW, PB = BN / 8 / NW;  // copies of 8 rows per wave and slice
+  static_assert(PA * 8 * NW == BM && PB * 8 * NW == BN && FM >= 1 && FN >= 2, "tile");
+};
+
+// LDS: a row of a slice is 128 bytes, its 16-byte chunk c at c ^ f8_swz(row), so that 16 rows' chunks of one number lie on
+// distinct banks (two rows fill the 64 banks once).
+__device__ __forceinline__ int f8_swz(int row) { return (row >> 1) & 7; }
+
+// A fragment of 32 rows x 64 k: the lane's row, 32 bytes
+__device__ __forceinline__ i32x8 f8_frag(const char* rows, const int* off) {
+  typedef int i32x4v __attribute__((ext_vector_type(4)));
+  const i32x4v a = *reinterpret_cast<const i32x4v*>(rows + off[0]);
+  const i32x4v b = *reinterpret_cast<const i32x4v*>(rows + off[1]);
+  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// The weights go in as the first operand, so a lane ends with one row of y (lane % 32) and, per group g of four, columns
+// 8 g + 4 (lane / 32) + 0..3 of the fragment.  S: byte of the scale words.
+template <int S>
+__device__ __forceinline__ f32x16 f8_mfma(i32x8 w, i32x8 x, f32x16 c, uint32_t sw, uint32_t sx) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, x, c, 0, 0, S, (int)sw, S, (int)sx);
+}
+
+__device__ __forceinline__ float row_scale_at(const void* s, int dt, int64_t i) {
+  if (dt == HMOE_DT_F32) return static_cast<const float*>(s)[i];
+  const uint16_t h = static_cast<const uint16_t*>(s)[i];
+  return dt == HMOE_DT_BF16 ? Elt<false>::one(h) : Elt<true>::one(h);
+}
+
+template <class C, int EPI, int CDT>
+__global__ __launch_bounds__(C::NT, C::LDS_BYTES > 81920 ? 1 : 2) void f8_gemm_kernel(F8Params p) {
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int wm = wave / C::WN, wn = wave % C::WN;
+  const int E = p.E;
+
+  // ---- the workgroup's tile: each wave scans the counts by itself, E / 64 experts a lane ----
+  const int per = (E + 63) / 64;
+  int64_t rs = 0;
+  for (int i = 0; i < per; ++i) {
+    const int e = lane * per + i;
+    if (e < E) rs += std::min(std::max(read_count(p.counts, p.counts64, e), (int64_t)0), p.M);
+  }
+  int64_t irs = rs;
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) {
+    const int64_t a = __shfl_up(irs, s, 64);
+    if (lane >= s) irs += a;
+  }
+  const int64_t st = irs - rs;  // the lane's first row
+  int tl = 0;
+  int64_t at_row = st;
+  for (int i = 0; i < per; ++i) {  // m-tiles of the lane's experts (rows past M do not exist)
+    const int e = lane * per + i;
+    if (e >= E) break;
+    const int64_t end = at_row + std::min(std::max(read_count(p.counts, p.counts64, e), (int64_t)0), p.M);
+    tl += (int)((std::min(end, p.M) - std::min(at_row, p.M) + C::BM - 1) / C::BM);
+    at_row = end;
+  }
+  int itl = tl;
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) {
+    const int a = __shfl_up(itl, s, 64);
+    if (lane >= s) itl += a;
+  }
+  const int total = __builtin_amdgcn_readfirstlane(__shfl(itl, 63, 64)) * p.nb;
+  // the tiles in runs of equal length over the 8 XCDs (workgroups go to them in turn)
+  const int share = (total + 7) >> 3, at = (int)blockIdx.x >> 3;
+  const int tile = ((int)blockIdx.x & 7) * share + at;
+  [[maybe_unused]] const int64_t counted = std::min<int64_t>(__shfl(irs, 63, 64), p.M);
+  // rows that no expert counts are zeros (where rows keep their places): every n-th of them for the n-th tile's workgroup
+  [[maybe_unused]] auto zero_rows = [&](int n, int of) __attribute__((always_inline)) {
+    constexpr int ES = CDT == HMOE_DT_F32 ? 4 : 2;
+    const int pieces = (int)((int64_t)p.halves * p.N * ES / 16);
+    for (int64_t row = counted + n; row < p.M; row += of)
+      for (int i = threadIdx.x; i < pieces; i += C::NT)
+        *reinterpret_cast<uint4*>(static_cast<char*>(p.C) + row * p.ldc * ES + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+  };
+  if (at >= share || tile >= total) {
+    if constexpr (EPI == F8_STORE)
+      if (total == 0 && !p.y_idx) zero_rows((int)blockIdx.x, (int)gridDim.x);
+    return;
+  }
+  const int mt = tile / p.nb;
+  const int ol = __builtin_ctzll(__ballot(itl > mt));
+  int mstart = __builtin_amdgcn_readfirstlane(__shfl(itl - tl, ol, 64));
+  int64_t first = __shfl(st, ol, 64);
+  int e = -1, mt_e = 0;
+  int64_t row_end = 0;
+  for (int i = 0; i < per; ++i) {
+    const int x = ol * per + i;
+    if (x >= E) break;
+    const int64_t end = first + std::min(std::max(read_count(p.counts, p.counts64, x), (int64_t)0), p.M);
+    const int n = (int)((std::min(end, p.M) - std::min(first, p.M) + C::BM - 1) / C::BM);
+    if (mt < mstart + n) {
+      e = x;
+      mt_e = n;
+      row_end = std::min(end, p.M);
+      break;
+    }
+    mstart += n;
+    first = end;
+  }
+  // bands of kF8BandM m-tiles of an expert, n-tile by n-tile
+  const int local = tile - mstart * p.nb, band = local / (kF8BandM * p.nb) * kF8BandM;
+  const int mc = min(kF8BandM, mt_e - band), r = local - band * p.nb;
+  e = __builtin_amdgcn_readfirstlane(e);
+  const int nbi = __builtin_amdgcn_readfirstlane(r / mc);
+  const int row0 = __builtin_amdgcn_readfirstlane((int)(first + (int64_t)(band + r % mc) * C::BM));
+  const int live = __builtin_amdgcn_readfirstlane((int)std::min<int64_t>(row_end - row0, C::BM));
+
+  // ---- columns: n0 the first of the half (store) or of act (SwiGLU) ----
+  const int nbh = EPI == F8_STORE ? p.nb / p.halves : p.nb;
+  const int half = EPI == F8_STORE ? nbi / nbh : 0;
+  const int n0 = (nbi - half * nbh) * (EPI == F8_SWIGLU ? C::BN / 2 : C::BN);
+
+  // ---- copy sources ----
+  const int K = p.K, nk = (K + kF8Slice - 1) / kF8Slice;
+  const i32x4 rsA = make_rsrc(p.a_idx ? p.A : p.A + (int64_t)row0 * p.lda);
+  const i32x4 rsB = make_rsrc(p.B + (int64_t)e * p.halves * p.N * K);
+  uint32_t vA[C::PA], vB[C::PB];
+  auto chunk_of = [&](int rr) { return (lane & 7) ^ f8_swz(rr); };
+#pragma unroll
+  for (int i = 0; i < C::PA; ++i) {
+    const int rr = 8 * (wave * C::PA + i) + (lane >> 3);
+    vA[i] = kOOB;
+    if (rr < live) {
+      const int64_t src = p.a_idx ? (int64_t)p.a_idx[row0 + rr] : (int64_t)rr;
+      vA[i] = (uint32_t)(src * p.lda + chunk_of(rr) * 16);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < C::PB; ++i) {
+    const int rr = 8 * (wave * C::PB + i) + (lane >> 3);
+    int col, row;  // column within the half, row of B
+    if constexpr (EPI == F8_SWIGLU) {
+      col = n0 + rr % (C::BN / 2);
+      row = rr / (C::BN / 2) * p.N + col;
+    } else {
+      col = n0 + rr;
+      row = half * p.N + col;
+    }
+    vB[i] = col < p.N ? (uint32_t)((int64_t)row * K + chunk_of(rr) * 16) : kOOB;
+  }
+  auto issue = [&](int kt) __attribute__((always_inline)) {  // slice kt into its stage
+    char* slot = smem + (kt % C::NS) * C::STAGE;
+    const int k0 = kt * kF8Slice;
+    if (k0 + kF8Slice <= K) {
+#pragma unroll
+      for (int i = 0; i < C::PA; ++i) buf2lds(vA[i], rsA, (uint32_t)k0, slot + (wave * C::PA + i) * 1024);
+#pragma unroll
+      for (int i = 0; i < C::PB; ++i) buf2lds(vB[i], rsB, (uint32_t)k0, slot + C::A_BYTES + (wave * C::PB + i) * 1024);
+    } else {  // chunks at or past K (and whole slices past it) read zeros
+#pragma unroll
+      for (int i = 0; i < C::PA; ++i)
+        buf2lds(k0 + chunk_of(8 * (wave * C::PA + i) + (lane >> 3)) * 16 < K ? vA[i] : kOOB, rsA, (uint32_t)k0,
+                slot + (wave * C::PA + i) * 1024);
+#pragma unroll
+      for (int i = 0; i < C::PB; ++i)
+        buf2lds(k0 + chunk_of(8 * (wave * C::PB + i) + (lane >> 3)) * 16 < K ? vB[i] : kOOB, rsB, (uint32_t)k0,
+                slot + C::A_BYTES + (wave * C::PB + i) * 1024);
+    }
+  };
+
+  // ---- per-row inputs of the lane's rows a*32 + lane%32 of the wave ----
+  const uint8_t* pa[C::FM];
+  [[maybe_unused]] int yr[C::FM];
+  [[maybe_unused]] float sc[C::FM];
+#pragma unroll
+  for (int a = 0; a < C::FM; ++a) {
+    const int rr = wm * C::TM + a * 32 + (lane & 31);
+    const int row = row0 + min(rr, live - 1);  // (a row past the tile's last takes that one's scales: its values are zeros)
+    pa[a] = p.As + (p.a_idx ? (int64_t)p.a_idx[row] : (int64_t)row) * p.ldas;
+    if constexpr (EPI == F8_STORE) {
+      yr[a] = p.y_idx ? p.y_idx[row] : row;
+      sc[a] = p.scale ? row_scale_at(p.scale, p.scale_dt, p.scale_by_y ? yr[a] : row) : 1.0f;
+    }
+  }
+  // scales of the wave's columns: one 128-column block (store), the gate's and the up's (SwiGLU)
+  const int sblk = EPI == F8_STORE ? min((n0 + wn * C::TN) / kF8Block, p.nbs - 1)
+                                   : min((n0 + wn * C::TN / 2) / kF8Block, p.nbs - 1);
+  const uint8_t* pb0 = p.Bs + ((int64_t)(e * p.halves + half) * p.nbs + sblk) * p.ldbs;
+  const uint8_t* pb1 = EPI == F8_SWIGLU ? pb0 + (int64_t)p.nbs * p.ldbs : pb0;
+
+  // ---- main loop ----
+  int off[2][2];
+#pragma unroll
+  for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      off[ks][j] = (lane & 31) * 128 + (((ks * 4 + (lane >> 5) * 2 + j) ^ f8_swz(lane & 31)) * 16);
+  auto b_row = [&](int b) {  // tile row of column fragment b
+    if constexpr (EPI == F8_SWIGLU)
+      return b < C::FN / 2 ? wn * (C::TN / 2) + b * 32 : C::BN / 2 + wn * (C::TN / 2) + (b - C::FN / 2) * 32;
+    else
+      return wn * C::TN + b * 32;
+  };
+  f32x16 acc[C::FM][C::FN];
+#pragma unroll
+  for (int a = 0; a < C::FM; ++a)
+#pragma unroll
+    for (int b = 0; b < C::FN; ++b)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) acc[a][b][v] = 0.0f;
+  uint4 sA[C::FM], sB0, sB1;
+  constexpr int LOADS = C::PA + C::PB;
+#pragma unroll
+  for (int s = 0; s < C::NS - 1; ++s) issue(s);
+  for (int k4 = 0; k4 < nk; k4 += 4) {
+    if ((k4 & 15) == 0) {
+#pragma unroll
+      for (int a = 0; a < C::FM; ++a) sA[a] = *reinterpret_cast<const uint4*>(pa[a] + k4);
+      sB0 = *reinterpret_cast<const uint4*>(pb0 + k4);
+      if constexpr (EPI == F8_SWIGLU) sB1 = *reinterpret_cast<const uint4*>(pb1 + k4);
+    }
+    static_for<4>([&](auto it) __attribute__((always_inline)) {
+      constexpr int I = decltype(it)::value;
+      const int kt = k4 + I;
+      if (kt < nk) {
+        wait_vm<(C::NS - 2) * LOADS>();  // this wave's copies of slice kt have landed
+        lds_barrier();                   // and the others'; all have read slice kt - 1, whose stage is filled next
+        issue(kt + C::NS - 1);
+        const char* sa = smem + (kt % C::NS) * C::STAGE;
+        const char* sb = sa + C::A_BYTES;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+          i32x8 xa[C::FM], wb[C::FN];
+#pragma unroll
+          for (int b = 0; b < C::FN; ++b) wb[b] = f8_frag(sb + b_row(b) * 128, off[ks]);
+#pragma unroll
+          for (int a = 0; a < C::FM; ++a) xa[a] = f8_frag(sa + (wm * C::TM + a * 32) * 128, off[ks]);
+#pragma unroll
+          for (int a = 0; a < C::FM; ++a)
+#pragma unroll
+            for (int b = 0; b < C::FN; ++b)
+              acc[a][b] = f8_mfma<I>(wb[b], xa[a], acc[a][b], EPI == F8_SWIGLU && b >= C::FN / 2 ? sB1.x : sB0.x, sA[a].x);
+        }
+      }
+    });
+    auto next = [](uint4& v) { v.x = v.y; v.y = v.z; v.z = v.w; };
+#pragma unroll
+    for (int a = 0; a < C::FM; ++a) next(sA[a]);
+    next(sB0);
+    if constexpr (EPI == F8_SWIGLU) next(sB1);
+  }
+  wait_vm<0>();   // (copies past the last slice move nothing, but still write zeros)
+  lds_barrier();  // the ring is free
+
+  const int lrow = lane & 31, lcol = 4 * (lane >> 5);
+  if constexpr (EPI == F8_STORE) {
+    // 32 rows of the wave at a time go through its own part of the LDS, chunk c of a row at c ^ row, and leave in whole rows
+    constexpr int ES = CDT == HMOE_DT_F32 ? 4 : 2, RB = C::TN * ES, CPR = RB / 16, RPI = 64 / CPR;
+    char* park = smem + wave * (32 * RB);
+#pragma unroll
+    for (int a = 0; a < C::FM; ++a) {
+      const int rbase = wm * C::TM + a * 32;
+      if (rbase >= live) break;
+#pragma unroll
+      for (int b = 0; b < C::FN; ++b)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const f32x16& v = acc[a][b];
+          const float o[4] = {v[4 * g] * sc[a], v[4 * g + 1] * sc[a], v[4 * g + 2] * sc[a], v[4 * g + 3] * sc[a]};
+          const int byte = (b * 32 + 8 * g + lcol) * ES;
+          char* at = park + lrow * RB + (((byte >> 4) ^ (lrow & (CPR - 1))) << 4) + (byte & 15);
+          if constexpr (CDT == HMOE_DT_F32) {
+            *reinterpret_cast<float4*>(at) = make_float4(o[0], o[1], o[2], o[3]);
+          } else {
+            using X = Elt<CDT == HMOE_DT_F16>;
+            *reinterpret_cast<uint2*>(at) = make_uint2(X::pack2(o[0], o[1]), X::pack2(o[2], o[3]));
+          }
+        }
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int i = 0; i < 32 / RPI; ++i) {
+        const int rr = i * RPI + lane / CPR, c = lane % CPR;
+        const uint4 v = *reinterpret_cast<const uint4*>(park + rr * RB + ((c ^ (rr & (CPR - 1))) << 4));
+        const int64_t y = __shfl(yr[a], rr, 64);
+        const int col = n0 + wn * C::TN + c * (16 / ES);
+        if (rbase + rr < live && col < p.N)
+          *reinterpret_cast<uint4*>(static_cast<char*>(p.C) + (y * p.ldc + half * p.N + col) * ES) = v;
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+    if (!p.y_idx && counted < p.M) zero_rows(tile, total);
+  } else {
+    // act = silu(g) u in fp32, in place of g; the largest of a row's 128 columns from the lanes l and l ^ 32 and, through
+    // LDS, the waves side by side; then e4m3 through LDS into whole 128-byte rows
+    float* s_max = reinterpret_cast<float*>(smem);  // [WN][BM]
+    char* park = smem + C::WN * C::BM * 4;          // [BM][128]
+    static_assert(C::BN / 2 == kF8Block && C::WN * C::BM * 4 + C::BM * 128 <= C::LDS_BYTES, "one block of act per tile");
+#pragma unroll
+    for (int a = 0; a < C::FM; ++a) {
+      float m = 0.0f;
+#pragma unroll
+      for (int b = 0; b < C::FN / 2; ++b)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const float act = silu_f(acc[a][b][v]) * acc[a][b + C::FN / 2][v];
+          acc[a][b][v] = act;
+          m = fmaxf(m, f8_abs(act));
+        }
+      m = bfly_max<32>(m);
+      if (lane < 32) s_max[wn * C::BM + wm * C::TM + a * 32 + lrow] = m;
+    }
+    lds_barrier();
+#pragma unroll
+    for (int a = 0; a < C::FM; ++a) {
+      const int rr = wm * C::TM + a * 32 + lrow;
+      float m = 0.0f;
+#pragma unroll
+      for (int w = 0; w < C::WN; ++w) m = fmaxf(m, s_max[w * C::BM + rr]);
+      const int ex = f8_exp(m);
+      const float inv = f8_inv(ex);
+      if (wn == 0 && lane < 32 && rr < live) p.Cs[(int64_t)(row0 + rr) * p.ldcs + nbi] = (uint8_t)(ex + 127);
+#pragma unroll
+      for (int b = 0; b < C::FN / 2; ++b)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const f32x16& v = acc[a][b];
+          const int byte = wn * (C::TN / 2) + b * 32 + 8 * g + lcol;
+          *reinterpret_cast<uint32_t*>(park + rr * 128 + (((byte >> 4) ^ f8_swz(rr)) << 4) + (byte & 15)) =
+              f8_pack4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3], inv);
+        }
+    }
+    lds_barrier();
+    for (int i = threadIdx.x; i < live * 8; i += C::NT) {
+      const int rr = i >> 3, c = i & 7;
+      if (n0 + c * 16 < p.N)
+        *reinterpret_cast<uint4*>(static_cast<char*>(p.C) + (int64_t)(row0 + rr) * p.ldc + n0 + c * 16) =
+            *reinterpret_cast<const uint4*>(park + rr * 128 + ((c ^ f8_swz(rr)) << 4));
+    }
+  }
+}
+
+template <class C, int EPI, int CDT>
+static int f8_launch(const F8Params& p, hipStream_t s) {
+  auto kern = f8_gemm_kernel<C, EPI, CDT>;
+  static std::atomic<bool> attr_set[64];  // per device
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return HMOE_ERR_DEVICE;
+  if (!attr_set[dev].load(std::memory_order_acquire)) {
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize,
+                            C::LDS_BYTES) != hipSuccess)
+      return HMOE_ERR_LAUNCH;
+    attr_set[dev].store(true, std::memory_order_release);
+  }
+  F8Params q = p;
+  q.nb = EPI == F8_SWIGLU ? (p.N + C::BN / 2 - 1) / (C::BN / 2) : p.halves * ((p.N + C::BN - 1) / C::BN);
+  // an m-tile for every expert with rows and at most M / BM further ones; the tiles in eights (one per XCD)
+  const int64_t tiles = (std::min<int64_t>(p.E, p.M) + p.M / C::BM) * q.nb;
+  if (tiles >= (1 << 23)) return HMOE_ERR_SHAPE;  // (a grid's threads stay below 2^32)
+  hipLaunchKernelGGL(kern, dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(C::NT), C::LDS_BYTES, s, q);
+  HMOE_CHECK_LAUNCH();
+  return HMOE_OK;
+}
+
+template <int EPI, int CDT>
+static int f8_pick(const F8Params& p, hipStream_t s) {
+  const int64_t rows = p.M / std::min<int64_t>(p.E, p.M);  // per expert
+  if (rows >= 160) return f8_launch<F8Cfg<256, 256, 2, 2, 2>, EPI, CDT>(p, s);
+  if (rows >= 64) return f8_launch<F8Cfg<128, 256, 2, 2, 2>, EPI, CDT>(p, s);
+  return f8_launch<F8Cfg<32, 256, 1, 4, 2>, EPI, CDT>(p, s);
+}
+
+static bool al(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+static int f8_check(const void* a, int64_t lda, const uint8_t* a_s, int64_t lda_s, const int32_t* a_idx, const void* w,
+                    const uint8_t* w_s, int64_t E, int64_t K, int64_t N, int halves, const void* counts, int counts_dtype,
+                    int64_t M) {
+  if (!counts || E <= 0 || M < 0) return HMOE_ERR_ARG;
+  if (E > kMaxEGemm || M > INT32_MAX - 256) return HMOE_ERR_SHAPE;
+  if (counts_dtype != HMOE_DT_I32 && counts_dtype != HMOE_DT_I64) return HMOE_ERR_DTYPE;
+  if (M == 0) return HMOE_OK;
+  if (!a || !a_s || !w || !w_s || K <= 0 || N <= 0 || halves < 1 || halves > 2 || N % halves) return HMOE_ERR_ARG;
+  if (K % 16 || N / halves % 16) return HMOE_ERR_SHAPE;
+  if (lda < K || lda % 16 || lda_s < f8_scale_ld(K) || lda_s % 16 || !al(a, 16) || !al(a_s, 16) || !al(w, 16) || !al(w_s, 16))
+    return HMOE_ERR_ARG;
+  // 32-bit copy offsets: one expert's weights, the rows of a tile, all rows where they are gathered
+  const int64_t lim = ((int64_t)1 << 31) - 32768;
+  if (K > lim / N || lda > lim / 256 || (a_idx && M > lim / lda)) return HMOE_ERR_SHAPE;
+  return HMOE_OK;
+}
+
+static F8Params f8_params(const void* a, int64_t lda, const uint8_t* a_s, int64_t lda_s, const int32_t* a_idx, const void* w,
+                          const uint8_t* w_s, int64_t E, int64_t K, int64_t N, int halves, const void* counts,
+                          int counts_dtype, int64_t M) {
+  F8Params p = {};
+  p.A = static_cast<const uint8_t*>(a);
+  p.lda = lda;
+  p.As = a_s;
+  p.ldas = lda_s;
+  p.a_idx = a_idx;
+  p.B = static_cast<const uint8_t*>(w);
+  p.Bs = w_s;
+  p.ldbs = f8_scale_ld(K);
+  p.counts = counts;
+  p.counts64 = counts_dtype == HMOE_DT_I64;
+  p.E = (int)E;
+  p.M = M;
+  p.K = (int)K;
+  p.N = (int)(N / halves);
+  p.halves = halves;
+  p.nbs = (p.N + kF8Block - 1) / kF8Block;
+  return p;
+}
+
+}  // namespace hmoe
+
+using namespace hmoe;
+
+extern "C" {
+
+size_t hmoe_f8_scale_ld(int64_t K) { return K > 0 ? static_cast<size_t>(f8_scale_ld(K)) : 0; }
+
+int hmoe_f8_quant_rows(const void* x, int64_t ldx, int dtype, int64_t M, int64_t K, void* q, int64_t ldq, uint8_t* s,
+                       int64_t lds, hmoe_stream_t stream) {
+  if (M < 0 || K <= 0) return HMOE_ERR_ARG;
+  if (dtype != HMOE_DT_BF16 && dtype != HMOE_DT_F16 && dtype != HMOE_DT_F32) return HMOE_ERR_DTYPE;
+  if (M == 0) return HMOE_OK;
+  if (!x || !q || !s) return HMOE_ERR_ARG;
+  if (K % 16 || K > INT32_MAX - 256) return HMOE_ERR_SHAPE;
+  if (ldx < K || ldx % 8 || ldq < K || ldq % 16 || lds < f8_scale_ld(K) || lds % 16 || !al(x, 16) || !al(q, 16) || !al(s, 16))
+    return HMOE_ERR_ARG;
+  const int nb = (int)((K + kF8Block - 1) / kF8Block);
+  const int64_t groups = (M * nb + 15) / 16;
+  const dim3 grid((unsigned)std::min<int64_t>(groups, 4096));
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  auto* q8 = static_cast<uint8_t*>(q);
+  if (dtype == HMOE_DT_BF16)
+    hipLaunchKernelGGL(quant_rows_kernel<HMOE_DT_BF16>, grid, dim3(256), 0, st, x, ldx, M, (int)K, nb, q8, ldq, s, lds);
+  else if (dtype == HMOE_DT_F16)
+    hipLaunchKernelGGL(quant_rows_kernel<HMOE_DT_F16>, grid, dim3(256), 0, st, x, ldx, M, (int)K, nb, q8, ldq, s, lds);
+  else
+    hipLaunchKernelGGL(quant_rows_kernel<HMOE_DT_F32>, grid, dim3(256), 0, st, x, ldx, M, (int)K, nb, q8, ldq, s, lds);
+  HMOE_CHECK_LAUNCH();
+  return HMOE_OK;
+}
+
+int hmoe_f8_dequant_rows(const void* q, int64_t ldq, const uint8_t* s, int64_t lds, int64_t M, int64_t K, int block, void* x,
+                         int64_t ldx, int dtype, hmoe_stream_t stream) {
+  if (M < 0 || K <= 0) return HMOE_ERR_ARG;
+  if (dtype != HMOE_DT_BF16 && dtype != HMOE_DT_F16 && dtype != HMOE_DT_F32) return HMOE_ERR_DTYPE;
+  if (block != 128 && block != 32) return HMOE_ERR_SHAPE;
+  if (M == 0) return HMOE_OK;
+  if (!q || !s || !x) return HMOE_ERR_ARG;
+  if (K % 8 || K > INT32_MAX - 256) return HMOE_ERR_SHAPE;
+  if (ldq < K || ldq % 8 || lds < (K + block - 1) / block || ldx < K || ldx % 8 || !al(q, 8) || !al(x, 16)) return HMOE_ERR_ARG;
+  const int k8 = (int)(K / 8), shift = block == 128 ? 7 : 5;
+  const dim3 grid((unsigned)std::min<int64_t>((M * k8 + 255) / 256, 8192));
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  auto* q8 = static_cast<const uint8_t*>(q);
+  if (dtype == HMOE_DT_BF16)
+    hipLaunchKernelGGL(dequant_rows_kernel<HMOE_DT_BF16>, grid, dim3(256), 0, st, q8, ldq, s, lds, M, k8, shift, x, ldx);
+  else if (dtype == HMOE_DT_F16)
+    hipLaunchKernelGGL(dequant_rows_kernel<HMOE_DT_F16>, grid, dim3(256), 0, st, q8, ldq, s, lds, M, k8, shift, x, ldx);
+  else
+    hipLaunchKernelGGL(dequant_rows_kernel<HMOE_DT_F32>, grid, dim3(256), 0, st, q8, ldq, s, lds, M, k8, shift, x, ldx);
+  HMOE_CHECK_LAUNCH();
+  return HMOE_OK;
+}
+
+int hmoe_f8_quant_stack(const void* w, int dtype, int64_t E, int64_t K, int64_t N, int64_t stride_we, int64_t stride_wk,
+                        int halves, int transpose, void* q, uint8_t* s, hmoe_stream_t stream) {
+  if (E <= 0 || K <= 0 || N <= 0 || halves < 1 || halves > 2 || N % halves) return HMOE_ERR_ARG;
+  if (dtype != HMOE_DT_BF16 && dtype != HMOE_DT_F16 && dtype != HMOE_DT_F32) return HMOE_ERR_DTYPE;
+  if (!w || !q || !s) return HMOE_ERR_ARG;
+  if (K % 16 || N / halves % 16 || E > kMaxEGemm || K > INT32_MAX - 256 || N > INT32_MAX - 256) return HMOE_ERR_SHAPE;
+  if (!transpose && halves != 1) return HMOE_ERR_SHAPE;  // blocks of a reduction run over all of it
+  if (stride_wk < N || stride_wk % 8 || stride_we % 8 || !al(w, 16) || !al(q, 16)) return HMOE_ERR_ARG;
+  const int kb = (int)((K + kF8Block - 1) / kF8Block), nh = (int)(N / halves), nbh = (nh + kF8Block - 1) / kF8Block;
+  if ((int64_t)kb * halves * nbh >= ((int64_t)1 << 23)) return HMOE_ERR_SHAPE;
+  const int64_t lds = f8_scale_ld(transpose ? K : N);
+  const dim3 grid((unsigned)(kb * halves * nbh), (unsigned)E);
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  auto* q8 = static_cast<uint8_t*>(q);
+  auto go = [&](auto dt, auto tr) {
+    hipLaunchKernelGGL((quant_stack_kernel<decltype(dt)::value, decltype(tr)::value>), grid, dim3(256), 0, st, w, stride_we,
+                       stride_wk, (int)K, nh, halves, q8, s, lds, kb, nbh);
+  };
+  auto by_dt = [&](auto tr) {
+    if (dtype == HMOE_DT_BF16) go(std::integral_constant<int, HMOE_DT_BF16>{}, tr);
+    else if (dtype == HMOE_DT_F16) go(std::integral_constant<int, HMOE_DT_F16>{}, tr);
+    else go(std::integral_constant<int, HMOE_DT_F32>{}, tr);
+  };
+  if (transpose) by_dt(std::true_type{});
+  else by_dt(std::false_type{});
+  HMOE_CHECK_LAUNCH();
+  return HMOE_OK;
+}
+
+int hmoe_f8_grouped_mm(const void* a, int64_t lda, const uint8_t* a_s, int64_t lda_s, const void* w, const uint8_t* w_s,
+                       int64_t E, int64_t K, int64_t N, int halves, const void* counts, int counts_dtype, int64_t M,
+                       const int32_t* a_idx, const int32_t* y_idx, const void* scale, int scale_dtype, int scale_by_y, void* y,
+                       int64_t ldy, int y_dtype, hmoe_stream_t stream) {
+  int rc = f8_check(a, lda, a_s, lda_s, a_idx, w, w_s, E, K, N, halves, counts, counts_dtype, M);
+  if (rc) return rc;
+  if (y_dtype != HMOE_DT_BF16 && y_dtype != HMOE_DT_F16 && y_dtype != HMOE_DT_F32) return HMOE_ERR_DTYPE;
+  if (scale && scale_dtype != HMOE_DT_BF16 && scale_dtype != HMOE_DT_F16 && scale_dtype != HMOE_DT_F32) return HMOE_ERR_DTYPE;
+  if (M == 0) return HMOE_OK;
+  if (!y || !al(y, 16) || ldy < N || ldy % 8) return HMOE_ERR_ARG;
+  F8Params p = f8_params(a, lda, a_s, lda_s, a_idx, w, w_s, E, K, N, halves, counts, counts_dtype, M);
+  p.C = y;
+  p.ldc = ldy;
+  p.y_idx = y_idx;
+  p.scale = scale;
+  p.scale_dt = scale_dtype;
+  p.scale_by_y = scale_by_y && y_idx;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (y_dtype == HMOE_DT_BF16) return f8_pick<F8_STORE, HMOE_DT_BF16>(p, s);
+  if (y_dtype == HMOE_DT_F16) return f8_pick<F8_STORE, HMOE_DT_F16>(p, s);
+  return f8_pick<F8_STORE, HMOE_DT_F32>(p, s);
+}
+
+int hmoe_f8_gate_up_swiglu(const void* x, int64_t ldx, const uint8_t* x_s, int64_t ldx_s, const int32_t* a_idx, const void* wgu,
+                           const uint8_t* wgu_s, int64_t E, int64_t d, int64_t h, const void* counts, int counts_dtype,
+                           int64_t M, void* act, uint8_t* act_s, hmoe_stream_t stream) {
+  if (h <= 0) return HMOE_ERR_ARG;
+  int rc = f8_check(x, ldx, x_s, ldx_s, a_idx, wgu, wgu_s, E, d, 2 * h, 2, counts, counts_dtype, M);
+  if (rc || M == 0) return rc;
+  if (!act || !act_s || !al(act, 16)) return HMOE_ERR_ARG;
+  F8Params p = f8_params(x, ldx, x_s, ldx_s, a_idx, wgu, wgu_s, E, d, 2 * h, 2, counts, counts_dtype, M);
+  p.C = act;
+  p.ldc = h;
+  p.Cs = act_s;
+  p.ldcs = f8_scale_ld(h);
+  return f8_pick<F8_SWIGLU, HMOE_DT_I8>(p, reinterpret_cast<hipStream_t>(stream));
+}
+
+}  // extern "C"
+
+// The experts of a routed layer for given routing: x quantised, dispatch, gate/up with SwiGLU and act quantised, down with the
+// routing weights (fp32 as given) and scatter, over one workspace.
+namespace {
+
+size_t al256(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
+
+struct F8Layout {
+  size_t x8, xs, counts, starts, order, a_idx, dws, act, act_s, total, dws_bytes;
+};
+
+bool f8_layout(int64_t T, int64_t d, int E, int k, int64_t h, F8Layout& L) {
+  if (T < 0 || d <= 0 || E <= 0 || k <= 0 || h <= 0 || T > INT32_MAX || d > INT32_MAX || h > INT32_MAX || k > 1024) return false;
+  const size_t t = static_cast<size_t>(T), M = t * static_cast<size_t>(k);
+  L.dws_bytes = hmoe_dispatch_workspace_size(T, k, E);
+  size_t o = 0;
+  auto take = [&](size_t bytes) {
+    const size_t at = o;
+    o += al256(bytes > 0 ? bytes : 1);
+    return at;
+  };
+  L.x8 = take(t * static_cast<size_t>(d));
+  L.xs = take(t * static_cast<size_t>(f8_scale_ld(d)));
+  L.counts = take(static_cast<size_t>(E) * 4);
+  L.starts = take(static_cast<size_t>(E + 1) * 4);
+  L.order = take(M * 4);
+  L.a_idx = take(M * 4);
+  L.dws = take(L.dws_bytes);
+  L.act = take(M * static_cast<size_t>(h));
+  L.act_s = take(M * static_cast<size_t>(f8_scale_ld(h)));
+  L.total = o;
+  return true;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t hmoe_f8_moe_experts_workspace_size(int64_t T, int64_t d, int E, int k, int64_t h) {
+  F8Layout L;
+  return f8_layout(T, d, E, k, h, L) ? L.total : 0;
+}
+
+int hmoe_f8_moe_experts(const void* x, int64_t ldx, int dtype, const void* topk_ids, int ids_dtype, const void* topk_w,
+                        int topk_w_dtype, const void* wgu, const uint8_t* wgu_s, const void* wd, const uint8_t* wd_s, int64_t T,
+                        int64_t d, int E, int k, int64_t h, void* y, int32_t* inv_pos, int32_t* n_invalid, void* workspace,
+                        size_t workspace_bytes, hmoe_stream_t stream) {
+  F8Layout L;
+  if (!f8_layout(T, d, E, k, h, L)) return HMOE_ERR_ARG;
+  if (dtype != HMOE_DT_BF16 && dtype != HMOE_DT_F16) return HMOE_ERR_DTYPE;
+  if (topk_w_dtype != HMOE_DT_F32 && topk_w_dtype != HMOE_DT_BF16 && topk_w_dtype != HMOE_DT_F16) return HMOE_ERR_DTYPE;
+  if (!workspace || workspace_bytes < L.total || (reinterpret_cast<uintptr_t>(workspace) & 255u)) return HMOE_ERR_WORKSPACE;
+  // every launch's limits ahead of the first, so that a refused call launches nothing (an empty input only runs the dispatch)
+  if (T > 0 && (!x || !topk_ids || !topk_w || !wgu || !wgu_s || !wd || !wd_s || !y || ldx < d || ldx % 8 || !al(x, 16) ||
+                !al(wgu, 16) || !al(wgu_s, 16) || !al(wd, 16) || !al(wd_s, 16) || !al(y, 16)))
+    return HMOE_ERR_ARG;
+  const int64_t lim = ((int64_t)1 << 31) - 32768, M = T * k;
+  if (d % 16 || h % 16 || E > kMaxEGemm || M > INT32_MAX - 256 || d > lim / (2 * h) || d > lim / 256 || h > lim / 256 ||
+      M > lim / d)
+    return HMOE_ERR_SHAPE;
+  char* ws = static_cast<char*>(workspace);
+  auto* counts = reinterpret_cast<int32_t*>(ws + L.counts);
+  auto* order = reinterpret_cast<int32_t*>(ws + L.order);
+  auto* a_idx = reinterpret_cast<int32_t*>(ws + L.a_idx);
+  auto* xs = reinterpret_cast<uint8_t*>(ws + L.xs);
+  auto* act_s = reinterpret_cast<uint8_t*>(ws + L.act_s);
+  int rc = hmoe_dispatch_tiles(topk_ids, ids_dtype, topk_w, topk_w_dtype, T, k, E, nullptr, 0, 0, nullptr, nullptr, counts,
+                               nullptr, reinterpret_cast<int32_t*>(ws + L.starts), order, a_idx, inv_pos, nullptr, n_invalid,
+                               ws + L.dws, L.dws_bytes, dtype, stream);
+  if (rc != HMOE_OK || M == 0) return rc;
+  rc = hmoe_f8_quant_rows(x, ldx, dtype, T, d, ws + L.x8, d, xs, f8_scale_ld(d), stream);
+  if (rc != HMOE_OK) return rc;
+  rc = hmoe_f8_gate_up_swiglu(ws + L.x8, d, xs, f8_scale_ld(d), a_idx, wgu, wgu_s, E, d, h, counts, HMOE_DT_I32, M, ws + L.act,
+                              act_s, stream);
+  if (rc != HMOE_OK) return rc;
+  return hmoe_f8_grouped_mm(ws + L.act, h, act_s, f8_scale_ld(h), wd, wd_s, E, h, d, 1, counts, HMOE_DT_I32, M, nullptr, order,
+                            topk_w, topk_w_dtype, 1, y, d, dtype, stream);
+}
+
+}  // extern "C"

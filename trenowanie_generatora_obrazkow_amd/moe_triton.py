@@ -11,6 +11,7 @@ from __future__ import annotations
 import torch
 
 from . import ops
+from .layer import _recorded
 
 BLOCK_M = 64  # aurora/moe_triton.py:13 -- the row granularity of make_schedule's blocks
 
@@ -38,7 +39,12 @@ def grouped_mm(a: torch.Tensor, w: torch.Tensor, counts: torch.Tensor, sched=Non
     a is bf16 or fp16 (the products run on the matching MFMA, the output has a's type); w has a's type, or is int8
     with w_scale (E, N) (aurora/moe_triton.py:44-51): the integers enter the 16-bit products exactly and the
     per-column scale multiplies the fp32 sum, before `scale`.  K and N need not be multiples of the copy granule:
-    such operands are zero-padded on the device first (pad_operands)."""
+    such operands are zero-padded on the device first (pad_operands).
+    w may be an ops.F8Stack: a is quantised to 8 bits (a scale per 128 columns) and the product runs in 8-bit floating point; K
+    and N are then multiples of 16.  That product is differentiable in a (sorted rows, without a_idx, y_idx and scale; the stack
+    made with grad=True): the gradient is quantised in the same way."""
+    if isinstance(w, ops.F8Stack):
+        return _grouped_mm_f8(a, w, counts, a_idx, y_idx, scale, w_scale)
     M = a_idx.numel() if a_idx is not None else a.shape[0]
     assert w.stride(2) == 1, "w must be (E, K, N) with contiguous rows"
     if a.dtype not in (torch.bfloat16, torch.float16) or w.dtype not in (a.dtype, torch.int8):
@@ -56,6 +62,39 @@ def grouped_mm(a: torch.Tensor, w: torch.Tensor, counts: torch.Tensor, sched=Non
     y = ops.grouped_mm(a, w, counts, M, a_idx=a_idx.contiguous() if a_idx is not None else None,
                        y_idx=y_idx.contiguous() if y_idx is not None else None, scale=scale, w_scale=w_scale)
     return y if y.shape[1] == N else y[:, :N].contiguous()
+
+
+def _grouped_mm_f8(a, w, counts, a_idx, y_idx, scale, w_scale):
+    if w_scale is not None:
+        raise ValueError("an F8Stack holds its own scales")
+    if a.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise TypeError(f"a: bf16, fp16 or fp32 expected (got {a.dtype})")
+    if _recorded(a, scale):
+        if a_idx is not None or y_idx is not None or scale is not None:
+            raise ValueError("an 8-bit grouped_mm with a gradient takes sorted rows: no a_idx, y_idx and scale")
+        if w.grad_q is None:
+            raise ValueError("a gradient of a needs an F8Stack made with grad=True")
+        return _GroupedMMF8.apply(a, w, counts)
+    a_idx, y_idx = (i if i is None else i.to(torch.int32).contiguous() for i in (a_idx, y_idx))
+    scale = scale if scale is None else scale.contiguous()
+    return ops.grouped_mm_f8(*ops.quant_rows(a.detach()), w, counts.contiguous(), a_idx=a_idx, y_idx=y_idx, scale=scale,
+                             dtype=a.dtype)
+
+
+class _GroupedMMF8(torch.autograd.Function):
+    """y = Q(a) w, and da = Q(dy) w^T: the gradient of the product, taken in the same 8 bits (Q itself as the identity)."""
+
+    @staticmethod
+    def forward(ctx, a, w, counts):
+        counts = counts.contiguous()
+        ctx.w = w
+        ctx.save_for_backward(counts)
+        return ops.grouped_mm_f8(*ops.quant_rows(a), w, counts, dtype=a.dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        return ops.grouped_mm_f8_bwd(dy.contiguous(), ctx.w, ctx.saved_tensors[0]), None, None
 
 
 def pad_operands(a, w, w_scale=None):

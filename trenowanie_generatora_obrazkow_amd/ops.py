@@ -191,7 +191,12 @@ def moe_experts(x, ids, tw, wgu, wd, wgu_s=None, wd_s=None):
     routed_gate_up (with inv_pos) and down_scatter with the same outputs.  x (T, d) bf16 or fp16 with contiguous rows;
     ids (T, k) int32 / int64; tw (T, k); wgu (E, d, 2h) and wd (E, h, d) of x's type, or int8 with scales wgu_s
     (E, 2h) and wd_s (E, d) -> (y (T*k, d) in (token, slot) order, inv_pos (T*k,) int32, n_invalid (1,) int32); the
-    combine (with inv_pos) sums y over the slots."""
+    combine (with inv_pos) sums y over the slots.  wgu and wd may be F8Stacks (of 2 halves and of one): x and the activation
+    are then quantised to 8 bits on the way, and the routing weights are not rounded."""
+    if isinstance(wgu, F8Stack) or isinstance(wd, F8Stack):
+        if wgu_s is not None or wd_s is not None:
+            raise ValueError("F8Stacks hold their own scales")
+        return _moe_experts_f8(x, ids, tw, wgu, wd)
     T, k = ids.shape
     if probe is not None and any(n in probe for n in _FWD_OPS):
         # event timing of single ops (bench.py's probe): the same entry points one by one
@@ -1085,3 +1090,225 @@ def grad_clip(grads, sq_norm, max_norm, out=None):
         raise ValueError("a tensor to be written lies over another gradient or output of the call, or over its own gradient "
                          "in another type") from e
     return norm
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# Experts in 8-bit floating point (e4m3 values, a power-of-two scale per block of 128)
+# ---------------------------------------------------------------------------------------------------------------
+_E4M3, _E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+
+
+def _f8_ld(K):
+    return -(-K // 2048) * 16  # hmoe_f8_scale_ld: one byte per 128 columns, in whole 16 bytes
+
+
+def quant_rows(x):
+    """Rows x (M, K) bf16, fp16 or fp32 in 8 bits with a scale per 128 columns -> (q (M, K) float8_e4m3fn, s
+    (M, ceil(K / 128)) float8_e8m0fnu): x is about q * s.  s is 2^e with the least e >= -126 that brings the block's largest finite
+    value to at most 448; infinities and NaNs become NaN.  K a multiple of 16."""
+    M, K, ld = _rows(x, "x")
+    if K % 16:
+        raise ValueError(f"x: width {K} must be a multiple of 16")
+    q = torch.empty(M, K, device=x.device, dtype=_E4M3)
+    s = torch.empty(M, _f8_ld(K), device=x.device, dtype=_E8M0)
+    _call_on(x.device, "hmoe_f8_quant_rows", L.ptr(x), ld, L.dt(x), M, K, L.ptr(q), K, L.ptr(s), s.shape[1])
+    return q, s[:, :-(-K // 128)]
+
+
+def _f8_rows(q, s, block=128):
+    """(M, K, row stride, scale row stride) of quantised rows."""
+    L.require_gpu(q, "q")
+    if q.dim() != 2 or q.dtype != _E4M3 or s.dtype != _E8M0:
+        raise TypeError(f"quantised rows are (M, K) float8_e4m3fn with float8_e8m0fnu scales (got {q.dtype}, {s.dtype})")
+    M, K = q.shape
+    if s.device != q.device:
+        raise ValueError(f"the scales are on {s.device}, the rows on {q.device}")
+    if tuple(s.shape) != (M, -(-K // block)):
+        raise ValueError(f"scales of shape {tuple(s.shape)}, expected {(M, -(-K // block))}")
+    ld = q.stride(0) if M > 1 else K
+    lds = s.stride(0) if M > 1 else max(s.stride(0), _f8_ld(K) if block == 128 else s.shape[1])
+    if (K and q.stride(1) != 1) or ld < K or (s.shape[1] > 1 and s.stride(1) != 1):
+        raise ValueError("quantised rows and their scales must be contiguous in themselves")
+    if block == 128 and (ld % 16 or lds % 16 or lds < _f8_ld(K) or q.data_ptr() % 16 or s.data_ptr() % 16):
+        raise ValueError("quantised rows and scale rows lie 16-byte aligned, as quant_rows gives them")
+    return M, K, ld, lds
+
+
+def dequant_rows(q, s, dtype=torch.float32, block=128):
+    """The values of quantised rows (quant_rows; block=32: swiglu_pack's) -> (M, K) of `dtype` (fp32 holds them exactly)."""
+    M, K, ld, lds = _f8_rows(q, s, block)
+    if dtype not in _FLOATS:
+        raise TypeError(f"dtype {dtype} not in {_FLOATS}")
+    x = torch.empty(M, K, device=q.device, dtype=dtype)
+    if K:
+        _call_on(q.device, "hmoe_f8_dequant_rows", L.ptr(q), ld, L.ptr(s), lds, M, K, block, L.ptr(x), K, L.dt(dtype))
+    return x
+
+
+@dataclass
+class F8Stack:
+    """Expert weights (E, K, N) in 8 bits, laid out for the products: q (E, N, K) float8_e4m3fn with its scales s, and, for the
+    gradient of the rows, grad_q (E, K, N) and grad_s.  halves = 2 for [gate | up] stacks (each half's blocks from its own first
+    column).  Frozen: no gradient reaches the weights."""
+
+    q: torch.Tensor
+    s: torch.Tensor
+    halves: int = 1
+    grad_q: torch.Tensor | None = None
+    grad_s: torch.Tensor | None = None
+
+    @property
+    def shape(self):
+        """(E, K, N), as of the stack it was made from."""
+        return torch.Size((self.q.shape[0], self.q.shape[2], self.q.shape[1]))
+
+    @property
+    def device(self):
+        return self.q.device
+
+    @classmethod
+    def from_weights(cls, w, halves=1, grad=False):
+        """w (E, K, N) bf16, fp16 or fp32, N contiguous; K and N / halves multiples of 16.  grad=True also keeps the layout that
+        the gradient of the rows reads (as many bytes again)."""
+        L.require_gpu(w, "w")
+        if w.dim() != 3 or w.dtype not in _FLOATS:
+            raise TypeError(f"w must be an (E, K, N) stack of bf16, fp16 or fp32 (got {tuple(w.shape)} {w.dtype})")
+        E, K, N = w.shape
+        if halves not in (1, 2) or min(E, K, N) < 1 or N % halves:
+            raise ValueError(f"w {tuple(w.shape)} in {halves} halves")
+        if K % 16 or N // halves % 16:
+            raise ValueError(f"w {tuple(w.shape)}: K and N / halves must be multiples of 16")
+        w = w.detach()
+        if w.stride(2) != 1 or w.stride(1) < N or w.stride(1) % 8 or w.stride(0) % 8 or w.data_ptr() % 16:
+            w = w.contiguous() if not w.is_contiguous() else w.clone()
+        nb = -(-(N // halves) // 128)
+        st = cls(torch.empty(E, N, K, device=w.device, dtype=_E4M3),
+                 torch.zeros(E, halves * nb, _f8_ld(K), device=w.device, dtype=torch.uint8).view(_E8M0), halves)
+        args = (L.ptr(w), L.dt(w), E, K, N, w.stride(0), w.stride(1))
+        _call_on(w.device, "hmoe_f8_quant_stack", *args, halves, 1, L.ptr(st.q), L.ptr(st.s))
+        if grad:
+            st.grad_q = torch.empty(E, K, N, device=w.device, dtype=_E4M3)
+            st.grad_s = torch.zeros(E, -(-K // 128), _f8_ld(N), device=w.device, dtype=torch.uint8).view(_E8M0)
+            _call_on(w.device, "hmoe_f8_quant_stack", *args, 1, 0, L.ptr(st.grad_q), L.ptr(st.grad_s))
+        return st
+
+    def to(self, device):
+        """The stack on another device."""
+        return F8Stack(*(t.to(device) if isinstance(t, torch.Tensor) else t
+                         for t in (self.q, self.s, self.halves, self.grad_q, self.grad_s)))
+
+    def dequant(self):
+        """The values it stands for, (E, K, N) fp32."""
+        E, K, N = self.shape
+        s = self.s.to(torch.float32)[:, :, :-(-K // 128)]
+        rows = torch.cat([torch.arange(N // self.halves, device=s.device) // 128 + i * (s.shape[1] // self.halves)
+                          for i in range(self.halves)])
+        return (self.q.to(torch.float32) * s[:, rows].repeat_interleave(128, 2)[:, :, :K]).transpose(1, 2).contiguous()
+
+
+def _f8_stack(w, name, dev, shape=None, halves=None):
+    """Checks a stack handed to a C entry point (its fields are public)."""
+    if not isinstance(w, F8Stack):
+        raise TypeError(f"{name}: an F8Stack expected (got {type(w).__name__})")
+    E, K, N = w.shape
+    if shape is not None and any(want is not None and got != want for got, want in zip((E, K, N), shape)):
+        raise ValueError(f"{name}: shape {(E, K, N)} does not match {shape}")
+    if halves is not None and w.halves != halves:
+        raise ValueError(f"{name}: a stack of {w.halves} halves, {halves} expected")
+    _on(w.q, name, dev, (E, N, K), (_E4M3,))
+    _on(w.s, name + " scales", dev, (E, w.halves * -(-(N // w.halves) // 128), _f8_ld(K)), (_E8M0,))
+    return E, K, N
+
+
+def _f8_mm(q, s, wq, ws, E, K, N, halves, counts, M, a_idx, y_idx, scale, dtype, scale_by_y=False):
+    """hmoe_f8_grouped_mm on checked stacks."""
+    rows, K_, ld, lds = _f8_rows(q, s)
+    dev = q.device
+    if K_ != K:
+        raise ValueError(f"a has {K_} columns, the stack {K} rows")
+    if dtype not in _FLOATS:
+        raise TypeError(f"dtype {dtype} not in {_FLOATS}")
+    counts = _on(counts if counts.dtype in (torch.int32, torch.int64) else counts.to(torch.int64), "counts", dev, (E,),
+                 (torch.int32, torch.int64))
+    a_idx = _on(a_idx, "a_idx", dev, (M,), _I32)
+    y_idx = _on(y_idx, "y_idx", dev, (M,), _I32)
+    if rows < (min(1, M) if a_idx is not None else M):
+        raise ValueError(f"a: {rows} rows for {M} of the product")
+    if a_idx is not None and rows * ld >= 2 ** 31 - 32768:
+        raise ValueError("a gathered through a_idx must span less than 2 GiB (32-bit row offsets)")
+    if scale is not None:
+        scale = _on(scale if scale.dtype in _FLOATS else scale.float(), "scale", dev, (M,), _FLOATS)
+    y = torch.empty(M, N, device=dev, dtype=dtype)
+    _call_on(dev, "hmoe_f8_grouped_mm", L.ptr(q), ld, L.ptr(s), lds, L.ptr(wq), L.ptr(ws), E, K, N, halves, L.ptr(counts),
+             L.dt(counts), M, L.ptr(a_idx), L.ptr(y_idx), L.ptr(scale), L.dt(scale) if scale is not None else 0,
+             int(scale_by_y), L.ptr(y), N, L.dt(dtype))
+    return y
+
+
+def grouped_mm_f8(q, s, w, counts, M=None, a_idx=None, y_idx=None, scale=None, dtype=torch.bfloat16):
+    """grouped_mm on rows in 8 bits (quant_rows) and an F8Stack: y[y_idx[r] or r] = scale[r] * a[a_idx[r] or r] @ w[e(r)] ->
+    (M, N) of `dtype` (bf16, fp16 or fp32), summed in fp32 and rounded once.  Index values are trusted, as in grouped_mm.  Rows
+    that counts name for no expert are zeros; with y_idx they are not written."""
+    E, K, N = _f8_stack(w, "w", q.device)
+    M = (a_idx.numel() if a_idx is not None else q.shape[0]) if M is None else M
+    return _f8_mm(q, s, w.q, w.s, E, K, N, w.halves, counts, M, a_idx, y_idx, scale, dtype)
+
+
+def grouped_mm_f8_bwd(dy, w, counts):
+    """The gradient of grouped_mm_f8's rows: dy (M, N) bf16, fp16 or fp32, sorted by expert, is quantised along N and multiplied
+    by the stack's other layout (F8Stack.from_weights(..., grad=True)) -> (M, K) of dy's type."""
+    E, K, N = _f8_stack(w, "w", dy.device)
+    if w.grad_q is None:
+        raise ValueError("this F8Stack was made without grad=True: it has no layout for the gradient of the rows")
+    _on(w.grad_q, "w.grad_q", dy.device, (E, K, N), (_E4M3,))
+    _on(w.grad_s, "w.grad_s", dy.device, (E, -(-K // 128), _f8_ld(N)), (_E8M0,))
+    q, s = quant_rows(dy)
+    return _f8_mm(q, s, w.grad_q, w.grad_s, E, N, K, 1, counts, dy.shape[0], None, None, None, dy.dtype)
+
+
+def gate_up_swiglu_f8(q, s, wgu, counts, M=None, a_idx=None):
+    """act = silu(g) * u of [g | u] = a[a_idx] @ wgu[e] in fp32, in 8 bits -> (act (M, h) float8_e4m3fn, its scales
+    (M, ceil(h / 128)) float8_e8m0fnu), ready for grouped_mm_f8 with the down stack.  wgu: an F8Stack (E, d, 2h) of 2 halves."""
+    E, d, h2 = _f8_stack(wgu, "wgu", q.device, halves=2)
+    rows, K, ld, lds = _f8_rows(q, s)
+    dev, h = q.device, h2 // 2
+    M = (a_idx.numel() if a_idx is not None else rows) if M is None else M
+    if K != d:
+        raise ValueError(f"a has {K} columns, wgu {d} rows")
+    counts = _on(counts if counts.dtype in (torch.int32, torch.int64) else counts.to(torch.int64), "counts", dev, (E,),
+                 (torch.int32, torch.int64))
+    a_idx = _on(a_idx, "a_idx", dev, (M,), _I32)
+    if rows < (min(1, M) if a_idx is not None else M):
+        raise ValueError(f"a: {rows} rows for {M} of the product")
+    if a_idx is not None and rows * ld >= 2 ** 31 - 32768:
+        raise ValueError("a gathered through a_idx must span less than 2 GiB (32-bit row offsets)")
+    act = torch.empty(M, h, device=dev, dtype=_E4M3)
+    act_s = torch.empty(M, _f8_ld(h), device=dev, dtype=_E8M0)
+    _call_on(dev, "hmoe_f8_gate_up_swiglu", L.ptr(q), ld, L.ptr(s), lds, L.ptr(a_idx), L.ptr(wgu.q), L.ptr(wgu.s), E, d, h,
+             L.ptr(counts), L.dt(counts), M, L.ptr(act), L.ptr(act_s))
+    return act, act_s[:, :-(-h // 128)]
+
+
+def _moe_experts_f8(x, ids, tw, wgu, wd):
+    """moe_experts over F8Stacks (hmoe_f8_moe_experts)."""
+    T, k = ids.shape
+    if x.dim() != 2 or x.shape[0] != T or x.stride(1) != 1:
+        raise ValueError(f"x must be a ({T}, d) matrix with contiguous rows (got {tuple(x.shape)})")
+    L.require_gpu(x, "x")
+    dt, d, dev = _act_dtype(x, "x"), x.shape[1], x.device
+    E, _, h2 = _f8_stack(wgu, "wgu", dev, (None, d, None), 2)
+    h = h2 // 2
+    _f8_stack(wd, "wd", dev, (E, h, d), 1)
+    _on(ids, "topk_ids", dev, (T, k), (torch.int32, torch.int64))
+    tw = _on(tw if tw.dtype in _FLOATS else tw.float(), "topk_weight", dev, (T, k), _FLOATS)
+    ws_bytes = L.lib().hmoe_f8_moe_experts_workspace_size(T, d, E, k, h)
+    if ws_bytes == 0:
+        raise ValueError(f"moe_experts: unsupported sizes T={T} d={d} E={E} k={k} h={h}")
+    ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
+    y = torch.empty(T * k, d, device=dev, dtype=x.dtype)
+    inv = torch.empty(T * k, device=dev, dtype=torch.int32)
+    n_invalid = torch.empty(1, device=dev, dtype=torch.int32)
+    _call_on(dev, "hmoe_f8_moe_experts", L.ptr(x), x.stride(0) if T > 1 else d, dt, L.ptr(ids), L.dt(ids), L.ptr(tw), L.dt(tw),
+             L.ptr(wgu.q), L.ptr(wgu.s), L.ptr(wd.q), L.ptr(wd.s), T, d, E, k, h, L.ptr(y), L.ptr(inv), L.ptr(n_invalid),
+             L.ptr(ws), ws_bytes)
+    return y, inv, n_invalid
