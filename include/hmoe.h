@@ -326,6 +326,10 @@ int hmoe_down_dgrad_swiglu_dw(const void* dy, const int32_t* a_idx, const uint16
                               const void* gu, void* dgu, const int32_t* order, float* dtopk_w, void* workspace,
                               size_t workspace_bytes, hmoe_stream_t stream);
 
+/* The same product alone: dh[r] = dy[a_idx[r] or r] @ wd[e]^T (M, h) bf16, not scaled (hmoe_swiglu_pack_bwd takes it). */
+int hmoe_down_dgrad(const void* dy, const int32_t* a_idx, const void* wd, int64_t E, int64_t h, int64_t d, const void* counts,
+                    int counts_dtype, int64_t M, void* dh, hmoe_stream_t stream);
+
 /* Backward of :79 to the sorted input rows: dxs[r] = dgu[r] @ wgu[e]^T, stored bf16 or fp32 (dxs_dtype). */
 int hmoe_gate_up_dgrad(const void* dgu, const void* wgu, int64_t E, int64_t d, int64_t h, const void* counts,
                        int counts_dtype, int64_t M, void* dxs, int dxs_dtype, hmoe_stream_t stream);
@@ -504,6 +508,20 @@ int hmoe_f8_moe_experts(const void* x, int64_t ldx, int dtype, const void* topk_
                         int topk_w_dtype, const void* wgu, const uint8_t* wgu_s, const void* wd, const uint8_t* wd_s, int64_t T,
                         int64_t d, int E, int k, int64_t h, void* y, int32_t* inv_pos, int32_t* n_invalid, void* workspace,
                         size_t workspace_bytes, hmoe_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------------------------------
+ * SwiGLU with an 8-bit checkpoint of [g | u] (e4m3, a power-of-two scale per 32 columns, as above)
+ * ------------------------------------------------------------------------------------------------------------- */
+
+/* act (M, h) = silu(g) * u of gu (M, 2h) = [g | u] (row stride ldgu), rounded once; q (M, 2h) e4m3 and s (M, 2 ceil(h / 32))
+ * keep g and u: a row's scales of g, then those of u.  bf16 or fp16 (dtype).  h % 8 == 0. */
+int hmoe_swiglu_pack(const void* gu, int64_t ldgu, int64_t M, int64_t h, void* act, void* q, uint8_t* s, int dtype,
+                     hmoe_stream_t stream);
+/* Its backward from what it kept, with da = w[r] * dh[r] (w (M,) fp32, bf16 or fp16; NULL = 1): dgu (M, 2h) = [dg | du]; act
+ * (M, h), the activation of the kept values (NULL to skip); dw[order[r] or r] = <dh[r], that activation before its rounding>
+ * fp32, in a fixed order (NULL to skip). */
+int hmoe_swiglu_pack_bwd(const void* dh, const void* q, const uint8_t* s, const void* w, int w_dtype, int64_t M, int64_t h,
+                         void* dgu, void* act, const int32_t* order, float* dw, int dtype, hmoe_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -117,3 +117,34 @@ def test_reference_against_torch():
         assert torch.equal((b / s).to(torch.float8_e4m3fn).double() * s, q[:, 128 * j:128 * j + 128])
         top = b.abs().amax(1, keepdim=True)
         assert (top <= 448 * s).all() and (top > 224 * s).all()
+
+
+def test_pack_codes(L):
+    def f(gu=P, ld=128, M=4, h=64, act=P, q=P, s=P, dt=BF):
+        return L.hmoe_swiglu_pack(gu, ld, M, h, act, q, s, dt, None)
+    assert f(M=0) == 0 and f(M=-1) == ARG and f(h=0) == ARG and f(h=60) == SHAPE and f(dt=FP) == DTYPE
+    assert f(gu=None) == ARG and f(act=None) == ARG and f(q=None) == ARG and f(s=None) == ARG
+    assert f(ld=120) == ARG and f(ld=132) == ARG and f(gu=P + 8) == ARG and f(act=P + 8) == ARG and f(q=P + 4) == ARG
+
+    def b(dh=P, q=P, s=P, w=P, wdt=FP, M=4, h=64, dgu=P, act=P, dt=BF):
+        return L.hmoe_swiglu_pack_bwd(dh, q, s, w, wdt, M, h, dgu, act, None, P, dt, None)
+    assert b(M=0) == 0 and b(h=60) == SHAPE and b(dt=FP) == DTYPE and b(wdt=I32) == DTYPE
+    assert b(dh=None) == ARG and b(q=None) == ARG and b(s=None) == ARG and b(dgu=None) == ARG
+    assert b(dh=P + 8) == ARG and b(dgu=P + 8) == ARG and b(act=P + 8) == ARG and b(q=P + 4) == ARG
+
+
+def test_down_dgrad_codes(L):
+    def f(dy=P, wd=P, E=2, h=64, d=32, c=P, cdt=I32, M=4, dh=P):
+        return L.hmoe_down_dgrad(dy, None, wd, E, h, d, c, cdt, M, dh, None)
+    assert f(M=0) == 0 and f(dy=None) == ARG and f(wd=None) == ARG and f(dh=None) == ARG and f(c=None) == ARG
+    assert f(h=60) == SHAPE and f(d=36) == SHAPE and f(cdt=FP) == DTYPE and f(dh=P + 8) == ARG
+
+
+def test_pack_wrappers():
+    from trenowanie_generatora_obrazkow_amd import MoESwiGLU, moe_swiglu, ops
+    with pytest.raises((RuntimeError, ValueError)):
+        ops.swiglu_pack(torch.zeros(2, 16, dtype=torch.bfloat16))
+    with pytest.raises(ValueError, match="checkpoint"):
+        MoESwiGLU(16, 16, 2, checkpoint="int8")
+    with pytest.raises(ValueError, match="checkpoint"):
+        moe_swiglu(torch.zeros(2, 16, dtype=torch.bfloat16), None, None, None, 1, checkpoint="bf16")

@@ -90,6 +90,9 @@ SIGNATURES = {
     "hmoe_grad_sq_norm": (_I32, [_P, _P, _P, _I32, _P, _P, _SZ, _P]),
     "hmoe_grad_clip": (_I32, [_P, _P, _P, _P, _P, _I32, _P, _F32, _P, _P]),
     "hmoe_grad_clip_f64": (_I32, [_P, _P, _P, _P, _P, _I32, _P, _F64, _P, _P]),
+    "hmoe_down_dgrad": (_I32, [_P, _P, _P, _I64, _I64, _I64, _P, _I32, _I64, _P, _P]),
+    "hmoe_swiglu_pack": (_I32, [_P, _I64, _I64, _I64, _P, _P, _P, _I32, _P]),
+    "hmoe_swiglu_pack_bwd": (_I32, [_P, _P, _P, _P, _I32, _I64, _I64, _P, _P, _P, _P, _I32, _P]),
     "hmoe_f8_scale_ld": (_SZ, [_I64]),
     "hmoe_f8_quant_rows": (_I32, [_P, _I64, _I32, _I64, _I64, _P, _I64, _P, _I64, _P]),
     "hmoe_f8_dequant_rows": (_I32, [_P, _I64, _P, _I64, _I64, _I64, _I32, _P, _I64, _I32, _P]),

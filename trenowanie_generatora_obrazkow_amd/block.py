@@ -14,12 +14,14 @@ unequal lengths, (d,) for all rows.
 Rows outside the samples are padding: their residual passes through and nothing else does."""
 from __future__ import annotations
 
+from dataclasses import replace
+
 import torch
 import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
 from . import ops
-from .layer import MoESwiGLU, _Experts, _experts_backward, _experts_forward, _experts_infer, _recorded
+from .layer import MoESwiGLU, _check_checkpoint, _experts_backward, _experts_forward, _experts_infer, _recorded
 
 
 def _flat(x):
@@ -120,11 +122,11 @@ def norm_residual(x, y, gate=None, weight=None, norm=True, starts=None, eps=1e-6
 class _MoEResidual(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, wr, wgu, wd, pre_w, scale, shift, post_w, res_gate, cfg):
-        (bias, k, renorm, gate, select_bias, norm, starts, eps, alpha) = cfg
+        (bias, k, renorm, gate, select_bias, norm, starts, eps, alpha, checkpoint) = cfg
         need = any(ctx.needs_input_grad[:9])
         pw, sc, sh, qw, rg = _par(pre_w), _par(scale), _par(shift), _par(post_w), _par(res_gate)
         h = ops.norm_modulate(x, pw, sc, sh, starts, eps, torch.bfloat16)
-        y, ids, tw, state = _experts_forward(h, wr, wgu, wd, bias, k, renorm, gate, select_bias, need)
+        y, ids, tw, state = _experts_forward(h, wr, wgu, wd, bias, k, renorm, gate, select_bias, need, checkpoint)
         out = ops.norm_residual(y, x, rg, qw, norm, starts, eps, alpha, k)
         if need:
             ctx.save_for_backward(x, y, pw, sc, sh, qw, rg, starts, *state.saved)
@@ -141,8 +143,7 @@ class _MoEResidual(torch.autograd.Function):
             return (None,) * 10
         norm, eps, alpha, k = ctx.cfg
         x, y, pw, sc, sh, qw, rg, starts, *saved = ctx.saved_tensors
-        st = ctx.state
-        state = _Experts(tuple(saved), st.k, st.renorm, st.gate, st.select, st.w_dtypes)
+        state = replace(ctx.state, saved=tuple(saved))
         n = ctx.needs_input_grad
         if dout is None:  # a loss on the routing weights alone
             dout = torch.zeros_like(x, memory_format=torch.contiguous_format)
@@ -160,20 +161,21 @@ class _MoEResidual(torch.autograd.Function):
 
 def moe_residual(x, router_weight, w_gu, w_d, top_k, pre_weight=None, scale=None, shift=None, post_weight=None, gate=None,
                  post_norm=True, starts=None, eps=1e-6, alpha=1.0, logit_bias=None, renorm=True, router=None,
-                 select_bias=None):
+                 select_bias=None, checkpoint=None):
     """out (T, d) = alpha * x + gate_b * post_weight * N(moe(N(x) * pre_weight * (1 + scale_b) + shift_b)) of x (T, d), bf16 or
     fp32 (the routed layer runs in bf16), N the RMS norm (post_norm=False: the layer's output itself) -> (out of x's type,
     topk_ids, topk_weight).  The routed layer and its options are moe_swiglu's (`router` its Gate); the other arguments are
     norm_modulate's and norm_residual's."""
     if x.dim() != 2 or x.dtype not in (torch.bfloat16, torch.float32):
         raise TypeError(f"x must be a (T, d) matrix in bf16 or fp32 (got {tuple(x.shape)} {x.dtype})")
+    _check_checkpoint(checkpoint)
     if not _recorded(x, router_weight, w_gu, w_d, pre_weight, scale, shift, post_weight, gate):
         x2 = _flat(x)
         h = ops.norm_modulate(x2, _par(pre_weight), _par(scale), _par(shift), starts, eps, torch.bfloat16)
         y, ids, tw, inv = _experts_infer(h, router_weight, w_gu, w_d, logit_bias, top_k, renorm, router, select_bias)
         out = ops.norm_residual(y, x2, _par(gate), _par(post_weight), post_norm, starts, eps, alpha, top_k, inv)
         return out, ids, tw
-    cfg = (logit_bias, top_k, renorm, router, select_bias, post_norm, starts, eps, alpha)
+    cfg = (logit_bias, top_k, renorm, router, select_bias, post_norm, starts, eps, alpha, checkpoint)
     return _MoEResidual.apply(_flat(x), router_weight, w_gu, w_d, pre_weight, scale, shift, post_weight, gate, cfg)
 
 
@@ -199,6 +201,6 @@ class MoEResidual(nn.Module):
         m = self.mlp
         out, ids, tw = moe_residual(x.reshape(-1, x.shape[-1]), m.router_weight, m.w_gu, m.w_d, m.top_k, self.norm_weight,
                                     scale, shift, self.post_weight, gate, self.post_norm, starts, self.eps, self.alpha,
-                                    m.logit_bias, m.renorm, m.gate, m.select_bias)
+                                    m.logit_bias, m.renorm, m.gate, m.select_bias, m.checkpoint)
         m.last_topk_ids, m.last_topk_weight = ids, tw
         return out.view(x.shape)

@@ -1601,6 +1601,16 @@ static GemmParams down_dgrad_params(const void* dy, const int32_t* a_idx, const 
   return p;
 }
 
+int hmoe_down_dgrad(const void* dy, const int32_t* a_idx, const void* wd, int64_t E, int64_t h, int64_t d, const void* counts,
+                    int counts_dtype, int64_t M, void* dh, hmoe_stream_t stream) {
+  int rc = HMOE_OK;
+  GemmParams p = down_dgrad_params(dy, a_idx, nullptr, wd, E, h, d, counts, counts_dtype, M, dh, dh, &rc);
+  if (rc || M == 0) return rc;
+  p.gu_in = nullptr;
+  p.ldc = h;
+  return launch_mgroup<MGROUP, false, false, EPI_STORE>(p, h, reinterpret_cast<hipStream_t>(stream));
+}
+
 int hmoe_down_dgrad_swiglu(const void* dy, const int32_t* a_idx, const uint16_t* w_sorted, const void* wd,
                            int64_t E, int64_t h, int64_t d, const void* counts, int counts_dtype, int64_t M,
                            const void* gu, void* dgu, hmoe_stream_t stream) {

@@ -107,9 +107,16 @@ class _Experts:
     gate: Gate | None
     select: bool  # the routing took a selection bias
     w_dtypes: tuple
+    packed: bool = False  # [g | u] is kept in 8 bits, and neither the activation nor the permuted rows
 
 
-def _experts_forward(x, wr, wgu, wd, bias, k, renorm, gate, select_bias, need_grad):
+def _check_checkpoint(checkpoint):
+    if checkpoint not in (None, "fp8"):
+        raise ValueError(f"checkpoint = {checkpoint!r}: None or 'fp8'")
+    return checkpoint is not None
+
+
+def _experts_forward(x, wr, wgu, wd, bias, k, renorm, gate, select_bias, need_grad, checkpoint=None):
     """Routing, dispatch and both projections of x (T, d) bf16 -> (y (T*k, d) in (token, slot) order, ids, weights, state)."""
     _check_layer_args(x, wr, wgu, wd, bias, k)
     if select_bias is not None and tuple(select_bias.shape) != (wgu.shape[0],):
@@ -118,6 +125,17 @@ def _experts_forward(x, wr, wgu, wd, bias, k, renorm, gate, select_bias, need_gr
     w_dtypes = (wr.dtype, wgu.dtype, wd.dtype)
     wr, wgu, wd = _bf16(wr), _bf16(wgu), _bf16(wd)
     logits, ids, tw = _route(x, wr, bias, k, renorm, gate, select_bias)
+    packed = _check_checkpoint(checkpoint) and need_grad
+    if packed:
+        # [g | u] by the plain product, then act and the 8-bit copy in one pass over it: the same bytes as the fused epilogue
+        # with a copy of [g | u], and nothing 16 bits wide stays behind
+        disp = ops.dispatch(ids, wgu.shape[0], topk_w=tw, want_xs=False, dtype=x.dtype)
+        act, kept = ops.swiglu_pack(ops.grouped_mm(x, wgu, disp.counts, M, a_idx=disp.a_idx))
+        y, _ = ops.down_scatter(act, wd, disp.counts, M, disp.w_sorted, disp.order)
+        saved = (x, wr, wgu, wd, logits, ids, disp.counts, disp.order, disp.a_idx, disp.inv_pos, disp.w_sorted, kept.q, kept.s)
+        if gate is not None or select_bias is not None:
+            saved += (tw,)
+        return y, ids, tw, _Experts(saved, k, renorm, gate, select_bias is not None, w_dtypes, True)
     # The dispatch writes the routed rows as row-group tiles for the gate/up GEMM; with a backward to follow,
     # also the row-major permuted copy xs (the gate/up weight gradient reads it).
     disp, act, gu = ops.routed_gate_up(x, ids, wgu.shape[0], wgu, topk_w=tw, keep_gu=need_grad, want_xs=need_grad,
@@ -135,7 +153,8 @@ def _experts_forward(x, wr, wgu, wd, bias, k, renorm, gate, select_bias, need_gr
 def _experts_backward(state, dout, dtw_out, need_x, need_wr, need_wgu, need_wd):
     """(dx, dwr, dwgu, dwd), None where not needed, from dout (T, d) bf16, the gradient of every slot of y, and dtw_out
     (T, k), that of the returned weights, or None."""
-    x, wr, wgu, wd, logits, ids, counts, order, a_idx, inv_pos, w_sorted, xs, gu, act, *tw = state.saved
+    x, wr, wgu, wd, logits, ids, counts, order, a_idx, inv_pos, w_sorted, xs, gu, *rest = state.saved
+    act, tw = (None, rest) if state.packed else (rest[0], rest[1:])  # (packed: xs and gu are the checkpoint's q and s)
     k = state.k
     T = x.shape[0]
     E = wgu.shape[0]
@@ -144,12 +163,18 @@ def _experts_backward(state, dout, dtw_out, need_x, need_wr, need_wgu, need_wd):
     disp = ops.Dispatch(counts, None, None, order, a_idx, inv_pos, w_sorted, xs)
     # One stream: every GEMM is a persistent launch sized to own all CUs, so two of them side by side only
     # queue each other's workgroups behind long-running tiles.
-    dys, _ = ops.combine_bwd(dout, None, disp, k)
-    dwd = dwgu = None
+    dys = dwd = dwgu = dgu = dtw = None
+    if state.packed:
+        kept = ops.PackedGU(xs, gu, torch.bfloat16)
+        dgu, act, dtw = ops.swiglu_pack_bwd(ops.down_dgrad(dout, wd, counts, M, a_idx=a_idx), kept, w_sorted, order, want_act=need_wd)
+        dtw = dtw.view(T, k)
+        xs = ops.dispatch(ids, E, x=x, want_inv=False).xs if need_wgu else None
     if need_wd:
+        dys, _ = ops.combine_bwd(dout, None, disp, k)
         dwd = _to_param(ops.grouped_wgrad(act, dys, counts, E, dtype=_grad_dtype(wd_dt)), wd_dt)
-    # dgu, and the routing-weight gradient <dout[t], act[r] @ wd[e]> from the same fp32 product
-    dgu, dtw = ops.down_dgrad_swiglu_dw(dout, wd, counts, M, gu, order, k, a_idx=a_idx, w_sorted=w_sorted)
+    if not state.packed:
+        # dgu, and the routing-weight gradient <dout[t], act[r] @ wd[e]> from the same fp32 product
+        dgu, dtw = ops.down_dgrad_swiglu_dw(dout, wd, counts, M, gu, order, k, a_idx=a_idx, w_sorted=w_sorted)
     if dtw_out is not None:  # the returned routing weights are outputs too: their gradient joins the combine's
         dtw = dtw + dtw_out.to(torch.float32)
     if need_wgu:
@@ -169,9 +194,9 @@ def _experts_backward(state, dout, dtw_out, need_x, need_wr, need_wgu, need_wd):
 
 class _MoEFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, wr, wgu, wd, bias, k, renorm, gate=None, select_bias=None):
+    def forward(ctx, x, wr, wgu, wd, bias, k, renorm, gate=None, select_bias=None, checkpoint=None):
         need_grad = any(ctx.needs_input_grad[:4])
-        y, ids, tw, state = _experts_forward(x, wr, wgu, wd, bias, k, renorm, gate, select_bias, need_grad)
+        y, ids, tw, state = _experts_forward(x, wr, wgu, wd, bias, k, renorm, gate, select_bias, need_grad, checkpoint)
         out = ops.combine(y, x.shape[0], k)
         if need_grad:
             ctx.save_for_backward(*state.saved)
@@ -183,7 +208,7 @@ class _MoEFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dout, _dids, dtw_out):
-        none = (None,) * 5
+        none = (None,) * 6
         if dout is None and dtw_out is None:
             return (None,) * 4 + none
         state = replace(ctx.state, saved=ctx.saved_tensors)
@@ -194,17 +219,20 @@ class _MoEFunction(torch.autograd.Function):
         return _experts_backward(state, dout, dtw_out, *ctx.needs_input_grad[:4]) + none
 
 
-def moe_swiglu(x, router_weight, w_gu, w_d, top_k, logit_bias=None, renorm=True, gate=None, select_bias=None):
+def moe_swiglu(x, router_weight, w_gu, w_d, top_k, logit_bias=None, renorm=True, gate=None, select_bias=None, checkpoint=None):
     """Functional form: x (T, d) bf16 -> (out (T, d) bf16, topk_ids (T, k) int32, topk_weight (T, k) fp32).
 
     router_weight (E, d), w_gu (E, d, 2h) = [gate | up], w_d (E, h, d): bf16, or fp32 / fp16 (rounded to bf16 for
     the products, gradients in the weights' dtype).  logit_bias (E,) fp32 is added to the router logits (no gradient).  Gradients reach
     x and the three weights from `out` and from `topk_weight` (softmax + renormalisation Jacobian).  gate: a Gate for sigmoid
     scores, groups or a factor on the weights; select_bias (E,) fp32 joins the scores for the selection only (a bias for
-    balance; no gradient).  Without a
+    balance; no gradient).  checkpoint="fp8" keeps [g | u] for the backward in 8 bits (ops.swiglu_pack), and neither the
+    activation nor the permuted rows: about a third of the memory; the forward is the same but for act's single rounding, the
+    gradients are those at the kept g and u.  Without a
     gradient to record (grad mode off, or no input requiring one) the forward runs as one C call
     (ops.moe_forward; with a gate or a selection bias, the routing and ops.moe_experts): the same kernels and outputs, a
     fraction of the host time."""
+    _check_checkpoint(checkpoint)
     if not _recorded(x, router_weight, w_gu, w_d):
         if gate is None and select_bias is None:
             _check_layer_args(x, router_weight, w_gu, w_d, logit_bias, top_k)
@@ -213,7 +241,7 @@ def moe_swiglu(x, router_weight, w_gu, w_d, top_k, logit_bias=None, renorm=True,
             return out, ids, tw
         y, ids, tw, inv = _experts_infer(x, router_weight, w_gu, w_d, logit_bias, top_k, renorm, gate, select_bias)
         return ops.combine(y, x.shape[0], top_k, inv_pos=inv), ids, tw
-    return _MoEFunction.apply(x, router_weight, w_gu, w_d, logit_bias, top_k, renorm, gate, select_bias)
+    return _MoEFunction.apply(x, router_weight, w_gu, w_d, logit_bias, top_k, renorm, gate, select_bias, checkpoint)
 
 
 def _experts_infer(x, wr, wgu, wd, bias, k, renorm, gate, select_bias):
@@ -263,14 +291,18 @@ class MoESwiGLU(nn.Module):
     fp32, which joins the scores for the selection only: a training script that balances its experts without a loss raises
     it for experts that got too few tokens and lowers it for the others.
 
+    `checkpoint="fp8"` keeps [g | u] for the backward in 8 bits and nothing else of the experts' activations (moe_swiglu).
+
     The products run in bf16 (any other input dtype is rounded to bf16 first); the output has the dtype the
     reference's SwiGLU would return: the autocast dtype inside autocast, else the input's dtype.  The routing of the
     last call is kept in `last_topk_ids` / `last_topk_weight` (the weights carry gradient)."""
 
     def __init__(self, dim: int, hidden: int, experts: int, top_k: int = 2, renorm: bool = True,
                  init_std: float | None = None, device=None, dtype=torch.bfloat16, gate: Gate | None = None,
-                 balance: bool = False):
+                 balance: bool = False, checkpoint: str | None = None):
         super().__init__()
+        _check_checkpoint(checkpoint)
+        self.checkpoint = checkpoint
         self.dim, self.hidden, self.experts, self.top_k, self.renorm = dim, hidden, experts, top_k, renorm
         self.gate = gate
         f = dict(device=device, dtype=dtype)
@@ -290,6 +322,7 @@ class MoESwiGLU(nn.Module):
     def __setstate__(self, state):
         super().__setstate__(state)
         self.__dict__.setdefault("gate", None)  # (pickled before the layer had gates)
+        self.__dict__.setdefault("checkpoint", None)
         if "select_bias" not in self._buffers:
             self.__dict__.setdefault("select_bias", None)
 
@@ -313,7 +346,7 @@ class MoESwiGLU(nn.Module):
         if x.dtype != torch.bfloat16:
             x = x.to(torch.bfloat16)
         out, ids, tw = moe_swiglu(x, self.router_weight, self.w_gu, self.w_d, self.top_k, self.logit_bias,
-                                  self.renorm, self.gate, self.select_bias)
+                                  self.renorm, self.gate, self.select_bias, self.checkpoint)
         self.last_topk_ids, self.last_topk_weight = ids, tw
         out = out.view(shape)
         return out if out.dtype == out_dtype else out.to(out_dtype)

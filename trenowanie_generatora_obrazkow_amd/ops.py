@@ -628,6 +628,20 @@ def down_dgrad_swiglu_dw(dy, wd, counts, M, gu, order, k, a_idx=None, w_sorted=N
     return dgu, dtw
 
 
+def down_dgrad(dy, wd, counts, M, a_idx=None):
+    """dh (M, h) bf16 = dy[a_idx[r] or r] @ wd[e]^T, not scaled: the product of down_dgrad_swiglu alone."""
+    _need(wd, "wd", (None, None, None), _BF16)
+    E, h, d = wd.shape
+    counts = _counts(counts, E)
+    a_idx = _rows_index(a_idx, "a_idx", M)
+    _need(dy, "dy", (None, d), _BF16, min_rows=min(1, M) if a_idx is not None else M)
+    dh = torch.empty(M, h, device=dy.device, dtype=torch.bfloat16)
+    with _Probe("down_dgrad"):
+        L.call("hmoe_down_dgrad", L.ptr(dy), L.ptr(a_idx), L.ptr(wd), E, h, d, L.ptr(counts), L.dt(counts), M, L.ptr(dh),
+               _dev_stream(dy))
+    return dh
+
+
 def dgrad_parts(M, wgu):
     """Parts the gate/up dgrad's reduction is best split into for M rows (1: not split)."""
     E, d, h2 = wgu.shape
@@ -1312,3 +1326,57 @@ def _moe_experts_f8(x, ids, tw, wgu, wd):
              L.ptr(wgu.q), L.ptr(wgu.s), L.ptr(wd.q), L.ptr(wd.s), T, d, E, k, h, L.ptr(y), L.ptr(inv), L.ptr(n_invalid),
              L.ptr(ws), ws_bytes)
     return y, inv, n_invalid
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# SwiGLU with an 8-bit checkpoint
+# ---------------------------------------------------------------------------------------------------------------
+@dataclass
+class PackedGU:
+    """[g | u] (M, 2h) in 8 bits: q (M, 2h) float8_e4m3fn, s (M, 2 ceil(h / 32)) float8_e8m0fnu, a scale per 32 columns of g, then
+    of u; dtype: the type it had."""
+
+    q: torch.Tensor
+    s: torch.Tensor
+    dtype: torch.dtype
+
+    def dequant(self, dtype=torch.float32):
+        """The values kept, (M, 2h)."""
+        h, nb = self.q.shape[1] // 2, self.s.shape[1] // 2
+        return torch.cat([dequant_rows(self.q[:, i * h:(i + 1) * h], self.s[:, i * nb:(i + 1) * nb], dtype, block=32)
+                          for i in range(2)], 1)
+
+
+def swiglu_pack(gu):
+    """gu (M, 2h) = [g | u] bf16 or fp16 -> (act (M, h) = silu(g) * u, rounded once; PackedGU, g and u in 8 bits).  h a multiple
+    of 8; infinities and NaNs are kept as NaN."""
+    M, h2, ld = _rows(gu, "gu", _H16)
+    if h2 % 16:
+        raise ValueError(f"gu: width {h2} must be twice a multiple of 8")
+    h, dev = h2 // 2, gu.device
+    act = torch.empty(M, h, device=dev, dtype=gu.dtype)
+    kept = PackedGU(torch.empty(M, h2, device=dev, dtype=_E4M3), torch.empty(M, 2 * -(-h // 32), device=dev, dtype=_E8M0), gu.dtype)
+    _call_on(dev, "hmoe_swiglu_pack", L.ptr(gu), ld, M, h, L.ptr(act), L.ptr(kept.q), L.ptr(kept.s), L.dt(gu))
+    return act, kept
+
+
+def swiglu_pack_bwd(dh, kept, w=None, order=None, want_act=True, want_dw=True):
+    """The backward of swiglu_pack from what it kept -> (dgu (M, 2h), act (M, h) or None, dw (M,) fp32 or None).  dh (M, h) of
+    gu's type; w (M,) multiplies its rows (the routing weight); act is the activation of the kept values and dw[order[r] or r]
+    = <dh[r], act[r]>, w's gradient."""
+    M, h, ld = _rows(dh, "dh", _H16)
+    dev = dh.device
+    if ld != h:
+        dh = dh.contiguous()
+    if dh.dtype != kept.dtype:
+        raise TypeError(f"dh: dtype {dh.dtype}, the checkpoint is of {kept.dtype}")
+    _on(kept.q, "the checkpoint", dev, (M, 2 * h), (_E4M3,))
+    _on(kept.s, "the checkpoint's scales", dev, (M, 2 * -(-h // 32)), (_E8M0,))
+    w = _on(w, "w", dev, (M,), _FLOATS)
+    order = _on(order, "order", dev, (M,), _I32)
+    dgu = torch.empty(M, 2 * h, device=dev, dtype=dh.dtype)
+    act = torch.empty(M, h, device=dev, dtype=dh.dtype) if want_act else None
+    dw = torch.empty(M, device=dev, dtype=torch.float32) if want_dw else None
+    _call_on(dev, "hmoe_swiglu_pack_bwd", L.ptr(dh), L.ptr(kept.q), L.ptr(kept.s), L.ptr(w), L.dt(w) if w is not None else 0, M, h,
+             L.ptr(dgu), L.ptr(act), L.ptr(order), L.ptr(dw), L.dt(dh))
+    return dgu, act, dw
