@@ -148,3 +148,34 @@ def test_pack_wrappers():
         MoESwiGLU(16, 16, 2, checkpoint="int8")
     with pytest.raises(ValueError, match="checkpoint"):
         moe_swiglu(torch.zeros(2, 16, dtype=torch.bfloat16), None, None, None, 1, checkpoint="bf16")
+
+
+def test_few_codes(L):
+    n = L.hmoe_few_workspace_size(4, 64, 3, 2, 48, BF, BF)
+    assert n > 0 and L.hmoe_few_workspace_size(17, 64, 3, 2, 48, BF, BF) == 0 and L.hmoe_few_workspace_size(4, 64, 3, 2, 48, HF, BF) == 0
+    P2 = 1 << 16  # 256-byte aligned
+
+    def f(x=P, ldx=64, dt=BF, ids=P, idt=I32, tw=P, twdt=FP, w1=P, s1=None, sdt=BF, w2=P, s2=None, wdt=BF, T=4, d=64, E=3, k=2,
+          h=48, add=None, out=P, ws=P2, n=1 << 24):
+        return L.hmoe_few_experts(x, ldx, dt, ids, idt, tw, twdt, w1, s1, sdt, w2, s2, sdt, wdt, T, d, E, k, h, add, out, ws, n, None)
+    assert f(T=0) == 0 and f(T=-1) == ARG and f(d=0) == ARG and f(k=0) == ARG
+    assert f(dt=FP) == DTYPE and f(wdt=HF) == DTYPE and f(dt=HF, wdt=BF) == DTYPE and f(idt=FP) == DTYPE and f(twdt=I32) == DTYPE
+    assert f(wdt=I8) == ARG and f(s1=P) == ARG and f(wdt=I8, s1=P, s2=P, sdt=HF) == DTYPE and f(wdt=6) == ARG
+    assert f(T=17) == SHAPE and f(k=17) == SHAPE and f(E=1025) == SHAPE and f(d=60, ldx=64) == SHAPE and f(h=44) == SHAPE
+    assert f(wdt=I8, s1=P, s2=P, h=40) == SHAPE
+    assert f(x=None) == ARG and f(ids=None) == ARG and f(tw=None) == ARG and f(w1=None) == ARG and f(w2=None) == ARG and f(out=None) == ARG
+    assert f(ldx=56) == ARG and f(ldx=68) == ARG and f(x=P + 8) == ARG and f(out=P + 8) == ARG and f(add=P + 8) == ARG and f(w1=P + 8) == ARG
+    assert f(ws=None) == WORKSPACE and f(n=n - 1) == WORKSPACE and f(ws=P2 + 64) == WORKSPACE
+
+    def g(wr=P, ids=P, tw=P, k=2, E=3, n=1 << 24):
+        return L.hmoe_few_forward(P, 64, wr, None, P, P, 4, 64, E, k, 48, 1, 1.0, None, P, ids, tw, P2, n, None)
+    assert g(wr=None) == ARG and g(ids=None) == ARG and g(tw=None) == ARG and g(k=4) == SHAPE and g(E=300, n=1 << 28) == SHAPE
+    assert g(n=16) == WORKSPACE
+
+
+def test_few_wrappers():
+    from trenowanie_generatora_obrazkow_amd import ops
+    x = torch.zeros(2, 64, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError):
+        ops.few_experts(x, torch.zeros(2, 1, dtype=torch.int32), torch.ones(2, 1), torch.zeros(1, 64, 32, dtype=torch.bfloat16),
+                        torch.zeros(1, 16, 64, dtype=torch.bfloat16))

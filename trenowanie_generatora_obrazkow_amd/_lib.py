@@ -13,7 +13,7 @@ import torch
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "libhmoe.so")
 
 ERR_OVERLAP = -8
-DT_BF16, DT_F16, DT_F32, DT_I32, DT_I64, DT_I8 = 0, 1, 2, 3, 4, 5
+DT_BF16, DT_F16, DT_F32, DT_I32, DT_I64, DT_I8, DT_F8 = 0, 1, 2, 3, 4, 5, 6
 _DT = {torch.bfloat16: DT_BF16, torch.float16: DT_F16, torch.float32: DT_F32, torch.int32: DT_I32,
        torch.int64: DT_I64, torch.int8: DT_I8}
 
@@ -93,6 +93,11 @@ SIGNATURES = {
     "hmoe_down_dgrad": (_I32, [_P, _P, _P, _I64, _I64, _I64, _P, _I32, _I64, _P, _P]),
     "hmoe_swiglu_pack": (_I32, [_P, _I64, _I64, _I64, _P, _P, _P, _I32, _P]),
     "hmoe_swiglu_pack_bwd": (_I32, [_P, _P, _P, _P, _I32, _I64, _I64, _P, _P, _P, _P, _I32, _P]),
+    "hmoe_few_workspace_size": (_SZ, [_I64, _I64, _I32, _I32, _I64, _I32, _I32]),
+    "hmoe_few_experts": (_I32, [_P, _I64, _I32, _P, _I32, _P, _I32, _P, _P, _I32, _P, _P, _I32, _I32, _I64, _I64, _I32, _I32,
+                                _I64, _P, _P, _P, _SZ, _P]),
+    "hmoe_few_forward": (_I32, [_P, _I64, _P, _P, _P, _P, _I64, _I64, _I32, _I32, _I64, _I32, _F32, _P, _P, _P, _P, _P, _SZ,
+                                _P]),
     "hmoe_f8_scale_ld": (_SZ, [_I64]),
     "hmoe_f8_quant_rows": (_I32, [_P, _I64, _I32, _I64, _I64, _P, _I64, _P, _I64, _P]),
     "hmoe_f8_dequant_rows": (_I32, [_P, _I64, _P, _I64, _I64, _I64, _I32, _P, _I64, _I32, _P]),

@@ -15,7 +15,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB_DIR = os.path.join(HERE, "_lib")
 LIB = os.path.join(LIB_DIR, "libhmoe.so")
-SOURCES = ["route.hip", "gemm.hip", "layer.hip", "norm.hip", "gate.hip", "clip.hip", "f8.hip", "pack.hip"]
+SOURCES = ["route.hip", "gemm.hip", "layer.hip", "norm.hip", "gate.hip", "clip.hip", "f8.hip", "pack.hip", "few.hip"]
 ARCH = os.environ.get("HMOE_ARCH", "gfx950")
 
 # -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 in generated code.

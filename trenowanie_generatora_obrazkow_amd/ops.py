@@ -1380,3 +1380,84 @@ def swiglu_pack_bwd(dh, kept, w=None, order=None, want_act=True, want_dw=True):
     _call_on(dev, "hmoe_swiglu_pack_bwd", L.ptr(dh), L.ptr(kept.q), L.ptr(kept.s), L.ptr(w), L.dt(w) if w is not None else 0, M, h,
              L.ptr(dgu), L.ptr(act), L.ptr(order), L.ptr(dw), L.dt(dh))
     return dgu, act, dw
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# A routed layer for a few tokens
+# ---------------------------------------------------------------------------------------------------------------
+FEW_TOKENS = 16  # the most a call takes
+
+
+def _few_args(x, k, wgu, wd, wgu_s, wd_s, add):
+    """Checks of few_experts and few_forward -> (T, d, row stride, E, h, weight pointers and types, workspace, out)."""
+    if x.dim() != 2 or not x.is_cuda:
+        L.require_gpu(x, "x")
+        raise ValueError(f"x must be a (T, d) matrix (got {tuple(x.shape)})")
+    dt, dev = _act_dtype(x, "x"), x.device
+    T, d = x.shape
+    if T > FEW_TOKENS or not 1 <= k <= 16:
+        raise ValueError(f"{T} tokens in {k} slots: at most {FEW_TOKENS} in 1 to 16")
+    ld = x.stride(0) if T > 1 else d
+    if T and (x.stride(1) != 1 or ld < d or ld % 8 or x.data_ptr() % 16):
+        raise ValueError(f"x: rows must be contiguous, 16-byte aligned, with a row stride of a multiple of 8 (strides {x.stride()})")
+    if isinstance(wgu, F8Stack) or isinstance(wd, F8Stack):
+        if wgu_s is not None or wd_s is not None:
+            raise ValueError("F8Stacks hold their own scales")
+        E, _, h2 = _f8_stack(wgu, "wgu", dev, (None, d, None), 2)
+        h = h2 // 2
+        _f8_stack(wd, "wd", dev, (E, h, d), 1)
+        w_dt = L.DT_F8
+        ws = (L.ptr(wgu.q), L.ptr(wgu.s), 0, L.ptr(wd.q), L.ptr(wd.s), 0, w_dt)
+    else:
+        if wgu.dim() != 3 or wd.dim() != 3 or wgu.dtype not in (x.dtype, torch.int8) or wd.dtype != wgu.dtype:
+            raise TypeError(f"wgu (E, d, 2h) and wd (E, h, d) of x's type, int8 or F8Stacks expected (got {wgu.dtype}, {wd.dtype})")
+        E, h = wgu.shape[0], wd.shape[1]
+        _on(wgu, "wgu", dev, (E, d, 2 * h), (wgu.dtype,))
+        _on(wd, "wd", dev, (E, h, d), (wd.dtype,))
+        wgu_s, wd_s = _w_scale(wgu, wgu_s, 2 * h), _w_scale(wd, wd_s, d)
+        for t, name in ((wgu_s, "wgu_s"), (wd_s, "wd_s")):
+            if t is not None:
+                _on(t, name, dev, t.shape, (t.dtype,))
+        w_dt = L.dt(wgu)
+        ws = (L.ptr(wgu), L.ptr(wgu_s), L.dt(wgu_s) if wgu_s is not None else 0, L.ptr(wd), L.ptr(wd_s),
+              L.dt(wd_s) if wd_s is not None else 0, w_dt)
+    _on(add, "add", dev, (T, d), (x.dtype,))
+    n = L.lib().hmoe_few_workspace_size(T, d, E, k, h, w_dt, dt)
+    if n == 0 and T:
+        raise ValueError(f"few tokens: unsupported sizes T={T} d={d} E={E} k={k} h={h}")
+    return T, d, ld, E, h, ws, torch.empty(n, device=dev, dtype=torch.uint8), torch.empty(T, d, device=dev, dtype=x.dtype)
+
+
+def few_experts(x, ids, tw, wgu, wd, wgu_s=None, wd_s=None, add=None):
+    """The experts of a routed layer and the sum over its slots for up to 16 tokens, in two kernels (hmoe_few_experts): moe_experts
+    and combine in fp32 throughout, rounded once -> out (T, d).  x (T, d) bf16 or fp16; ids (T, k) int32 / int64, those outside
+    [0, E) add nothing; tw (T, k); wgu (E, d, 2h) and wd (E, h, d) of x's type, int8 with scales, or F8Stacks; add (T, d) of x's
+    type (a shared expert's output) joins the sum."""
+    T, k = ids.shape
+    T_, d, ld, E, h, w, ws, out = _few_args(x, k, wgu, wd, wgu_s, wd_s, add)
+    dev = x.device
+    _on(ids, "topk_ids", dev, (T_, k), (torch.int32, torch.int64))
+    tw = _on(tw if tw.dtype in _FLOATS else tw.float(), "topk_weight", dev, (T_, k), _FLOATS)
+    _call_on(dev, "hmoe_few_experts", L.ptr(x), ld, L.dt(x), L.ptr(ids), L.dt(ids), L.ptr(tw), L.dt(tw), *w, T, d, E, k, h,
+             L.ptr(add), L.ptr(out), L.ptr(ws), ws.numel())
+    return out
+
+
+def few_forward(x, wr, wgu, wd, k, bias=None, renorm=True, scaling=1.0, add=None):
+    """moe_forward for up to 16 tokens in two kernels (hmoe_few_forward), in fp32 throughout and rounded once -> (out (T, d),
+    topk_ids (T, k) int32, topk_w (T, k) fp32: those of route_topk).  bf16; add (T, d) joins the sum."""
+    _router_args(x, wr)
+    T, d, ld, E, h, w, ws, out = _few_args(x, k, wgu, wd, None, None, add)
+    dev = x.device
+    if isinstance(wgu, F8Stack) or wgu.dtype != torch.bfloat16:
+        raise TypeError("few_forward takes bf16 experts (few_experts any, with the routing given)")
+    _on(wr, "router weight", dev, (E, d), _BF16)
+    if not 1 <= k <= E:
+        raise ValueError(f"top_k = {k} must lie in [1, {E}]")
+    if bias is not None:
+        bias = _on(bias.to(torch.float32), "logit bias", dev, (E,), (torch.float32,))
+    ids = torch.empty(T, k, device=dev, dtype=torch.int32)
+    tw = torch.empty(T, k, device=dev, dtype=torch.float32)
+    _call_on(dev, "hmoe_few_forward", L.ptr(x), ld, L.ptr(wr), L.ptr(bias), w[0], w[3], T, d, E, k, h, int(bool(renorm)),
+             float(scaling), L.ptr(add), L.ptr(out), L.ptr(ids), L.ptr(tw), L.ptr(ws), ws.numel())
+    return out, ids, tw
