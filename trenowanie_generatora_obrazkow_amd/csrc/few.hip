@@ -24,7 +24,7 @@ namespace hmoe {
 constexpr int kFewT = 16;                // tokens
 constexpr int kFewK = 16;                // slots
 constexpr int kFewM = kFewT * kFewK;     // routed rows
-constexpr int kFewMaxS1 = 8, kFewMaxS2 = 16;
+constexpr int kFewMaxS1 = 4, kFewMaxS2 = 16;
 enum FewW { FW_BF16 = 0, FW_F16 = 1, FW_I8 = 2, FW_F8 = 3 };
 
 // the first kernel leaves the grouping for the second
@@ -428,129 +428,203 @@ __global__ __launch_bounds__(256, 1) void few_up_kernel(FewParams p) {
 // ----------------------------------------------------------------------------------------------------------------
 // The output's columns of one expert's rows over a part of h; the last workgroup of a run of columns sums up
 // ----------------------------------------------------------------------------------------------------------------
+// The parts of the output pass between workgroups of one launch, on XCDs with an L2 each.  They are written and read as
+// agent-scope atomics: these go through to memory and are read from there, so no workgroup has to write a whole L2 back or
+// discard it (a release and an acquire fence per workgroup: 181 us instead of TIME_FEW16 for 16 tokens over 51 experts).
+__device__ __forceinline__ void put_agent(float* p, float a, float b) {
+  const uint64_t v = (uint64_t)__float_as_uint(a) | (uint64_t)__float_as_uint(b) << 32;
+  __hip_atomic_store(reinterpret_cast<uint64_t*>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 get_agent(const float* p) {
+  const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
+}
+
+// act = silu(g) u of a chunk of kFewChunk columns of up to 16 rows, in LDS rows of kFewActLd numbers: the workgroup adds the parts
+// of [g | u] once, eight columns a thread, all loads of a thread in flight together.  16-bit and int8 experts read it as two
+// bf16 numbers; 8-bit floats as the one that Q(act) is (16 threads hold a block of 128).
+constexpr int kFewChunk = 512, kFewActLd = kFewChunk + 8;
+template <int S1, bool F8>
+__device__ __forceinline__ void few_act(const float* __restrict__ p1, int64_t part_stride, const int* rows, int nr, int h, int k0,
+                                        int k1, uint16_t* hi, uint16_t* lo) {
+  const int pieces = (k1 - k0 + 7) / 8, all = F8 ? (pieces + 15) & ~15 : pieces;  // (whole blocks)
+  for (int i = threadIdx.x; i < nr * all; i += 256) {
+    const int r = i / all, c = (i - r * all) * 8, k = k0 + c;
+    float4 x[S1][4];
+    const float* pg = p1 + (int64_t)rows[r] * 2 * h + k;
+    const bool in = k < h && c < k1 - k0;
+#pragma unroll
+    for (int s = 0; s < S1; ++s)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        x[s][j] = in ? *reinterpret_cast<const float4*>(pg + s * part_stride + (j >> 1) * h + (j & 1) * 4)
+                     : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int s = 1; s < S1; ++s)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[0][j].x += x[s][j].x; x[0][j].y += x[s][j].y; x[0][j].z += x[s][j].z; x[0][j].w += x[s][j].w;
+      }
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      v[4 * j] = silu_f(x[0][j].x) * x[0][j + 2].x;
+      v[4 * j + 1] = silu_f(x[0][j].y) * x[0][j + 2].y;
+      v[4 * j + 2] = silu_f(x[0][j].z) * x[0][j + 2].z;
+      v[4 * j + 3] = silu_f(x[0][j].w) * x[0][j + 2].w;
+    }
+    u32x4 a, b;
+    if constexpr (F8) {
+      float m = 0.0f;
+#pragma unroll
+      for (int t = 0; t < 8; ++t) m = fmaxf(m, f8_abs(v[t]));
+      m = bfly_max<8>(bfly_max<4>(bfly_max<2>(bfly_max<1>(m))));
+      const int e = f8_exp(m);
+      const float inv = f8_inv(e);
+      a = f8_widen(make_uint2(f8_pack4(v[0], v[1], v[2], v[3], inv), f8_pack4(v[4], v[5], v[6], v[7], inv)), f8_pow(e));
+    } else {
+      split8(v, a, b);
+      *reinterpret_cast<u32x4*>(lo + r * kFewActLd + c) = b;
+    }
+    *reinterpret_cast<u32x4*>(hi + r * kFewActLd + c) = a;
+  }
+}
+
 template <int W, bool F16>
 __global__ __launch_bounds__(256, 1) void few_down_kernel(FewParams p) {
   using S = FewShape<W>;
   extern __shared__ __attribute__((aligned(16))) float red[];
-  __shared__ int s_last;
+  __shared__ __attribute__((aligned(16))) uint16_t s_hi[16 * kFewActLd], s_lo[W == FW_F8 ? 8 : 16 * kFewActLd];
+  __shared__ int s_row[16];
+  __shared__ float s_w[kFewM];
+  __shared__ int s_ok[kFewM], s_last;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15, q = lane >> 4;
   const int M = p.M;
   const FewHead& hd = *p.head;
   const int part = blockIdx.x % p.S2, run = blockIdx.x / p.S2 % p.runs2, a = blockIdx.x / (p.S2 * p.runs2);
   const int A = hd.active, e = hd.expert[a], n = hd.rows[a], base = hd.base[a];
+  if (tid < M) {
+    s_w[tid] = hd.w[tid];
+    s_ok[tid] = hd.flat_ok[tid];
+  }
   if (a >= A && !(A == 0 && a == 0 && part == 0)) return;
   const int steps = (p.h + S::STEP - 1) / S::STEP;
-  const int k_end = min(steps, (part + 1) * p.per2);
+  const int k_begin = part * p.per2, k_end = min(steps, (part + 1) * p.per2);
+  constexpr int CS = kFewChunk / S::STEP;  // steps per chunk of act
   if (A > 0) {
     for (int r0 = 0; r0 < n; r0 += 16) {
       const int nr = min(16, n - r0);
       const bool has = l16 < nr;
-      const int flat = has ? hd.row[base + r0 + l16] : 0;
-      const float* pg = p.p1 + (int64_t)flat * 2 * p.h;
-      const int64_t pstride = (int64_t)M * 2 * p.h;
-      // act of NV consecutive columns from k on
-      auto act_of = [&](int k, auto nv, float* v) __attribute__((always_inline)) {
-        constexpr int NV = decltype(nv)::value;
-        float gs[NV], us[NV];
-#pragma unroll
-        for (int i = 0; i < NV; ++i) gs[i] = us[i] = 0.0f;
-        if (has) {
-          for (int s = 0; s < p.S1; ++s) {
-#pragma unroll
-            for (int i = 0; i < NV; i += 4) {
-              if (k + i < p.h) {
-                const float4 x = *reinterpret_cast<const float4*>(pg + s * pstride + k + i);
-                const float4 y = *reinterpret_cast<const float4*>(pg + s * pstride + p.h + k + i);
-                gs[i] += x.x; gs[i + 1] += x.y; gs[i + 2] += x.z; gs[i + 3] += x.w;
-                us[i] += y.x; us[i + 1] += y.y; us[i + 2] += y.z; us[i + 3] += y.w;
-              }
-            }
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < NV; ++i) v[i] = silu_f(gs[i]) * us[i];
-      };
+      if (r0 > 0) __syncthreads();
+      if (tid < 16) s_row[tid] = hd.row[base + r0 + min(tid, nr - 1)];
+      __syncthreads();
       f32x4 acc[S::FR];
 #pragma unroll
       for (int j = 0; j < S::FR; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      if constexpr (W != FW_F8) {
-        constexpr int ES = W == FW_I8 ? 1 : 2;
-        const int col = run * S::COLS + l16 * S::NC;
-        const bool cin = col < p.d;
-        const char* pw = static_cast<const char*>(p.wd) + ((int64_t)e * p.h * p.d + col) * ES;
-        for (int st = part * p.per2 + wave; st < k_end; st += 4) {
-          const int k = st * 32 + q * 8;
-          const bool in = k < p.h;
-          uint4 w[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            w[i] = in && cin ? *reinterpret_cast<const uint4*>(pw + (int64_t)(k + i) * p.d * ES) : make_uint4(0, 0, 0, 0);
-          float v[8];
-          act_of(k, std::integral_constant<int, 8>{}, v);
-          u32x4 hi, lo;
-          split8(v, hi, lo);
-#pragma unroll
-          for (int j = 0; j < S::FR; ++j) {
-            if constexpr (W == FW_F16) {  // the weights' 11 bits as two bf16 numbers
-              const u32x4 c = few_column<false, true>(w, j);
-              float f[8];
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                f[2 * i] = h_lo(c[i]);
-                f[2 * i + 1] = h_hi(c[i]);
-              }
-              u32x4 wh, wl;
-              split8(f, wh, wl);
-              acc[j] = few_mfma<false>(wl, hi, acc[j]);
-              acc[j] = few_mfma<false>(wh, lo, acc[j]);
-              acc[j] = few_mfma<false>(wh, hi, acc[j]);
-            } else {
-              const u32x4 c = few_column<W == FW_I8, false>(w, j);
-              acc[j] = few_mfma<false>(c, lo, acc[j]);
-              acc[j] = few_mfma<false>(c, hi, acc[j]);
-            }
-          }
-        }
-      } else {
-        const uint8_t* pw[4];
-        const uint8_t* ps[4];
-        bool cin[4];
+      // the weights of a step: 8 loads of 16 bytes a lane
+      uint4 w[8];
+      [[maybe_unused]] uint8_t sb[4];
+      constexpr int ES = W == FW_I8 ? 1 : 2;
+      const int col0 = run * S::COLS + l16 * S::NC;
+      [[maybe_unused]] const char* pw16 = static_cast<const char*>(p.wd) + ((int64_t)e * p.h * p.d + col0) * ES;
+      [[maybe_unused]] const uint8_t* pw8[4];
+      [[maybe_unused]] const uint8_t* ps[4];
+      if constexpr (W == FW_F8) {
         const int nbs = (p.d + kF8Block - 1) / kF8Block;
         const int64_t lds = (p.h + 2047) / 2048 * 16;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int col = run * S::COLS + j * 16 + l16;
-          cin[j] = col < p.d;
-          pw[j] = static_cast<const uint8_t*>(p.wd) + ((int64_t)e * p.d + min(col, p.d - 1)) * p.h;
+          pw8[j] = static_cast<const uint8_t*>(p.wd) + ((int64_t)e * p.d + min(run * S::COLS + j * 16 + l16, p.d - 1)) * p.h;
           ps[j] = static_cast<const uint8_t*>(p.s2) + ((int64_t)e * nbs + min(run * S::COLS + j * 16, p.d - 1) / kF8Block) * lds;
         }
-        for (int st = part * p.per2 + wave; st < k_end; st += 4) {
+      }
+      auto load = [&](int st) __attribute__((always_inline)) {
+        if constexpr (W != FW_F8) {
+          const int k = st * 32 + q * 8;
+          const bool in = k < p.h && col0 < p.d;
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            w[i] = in ? *reinterpret_cast<const uint4*>(pw16 + (int64_t)(k + i) * p.d * ES) : make_uint4(0, 0, 0, 0);
+        } else {
           const int k = st * 128 + q * 32;
-          uint4 w[4][2];
-          float sc[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
+            const bool cin = run * S::COLS + j * 16 + l16 < p.d;
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-              w[j][i] = cin[j] && k + 16 * i < p.h ? *reinterpret_cast<const uint4*>(pw[j] + k + 16 * i) : make_uint4(0, 0, 0, 0);
-            sc[j] = f8_pow((int)ps[j][st] - 127);
+              w[2 * j + i] = cin && k + 16 * i < p.h ? *reinterpret_cast<const uint4*>(pw8[j] + k + 16 * i) : make_uint4(0, 0, 0, 0);
+            sb[j] = ps[j][st];
           }
-          float v[32];
-          act_of(k, std::integral_constant<int, 32>{}, v);
-          u32x4 xf[4];
-          f8_requant(v, xf);
+        }
+      };
+      if (k_begin + wave < k_end) load(k_begin + wave);
+      for (int c0 = k_begin; c0 < k_end; c0 += CS) {
+        const int c1 = min(k_end, c0 + CS);
+        if (c0 > k_begin) __syncthreads();  // the last chunk has been read
+        const int64_t ps1 = (int64_t)M * 2 * p.h;
+        const int ka = c0 * S::STEP, kb = min(p.h, c1 * S::STEP);
+        switch (p.S1) {
+          case 1: few_act<1, W == FW_F8>(p.p1, ps1, s_row, nr, p.h, ka, kb, s_hi, s_lo); break;
+          case 2: few_act<2, W == FW_F8>(p.p1, ps1, s_row, nr, p.h, ka, kb, s_hi, s_lo); break;
+          case 3: few_act<3, W == FW_F8>(p.p1, ps1, s_row, nr, p.h, ka, kb, s_hi, s_lo); break;
+          default: few_act<4, W == FW_F8>(p.p1, ps1, s_row, nr, p.h, ka, kb, s_hi, s_lo); break;
+        }
+        __syncthreads();
+        // steps wave, wave + 4, ... of the part (a chunk is a multiple of four steps)
+        for (int st = c0 + wave; st < c1; st += 4) {
+          uint4 c[8];
+          [[maybe_unused]] float sc[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint2 b[4] = {make_uint2(w[j][0].x, w[j][0].y), make_uint2(w[j][0].z, w[j][0].w),
-                                make_uint2(w[j][1].x, w[j][1].y), make_uint2(w[j][1].z, w[j][1].w)};
+          for (int i = 0; i < 8; ++i) c[i] = w[i];
+          if constexpr (W == FW_F8) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[j] = few_mfma<false>(f8_widen(b[i], sc[j]), xf[i], acc[j]);
+            for (int j = 0; j < 4; ++j) sc[j] = f8_pow((int)sb[j] - 127);
+          }
+          if (st + 4 < k_end) load(st + 4);
+          const u32x4 zero = {0, 0, 0, 0};
+          if constexpr (W != FW_F8) {
+            const int at = l16 * kFewActLd + (st - c0) * 32 + q * 8;
+            const bool on = has && st * 32 + q * 8 < p.h;
+            const u32x4 hi = on ? *reinterpret_cast<const u32x4*>(s_hi + at) : zero;
+            const u32x4 lo = on ? *reinterpret_cast<const u32x4*>(s_lo + at) : zero;
+#pragma unroll
+            for (int j = 0; j < S::FR; ++j) {
+              if constexpr (W == FW_F16) {  // the weights' 11 bits as two bf16 numbers
+                const u32x4 v = few_column<false, true>(c, j);
+                float f[8];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  f[2 * i] = h_lo(v[i]);
+                  f[2 * i + 1] = h_hi(v[i]);
+                }
+                u32x4 wh, wl;
+                split8(f, wh, wl);
+                acc[j] = few_mfma<false>(wl, hi, acc[j]);
+                acc[j] = few_mfma<false>(wh, lo, acc[j]);
+                acc[j] = few_mfma<false>(wh, hi, acc[j]);
+              } else {
+                const u32x4 v = few_column<W == FW_I8, false>(c, j);
+                acc[j] = few_mfma<false>(v, lo, acc[j]);
+                acc[j] = few_mfma<false>(v, hi, acc[j]);
+              }
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const u32x4 xf = has && st * 128 + q * 32 + 8 * i < p.h
+                                   ? *reinterpret_cast<const u32x4*>(s_hi + l16 * kFewActLd + (st - c0) * 128 + q * 32 + 8 * i)
+                                   : zero;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const uint4 v = c[2 * j + (i >> 1)];
+                acc[j] = few_mfma<false>(f8_widen(i & 1 ? make_uint2(v.z, v.w) : make_uint2(v.x, v.y), sc[j]), xf, acc[j]);
+              }
+            }
           }
         }
       }
       constexpr int LD = S::COLS + 4;
-      if (r0 > 0) __syncthreads();
       if (has) {
 #pragma unroll
         for (int j = 0; j < S::FR; ++j)
@@ -558,48 +632,81 @@ __global__ __launch_bounds__(256, 1) void few_down_kernel(FewParams p) {
           for (int v = 0; v < 4; ++v) red[(wave * 16 + l16) * LD + S::col(j, v, q)] = acc[j][v];
       }
       __syncthreads();
-      for (int i = tid; i < nr * S::COLS; i += 256) {
-        const int r = i / S::COLS, c = i - r * S::COLS, col = run * S::COLS + c;
+      for (int i = tid; i < nr * (S::COLS / 2); i += 256) {
+        const int r = i / (S::COLS / 2), c = (i - r * (S::COLS / 2)) * 2, col = run * S::COLS + c;
         if (col >= p.d) continue;
-        float v = (red[r * LD + c] + red[(16 + r) * LD + c]) + (red[(32 + r) * LD + c] + red[(48 + r) * LD + c]);
-        if constexpr (W == FW_I8) {
-          const int64_t at = (int64_t)e * p.d + col;
-          v *= p.s2_f32 ? static_cast<const float*>(p.s2)[at] : Elt<false>::one(static_cast<const uint16_t*>(p.s2)[at]);
+        float v[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          v[t] = (red[r * LD + c + t] + red[(16 + r) * LD + c + t]) + (red[(32 + r) * LD + c + t] + red[(48 + r) * LD + c + t]);
+          if constexpr (W == FW_I8) {
+            const int64_t at = (int64_t)e * p.d + col + t;
+            v[t] *= p.s2_f32 ? static_cast<const float*>(p.s2)[at] : Elt<false>::one(static_cast<const uint16_t*>(p.s2)[at]);
+          }
         }
-        p.p2[((int64_t)part * M + hd.row[base + r0 + r]) * p.d + col] = v;
+        put_agent(p.p2 + ((int64_t)part * M + s_row[r]) * p.d + col, v[0], v[1]);
       }
     }
-    // the last of the run's A * S2 workgroups to come here has every other one's sums before it
-    __threadfence();
+    // every thread's sums are in memory before the workgroup counts itself; the last of the run's A * S2 has all before it
+    __builtin_amdgcn_s_waitcnt(0);
+    asm volatile("" ::: "memory");
     __syncthreads();
-    if (tid == 0) s_last = atomicAdd(p.counter + run, 1u) == (unsigned)(A * p.S2 - 1);
+    if (tid == 0)
+      s_last = __hip_atomic_fetch_add(p.counter + run, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)(A * p.S2 - 1);
     __syncthreads();
     if (!s_last) return;
-    __threadfence();
+    asm volatile("" ::: "memory");
+  } else {
+    __syncthreads();
   }
+  // the run's columns of every token, two a thread: the terms (slot, part) are dealt to G groups of threads where there are
+  // fewer columns than threads, each with eight loads in flight, and the groups' sums added in LDS, always in the same order
   using X = Elt<F16>;
-  for (int i = tid; i < p.T * (S::COLS / 2); i += 256) {
+  const int items = p.T * (S::COLS / 2);
+  const int G = items * 4 <= 256 ? 4 : items * 2 <= 256 ? 2 : 1;
+  const int terms = A > 0 ? p.k * p.S2 : 0;
+  float2* s_sum = reinterpret_cast<float2*>(red);
+  for (int i0 = 0; i0 < items * G; i0 += 256) {
+    const int i = (i0 + tid) % items, grp = (i0 + tid) / items;
     const int t = i / (S::COLS / 2), col = run * S::COLS + (i - t * (S::COLS / 2)) * 2;
-    if (col >= p.d) continue;
+    const bool on = i0 + tid < items * G && col < p.d;
     float o0 = 0.0f, o1 = 0.0f;
-    for (int s = 0; s < p.k; ++s) {
-      const int f = t * p.k + s;
-      if (!hd.flat_ok[f]) continue;
-      float y0 = 0.0f, y1 = 0.0f;
-      for (int j = 0; j < p.S2; ++j) {
-        const float2 v = *reinterpret_cast<const float2*>(p.p2 + ((int64_t)j * M + f) * p.d + col);
-        y0 += v.x;
-        y1 += v.y;
+    if (on) {
+      for (int t0 = grp; t0 < terms; t0 += 8 * G) {
+        float2 v[8];
+        float wv[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int term = t0 + j * G, s = term / p.S2, f = t * p.k + s;
+          const bool ok = term < terms && s_ok[f];
+          v[j] = ok ? get_agent(p.p2 + ((int64_t)(term - s * p.S2) * M + f) * p.d + col) : make_float2(0.0f, 0.0f);
+          wv[j] = ok ? s_w[f] : 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          o0 = __builtin_fmaf(wv[j], v[j].x, o0);
+          o1 = __builtin_fmaf(wv[j], v[j].y, o1);
+        }
       }
-      o0 = __builtin_fmaf(hd.w[f], y0, o0);
-      o1 = __builtin_fmaf(hd.w[f], y1, o1);
     }
-    if (p.add) {
-      const uint32_t w = *reinterpret_cast<const uint32_t*>(p.add + (int64_t)t * p.d + col);
-      o0 += X::lo(w);
-      o1 += X::hi(w);
+    if (G > 1) {  // (one round: items * G <= 256)
+      s_sum[tid] = make_float2(o0, o1);
+      __syncthreads();
+      for (int j = 1; j < G; ++j) {
+        if (grp == 0 && on) {
+          o0 += s_sum[tid + j * items].x;
+          o1 += s_sum[tid + j * items].y;
+        }
+      }
     }
-    *reinterpret_cast<uint32_t*>(p.out + (int64_t)t * p.d + col) = X::pack2(o0, o1);
+    if (on && grp == 0) {
+      if (p.add) {
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(p.add + (int64_t)t * p.d + col);
+        o0 += X::lo(w);
+        o1 += X::hi(w);
+      }
+      *reinterpret_cast<uint32_t*>(p.out + (int64_t)t * p.d + col) = X::pack2(o0, o1);
+    }
   }
 }
 
@@ -654,9 +761,9 @@ template <int W, bool F16>
 static int few_launch(const FewParams& p, hipStream_t s) {
   const unsigned chosen = (unsigned)std::min(p.E, p.M);
   const size_t lds = FewShape<W>::RED;
-  static_assert(FewShape<W>::RED <= 150 * 1024 && FewShape<W>::RED >= 4096, "LDS");
-  auto big = [&](const void* f) {  // (asked for above 64 KB)
-    return lds <= 48 * 1024 || hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) == hipSuccess;
+  static_assert(FewShape<W>::RED + 2 * 16 * kFewActLd * 2 + 8 * kFewM <= 150 * 1024 && FewShape<W>::RED >= 4096, "LDS");
+  auto big = [&](const void* f) {  // (beyond what a kernel gets unasked)
+    return lds <= 16 * 1024 || hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) == hipSuccess;
   };
   const dim3 g1(chosen * (unsigned)(p.runs1 * p.S1)), g2(chosen * (unsigned)(p.runs2 * p.S2));
   if (p.wr) {
