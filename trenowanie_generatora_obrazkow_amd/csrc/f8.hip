@@ -208,6 +208,25 @@ struct F8Cfg {
 // distinct banks (two rows fill the 64 banks once).
 __device__ __forceinline__ int f8_swz(int row) { return (row >> 1) & 7; }
 
+// buf2lds (gemm_common.h) by LDS address
+__device__ __forceinline__ void f8_copy(uint32_t voff, i32x4 rsrc, uint32_t soff, uint32_t lds32) {
+  const uint32_t m0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds32);
+  rsrc.x = __builtin_amdgcn_readfirstlane(rsrc.x);
+  rsrc.y = __builtin_amdgcn_readfirstlane(rsrc.y);
+  rsrc.z = __builtin_amdgcn_readfirstlane(rsrc.z);
+  rsrc.w = __builtin_amdgcn_readfirstlane(rsrc.w);
+  soff = (uint32_t)__builtin_amdgcn_readfirstlane((int)soff);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+               :: "s"(m0), "v"(voff), "s"(rsrc), "s"(soff) : "memory", "m0");
+}
+
+// The lane's number as a value of this place: what is computed from it is not moved out of the tile loop, where it would be
+// kept, that is spilled, through the main loop (and a spill's reload waits for every store before it)
+__device__ __forceinline__ int here(int lane) {
+  asm volatile("" : "+v"(lane));
+  return lane;
+}
+
 // A fragment of 32 rows x 64 k: the lane's row, 32 bytes
 __device__ __forceinline__ i32x8 f8_frag(const char* rows, const int* off) {
   typedef int i32x4v __attribute__((ext_vector_type(4)));
@@ -217,10 +236,16 @@ __device__ __forceinline__ i32x8 f8_frag(const char* rows, const int* off) {
 }
 
 // The weights go in as the first operand, so a lane ends with one row of y (lane % 32) and, per group g of four, columns
-// 8 g + 4 (lane / 32) + 0..3 of the fragment.  S: byte of the scale words.
-template <int S>
+// 8 g + 4 (lane / 32) + 0..3 of the fragment.  The scales are the words' lowest bytes.
 __device__ __forceinline__ f32x16 f8_mfma(i32x8 w, i32x8 x, f32x16 c, uint32_t sw, uint32_t sx) {
-  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, x, c, 0, 0, S, (int)sw, S, (int)sx);
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, x, c, 0, 0, 0, (int)sw, 0, (int)sx);
+}
+// 16 slices' scales of a row: to the next slice's
+__device__ __forceinline__ void f8_next_scale(uint4& v) {
+  v.x = __builtin_amdgcn_alignbit(v.y, v.x, 8);
+  v.y = __builtin_amdgcn_alignbit(v.z, v.y, 8);
+  v.z = __builtin_amdgcn_alignbit(v.w, v.z, 8);
+  v.w >>= 8;
 }
 
 __device__ __forceinline__ float row_scale_at(const void* s, int dt, int64_t i) {
@@ -229,163 +254,142 @@ __device__ __forceinline__ float row_scale_at(const void* s, int dt, int64_t i) 
   return dt == HMOE_DT_BF16 ? Elt<false>::one(h) : Elt<true>::one(h);
 }
 
+// One workgroup per CU (two with the small tile) walks tiles; the ring of two slices runs on from one tile into the next: the
+// last slice's place in the copy stream is taken by the next tile's first slice, so that its latency and the tile search hide
+// behind the last products and the epilogue, which parks its output in the stage that the last slice has left.
 template <class C, int EPI, int CDT>
 __global__ __launch_bounds__(C::NT, C::LDS_BYTES > 81920 ? 1 : 2) void f8_gemm_kernel(F8Params p) {
+  static_assert(C::NS == 2, "two stages");
   extern __shared__ __attribute__((aligned(1024))) char smem[];
+  // behind the ring: where a tile's rows go and their scales, by turns of the tiles (the waves are at most one tile apart);
+  // m-tiles up to and with expert e; expert e's first row, [E]: rows counted (at most M)
+  constexpr int kRowTab = 2 * C::BM * 8;
+  int* const s_tl = reinterpret_cast<int*>(smem + C::LDS_BYTES + kRowTab);
+  int* const s_r0 = s_tl + p.E;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int wm = wave / C::WN, wn = wave % C::WN;
-  const int E = p.E;
+  const int E = p.E, per = (E + 63) / 64;
 
-  // ---- the workgroup's tile: each wave scans the counts by itself, E / 64 experts a lane ----
-  const int per = (E + 63) / 64;
-  int64_t rs = 0;
-  for (int i = 0; i < per; ++i) {
-    const int e = lane * per + i;
-    if (e < E) rs += std::min(std::max(read_count(p.counts, p.counts64, e), (int64_t)0), p.M);
-  }
-  int64_t irs = rs;
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) {
-    const int64_t a = __shfl_up(irs, s, 64);
-    if (lane >= s) irs += a;
-  }
-  const int64_t st = irs - rs;  // the lane's first row
-  int tl = 0;
-  int64_t at_row = st;
-  for (int i = 0; i < per; ++i) {  // m-tiles of the lane's experts (rows past M do not exist)
-    const int e = lane * per + i;
-    if (e >= E) break;
-    const int64_t end = at_row + std::min(std::max(read_count(p.counts, p.counts64, e), (int64_t)0), p.M);
-    tl += (int)((std::min(end, p.M) - std::min(at_row, p.M) + C::BM - 1) / C::BM);
-    at_row = end;
-  }
-  int itl = tl;
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) {
-    const int a = __shfl_up(itl, s, 64);
-    if (lane >= s) itl += a;
-  }
-  const int total = __builtin_amdgcn_readfirstlane(__shfl(itl, 63, 64)) * p.nb;
-  // the tiles in runs of equal length over the 8 XCDs (workgroups go to them in turn)
-  const int share = (total + 7) >> 3, at = (int)blockIdx.x >> 3;
-  const int tile = ((int)blockIdx.x & 7) * share + at;
-  [[maybe_unused]] const int64_t counted = std::min<int64_t>(__shfl(irs, 63, 64), p.M);
-  // rows that no expert counts are zeros (where rows keep their places): every n-th of them for the n-th tile's workgroup
-  [[maybe_unused]] auto zero_rows = [&](int n, int of) __attribute__((always_inline)) {
-    constexpr int ES = CDT == HMOE_DT_F32 ? 4 : 2;
-    const int pieces = (int)((int64_t)p.halves * p.N * ES / 16);
-    for (int64_t row = counted + n; row < p.M; row += of)
-      for (int i = threadIdx.x; i < pieces; i += C::NT)
-        *reinterpret_cast<uint4*>(static_cast<char*>(p.C) + row * p.ldc * ES + i * 16) = make_uint4(0u, 0u, 0u, 0u);
-  };
-  if (at >= share || tile >= total) {
-    if constexpr (EPI == F8_STORE)
-      if (total == 0 && !p.y_idx) zero_rows((int)blockIdx.x, (int)gridDim.x);
-    return;
-  }
-  const int mt = tile / p.nb;
-  const int ol = __builtin_ctzll(__ballot(itl > mt));
-  int mstart = __builtin_amdgcn_readfirstlane(__shfl(itl - tl, ol, 64));
-  int64_t first = __shfl(st, ol, 64);
-  int e = -1, mt_e = 0;
-  int64_t row_end = 0;
-  for (int i = 0; i < per; ++i) {
-    const int x = ol * per + i;
-    if (x >= E) break;
-    const int64_t end = first + std::min(std::max(read_count(p.counts, p.counts64, x), (int64_t)0), p.M);
-    const int n = (int)((std::min(end, p.M) - std::min(first, p.M) + C::BM - 1) / C::BM);
-    if (mt < mstart + n) {
-      e = x;
-      mt_e = n;
-      row_end = std::min(end, p.M);
-      break;
+  // ---- the experts' rows and m-tiles: one wave scans the counts, E / 64 experts a lane ----
+  if (wave == 0) {
+    auto count = [&](int e) __attribute__((always_inline)) {
+      return std::min(std::max(read_count(p.counts, p.counts64, e), (int64_t)0), p.M);
+    };
+    int64_t rs = 0;
+    for (int i = 0; i < per; ++i) {
+      const int e = lane * per + i;
+      if (e < E) rs += count(e);
     }
-    mstart += n;
-    first = end;
+    int64_t irs = rs;
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) {
+      const int64_t a = __shfl_up(irs, s, 64);
+      if (lane >= s) irs += a;
+    }
+    int64_t at = irs - rs;
+    int tl = 0;
+    for (int i = 0; i < per; ++i) {  // (rows past M do not exist)
+      const int e = lane * per + i;
+      if (e >= E) break;
+      const int64_t end = at + count(e);
+      const int lo = (int)std::min(at, p.M), hi = (int)std::min(end, p.M);
+      tl += (hi - lo + C::BM - 1) / C::BM;
+      s_r0[e] = lo;
+      s_tl[e] = tl;
+      at = end;
+    }
+    int itl = tl;
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) {
+      const int a = __shfl_up(itl, s, 64);
+      if (lane >= s) itl += a;
+    }
+    for (int i = 0; i < per; ++i) {
+      const int e = lane * per + i;
+      if (e < E) s_tl[e] += itl - tl;
+    }
+    if (lane == 63) s_r0[E] = (int)std::min(irs, p.M);
   }
-  // bands of kF8BandM m-tiles of an expert, n-tile by n-tile
-  const int local = tile - mstart * p.nb, band = local / (kF8BandM * p.nb) * kF8BandM;
-  const int mc = min(kF8BandM, mt_e - band), r = local - band * p.nb;
-  e = __builtin_amdgcn_readfirstlane(e);
-  const int nbi = __builtin_amdgcn_readfirstlane(r / mc);
-  const int row0 = __builtin_amdgcn_readfirstlane((int)(first + (int64_t)(band + r % mc) * C::BM));
-  const int live = __builtin_amdgcn_readfirstlane((int)std::min<int64_t>(row_end - row0, C::BM));
+  __syncthreads();
+  const int counted = __builtin_amdgcn_readfirstlane(s_r0[E]);
+  const int total = __builtin_amdgcn_readfirstlane(s_tl[E - 1]) * p.nb;
+  const int share = (total + 7) >> 3;  // the tiles in runs of equal length over the 8 XCDs (workgroups go to them in turn)
 
-  // ---- columns: n0 the first of the half (store) or of act (SwiGLU) ----
+  struct Tile {
+    int e, nbi, row0, live;
+  };
+  // the workgroup's j-th tile: bands of kF8BandM m-tiles of an expert, n-tile by n-tile
+  auto find = [&](int j, Tile& t) __attribute__((always_inline)) {
+    const int v = (int)blockIdx.x + j * (int)gridDim.x, at = v >> 3, tile = (v & 7) * share + at;
+    if (at >= share || tile >= total) return false;
+    const int mt = tile / p.nb;
+    int e = 0;
+    for (int i = 0; i < per; ++i) {
+      const int x = i * 64 + lane;
+      e += __builtin_popcountll(__ballot((x < E ? s_tl[x] : INT32_MAX) <= mt));
+    }
+    const int m0 = e > 0 ? s_tl[e - 1] : 0, mt_e = s_tl[e] - m0, first = s_r0[e], end = s_r0[e + 1];
+    const int local = tile - m0 * p.nb, band = local / (kF8BandM * p.nb) * kF8BandM;
+    const int mc = min(kF8BandM, mt_e - band), r = local - band * p.nb;
+    t.e = e;
+    t.nbi = __builtin_amdgcn_readfirstlane(r / mc);
+    t.row0 = __builtin_amdgcn_readfirstlane(first + (band + r % mc) * C::BM);
+    t.live = __builtin_amdgcn_readfirstlane(min(end - t.row0, C::BM));
+    return true;
+  };
   const int nbh = EPI == F8_STORE ? p.nb / p.halves : p.nb;
-  const int half = EPI == F8_STORE ? nbi / nbh : 0;
-  const int n0 = (nbi - half * nbh) * (EPI == F8_SWIGLU ? C::BN / 2 : C::BN);
+  // the half a tile lies in, and its first column there (store), or its first column of act (SwiGLU)
+  auto half_of = [&](const Tile& t) { return EPI == F8_STORE ? t.nbi / nbh : 0; };
+  auto n0_of = [&](const Tile& t) { return (t.nbi - half_of(t) * nbh) * (EPI == F8_SWIGLU ? C::BN / 2 : C::BN); };
 
-  // ---- copy sources ----
+  // ---- copy sources of the tile whose slices are being copied ----
   const int K = p.K, nk = (K + kF8Slice - 1) / kF8Slice;
-  const i32x4 rsA = make_rsrc(p.a_idx ? p.A : p.A + (int64_t)row0 * p.lda);
-  const i32x4 rsB = make_rsrc(p.B + (int64_t)e * p.halves * p.N * K);
+  i32x4 rsA, rsB;
   uint32_t vA[C::PA], vB[C::PB];
-  auto chunk_of = [&](int rr) { return (lane & 7) ^ f8_swz(rr); };
+  auto chunk_of = [&](int ln, int rr) { return (ln & 7) ^ f8_swz(rr); };
+  auto set_sources = [&](const Tile& t) __attribute__((always_inline)) {
+    const int ln = here(lane);
+    rsA = make_rsrc(p.a_idx ? p.A : p.A + (int64_t)t.row0 * p.lda);
+    rsB = make_rsrc(p.B + (int64_t)t.e * p.halves * p.N * K);
+    const int half = half_of(t), n0 = n0_of(t);
 #pragma unroll
-  for (int i = 0; i < C::PA; ++i) {
-    const int rr = 8 * (wave * C::PA + i) + (lane >> 3);
-    vA[i] = kOOB;
-    if (rr < live) {
-      const int64_t src = p.a_idx ? (int64_t)p.a_idx[row0 + rr] : (int64_t)rr;
-      vA[i] = (uint32_t)(src * p.lda + chunk_of(rr) * 16);
+    for (int i = 0; i < C::PA; ++i) {
+      const int rr = 8 * (wave * C::PA + i) + (ln >> 3);
+      vA[i] = kOOB;
+      if (rr < t.live) {
+        const int64_t src = p.a_idx ? (int64_t)p.a_idx[t.row0 + rr] : (int64_t)rr;
+        vA[i] = (uint32_t)(src * p.lda + chunk_of(ln, rr) * 16);
+      }
     }
-  }
 #pragma unroll
-  for (int i = 0; i < C::PB; ++i) {
-    const int rr = 8 * (wave * C::PB + i) + (lane >> 3);
-    int col, row;  // column within the half, row of B
-    if constexpr (EPI == F8_SWIGLU) {
-      col = n0 + rr % (C::BN / 2);
-      row = rr / (C::BN / 2) * p.N + col;
-    } else {
-      col = n0 + rr;
-      row = half * p.N + col;
-    }
-    vB[i] = col < p.N ? (uint32_t)((int64_t)row * K + chunk_of(rr) * 16) : kOOB;
-  }
-  auto issue = [&](int kt) __attribute__((always_inline)) {  // slice kt into its stage
-    char* slot = smem + (kt % C::NS) * C::STAGE;
-    const int k0 = kt * kF8Slice;
-    if (k0 + kF8Slice <= K) {
-#pragma unroll
-      for (int i = 0; i < C::PA; ++i) buf2lds(vA[i], rsA, (uint32_t)k0, slot + (wave * C::PA + i) * 1024);
-#pragma unroll
-      for (int i = 0; i < C::PB; ++i) buf2lds(vB[i], rsB, (uint32_t)k0, slot + C::A_BYTES + (wave * C::PB + i) * 1024);
-    } else {  // chunks at or past K (and whole slices past it) read zeros
-#pragma unroll
-      for (int i = 0; i < C::PA; ++i)
-        buf2lds(k0 + chunk_of(8 * (wave * C::PA + i) + (lane >> 3)) * 16 < K ? vA[i] : kOOB, rsA, (uint32_t)k0,
-                slot + (wave * C::PA + i) * 1024);
-#pragma unroll
-      for (int i = 0; i < C::PB; ++i)
-        buf2lds(k0 + chunk_of(8 * (wave * C::PB + i) + (lane >> 3)) * 16 < K ? vB[i] : kOOB, rsB, (uint32_t)k0,
-                slot + C::A_BYTES + (wave * C::PB + i) * 1024);
+    for (int i = 0; i < C::PB; ++i) {
+      const int rr = 8 * (wave * C::PB + i) + (ln >> 3);
+      int col, row;  // column within the half, row of B
+      if constexpr (EPI == F8_SWIGLU) {
+        col = n0 + rr % (C::BN / 2);
+        row = rr / (C::BN / 2) * p.N + col;
+      } else {
+        col = n0 + rr;
+        row = half * p.N + col;
+      }
+      vB[i] = col < p.N ? (uint32_t)((int64_t)row * K + chunk_of(ln, rr) * 16) : kOOB;
     }
   };
-
-  // ---- per-row inputs of the lane's rows a*32 + lane%32 of the wave ----
-  const uint8_t* pa[C::FM];
-  [[maybe_unused]] int yr[C::FM];
-  [[maybe_unused]] float sc[C::FM];
+  const uint32_t ring = lds_addr(smem);
+  auto issue = [&](int kt, int stage) __attribute__((always_inline)) {  // slice kt, whole or not, into a stage
+    const uint32_t slot = ring + stage * C::STAGE;
+    const int k0 = kt * kF8Slice, ln = here(lane);
 #pragma unroll
-  for (int a = 0; a < C::FM; ++a) {
-    const int rr = wm * C::TM + a * 32 + (lane & 31);
-    const int row = row0 + min(rr, live - 1);  // (a row past the tile's last takes that one's scales: its values are zeros)
-    pa[a] = p.As + (p.a_idx ? (int64_t)p.a_idx[row] : (int64_t)row) * p.ldas;
-    if constexpr (EPI == F8_STORE) {
-      yr[a] = p.y_idx ? p.y_idx[row] : row;
-      sc[a] = p.scale ? row_scale_at(p.scale, p.scale_dt, p.scale_by_y ? yr[a] : row) : 1.0f;
-    }
-  }
-  // scales of the wave's columns: one 128-column block (store), the gate's and the up's (SwiGLU)
-  const int sblk = EPI == F8_STORE ? min((n0 + wn * C::TN) / kF8Block, p.nbs - 1)
-                                   : min((n0 + wn * C::TN / 2) / kF8Block, p.nbs - 1);
-  const uint8_t* pb0 = p.Bs + ((int64_t)(e * p.halves + half) * p.nbs + sblk) * p.ldbs;
-  const uint8_t* pb1 = EPI == F8_SWIGLU ? pb0 + (int64_t)p.nbs * p.ldbs : pb0;
+    for (int i = 0; i < C::PA; ++i)
+      f8_copy(k0 + chunk_of(ln, 8 * (wave * C::PA + i) + (ln >> 3)) * 16 < K ? vA[i] : kOOB, rsA, (uint32_t)k0,
+              slot + (wave * C::PA + i) * 1024);
+#pragma unroll
+    for (int i = 0; i < C::PB; ++i)
+      f8_copy(k0 + chunk_of(ln, 8 * (wave * C::PB + i) + (ln >> 3)) * 16 < K ? vB[i] : kOOB, rsB, (uint32_t)k0,
+              slot + C::A_BYTES + (wave * C::PB + i) * 1024);
+  };
 
-  // ---- main loop ----
   int off[2][2];
 #pragma unroll
   for (int ks = 0; ks < 2; ++ks)
@@ -399,161 +403,282 @@ __global__ __launch_bounds__(C::NT, C::LDS_BYTES > 81920 ? 1 : 2) void f8_gemm_k
       return wn * C::TN + b * 32;
   };
   f32x16 acc[C::FM][C::FN];
-#pragma unroll
-  for (int a = 0; a < C::FM; ++a)
-#pragma unroll
-    for (int b = 0; b < C::FN; ++b)
-#pragma unroll
-      for (int v = 0; v < 16; ++v) acc[a][b][v] = 0.0f;
   uint4 sA[C::FM], sB0, sB1;
-  constexpr int LOADS = C::PA + C::PB;
+
+  // One slice's products, the copies of the slice that follows dealt between them (FAST: one that lies inside K; otherwise
+  // they have been issued)
+  auto products = [&](auto fast_tag, int stage, int k0) __attribute__((always_inline)) {
+    constexpr bool FAST = decltype(fast_tag)::value;
+    constexpr int NM = 2 * C::FM * C::FN, NC = C::PA + C::PB;  // products, copies
+    const char* sa = smem + stage * C::STAGE;
+    const char* sb = sa + C::A_BYTES;
+    const uint32_t fa = ring + (stage ^ 1) * C::STAGE + wave * (C::PA * 1024);
+    const uint32_t fb = ring + (stage ^ 1) * C::STAGE + C::A_BYTES + wave * (C::PB * 1024);
+    const uint32_t so = (uint32_t)k0;
+    i32x8 xa[2][C::FM], wb[2][C::FN];
+    auto read_a = [&](int ks, int a) { xa[ks][a] = f8_frag(sa + (wm * C::TM + a * 32) * 128, off[ks]); };
+    auto read_b = [&](int ks, int b) { wb[ks][b] = f8_frag(sb + b_row(b) * 128, off[ks]); };
 #pragma unroll
-  for (int s = 0; s < C::NS - 1; ++s) issue(s);
-  for (int k4 = 0; k4 < nk; k4 += 4) {
-    if ((k4 & 15) == 0) {
+    for (int b = 0; b < C::FN; ++b) read_b(0, b);
 #pragma unroll
-      for (int a = 0; a < C::FM; ++a) sA[a] = *reinterpret_cast<const uint4*>(pa[a] + k4);
-      sB0 = *reinterpret_cast<const uint4*>(pb0 + k4);
-      if constexpr (EPI == F8_SWIGLU) sB1 = *reinterpret_cast<const uint4*>(pb1 + k4);
-    }
-    static_for<4>([&](auto it) __attribute__((always_inline)) {
-      constexpr int I = decltype(it)::value;
-      const int kt = k4 + I;
-      if (kt < nk) {
-        wait_vm<(C::NS - 2) * LOADS>();  // this wave's copies of slice kt have landed
-        lds_barrier();                   // and the others'; all have read slice kt - 1, whose stage is filled next
-        issue(kt + C::NS - 1);
-        const char* sa = smem + (kt % C::NS) * C::STAGE;
-        const char* sb = sa + C::A_BYTES;
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-          i32x8 xa[C::FM], wb[C::FN];
-#pragma unroll
-          for (int b = 0; b < C::FN; ++b) wb[b] = f8_frag(sb + b_row(b) * 128, off[ks]);
-#pragma unroll
-          for (int a = 0; a < C::FM; ++a) xa[a] = f8_frag(sa + (wm * C::TM + a * 32) * 128, off[ks]);
-#pragma unroll
-          for (int a = 0; a < C::FM; ++a)
-#pragma unroll
-            for (int b = 0; b < C::FN; ++b)
-              acc[a][b] = f8_mfma<I>(wb[b], xa[a], acc[a][b], EPI == F8_SWIGLU && b >= C::FN / 2 ? sB1.x : sB0.x, sA[a].x);
-        }
+    for (int a = 0; a < C::FM; ++a) read_a(0, a);
+    static_for<NM>([&](auto n_tag) __attribute__((always_inline)) {
+      constexpr int n = decltype(n_tag)::value, ks = n / (C::FM * C::FN), a = n / C::FN % C::FM, b = n % C::FN;
+      acc[a][b] = f8_mfma(wb[ks][b], xa[ks][a], acc[a][b], EPI == F8_SWIGLU && b >= C::FN / 2 ? sB1.x : sB0.x, sA[a].x);
+      if constexpr (FAST) {
+        constexpr int c0 = n * NC / NM, c1 = (n + 1) * NC / NM;
+        static_for<c1 - c0>([&](auto j) __attribute__((always_inline)) {
+          constexpr int c = c0 + decltype(j)::value;
+          if constexpr (c < C::PA)
+            buf2lds_inner<c * 1024>(vA[c], rsA, so, fa);
+          else
+            buf2lds_inner<(c - C::PA) * 1024>(vB[c - C::PA], rsB, so, fb);
+        });
+      }
+      if constexpr (ks == 0) {  // the second half's fragments behind the first half's products
+        if constexpr (b == 0) read_a(1, a);
+        constexpr int per_b = (C::FN + C::FM - 1) / C::FM;
+        if constexpr (b < per_b && a * per_b + b < C::FN) read_b(1, a * per_b + b);
       }
     });
-    auto next = [](uint4& v) { v.x = v.y; v.y = v.z; v.z = v.w; };
-#pragma unroll
-    for (int a = 0; a < C::FM; ++a) next(sA[a]);
-    next(sB0);
-    if constexpr (EPI == F8_SWIGLU) next(sB1);
-  }
-  wait_vm<0>();   // (copies past the last slice move nothing, but still write zeros)
-  lds_barrier();  // the ring is free
+  };
 
-  const int lrow = lane & 31, lcol = 4 * (lane >> 5);
-  if constexpr (EPI == F8_STORE) {
-    // 32 rows of the wave at a time go through its own part of the LDS, chunk c of a row at c ^ row, and leave in whole rows
-    constexpr int ES = CDT == HMOE_DT_F32 ? 4 : 2, RB = C::TN * ES, CPR = RB / 16, RPI = 64 / CPR;
-    char* park = smem + wave * (32 * RB);
+  // rows that no expert counts are zeros (where rows keep their places)
+  auto zero_rows = [&]() __attribute__((always_inline)) {
+    constexpr int ES = CDT == HMOE_DT_F32 ? 4 : 2;
+    const int pieces = (int)((int64_t)p.halves * p.N * ES / 16);
+    for (int64_t row = counted + (int64_t)blockIdx.x; row < p.M; row += gridDim.x)
+      for (int i = threadIdx.x; i < pieces; i += C::NT)
+        *reinterpret_cast<uint4*>(static_cast<char*>(p.C) + row * p.ldc * ES + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+  };
+  if constexpr (EPI == F8_STORE)
+    if (!p.y_idx && counted < p.M) zero_rows();
+
+  const uint8_t* pa[C::FM];  // scales of the lane's rows a*32 + lane%32 of the wave, and of the wave's columns
+  const uint8_t *pb0, *pb1;
+  auto set_scales = [&](const Tile& t) __attribute__((always_inline)) {
+    const int lrow = here(lane) & 31;
 #pragma unroll
     for (int a = 0; a < C::FM; ++a) {
-      const int rbase = wm * C::TM + a * 32;
-      if (rbase >= live) break;
+      const int row = t.row0 + min(wm * C::TM + a * 32 + lrow, t.live - 1);  // (past the last row: its values are zeros)
+      pa[a] = p.As + (p.a_idx ? (int64_t)p.a_idx[row] : (int64_t)row) * p.ldas;
+    }
+    // one 128-column block (store), the gate's and the up's (SwiGLU)
+    const int sblk = min((n0_of(t) + wn * (EPI == F8_STORE ? C::TN : C::TN / 2)) / kF8Block, p.nbs - 1);
+    pb0 = p.Bs + ((int64_t)(t.e * p.halves + half_of(t)) * p.nbs + sblk) * p.ldbs;
+    pb1 = EPI == F8_SWIGLU ? pb0 + (int64_t)p.nbs * p.ldbs : pb0;
+  };
+  auto load_scales = [&](int kt) __attribute__((always_inline)) {  // of slices kt .. kt + 15
+#pragma unroll
+    for (int a = 0; a < C::FM; ++a) sA[a] = *reinterpret_cast<const uint4*>(pa[a] + kt);
+    sB0 = *reinterpret_cast<const uint4*>(pb0 + kt);
+    if constexpr (EPI == F8_SWIGLU) sB1 = *reinterpret_cast<const uint4*>(pb1 + kt);
+  };
+
+  Tile t;
+  if (!find(0, t)) return;
+  set_sources(t);
+  issue(0, 0);
+  set_scales(t);
+  load_scales(0);
+  wait_vm<0>();
+  int stage = 0;
+  for (int j = 1;; ++j) {  // (the tile's first slice and scales have landed)
+    const int half = half_of(t), n0 = n0_of(t);
+    [[maybe_unused]] int* const s_y = reinterpret_cast<int*>(smem + C::LDS_BYTES + (j & 1) * (C::BM * 8));
+    [[maybe_unused]] float* const s_sc = reinterpret_cast<float*>(s_y + C::BM);
+    if constexpr (EPI == F8_STORE) {  // where the tile's rows go, and their scales (read behind the main loop's barriers)
+      for (int i = wave * 64 + here(lane); i < t.live; i += C::NT) {
+        const int row = t.row0 + i, y = p.y_idx ? p.y_idx[row] : row;
+        s_y[i] = y;
+        s_sc[i] = p.scale ? row_scale_at(p.scale, p.scale_dt, p.scale_by_y ? y : row) : 1.0f;
+      }
+    }
+#pragma unroll
+    for (int a = 0; a < C::FM; ++a)
 #pragma unroll
       for (int b = 0; b < C::FN; ++b)
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const f32x16& v = acc[a][b];
-          const float o[4] = {v[4 * g] * sc[a], v[4 * g + 1] * sc[a], v[4 * g + 2] * sc[a], v[4 * g + 3] * sc[a]};
-          const int byte = (b * 32 + 8 * g + lcol) * ES;
-          char* at = park + lrow * RB + (((byte >> 4) ^ (lrow & (CPR - 1))) << 4) + (byte & 15);
-          if constexpr (CDT == HMOE_DT_F32) {
-            *reinterpret_cast<float4*>(at) = make_float4(o[0], o[1], o[2], o[3]);
-          } else {
-            using X = Elt<CDT == HMOE_DT_F16>;
-            *reinterpret_cast<uint2*>(at) = make_uint2(X::pack2(o[0], o[1]), X::pack2(o[2], o[3]));
-          }
-        }
-      __builtin_amdgcn_wave_barrier();
-#pragma unroll
-      for (int i = 0; i < 32 / RPI; ++i) {
-        const int rr = i * RPI + lane / CPR, c = lane % CPR;
-        const uint4 v = *reinterpret_cast<const uint4*>(park + rr * RB + ((c ^ (rr & (CPR - 1))) << 4));
-        const int64_t y = __shfl(yr[a], rr, 64);
-        const int col = n0 + wn * C::TN + c * (16 / ES);
-        if (rbase + rr < live && col < p.N)
-          *reinterpret_cast<uint4*>(static_cast<char*>(p.C) + (y * p.ldc + half * p.N + col) * ES) = v;
+        for (int v = 0; v < 16; ++v) acc[a][b][v] = 0.0f;
+
+    // ---- main loop ----
+    Tile next;
+    bool more = false;
+    auto begin_slice = [&](int kt) __attribute__((always_inline)) {
+      if (kt > 0) {
+        if ((kt & 15) == 0) load_scales(kt);
+        wait_vm<0>();  // this wave's copies of slice kt have landed
       }
-      __builtin_amdgcn_wave_barrier();
+      lds_barrier();  // and the others'; all have read the slice before, whose stage is filled next
+    };
+    auto end_slice = [&]() __attribute__((always_inline)) {
+#pragma unroll
+      for (int a = 0; a < C::FM; ++a) f8_next_scale(sA[a]);
+      f8_next_scale(sB0);
+      if constexpr (EPI == F8_SWIGLU) f8_next_scale(sB1);
+      stage ^= 1;
+    };
+    int kt = 0;
+    for (; (kt + 2) * kF8Slice <= K; ++kt) {
+      begin_slice(kt);
+      products(std::true_type{}, stage, (kt + 1) * kF8Slice);
+      end_slice();
     }
-    if (!p.y_idx && counted < p.M) zero_rows(tile, total);
-  } else {
-    // act = silu(g) u in fp32, in place of g; the largest of a row's 128 columns from the lanes l and l ^ 32 and, through
-    // LDS, the waves side by side; then e4m3 through LDS into whole 128-byte rows
-    float* s_max = reinterpret_cast<float*>(smem);  // [WN][BM]
-    char* park = smem + C::WN * C::BM * 4;          // [BM][128]
-    static_assert(C::BN / 2 == kF8Block && C::WN * C::BM * 4 + C::BM * 128 <= C::LDS_BYTES, "one block of act per tile");
-#pragma unroll
-    for (int a = 0; a < C::FM; ++a) {
-      float m = 0.0f;
-#pragma unroll
-      for (int b = 0; b < C::FN / 2; ++b)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          const float act = silu_f(acc[a][b][v]) * acc[a][b + C::FN / 2][v];
-          acc[a][b][v] = act;
-          m = fmaxf(m, f8_abs(act));
+    for (; kt < nk; ++kt) {
+      begin_slice(kt);
+      if (kt + 1 < nk) {
+        issue(kt + 1, stage ^ 1);
+      } else {
+        more = find(j, next);
+        if (more) {
+          set_sources(next);
+          issue(0, stage ^ 1);
         }
-      m = bfly_max<32>(m);
-      if (lane < 32) s_max[wn * C::BM + wm * C::TM + a * 32 + lrow] = m;
+      }
+      products(std::false_type{}, stage, 0);
+      end_slice();
     }
-    lds_barrier();
+    if (more) set_scales(next);
+    if (more) load_scales(0);
+    lds_barrier();  // all have read the last slice: its stage (the next tile's first slice goes to the other) takes the output
+    char* const park = smem + (stage ^ 1) * C::STAGE;
+    const int ln = here(lane), lrow = ln & 31, lcol = 4 * (ln >> 5);
+
+    if constexpr (EPI == F8_STORE) {
+      // 32 rows of the wave at a time go through its own part of the stage, chunk c of a row at c ^ row, and leave in whole
+      // rows; in two turns where they fit, so that one's rows are written while the other's are read back
+      constexpr int ES = CDT == HMOE_DT_F32 ? 4 : 2;
+      constexpr int FP = ES == 4 ? C::FN / 2 : C::FN;  // column fragments of a pass
+      constexpr int RB = FP * 32 * ES, CPR = RB / 16, RPI = 64 / CPR;
+      constexpr int TURNS = 2 * 32 * RB * C::NW <= C::STAGE ? 2 : 1;
+      static_assert(32 * RB * C::NW <= C::STAGE, "a pass of every wave in a stage");
+      char* const own = park + wave * (TURNS * 32 * RB);
 #pragma unroll
-    for (int a = 0; a < C::FM; ++a) {
-      const int rr = wm * C::TM + a * 32 + lrow;
-      float m = 0.0f;
+      for (int a = 0; a < C::FM; ++a) {
+        const int rbase = wm * C::TM + a * 32;
+        if (rbase >= t.live) break;
+        const float sc = s_sc[min(rbase + lrow, t.live - 1)];
 #pragma unroll
-      for (int w = 0; w < C::WN; ++w) m = fmaxf(m, s_max[w * C::BM + rr]);
-      const int ex = f8_exp(m);
-      const float inv = f8_inv(ex);
-      if (wn == 0 && lane < 32 && rr < live) p.Cs[(int64_t)(row0 + rr) * p.ldcs + nbi] = (uint8_t)(ex + 127);
+        for (int b0 = 0; b0 < C::FN; b0 += FP) {
+          char* const buf = own + (a * (C::FN / FP) + b0 / FP) % TURNS * (32 * RB);
 #pragma unroll
-      for (int b = 0; b < C::FN / 2; ++b)
+          for (int b = 0; b < FP; ++b)
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const f32x16& v = acc[a][b];
-          const int byte = wn * (C::TN / 2) + b * 32 + 8 * g + lcol;
-          *reinterpret_cast<uint32_t*>(park + rr * 128 + (((byte >> 4) ^ f8_swz(rr)) << 4) + (byte & 15)) =
-              f8_pack4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3], inv);
+            for (int g = 0; g < 4; ++g) {
+              const f32x16& v = acc[a][b0 + b];
+              const float o[4] = {v[4 * g] * sc, v[4 * g + 1] * sc, v[4 * g + 2] * sc, v[4 * g + 3] * sc};
+              const int byte = (b * 32 + 8 * g + lcol) * ES;
+              char* at = buf + lrow * RB + (((byte >> 4) ^ (lrow & (CPR - 1))) << 4) + (byte & 15);
+              if constexpr (CDT == HMOE_DT_F32) {
+                *reinterpret_cast<float4*>(at) = make_float4(o[0], o[1], o[2], o[3]);
+              } else {
+                using X = Elt<CDT == HMOE_DT_F16>;
+                *reinterpret_cast<uint2*>(at) = make_uint2(X::pack2(o[0], o[1]), X::pack2(o[2], o[3]));
+              }
+            }
+          __builtin_amdgcn_wave_barrier();
+          // the next tile's first slice and scales have landed before the first store: no slice waits for the stores
+          if (a == 0 && b0 == 0) wait_vm<0>();
+#pragma unroll
+          for (int i = 0; i < 32 / RPI; ++i) {
+            const int rr = i * RPI + ln / CPR, c = ln % CPR;
+            const uint4 v = *reinterpret_cast<const uint4*>(buf + rr * RB + ((c ^ (rr & (CPR - 1))) << 4));
+            const int64_t y = s_y[min(rbase + rr, t.live - 1)];
+            const int col = n0 + wn * C::TN + b0 * 32 + c * (16 / ES);
+            if (rbase + rr < t.live && col < p.N)
+              *reinterpret_cast<uint4*>(static_cast<char*>(p.C) + (y * p.ldc + half * p.N + col) * ES) = v;
+          }
+          __builtin_amdgcn_wave_barrier();
         }
+      }
+    } else {
+      // act = silu(g) u in fp32, in place of g; the largest of a row's 128 columns from the lanes l and l ^ 32 and, through
+      // LDS, the waves side by side; then e4m3 through LDS into whole 128-byte rows
+      float* s_max = reinterpret_cast<float*>(park);  // [WN][BM]
+      char* const rows = park + C::WN * C::BM * 4;    // [BM][128]
+      static_assert(C::BN / 2 == kF8Block && C::WN * C::BM * 4 + C::BM * 128 <= C::STAGE, "one block of act per tile");
+#pragma unroll
+      for (int a = 0; a < C::FM; ++a) {
+        float m = 0.0f;
+#pragma unroll
+        for (int b = 0; b < C::FN / 2; ++b)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) {
+            const float act = silu_f(acc[a][b][v]) * acc[a][b + C::FN / 2][v];
+            acc[a][b][v] = act;
+            m = fmaxf(m, f8_abs(act));
+          }
+        m = bfly_max<32>(m);
+        if (ln < 32) s_max[wn * C::BM + wm * C::TM + a * 32 + lrow] = m;
+      }
+      lds_barrier();
+#pragma unroll
+      for (int a = 0; a < C::FM; ++a) {
+        const int rr = wm * C::TM + a * 32 + lrow;
+        float m = 0.0f;
+#pragma unroll
+        for (int w = 0; w < C::WN; ++w) m = fmaxf(m, s_max[w * C::BM + rr]);
+        const int ex = f8_exp(m);
+        const float inv = f8_inv(ex);
+        if (a == 0) wait_vm<0>();  // as above
+        if (wn == 0 && ln < 32 && rr < t.live) p.Cs[(int64_t)(t.row0 + rr) * p.ldcs + t.nbi] = (uint8_t)(ex + 127);
+#pragma unroll
+        for (int b = 0; b < C::FN / 2; ++b)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const f32x16& v = acc[a][b];
+            const int byte = wn * (C::TN / 2) + b * 32 + 8 * g + lcol;
+            *reinterpret_cast<uint32_t*>(rows + rr * 128 + (((byte >> 4) ^ f8_swz(rr)) << 4) + (byte & 15)) =
+                f8_pack4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3], inv);
+          }
+      }
+      lds_barrier();
+      for (int i = wave * 64 + ln; i < t.live * 8; i += C::NT) {
+        const int rr = i >> 3, c = i & 7;
+        if (n0 + c * 16 < p.N)
+          *reinterpret_cast<uint4*>(static_cast<char*>(p.C) + (int64_t)(t.row0 + rr) * p.ldc + n0 + c * 16) =
+              *reinterpret_cast<const uint4*>(rows + rr * 128 + ((c ^ f8_swz(rr)) << 4));
+      }
     }
-    lds_barrier();
-    for (int i = threadIdx.x; i < live * 8; i += C::NT) {
-      const int rr = i >> 3, c = i & 7;
-      if (n0 + c * 16 < p.N)
-        *reinterpret_cast<uint4*>(static_cast<char*>(p.C) + (int64_t)(row0 + rr) * p.ldc + n0 + c * 16) =
-            *reinterpret_cast<const uint4*>(park + rr * 128 + ((c ^ f8_swz(rr)) << 4));
-    }
+    if (!more) break;
+    t = next;
   }
+}
+
+static int f8_cus() {
+  static std::atomic<int> n[64];
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 0;
+  int v = n[dev].load(std::memory_order_relaxed);
+  if (v == 0) {
+    if (hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || v <= 0) return 0;
+    n[dev].store(v, std::memory_order_relaxed);
+  }
+  return v;
 }
 
 template <class C, int EPI, int CDT>
 static int f8_launch(const F8Params& p, hipStream_t s) {
   auto kern = f8_gemm_kernel<C, EPI, CDT>;
+  constexpr int kLds = C::LDS_BYTES + 2 * C::BM * 8 + 16;  // and 8 bytes per expert
   static std::atomic<bool> attr_set[64];  // per device
   int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return HMOE_ERR_DEVICE;
+  const int cus = f8_cus();
+  if (cus <= 0 || hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return HMOE_ERR_DEVICE;
   if (!attr_set[dev].load(std::memory_order_acquire)) {
     if (hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize,
-                            C::LDS_BYTES) != hipSuccess)
+                            kLds + kMaxEGemm * 8) !=
+        hipSuccess)
       return HMOE_ERR_LAUNCH;
     attr_set[dev].store(true, std::memory_order_release);
   }
   F8Params q = p;
   q.nb = EPI == F8_SWIGLU ? (p.N + C::BN / 2 - 1) / (C::BN / 2) : p.halves * ((p.N + C::BN - 1) / C::BN);
-  // an m-tile for every expert with rows and at most M / BM further ones; the tiles in eights (one per XCD)
+  // an m-tile for every expert with rows and at most M / BM further ones; the workgroups in eights (one per XCD)
   const int64_t tiles = (std::min<int64_t>(p.E, p.M) + p.M / C::BM) * q.nb;
-  if (tiles >= (1 << 23)) return HMOE_ERR_SHAPE;  // (a grid's threads stay below 2^32)
-  hipLaunchKernelGGL(kern, dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(C::NT), C::LDS_BYTES, s, q);
+  if (tiles >= (1 << 28)) return HMOE_ERR_SHAPE;
+  const int64_t wgs = std::min<int64_t>(tiles, (int64_t)cus * (C::LDS_BYTES > 81920 ? 1 : 2));
+  hipLaunchKernelGGL(kern, dim3((unsigned)((wgs + 7) / 8 * 8)), dim3(C::NT), kLds + p.E * 8, s, q);
   HMOE_CHECK_LAUNCH();
   return HMOE_OK;
 }
