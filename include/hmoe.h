@@ -498,12 +498,14 @@ int hmoe_f8_grouped_mm(const void* a, int64_t lda, const uint8_t* a_s, int64_t l
                        const int32_t* a_idx, const int32_t* y_idx, const void* scale, int scale_dtype, int scale_by_y, void* y,
                        int64_t ldy, int y_dtype, hmoe_stream_t stream);
 /* act = silu(g) * u of [g | u] = x[a_idx] @ wgu[e], all in fp32, quantised: act (M, h) e4m3, act_s (M, scale_ld(h)).  wgu
- * (E, 2h, d) with halves = 2. */
+ * (E, 2h, d) with halves = 2.  The 8-bit matrix instructions drop what lies below 2^-13 of the largest of eight products: some
+ * 2^-16 of a sum, which moves about one act in a thousand across a border of its 8 bits.  wide = 1 multiplies the same values
+ * as bf16 numbers instead, exactly but for the fp32 sums, at half the rate. */
 int hmoe_f8_gate_up_swiglu(const void* x, int64_t ldx, const uint8_t* x_s, int64_t ldx_s, const int32_t* a_idx, const void* wgu,
                            const uint8_t* wgu_s, int64_t E, int64_t d, int64_t h, const void* counts, int counts_dtype,
-                           int64_t M, void* act, uint8_t* act_s, hmoe_stream_t stream);
+                           int64_t M, int wide, void* act, uint8_t* act_s, hmoe_stream_t stream);
 /* hmoe_moe_experts with such stacks: x (T, d) bf16 or fp16 is quantised, y (T * k, d) of its type; the routing weights enter
- * as given (not rounded). */
+ * as given (not rounded).  fp16: the gate/up products are wide (hmoe_f8_gate_up_swiglu). */
 size_t hmoe_f8_moe_experts_workspace_size(int64_t T, int64_t d, int E, int k, int64_t h);
 int hmoe_f8_moe_experts(const void* x, int64_t ldx, int dtype, const void* topk_ids, int ids_dtype, const void* topk_w,
                         int topk_w_dtype, const void* wgu, const uint8_t* wgu_s, const void* wd, const uint8_t* wd_s, int64_t T,

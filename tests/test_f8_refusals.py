@@ -67,7 +67,7 @@ def test_grouped_mm_codes(L):
 
 def test_gate_up_codes(L):
     def f(x=P, M=4, d=64, h=48, act=P, act_s=P, E=2):
-        return L.hmoe_f8_gate_up_swiglu(x, d, P, 16, None, P, P, E, d, h, P, I32, M, act, act_s, None)
+        return L.hmoe_f8_gate_up_swiglu(x, d, P, 16, None, P, P, E, d, h, P, I32, M, 0, act, act_s, None)
     assert f(M=0) == 0 and f(h=0) == ARG and f(h=40) == SHAPE and f(act=None) == ARG and f(act_s=None) == ARG and f(act=P + 8) == ARG
 
 

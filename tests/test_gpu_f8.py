@@ -30,13 +30,15 @@ def rand(*shape, seed=0, dtype=torch.bfloat16, spread=True):
     return x.to(dtype).to(DEV)
 
 
-def lost(a, b):
+def lost(a, b, wide=False):
     """Bound of what the products a (M, K) @ b (K, N) lose in their groups of eight."""
+    if wide:  # products of bf16 numbers: none
+        return 0.0
     ga, gb = (t.abs().unflatten(dim, (-1, 8)).amax(-1 if dim else 1) for t, dim in ((a, 1), (b, 0)))
     return 7 * 2.0 ** -13 * (ga @ gb)
 
 
-def products(a, b, e):
+def products(a, b, e, wide=False):
     """a[r] @ b[e[r]] in 64 bits, and the bound of the 8-bit products' own error, sorted rows."""
     M, K = a.shape
     ref = torch.empty(M, b.shape[2], dtype=torch.float64, device=a.device)
@@ -44,7 +46,7 @@ def products(a, b, e):
     for i in e.unique().tolist():
         r = e == i
         ref[r] = a[r] @ b[i]
-        err[r] = lost(a[r], b[i]) + (K + 8) * 2.0 ** -23 * (a[r].abs() @ b[i].abs())
+        err[r] = lost(a[r], b[i], wide) + (K + 8) * 2.0 ** -23 * (a[r].abs() @ b[i].abs())
     return ref, err
 
 
@@ -193,19 +195,20 @@ def test_nan_rows_stay_in_their_rows():
     assert torch.isnan(y[[3, 66]]).all() and int(bad.sum()) == 2
 
 
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("E,M,d,h,kind", [(1, 1, 16, 16, "even"), (3, 50, 272, 336, "skew"), (4, 600, 400, 144, "skew"),
                                           (2, 600, 128, 272, "one"), (40, 300, 2064, 64, "skew")])
-def test_gate_up(E, M, d, h, kind):
+def test_gate_up(E, M, d, h, kind, wide):
     """act within half an e4m3 step of silu(g) u in 64 bits, plus the step that act's own error may move it by."""
     o = ops()
     x, w = rand(M, d, seed=M, spread=False), rand(E, d, 2 * h, seed=h, spread=False) * d ** -0.5
     q, s = o.quant_rows(x)
     st = o.F8Stack.from_weights(w, halves=2)
     counts = R.counts_of(M, E, kind)
-    act, act_s = o.gate_up_swiglu_f8(q, s, st, counts.to(DEV))
+    act, act_s = o.gate_up_swiglu_f8(q, s, st, counts.to(DEV), wide=wide)
     a, b = o.dequant_rows(q, s).double(), st.dequant().double()
     e = torch.repeat_interleave(torch.arange(E), counts.long()).to(DEV)
-    gu, mag = products(a, b, e)
+    gu, mag = products(a, b, e, wide)
     g, u = gu.split(h, 1)
     ref = g * torch.sigmoid(g) * u
     # |silu'| <= 1.1; silu in fp32 with an approximate exp and reciprocal: 8 steps of 2^-24
@@ -239,7 +242,7 @@ def test_moe_experts(T, E, k, d, h, dtype):
     y, inv, bad = o.moe_experts(x, ids, tw, gu, dn)
     disp = o.dispatch(ids, E, want_xs=False)
     M = T * k
-    act, act_s = o.gate_up_swiglu_f8(*o.quant_rows(x), gu, disp.counts, M, a_idx=disp.a_idx)
+    act, act_s = o.gate_up_swiglu_f8(*o.quant_rows(x), gu, disp.counts, M, a_idx=disp.a_idx, wide=dtype is torch.float16)
     n = int(disp.counts.sum())
     flat = disp.order[:n].long()
     # (positions past the counted rows carry no index: a permutation stands in for them)

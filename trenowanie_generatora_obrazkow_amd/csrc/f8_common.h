@@ -49,4 +49,15 @@ __device__ __forceinline__ void f8_unpack2(uint32_t w, float& a, float& b) {
   b = v[1];
 }
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+// eight e4m3 values times 2^e as bf16, exactly
+__device__ __forceinline__ u32x4 f8_widen(uint2 v, float scale) {
+  u32x4 f;
+  f[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v.x, scale, false));
+  f[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v.x, scale, true));
+  f[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v.y, scale, false));
+  f[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v.y, scale, true));
+  return f;
+}
+
 }  // namespace hmoe

@@ -63,8 +63,6 @@ struct FewParams {
 };
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x2v __attribute__((ext_vector_type(2)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 template <bool F16>
 __device__ __forceinline__ f32x4 few_mfma(u32x4 a, u32x4 b, f32x4 c) {
@@ -99,16 +97,6 @@ __device__ __forceinline__ u32x4 few_column(const uint4 (&r)[8], int j) {
       f[i] = __builtin_amdgcn_perm(b[j / 2], a[j / 2], j & 1 ? 0x07060302u : 0x05040100u);
     }
   }
-  return f;
-}
-
-// eight e4m3 values times 2^e as bf16, exactly
-__device__ __forceinline__ u32x4 f8_widen(uint2 v, float scale) {
-  u32x4 f;
-  f[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v.x, scale, false));
-  f[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v.x, scale, true));
-  f[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v.y, scale, false));
-  f[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v.y, scale, true));
   return f;
 }
 

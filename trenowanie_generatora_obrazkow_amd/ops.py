@@ -1280,9 +1280,11 @@ def grouped_mm_f8_bwd(dy, w, counts):
     return _f8_mm(q, s, w.grad_q, w.grad_s, E, N, K, 1, counts, dy.shape[0], None, None, None, dy.dtype)
 
 
-def gate_up_swiglu_f8(q, s, wgu, counts, M=None, a_idx=None):
+def gate_up_swiglu_f8(q, s, wgu, counts, M=None, a_idx=None, wide=False):
     """act = silu(g) * u of [g | u] = a[a_idx] @ wgu[e] in fp32, in 8 bits -> (act (M, h) float8_e4m3fn, its scales
-    (M, ceil(h / 128)) float8_e8m0fnu), ready for grouped_mm_f8 with the down stack.  wgu: an F8Stack (E, d, 2h) of 2 halves."""
+    (M, ceil(h / 128)) float8_e8m0fnu), ready for grouped_mm_f8 with the down stack.  wgu: an F8Stack (E, d, 2h) of 2 halves.
+    wide: the products on the bf16 matrix instructions, exact but for the fp32 sums, at half the rate (the 8-bit ones drop some
+    2^-16 of a sum, which moves about one act in a thousand across a border of its 8 bits); moe_experts takes it for fp16."""
     E, d, h2 = _f8_stack(wgu, "wgu", q.device, halves=2)
     rows, K, ld, lds = _f8_rows(q, s)
     dev, h = q.device, h2 // 2
@@ -1299,7 +1301,7 @@ def gate_up_swiglu_f8(q, s, wgu, counts, M=None, a_idx=None):
     act = torch.empty(M, h, device=dev, dtype=_E4M3)
     act_s = torch.empty(M, _f8_ld(h), device=dev, dtype=_E8M0)
     _call_on(dev, "hmoe_f8_gate_up_swiglu", L.ptr(q), ld, L.ptr(s), lds, L.ptr(a_idx), L.ptr(wgu.q), L.ptr(wgu.s), E, d, h,
-             L.ptr(counts), L.dt(counts), M, L.ptr(act), L.ptr(act_s))
+             L.ptr(counts), L.dt(counts), M, int(bool(wide)), L.ptr(act), L.ptr(act_s))
     return act, act_s[:, :-(-h // 128)]
 
 
