@@ -532,14 +532,14 @@ int hmoe_swiglu_pack_bwd(const void* dh, const void* q, const uint8_t* s, const 
  * rounded once (the bits differ from those of hmoe_moe_forward / hmoe_moe_experts, which round on the way).  T <= 16, k <= 16,
  * E <= 1024; d and h multiples of 8 (int8 and 8-bit floats: 16).  Experts as hmoe_moe_experts takes them (x's type, or int8
  * with bf16 / fp32 scales), or w_dtype = HMOE_DT_F8: stacks (E, 2h, d) and (E, d, h) of hmoe_f8_quant_stack with their scales.
- * Ids outside [0, E) add nothing; one expert may come several times.  add (T, d) of x's type or NULL; out (T, d), not over an
+ * Ids outside [0, E) add nothing, their number goes to n_invalid (1,) (NULL to skip); one expert may come several times.  add (T, d) of x's type or NULL; out (T, d), not over an
  * input of the call.  workspace: hmoe_few_workspace_size bytes, 256-byte aligned, not shared by calls that may run at once.
  * ------------------------------------------------------------------------------------------------------------- */
 size_t hmoe_few_workspace_size(int64_t T, int64_t d, int E, int k, int64_t h, int w_dtype, int dtype);
 int hmoe_few_experts(const void* x, int64_t ldx, int dtype, const void* topk_ids, int ids_dtype, const void* topk_w,
                      int topk_w_dtype, const void* wgu, const void* wgu_s, int wgu_s_dtype, const void* wd, const void* wd_s,
                      int wd_s_dtype, int w_dtype, int64_t T, int64_t d, int E, int k, int64_t h, const void* add, void* out,
-                     void* workspace, size_t workspace_bytes, hmoe_stream_t stream);
+                     int32_t* n_invalid, void* workspace, size_t workspace_bytes, hmoe_stream_t stream);
 /* The same with the softmax router of hmoe_route_topk (the same ids and weights; E <= 256) for bf16 experts: in the first
  * kernel for E <= 16, ahead of it otherwise. */
 int hmoe_few_forward(const void* x, int64_t ldx, const void* wr, const float* bias, const void* wgu, const void* wd, int64_t T,

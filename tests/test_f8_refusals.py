@@ -157,7 +157,7 @@ def test_few_codes(L):
 
     def f(x=P, ldx=64, dt=BF, ids=P, idt=I32, tw=P, twdt=FP, w1=P, s1=None, sdt=BF, w2=P, s2=None, wdt=BF, T=4, d=64, E=3, k=2,
           h=48, add=None, out=P, ws=P2, n=1 << 24):
-        return L.hmoe_few_experts(x, ldx, dt, ids, idt, tw, twdt, w1, s1, sdt, w2, s2, sdt, wdt, T, d, E, k, h, add, out, ws, n, None)
+        return L.hmoe_few_experts(x, ldx, dt, ids, idt, tw, twdt, w1, s1, sdt, w2, s2, sdt, wdt, T, d, E, k, h, add, out, None, ws, n, None)
     assert f(T=0) == 0 and f(T=-1) == ARG and f(d=0) == ARG and f(k=0) == ARG
     assert f(dt=FP) == DTYPE and f(wdt=HF) == DTYPE and f(dt=HF, wdt=BF) == DTYPE and f(idt=FP) == DTYPE and f(twdt=I32) == DTYPE
     assert f(wdt=I8) == ARG and f(s1=P) == ARG and f(wdt=I8, s1=P, s2=P, sdt=HF) == DTYPE and f(wdt=6) == ARG

@@ -95,7 +95,7 @@ SIGNATURES = {
     "hmoe_swiglu_pack_bwd": (_I32, [_P, _P, _P, _P, _I32, _I64, _I64, _P, _P, _P, _P, _I32, _P]),
     "hmoe_few_workspace_size": (_SZ, [_I64, _I64, _I32, _I32, _I64, _I32, _I32]),
     "hmoe_few_experts": (_I32, [_P, _I64, _I32, _P, _I32, _P, _I32, _P, _P, _I32, _P, _P, _I32, _I32, _I64, _I64, _I32, _I32,
-                                _I64, _P, _P, _P, _SZ, _P]),
+                                _I64, _P, _P, _P, _P, _SZ, _P]),
     "hmoe_few_forward": (_I32, [_P, _I64, _P, _P, _P, _P, _I64, _I64, _I32, _I32, _I64, _I32, _F32, _P, _P, _P, _P, _P, _SZ,
                                 _P]),
     "hmoe_f8_scale_ld": (_SZ, [_I64]),

@@ -51,6 +51,7 @@ struct FewParams {
   float scaling;
   int32_t* out_ids;
   float* out_w;
+  int32_t* n_invalid;
   const void *wgu, *wd;
   const void *s1, *s2;     // int8: scales per column; 8-bit floats: per block
   int s1_f32, s2_f32;
@@ -271,7 +272,10 @@ __global__ __launch_bounds__(256, 1) void few_up_kernel(FewParams p) {
   const int A = few_group(g, M);
   if (blockIdx.x == 0) {
     FewHead& h = *p.head;
-    if (tid == 0) h.active = A;
+    if (tid == 0) {
+      h.active = A;
+      if (p.n_invalid) *p.n_invalid = M - (A > 0 ? g.base[A - 1] + g.rows[A - 1] : 0);
+    }
     if (tid < A) {
       h.expert[tid] = g.expert[tid];
       h.rows[tid] = g.rows[tid];
@@ -833,7 +837,7 @@ size_t hmoe_few_workspace_size(int64_t T, int64_t d, int E, int k, int64_t h, in
 int hmoe_few_experts(const void* x, int64_t ldx, int dtype, const void* topk_ids, int ids_dtype, const void* topk_w,
                      int topk_w_dtype, const void* wgu, const void* wgu_s, int wgu_s_dtype, const void* wd, const void* wd_s,
                      int wd_s_dtype, int w_dtype, int64_t T, int64_t d, int E, int k, int64_t h, const void* add, void* out,
-                     void* workspace, size_t workspace_bytes, hmoe_stream_t stream) {
+                     int32_t* n_invalid, void* workspace, size_t workspace_bytes, hmoe_stream_t stream) {
   FewPlan P;
   int w = 0;
   int rc = few_check(x, ldx, dtype, wgu, wgu_s, wgu_s_dtype, wd, wd_s, wd_s_dtype, w_dtype, T, d, E, k, h, add, out, workspace,
@@ -850,6 +854,7 @@ int hmoe_few_experts(const void* x, int64_t ldx, int dtype, const void* topk_ids
   p.ids64 = ids_dtype == HMOE_DT_I64;
   p.tw = topk_w;
   p.tw_dt = topk_w_dtype;
+  p.n_invalid = n_invalid;
   p.wgu = wgu; p.wd = wd; p.s1 = wgu_s; p.s2 = wd_s;
   p.s1_f32 = wgu_s_dtype == HMOE_DT_F32;
   p.s2_f32 = wd_s_dtype == HMOE_DT_F32;

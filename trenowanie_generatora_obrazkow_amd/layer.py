@@ -219,7 +219,8 @@ class _MoEFunction(torch.autograd.Function):
         return _experts_backward(state, dout, dtw_out, *ctx.needs_input_grad[:4]) + none
 
 
-def moe_swiglu(x, router_weight, w_gu, w_d, top_k, logit_bias=None, renorm=True, gate=None, select_bias=None, checkpoint=None):
+def moe_swiglu(x, router_weight, w_gu, w_d, top_k, logit_bias=None, renorm=True, gate=None, select_bias=None, checkpoint=None,
+               few_tokens=0):
     """Functional form: x (T, d) bf16 -> (out (T, d) bf16, topk_ids (T, k) int32, topk_weight (T, k) fp32).
 
     router_weight (E, d), w_gu (E, d, 2h) = [gate | up], w_d (E, h, d): bf16, or fp32 / fp16 (rounded to bf16 for
@@ -228,12 +229,17 @@ def moe_swiglu(x, router_weight, w_gu, w_d, top_k, logit_bias=None, renorm=True,
     scores, groups or a factor on the weights; select_bias (E,) fp32 joins the scores for the selection only (a bias for
     balance; no gradient).  checkpoint="fp8" keeps [g | u] for the backward in 8 bits (ops.swiglu_pack), and neither the
     activation nor the permuted rows: about a third of the memory; the forward is the same but for act's single rounding, the
-    gradients are those at the kept g and u.  Without a
+    gradients are those at the kept g and u.  few_tokens: without a gradient, calls of at most that many tokens (up to 16) run as
+    two kernels (ops.few_forward, ops.few_experts), rounded once, so that their last bits differ from a larger call's.  Without a
     gradient to record (grad mode off, or no input requiring one) the forward runs as one C call
     (ops.moe_forward; with a gate or a selection bias, the routing and ops.moe_experts): the same kernels and outputs, a
     fraction of the host time."""
     _check_checkpoint(checkpoint)
+    if not 0 <= few_tokens <= ops.FEW_TOKENS:
+        raise ValueError(f"few_tokens = {few_tokens}: 0 to {ops.FEW_TOKENS}")
     if not _recorded(x, router_weight, w_gu, w_d):
+        if 0 < x.shape[0] <= few_tokens and top_k <= 16:
+            return _few_infer(x, router_weight, w_gu, w_d, logit_bias, top_k, renorm, gate, select_bias)
         if gate is None and select_bias is None:
             _check_layer_args(x, router_weight, w_gu, w_d, logit_bias, top_k)
             out, ids, tw, _ = ops.moe_forward(x, _bf16(router_weight), _bf16(w_gu), _bf16(w_d), top_k, bias=logit_bias,
@@ -252,6 +258,18 @@ def _experts_infer(x, wr, wgu, wd, bias, k, renorm, gate, select_bias):
     _, ids, tw = _route(x, _bf16(wr), bias, k, renorm, gate, select_bias)
     y, inv, _ = ops.moe_experts(x, ids, tw, _bf16(wgu), _bf16(wd))
     return y, ids, tw, inv
+
+
+def _few_infer(x, wr, wgu, wd, bias, k, renorm, gate, select_bias):
+    """The layer on a few tokens in two kernels -> (out, ids, weights)."""
+    _check_layer_args(x, wr, wgu, wd, bias, k)
+    if select_bias is not None and tuple(select_bias.shape) != (wgu.shape[0],):
+        raise ValueError(f"select_bias: shape {tuple(select_bias.shape)}, expected ({wgu.shape[0]},)")
+    wr, wgu, wd = _bf16(wr), _bf16(wgu), _bf16(wd)
+    if gate is None and select_bias is None:
+        return ops.few_forward(x, wr, wgu, wd, k, bias=bias, renorm=renorm)
+    _, ids, tw = _route(x, wr, bias, k, renorm, gate, select_bias)
+    return ops.few_experts(x, ids, tw, wgu, wd), ids, tw
 
 
 class _ExpertStackProj:
@@ -291,6 +309,7 @@ class MoESwiGLU(nn.Module):
     fp32, which joins the scores for the selection only: a training script that balances its experts without a loss raises
     it for experts that got too few tokens and lowers it for the others.
 
+    `few_tokens` (up to 16): calls of at most that many tokens without a gradient run as two kernels (moe_swiglu).
     `checkpoint="fp8"` keeps [g | u] for the backward in 8 bits and nothing else of the experts' activations (moe_swiglu).
 
     The products run in bf16 (any other input dtype is rounded to bf16 first); the output has the dtype the
@@ -299,10 +318,10 @@ class MoESwiGLU(nn.Module):
 
     def __init__(self, dim: int, hidden: int, experts: int, top_k: int = 2, renorm: bool = True,
                  init_std: float | None = None, device=None, dtype=torch.bfloat16, gate: Gate | None = None,
-                 balance: bool = False, checkpoint: str | None = None):
+                 balance: bool = False, checkpoint: str | None = None, few_tokens: int = 0):
         super().__init__()
         _check_checkpoint(checkpoint)
-        self.checkpoint = checkpoint
+        self.checkpoint, self.few_tokens = checkpoint, few_tokens
         self.dim, self.hidden, self.experts, self.top_k, self.renorm = dim, hidden, experts, top_k, renorm
         self.gate = gate
         f = dict(device=device, dtype=dtype)
@@ -323,6 +342,7 @@ class MoESwiGLU(nn.Module):
         super().__setstate__(state)
         self.__dict__.setdefault("gate", None)  # (pickled before the layer had gates)
         self.__dict__.setdefault("checkpoint", None)
+        self.__dict__.setdefault("few_tokens", 0)
         if "select_bias" not in self._buffers:
             self.__dict__.setdefault("select_bias", None)
 
@@ -346,7 +366,7 @@ class MoESwiGLU(nn.Module):
         if x.dtype != torch.bfloat16:
             x = x.to(torch.bfloat16)
         out, ids, tw = moe_swiglu(x, self.router_weight, self.w_gu, self.w_d, self.top_k, self.logit_bias,
-                                  self.renorm, self.gate, self.select_bias, self.checkpoint)
+                                  self.renorm, self.gate, self.select_bias, self.checkpoint, self.few_tokens)
         self.last_topk_ids, self.last_topk_weight = ids, tw
         out = out.view(shape)
         return out if out.dtype == out_dtype else out.to(out_dtype)

@@ -1430,19 +1430,20 @@ def _few_args(x, k, wgu, wd, wgu_s, wd_s, add):
     return T, d, ld, E, h, ws, torch.empty(n, device=dev, dtype=torch.uint8), torch.empty(T, d, device=dev, dtype=x.dtype)
 
 
-def few_experts(x, ids, tw, wgu, wd, wgu_s=None, wd_s=None, add=None):
+def few_experts(x, ids, tw, wgu, wd, wgu_s=None, wd_s=None, add=None, want_invalid=False):
     """The experts of a routed layer and the sum over its slots for up to 16 tokens, in two kernels (hmoe_few_experts): moe_experts
     and combine in fp32 throughout, rounded once -> out (T, d).  x (T, d) bf16 or fp16; ids (T, k) int32 / int64, those outside
     [0, E) add nothing; tw (T, k); wgu (E, d, 2h) and wd (E, h, d) of x's type, int8 with scales, or F8Stacks; add (T, d) of x's
-    type (a shared expert's output) joins the sum."""
+    type (a shared expert's output) joins the sum.  want_invalid: (out, n_invalid (1,) int32), how many ids named no expert."""
     T, k = ids.shape
     T_, d, ld, E, h, w, ws, out = _few_args(x, k, wgu, wd, wgu_s, wd_s, add)
     dev = x.device
     _on(ids, "topk_ids", dev, (T_, k), (torch.int32, torch.int64))
     tw = _on(tw if tw.dtype in _FLOATS else tw.float(), "topk_weight", dev, (T_, k), _FLOATS)
+    bad = torch.zeros(1, device=dev, dtype=torch.int32) if want_invalid else None
     _call_on(dev, "hmoe_few_experts", L.ptr(x), ld, L.dt(x), L.ptr(ids), L.dt(ids), L.ptr(tw), L.dt(tw), *w, T, d, E, k, h,
-             L.ptr(add), L.ptr(out), L.ptr(ws), ws.numel())
-    return out
+             L.ptr(add), L.ptr(out), L.ptr(bad), L.ptr(ws), ws.numel())
+    return (out, bad) if want_invalid else out
 
 
 def few_forward(x, wr, wgu, wd, k, bias=None, renorm=True, scaling=1.0, add=None):
