@@ -8,6 +8,7 @@
 // per row of a and one per 128 columns of w.
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 
 #include "f8_common.h"
 #include "gemm_common.h"
@@ -591,6 +592,7 @@ __global__ __launch_bounds__(C::NT, C::LDS_BYTES > 81920 ? 1 : 2) void f8_gemm_k
       constexpr int TURNS = 2 * 32 * RB * C::NW <= C::STAGE ? 2 : 1;
       static_assert(32 * RB * C::NW <= C::STAGE, "a pass of every wave in a stage");
       char* const own = park + wave * (TURNS * 32 * RB);
+      if (wm * C::TM >= t.live) wait_vm<0>();  // (a wave without rows: see below)
 #pragma unroll
       for (int a = 0; a < C::FM; ++a) {
         const int rbase = wm * C::TM + a * 32;
@@ -615,7 +617,7 @@ __global__ __launch_bounds__(C::NT, C::LDS_BYTES > 81920 ? 1 : 2) void f8_gemm_k
               }
             }
           __builtin_amdgcn_wave_barrier();
-          // the next tile's first slice and scales have landed before the first store: no slice waits for the stores
+          // the next tile's first slice and scales have landed before the first store: that slice does not wait for the stores
           if (a == 0 && b0 == 0) wait_vm<0>();
 #pragma unroll
           for (int i = 0; i < 32 / RPI; ++i) {
@@ -721,12 +723,28 @@ static int f8_launch(const F8Params& p, hipStream_t s) {
   return HMOE_OK;
 }
 
+// Tile height: 32 rows (two workgroups per CU, for few rows per expert: the launch streams weights), 128 or 256.  Each is
+// priced by its rounds over the CUs, a round by its slices; the prices (us, of launches with 2 to 20 rounds and random counts:
+// 32 rows 4 + 0.9 per slice, 128 6 + 1.0, 256 8 + 1.45) follow 40 layers of 8 to 128 experts, 4 to 600 rows each, d 768-2048, h
+// 320-4096, all tiles timed in turn.  Over these the choice is the fastest or within 10% of it in all but two launches (15%);
+// one line by rows per expert (256 from 160 on, 128 from 64 on) took up to 1.9 times the fastest: 1024 -> 1024 x 2048 rows over
+// 8 experts of 300 31 instead of 19 us, 16 experts of 160 rows, 4096 -> 1536, 60 instead of 50.
 template <int EPI, int CDT, bool WIDE = false>
 static int f8_pick(const F8Params& p, hipStream_t s) {
-  const int64_t rows = p.M / std::min<int64_t>(p.E, p.M);  // per expert
-  if (rows >= 160) return f8_launch<F8Cfg<256, 256, 2, 2, 2>, EPI, CDT, WIDE>(p, s);
-  if (rows >= 64) return f8_launch<F8Cfg<128, 256, 2, 2, 2>, EPI, CDT, WIDE>(p, s);
-  return f8_launch<F8Cfg<32, 256, 1, 4, 2>, EPI, CDT, WIDE>(p, s);
+  const int cus = f8_cus();
+  if (cus <= 0) return HMOE_ERR_DEVICE;
+  const double hit = (double)std::min<int64_t>(p.E, p.M), rows = (double)p.M / hit, nk = (p.K + kF8Slice - 1) / kF8Slice;
+  const double nb = EPI == F8_SWIGLU ? (p.N + 127) / 128 : p.halves * ((p.N + 255) / 256);
+  auto price = [&](double bm, double slots, double fixed, double slice) {
+    const double rounds = 1.08 * hit * std::max(1.0, rows / bm + 0.5) * nb / slots;  // (uneven counts make some tiles more)
+    return (rounds < 4 ? std::ceil(rounds) : rounds) * (fixed + slice * nk);
+  };
+  const double wide = WIDE ? 1.0 : 0.0;  // (a wide slice's products take 0.85 us more with 256 rows)
+  const double t32 = price(32, 2 * cus, 4, 0.9 + 0.1 * wide), t128 = price(128, cus, 6, 1.0 + 0.42 * wide),
+               t256 = price(256, cus, 8, 1.45 + 0.85 * wide);
+  if (t32 <= t128 && t32 <= t256) return f8_launch<F8Cfg<32, 256, 1, 4, 2>, EPI, CDT, WIDE>(p, s);
+  if (t128 <= t256) return f8_launch<F8Cfg<128, 256, 2, 2, 2>, EPI, CDT, WIDE>(p, s);
+  return f8_launch<F8Cfg<256, 256, 2, 2, 2>, EPI, CDT, WIDE>(p, s);
 }
 
 static bool al(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
