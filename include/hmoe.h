@@ -497,6 +497,12 @@ int hmoe_f8_grouped_mm(const void* a, int64_t lda, const uint8_t* a_s, int64_t l
                        int64_t E, int64_t K, int64_t N, int halves, const void* counts, int counts_dtype, int64_t M,
                        const int32_t* a_idx, const int32_t* y_idx, const void* scale, int scale_dtype, int scale_by_y, void* y,
                        int64_t ldy, int y_dtype, hmoe_stream_t stream);
+/* Both in one call: x (rows, K) bf16, fp16 or fp32 quantised into the workspace (16-byte aligned), then the product of its rows. */
+size_t hmoe_f8_quant_mm_workspace_size(int64_t rows, int64_t K);
+int hmoe_f8_quant_mm(const void* x, int64_t ldx, int x_dtype, int64_t rows, const void* w, const uint8_t* w_s, int64_t E,
+                     int64_t K, int64_t N, int halves, const void* counts, int counts_dtype, int64_t M, const int32_t* a_idx,
+                     const int32_t* y_idx, const void* scale, int scale_dtype, int scale_by_y, void* y, int64_t ldy, int y_dtype,
+                     void* workspace, size_t workspace_bytes, hmoe_stream_t stream);
 /* act = silu(g) * u of [g | u] = x[a_idx] @ wgu[e], all in fp32, quantised: act (M, h) e4m3, act_s (M, scale_ld(h)).  wgu
  * (E, 2h, d) with halves = 2.  The 8-bit matrix instructions drop what lies below 2^-13 of the largest of eight products: some
  * 2^-16 of a sum, which moves about one act in a thousand across a border of its 8 bits.  wide = 1 multiplies the same values

@@ -65,6 +65,18 @@ def test_grouped_mm_codes(L):
     assert f(M=1 << 26, ai=P) == SHAPE                                           # gathered rows past 2 GiB
 
 
+def test_quant_mm_codes(L):
+    n = L.hmoe_f8_quant_mm_workspace_size(4, 64)
+    assert n >= 4 * (64 + 16) and L.hmoe_f8_quant_mm_workspace_size(-1, 64) == 0
+
+    def f(x=P, ldx=64, dt=BF, rows=4, w=P, K=64, N=96, halves=1, cdt=I32, M=4, sc=None, sdt=FP, y=P, ldy=96, ydt=BF, ws=P, n=n):
+        return L.hmoe_f8_quant_mm(x, ldx, dt, rows, w, P, 2, K, N, halves, P, cdt, M, None, None, sc, sdt, 0, y, ldy, ydt, ws, n, None)
+    assert f(M=0) == 0 and f(rows=-1) == ARG and f(M=-1) == ARG and f(rows=3) == ARG and f(x=None) == ARG and f(w=None) == ARG
+    assert f(ws=None) == WORKSPACE and f(n=n - 1) == WORKSPACE and f(ws=P + 8) == WORKSPACE
+    assert f(dt=I8) == DTYPE and f(ydt=I8) == DTYPE and f(sc=P, sdt=I32) == DTYPE and f(cdt=FP) == DTYPE
+    assert f(K=72, n=1 << 20) == SHAPE and f(N=104, ldy=104) == SHAPE and f(ldy=88) == ARG and f(y=P + 8) == ARG and f(ldx=68) == ARG
+
+
 def test_gate_up_codes(L):
     def f(x=P, M=4, d=64, h=48, act=P, act_s=P, E=2):
         return L.hmoe_f8_gate_up_swiglu(x, d, P, 16, None, P, P, E, d, h, P, I32, M, 0, act, act_s, None)

@@ -303,11 +303,27 @@ def test_tail_gradient_is_zero():
     assert torch.equal(a.grad[17:], torch.zeros_like(a.grad[17:])) and torch.equal(y[17:], torch.zeros_like(y[17:]))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_one_call(dtype):
+    """The product with its rows quantised on the way has the bits of the two calls."""
+    o = ops()
+    x = rand(60, 400, seed=2, dtype=dtype)[:, 16:16 + 272]
+    st = o.F8Stack.from_weights(rand(3, 272, 96, seed=4), halves=2)
+    c = torch.tensor([20, 0, 25], device=DEV)
+    a = torch.randint(0, 60, (45,), generator=torch.Generator().manual_seed(0)).int().to(DEV)
+    y_idx, sc = torch.randperm(45).int().to(DEV), torch.rand(45, device=DEV)
+    q, s = o.quant_rows(x)
+    assert torch.equal(o.quant_mm_f8(x, st, c, a_idx=a, y_idx=y_idx, scale=sc), o.grouped_mm_f8(q, s, st, c, 45, a, y_idx, sc, dtype))
+    assert torch.equal(o.quant_mm_f8(x, st, c, dtype=torch.float32), o.grouped_mm_f8(q, s, st, c, dtype=torch.float32))
+
+
 def test_empty():
     o = ops()
     st = o.F8Stack.from_weights(rand(2, 64, 32, seed=4))
     q, s = o.quant_rows(torch.empty(0, 64, device=DEV, dtype=torch.bfloat16))
-    assert o.grouped_mm_f8(q, s, st, torch.zeros(2, dtype=torch.int32, device=DEV)).shape == (0, 32)
+    zero = torch.zeros(2, dtype=torch.int32, device=DEV)
+    assert o.grouped_mm_f8(q, s, st, zero).shape == (0, 32)
+    assert o.quant_mm_f8(torch.empty(0, 64, device=DEV), st, zero).shape == (0, 32)
 
 
 def test_graph_and_stream():

@@ -896,6 +896,32 @@ int hmoe_f8_grouped_mm(const void* a, int64_t lda, const uint8_t* a_s, int64_t l
   return f8_pick<F8_STORE, HMOE_DT_F32>(p, s);
 }
 
+size_t hmoe_f8_quant_mm_workspace_size(int64_t rows, int64_t K) {
+  if (rows < 0 || K <= 0 || K > INT32_MAX - 256 || rows > INT32_MAX) return 0;
+  return static_cast<size_t>(rows) * static_cast<size_t>((K + 15) / 16 * 16 + f8_scale_ld(K)) + 16;
+}
+
+int hmoe_f8_quant_mm(const void* x, int64_t ldx, int x_dtype, int64_t rows, const void* w, const uint8_t* w_s, int64_t E,
+                     int64_t K, int64_t N, int halves, const void* counts, int counts_dtype, int64_t M, const int32_t* a_idx,
+                     const int32_t* y_idx, const void* scale, int scale_dtype, int scale_by_y, void* y, int64_t ldy, int y_dtype,
+                     void* workspace, size_t workspace_bytes, hmoe_stream_t stream) {
+  if (rows < 0 || K <= 0) return HMOE_ERR_ARG;
+  const size_t need = hmoe_f8_quant_mm_workspace_size(rows, K);
+  if (!workspace || need == 0 || workspace_bytes < need || !al(workspace, 16)) return HMOE_ERR_WORKSPACE;
+  auto* q = static_cast<uint8_t*>(workspace);
+  auto* s = q + rows * ((K + 15) / 16 * 16);
+  // the product's limits ahead of the first launch, so that a refused call launches nothing
+  int rc = f8_check(q, K, s, f8_scale_ld(K), a_idx, w, w_s, E, K, N, halves, counts, counts_dtype, M);
+  if (rc) return rc;
+  if (y_dtype != HMOE_DT_BF16 && y_dtype != HMOE_DT_F16 && y_dtype != HMOE_DT_F32) return HMOE_ERR_DTYPE;
+  if (scale && scale_dtype != HMOE_DT_BF16 && scale_dtype != HMOE_DT_F16 && scale_dtype != HMOE_DT_F32) return HMOE_ERR_DTYPE;
+  if (M > 0 && (!y || !al(y, 16) || ldy < N || ldy % 8 || rows < (a_idx ? 1 : M))) return HMOE_ERR_ARG;
+  rc = hmoe_f8_quant_rows(x, ldx, x_dtype, M == 0 ? 0 : rows, K, q, K, s, f8_scale_ld(K), stream);
+  if (rc) return rc;
+  return hmoe_f8_grouped_mm(q, K, s, f8_scale_ld(K), w, w_s, E, K, N, halves, counts, counts_dtype, M, a_idx, y_idx, scale,
+                            scale_dtype, scale_by_y, y, ldy, y_dtype, stream);
+}
+
 int hmoe_f8_gate_up_swiglu(const void* x, int64_t ldx, const uint8_t* x_s, int64_t ldx_s, const int32_t* a_idx, const void* wgu,
                            const uint8_t* wgu_s, int64_t E, int64_t d, int64_t h, const void* counts, int counts_dtype,
                            int64_t M, int wide, void* act, uint8_t* act_s, hmoe_stream_t stream) {

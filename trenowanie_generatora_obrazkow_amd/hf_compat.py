@@ -63,7 +63,7 @@ def _f8_stacks(mod):
 
 
 def _mm_f8(a, w, counts, M, a_idx=None, y_idx=None, scale=None, w_scale=None):
-    return ops.grouped_mm_f8(*ops.quant_rows(a), w, counts, M, a_idx, y_idx, scale, a.dtype)
+    return ops.quant_mm_f8(a, w, counts, M, a_idx, y_idx, scale)
 
 
 def _is_silu(act):

@@ -77,8 +77,7 @@ def _grouped_mm_f8(a, w, counts, a_idx, y_idx, scale, w_scale):
         return _GroupedMMF8.apply(a, w, counts)
     a_idx, y_idx = (i if i is None else i.to(torch.int32).contiguous() for i in (a_idx, y_idx))
     scale = scale if scale is None else scale.contiguous()
-    return ops.grouped_mm_f8(*ops.quant_rows(a.detach()), w, counts.contiguous(), a_idx=a_idx, y_idx=y_idx, scale=scale,
-                             dtype=a.dtype)
+    return ops.quant_mm_f8(a, w, counts.contiguous(), None, a_idx, y_idx, scale)
 
 
 class _GroupedMMF8(torch.autograd.Function):
@@ -89,7 +88,7 @@ class _GroupedMMF8(torch.autograd.Function):
         counts = counts.contiguous()
         ctx.w = w
         ctx.save_for_backward(counts)
-        return ops.grouped_mm_f8(*ops.quant_rows(a), w, counts, dtype=a.dtype)
+        return ops.quant_mm_f8(a, w, counts)
 
     @staticmethod
     @torch.autograd.function.once_differentiable

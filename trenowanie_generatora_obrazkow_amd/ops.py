@@ -1234,6 +1234,48 @@ def _f8_stack(w, name, dev, shape=None, halves=None):
     return E, K, N
 
 
+def _f8_idx(counts, a_idx, y_idx, scale, dev, E, M, rows, ld):
+    """The checks that the grouped products share -> (counts, scale)."""
+    counts = _on(counts if counts.dtype in (torch.int32, torch.int64) else counts.to(torch.int64), "counts", dev, (E,),
+                 (torch.int32, torch.int64))
+    if a_idx is not None:
+        _on(a_idx, "a_idx", dev, (M,), _I32)
+        if rows * ld >= 2 ** 31 - 32768:
+            raise ValueError("a gathered through a_idx must span less than 2 GiB (32-bit row offsets)")
+    if rows < (min(1, M) if a_idx is not None else M):
+        raise ValueError(f"a: {rows} rows for {M} of the product")
+    _on(y_idx, "y_idx", dev, (M,), _I32)
+    if scale is not None:
+        scale = _on(scale if scale.dtype in _FLOATS else scale.float(), "scale", dev, (M,), _FLOATS)
+    return counts, scale
+
+
+def quant_mm_f8(x, w, counts, M=None, a_idx=None, y_idx=None, scale=None, dtype=None):
+    """grouped_mm_f8 of x's rows quantised on the way (quant_rows), in one call: x (rows, K) bf16, fp16 or fp32 -> (M, N) of
+    `dtype`, x's type by default."""
+    E, K, N = _f8_stack(w, "w", x.device)
+    return _quant_mm(x, w.q, w.s, E, K, N, w.halves, counts, M, a_idx, y_idx, scale, dtype)
+
+
+def _quant_mm(x, wq, ws, E, K, N, halves, counts, M, a_idx, y_idx, scale, dtype):
+    rows, K_, ld = _rows(x, "x")
+    if K_ != K:
+        raise ValueError(f"x has {K_} columns, the stack {K} rows")
+    dtype = x.dtype if dtype is None else dtype
+    if dtype not in _FLOATS:
+        raise TypeError(f"dtype {dtype} not in {_FLOATS}")
+    dev = x.device
+    M = (a_idx.numel() if a_idx is not None else rows) if M is None else M
+    counts, scale = _f8_idx(counts, a_idx, y_idx, scale, dev, E, M, rows, K)
+    n = rows * (K + _f8_ld(K)) + 16
+    tmp = torch.empty(n, device=dev, dtype=torch.uint8)
+    y = torch.empty(M, N, device=dev, dtype=dtype)
+    _call_on(dev, "hmoe_f8_quant_mm", x.data_ptr(), ld, L.dt(x), rows, wq.data_ptr(), ws.data_ptr(), E, K, N, halves,
+             counts.data_ptr(), L.dt(counts), M, L.ptr(a_idx), L.ptr(y_idx), L.ptr(scale),
+             L.dt(scale) if scale is not None else 0, 0, y.data_ptr(), N, L.dt(dtype), tmp.data_ptr(), n)
+    return y
+
+
 def _f8_mm(q, s, wq, ws, E, K, N, halves, counts, M, a_idx, y_idx, scale, dtype, scale_by_y=False):
     """hmoe_f8_grouped_mm on checked stacks."""
     rows, K_, ld, lds = _f8_rows(q, s)
@@ -1242,16 +1284,7 @@ def _f8_mm(q, s, wq, ws, E, K, N, halves, counts, M, a_idx, y_idx, scale, dtype,
         raise ValueError(f"a has {K_} columns, the stack {K} rows")
     if dtype not in _FLOATS:
         raise TypeError(f"dtype {dtype} not in {_FLOATS}")
-    counts = _on(counts if counts.dtype in (torch.int32, torch.int64) else counts.to(torch.int64), "counts", dev, (E,),
-                 (torch.int32, torch.int64))
-    a_idx = _on(a_idx, "a_idx", dev, (M,), _I32)
-    y_idx = _on(y_idx, "y_idx", dev, (M,), _I32)
-    if rows < (min(1, M) if a_idx is not None else M):
-        raise ValueError(f"a: {rows} rows for {M} of the product")
-    if a_idx is not None and rows * ld >= 2 ** 31 - 32768:
-        raise ValueError("a gathered through a_idx must span less than 2 GiB (32-bit row offsets)")
-    if scale is not None:
-        scale = _on(scale if scale.dtype in _FLOATS else scale.float(), "scale", dev, (M,), _FLOATS)
+    counts, scale = _f8_idx(counts, a_idx, y_idx, scale, dev, E, M, rows, ld)
     y = torch.empty(M, N, device=dev, dtype=dtype)
     _call_on(dev, "hmoe_f8_grouped_mm", L.ptr(q), ld, L.ptr(s), lds, L.ptr(wq), L.ptr(ws), E, K, N, halves, L.ptr(counts),
              L.dt(counts), M, L.ptr(a_idx), L.ptr(y_idx), L.ptr(scale), L.dt(scale) if scale is not None else 0,
@@ -1276,8 +1309,7 @@ def grouped_mm_f8_bwd(dy, w, counts):
         raise ValueError("this F8Stack was made without grad=True: it has no layout for the gradient of the rows")
     _on(w.grad_q, "w.grad_q", dy.device, (E, K, N), (_E4M3,))
     _on(w.grad_s, "w.grad_s", dy.device, (E, -(-K // 128), _f8_ld(N)), (_E8M0,))
-    q, s = quant_rows(dy)
-    return _f8_mm(q, s, w.grad_q, w.grad_s, E, N, K, 1, counts, dy.shape[0], None, None, None, dy.dtype)
+    return _quant_mm(dy, w.grad_q, w.grad_s, E, N, K, 1, counts, None, None, None, None, None)
 
 
 def gate_up_swiglu_f8(q, s, wgu, counts, M=None, a_idx=None, wide=False):
@@ -1291,13 +1323,7 @@ def gate_up_swiglu_f8(q, s, wgu, counts, M=None, a_idx=None, wide=False):
     M = (a_idx.numel() if a_idx is not None else rows) if M is None else M
     if K != d:
         raise ValueError(f"a has {K} columns, wgu {d} rows")
-    counts = _on(counts if counts.dtype in (torch.int32, torch.int64) else counts.to(torch.int64), "counts", dev, (E,),
-                 (torch.int32, torch.int64))
-    a_idx = _on(a_idx, "a_idx", dev, (M,), _I32)
-    if rows < (min(1, M) if a_idx is not None else M):
-        raise ValueError(f"a: {rows} rows for {M} of the product")
-    if a_idx is not None and rows * ld >= 2 ** 31 - 32768:
-        raise ValueError("a gathered through a_idx must span less than 2 GiB (32-bit row offsets)")
+    counts, _ = _f8_idx(counts, a_idx, None, None, dev, E, M, rows, ld)
     act = torch.empty(M, h, device=dev, dtype=_E4M3)
     act_s = torch.empty(M, _f8_ld(h), device=dev, dtype=_E8M0)
     _call_on(dev, "hmoe_f8_gate_up_swiglu", L.ptr(q), ld, L.ptr(s), lds, L.ptr(a_idx), L.ptr(wgu.q), L.ptr(wgu.s), E, d, h,
