@@ -33,6 +33,7 @@ struct FewHead {
   int pad[3];
   int expert[kFewM], rows[kFewM], base[kFewM];  // each one's id, its routed rows, where they begin in `row`
   int row[kFewM];          // flat rows (token * k + slot), grouped by expert, in order
+  int row16[kFewM][16];    // the first sixteen of each expert again, where they are found without `base`
   float w[kFewM];          // routing weights by flat row, 0 for an id that names no expert
   int flat_ok[kFewM];      // whether a flat row's id names an expert
 };
@@ -119,7 +120,8 @@ __device__ __forceinline__ void f8_requant(const float (&v)[32], u32x4 (&f)[4]) 
 // Grouping: ids (flat rows, -1: none) -> the chosen experts in the order of their first rows, each with its rows in order
 // ----------------------------------------------------------------------------------------------------------------
 struct FewGroups {
-  int id[kFewM], expert[kFewM], rows[kFewM], base[kFewM], row[kFewM];
+  __attribute__((aligned(16))) int id[kFewM];
+  int expert[kFewM], rows[kFewM], base[kFewM], row[kFewM];
   int wave_n[4], wave_rows[4];
 };
 
@@ -128,11 +130,16 @@ __device__ __forceinline__ int few_group(FewGroups& g, int M) {
   const int my = i < M ? g.id[i] : -1;
   int before = 0, all = 0, first = i;
   if (my >= 0) {
-    for (int j = M - 1; j >= 0; --j) {
-      const bool same = g.id[j] == my;
-      all += same;
-      before += same && j < i;
-      if (same) first = j;
+    for (int j = 0; j < M; j += 4) {  // (ids past M are -1)
+      const int4 v = *reinterpret_cast<const int4*>(g.id + j);
+      const int id[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const bool same = id[t] == my;
+        all += same;
+        before += same && j + t < i;
+        if (same) first = min(first, j + t);
+      }
     }
   }
   const bool lead = my >= 0 && before == 0;
@@ -257,11 +264,14 @@ __global__ __launch_bounds__(256, 1) void few_up_kernel(FewParams p) {
     for (int i = 0; i < 4; ++i) red[wave * 256 + (4 * q + i) * 16 + l16] = acc[i];
     __syncthreads();
     const float* pt = red + (4 * wave + q) * 16 + l16;
+    if (tid < kFewM) g.id[tid] = -1;
+    __syncthreads();
     float lg[1] = {__fadd_rn(__fadd_rn(pt[0], pt[256]), __fadd_rn(pt[512], pt[768]))};
     if (p.bias && l16 < p.E) lg[0] = __fadd_rn(lg[0], p.bias[l16]);
     route_select16<1>(lg, 4 * wave, lane, p.T, p.E, p.k, p.renorm, p.scaling, nullptr, g.id, s_w);
     __syncthreads();
   } else {
+    g.id[tid] = -1;
     if (tid < M) {
       const int64_t id = p.ids64 ? static_cast<const int64_t*>(p.ids)[tid] : (int64_t) static_cast<const int32_t*>(p.ids)[tid];
       g.id[tid] = id >= 0 && id < p.E ? (int)id : -1;
@@ -289,6 +299,10 @@ __global__ __launch_bounds__(256, 1) void few_up_kernel(FewParams p) {
       h.w[tid] = ROUTE ? s_w[tid] : few_w(p.tw, p.tw_dt, tid);
       h.flat_ok[tid] = my >= 0;
       if (A > 0 && tid < g.base[A - 1] + g.rows[A - 1]) h.row[tid] = g.row[tid];
+    }
+    for (int i = tid; i < A * 16; i += 256) {
+      const int x = i >> 4, r = i & 15;
+      h.row16[x][r] = r < g.rows[x] ? g.row[g.base[x] + r] : 0;
     }
     for (int i = tid; i < p.runs2; i += 256) p.counter[i] = 0;
   }
@@ -422,7 +436,7 @@ __global__ __launch_bounds__(256, 1) void few_up_kernel(FewParams p) {
 // ----------------------------------------------------------------------------------------------------------------
 // The parts of the output pass between workgroups of one launch, on XCDs with an L2 each.  They are written and read as
 // agent-scope atomics: these go through to memory and are read from there, so no workgroup has to write a whole L2 back or
-// discard it (a release and an acquire fence per workgroup: 181 us instead of TIME_FEW16 for 16 tokens over 51 experts).
+// discard it (a release and an acquire fence per workgroup: 185 us instead of 40 for 16 tokens over 51 experts).
 __device__ __forceinline__ void put_agent(float* p, float a, float b) {
   const uint64_t v = (uint64_t)__float_as_uint(a) | (uint64_t)__float_as_uint(b) << 32;
   __hip_atomic_store(reinterpret_cast<uint64_t*>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -496,6 +510,7 @@ __global__ __launch_bounds__(256, 1) void few_down_kernel(FewParams p) {
   const FewHead& hd = *p.head;
   const int part = blockIdx.x % p.S2, run = blockIdx.x / p.S2 % p.runs2, a = blockIdx.x / (p.S2 * p.runs2);
   const int A = hd.active, e = hd.expert[a], n = hd.rows[a], base = hd.base[a];
+  const int row16 = hd.row16[a][l16];  // (these loads are all under way together)
   if (tid < M) {
     s_w[tid] = hd.w[tid];
     s_ok[tid] = hd.flat_ok[tid];
@@ -509,7 +524,7 @@ __global__ __launch_bounds__(256, 1) void few_down_kernel(FewParams p) {
       const int nr = min(16, n - r0);
       const bool has = l16 < nr;
       if (r0 > 0) __syncthreads();
-      if (tid < 16) s_row[tid] = hd.row[base + r0 + min(tid, nr - 1)];
+      if (tid < 16) s_row[tid] = r0 == 0 ? row16 : hd.row[base + r0 + min(tid, nr - 1)];
       __syncthreads();
       f32x4 acc[S::FR];
 #pragma unroll
@@ -710,23 +725,26 @@ struct FewPlan {
   size_t head, counter, p1, p2, total;
 };
 
-// How the work is cut: column runs of fixed width; the sums in parts until there are two workgroups per CU were every chosen
-// expert another one, at least four steps to a part (one for each wave).
+// How the work is cut: column runs of fixed width; the sums in parts until there is about one workgroup per CU in the first
+// kernel and one for every other CU in the second (were every chosen expert another one), at least four steps to a part (one for
+// each wave).  More parts cost more than they bring: with 512, 256 and 128 workgroups wanted one bf16 token over 2 experts of
+// d 1536, h 4096 took 20.4, 17.6 and 20.4 us (with the router, which every workgroup runs) and 12.2, 11.4 and 11.4, seven fp16
+// tokens over 9 experts of d 1000, h 712 11.4, 12.4 and 12.7 and 19.5, 15.8 and 11.9 (its last workgroups add 18, 12 and 6 parts).
 static bool few_plan(int64_t T, int64_t d, int E, int k, int64_t h, int w, FewPlan& P) {
   if (T < 1 || T > kFewT || k < 1 || k > kFewK || E < 1 || d < 1 || h < 1 || d > (1 << 24) || h > (1 << 24)) return false;
   const int cols = w == FW_F8 ? 64 : w == FW_I8 ? 256 : 128, step = w == FW_F8 ? 128 : 32;
   const int64_t M = T * k, chosen = std::min<int64_t>(E, M);
   P.runs1 = (int)((h + cols / 2 - 1) / (cols / 2));
   P.runs2 = (int)((d + cols - 1) / cols);
-  auto cut = [&](int64_t pieces, int64_t len, int most, int& parts, int& per) {
+  auto cut = [&](int64_t wanted, int64_t pieces, int64_t len, int most, int& parts, int& per) {
     const int64_t steps = (len + step - 1) / step;
-    int64_t s = std::min<int64_t>({(512 + pieces - 1) / pieces, most, (steps + 3) / 4});
+    int64_t s = std::min<int64_t>({(wanted + pieces - 1) / pieces, most, (steps + 3) / 4});
     s = std::max<int64_t>(s, 1);
     per = (int)((steps + s - 1) / s);
     parts = (int)((steps + per - 1) / per);
   };
-  cut(chosen * P.runs1, d, kFewMaxS1, P.S1, P.per1);
-  cut(chosen * P.runs2, h, kFewMaxS2, P.S2, P.per2);
+  cut(256, chosen * P.runs1, d, kFewMaxS1, P.S1, P.per1);
+  cut(128, chosen * P.runs2, h, kFewMaxS2, P.S2, P.per2);
   size_t o = 0;
   auto take = [&](size_t n) {
     const size_t at = o;
