@@ -255,7 +255,7 @@ __device__ __forceinline__ float row_scale_at(const void* s, int dt, int64_t i) 
   return dt == HMOE_DT_BF16 ? Elt<false>::one(h) : Elt<true>::one(h);
 }
 
-// One workgroup per CU (two with the small tile) walks tiles; the ring of two slices runs on from one tile into the next: the
+// One workgroup per CU (two with the tiles of up to 80 KB) walks tiles; the ring of two slices runs on from one tile into the next: the
 // last slice's place in the copy stream is taken by the next tile's first slice, so that its latency and the tile search hide
 // behind the last products and the epilogue, which parks its output in the stage that the last slice has left.
 //
@@ -723,28 +723,44 @@ static int f8_launch(const F8Params& p, hipStream_t s) {
   return HMOE_OK;
 }
 
-// Tile height: 32 rows (two workgroups per CU, for few rows per expert: the launch streams weights), 128 or 256.  Each is
-// priced by its rounds over the CUs, a round by its slices; the prices (us, of launches with 2 to 20 rounds and random counts:
-// 32 rows 4 + 0.9 per slice, 128 6 + 1.0, 256 8 + 1.45) follow 40 layers of 8 to 128 experts, 4 to 600 rows each, d 768-2048, h
-// 320-4096, all tiles timed in turn.  Over these the choice is the fastest or within 10% of it in all but two launches (15%);
-// one line by rows per expert (256 from 160 on, 128 from 64 on) took up to 1.9 times the fastest: 1024 -> 1024 x 2048 rows over
-// 8 experts of 300 31 instead of 19 us, 16 experts of 160 rows, 4096 -> 1536, 60 instead of 50.
+// Tiles: 32 x 256 (two workgroups per CU: few rows per expert, the launch streams weights); 128 x 128, two workgroups per CU,
+// one's epilogue under the other's products (gate/up, whose tile makes one block of act: 128 x 256, one workgroup of 8 waves);
+// 256 x 256.  Each is priced by its rounds over the CUs, a round by its slices; the prices (us) follow 76 launches of each kind:
+// 1 to 128 experts of random load, 4 to 8192 rows each, d 768-8192, h 320-8192, every tile timed in turn.  Over these the
+// choice takes 1% more than the fastest tile on average (gate/up 2%) and at most 15% (17%; wide 40%, where 1.4 rounds of 32
+// rows would have been one of 128).  A line by rows per expert took up to 1.9 times the fastest: 1024 -> 1024 x 2048 rows over
+// 8 experts of 300 31 instead of 19 us.
+// 8 waves for a tile of 256 x 256: twice the LDS reads per product of 4 waves, but two waves per SIMD, of which one computes
+// while the other waits or is in the epilogue: gate/up 16 x 2048 rows, 1536 -> 8192, 482 -> 440 us, in 16 bits 788 -> 738;
+// plain outputs 510 -> 504 there, 600 rows of 1024 x 768 over 32 experts 41 -> 35.  From K = 4096 on a plain output's epilogue
+// is a small part and 4 waves are ahead (8192^3: 454 -> 440).
 template <int EPI, int CDT, bool WIDE = false>
 static int f8_pick(const F8Params& p, hipStream_t s) {
   const int cus = f8_cus();
   if (cus <= 0) return HMOE_ERR_DEVICE;
   const double hit = (double)std::min<int64_t>(p.E, p.M), rows = (double)p.M / hit, nk = (p.K + kF8Slice - 1) / kF8Slice;
-  const double nb = EPI == F8_SWIGLU ? (p.N + 127) / 128 : p.halves * ((p.N + 255) / 256);
-  auto price = [&](double bm, double slots, double fixed, double slice) {
-    const double rounds = 1.08 * hit * std::max(1.0, rows / bm + 0.5) * nb / slots;  // (uneven counts make some tiles more)
+  auto price = [&](double bm, double bn, double slots, double fixed, double slice) {
+    const double nb = EPI == F8_SWIGLU ? std::ceil(p.N / (bn / 2)) : p.halves * std::ceil(p.N / bn);
+    // (uneven counts make some tiles more)
+    const double rounds = 1.08 * hit * std::max(1.0, rows / bm + 0.5) * nb / slots;
     return (rounds < 4 ? std::ceil(rounds) : rounds) * (fixed + slice * nk);
   };
-  const double wide = WIDE ? 1.0 : 0.0;  // (a wide slice's products take 0.85 us more with 256 rows)
-  const double t32 = price(32, 2 * cus, 4, 0.9 + 0.1 * wide), t128 = price(128, cus, 6, 1.0 + 0.42 * wide),
-               t256 = price(256, cus, 8, 1.45 + 0.85 * wide);
+  double t32, t128, t256;
+  if constexpr (EPI == F8_STORE) {
+    t32 = price(32, 256, 2 * cus, 7, 0.7), t128 = price(128, 128, 2 * cus, 5, 0.7), t256 = price(256, 256, cus, 8, 1.15);
+  } else if constexpr (WIDE) {
+    t32 = price(32, 256, 2 * cus, 3, 1.3), t128 = price(128, 256, cus, 4, 1.65), t256 = price(256, 256, cus, 8, 2.75);
+  } else {
+    t32 = price(32, 256, 2 * cus, 2.5, 1.1), t128 = price(128, 256, cus, 2, 1.3), t256 = price(256, 256, cus, 5, 1.75);
+  }
   if (t32 <= t128 && t32 <= t256) return f8_launch<F8Cfg<32, 256, 1, 4, 2>, EPI, CDT, WIDE>(p, s);
-  if (t128 <= t256) return f8_launch<F8Cfg<128, 256, 2, 2, 2>, EPI, CDT, WIDE>(p, s);
-  return f8_launch<F8Cfg<256, 256, 2, 2, 2>, EPI, CDT, WIDE>(p, s);
+  if constexpr (EPI == F8_STORE) {
+    if (t128 <= t256) return f8_launch<F8Cfg<128, 128, 2, 2, 2>, EPI, CDT, WIDE>(p, s);
+    if (p.K >= 4096) return f8_launch<F8Cfg<256, 256, 2, 2, 2>, EPI, CDT, WIDE>(p, s);
+  } else {
+    if (t128 <= t256) return f8_launch<F8Cfg<128, 256, 2, 4, 2>, EPI, CDT, WIDE>(p, s);
+  }
+  return f8_launch<F8Cfg<256, 256, 2, 4, 2>, EPI, CDT, WIDE>(p, s);
 }
 
 static bool al(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
