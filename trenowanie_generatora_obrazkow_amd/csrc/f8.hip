@@ -259,6 +259,11 @@ __device__ __forceinline__ float row_scale_at(const void* s, int dt, int64_t i) 
 // last slice's place in the copy stream is taken by the next tile's first slice, so that its latency and the tile search hide
 // behind the last products and the epilogue, which parks its output in the stage that the last slice has left.
 //
+// The outputs leave with non-temporal stores: a large one would push the rows and weights that the XCD's next tiles share out
+// of its L2.  16 x 2048 rows, 1536 -> 8192: 465 -> 373 us (gate/up, half the columns of one byte, 408 -> 385), one expert 402 ->
+// 380; 4096 -> 1536 185 -> 170; the layer of 16384 tokens with the sum over its rows 768 -> 745.  Outputs that the next kernel
+// could have read from a cache are at most 1 us slower to it.
+//
 // WIDE: the operands are widened exactly to bf16 (their scales with them) and multiplied there, at half the rate.  The 8-bit
 // instructions add eight products at the exponent of the largest and drop what lies below 2^-13 of it: some 2^-16 of a sum's
 // size, nothing to a bf16 result, but where act is quantised again it moves a value in some thousand across a border of the 8
@@ -622,11 +627,12 @@ __global__ __launch_bounds__(C::NT, C::LDS_BYTES > 81920 ? 1 : 2) void f8_gemm_k
 #pragma unroll
           for (int i = 0; i < 32 / RPI; ++i) {
             const int rr = i * RPI + ln / CPR, c = ln % CPR;
-            const uint4 v = *reinterpret_cast<const uint4*>(buf + rr * RB + ((c ^ (rr & (CPR - 1))) << 4));
+            const u32x4 v = *reinterpret_cast<const u32x4*>(buf + rr * RB + ((c ^ (rr & (CPR - 1))) << 4));
             const int64_t y = s_y[min(rbase + rr, t.live - 1)];
             const int col = n0 + wn * C::TN + b0 * 32 + c * (16 / ES);
             if (rbase + rr < t.live && col < p.N)
-              *reinterpret_cast<uint4*>(static_cast<char*>(p.C) + (y * p.ldc + half * p.N + col) * ES) = v;
+              __builtin_nontemporal_store(
+                  v, reinterpret_cast<u32x4*>(static_cast<char*>(p.C) + (y * p.ldc + half * p.N + col) * ES));
           }
           __builtin_amdgcn_wave_barrier();
         }
@@ -676,8 +682,9 @@ __global__ __launch_bounds__(C::NT, C::LDS_BYTES > 81920 ? 1 : 2) void f8_gemm_k
       for (int i = wave * 64 + ln; i < t.live * 8; i += C::NT) {
         const int rr = i >> 3, c = i & 7;
         if (n0 + c * 16 < p.N)
-          *reinterpret_cast<uint4*>(static_cast<char*>(p.C) + (int64_t)(t.row0 + rr) * p.ldc + n0 + c * 16) =
-              *reinterpret_cast<const uint4*>(rows + rr * 128 + ((c ^ f8_swz(rr)) << 4));
+          __builtin_nontemporal_store(
+              *reinterpret_cast<const u32x4*>(rows + rr * 128 + ((c ^ f8_swz(rr)) << 4)),
+              reinterpret_cast<u32x4*>(static_cast<char*>(p.C) + (int64_t)(t.row0 + rr) * p.ldc + n0 + c * 16));
       }
     }
     if (!more) break;
