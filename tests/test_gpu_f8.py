@@ -195,6 +195,35 @@ def test_nan_rows_stay_in_their_rows():
     assert torch.isnan(y[[3, 66]]).all() and int(bad.sum()) == 2
 
 
+@pytest.mark.parametrize("form", ["store", "gate_up", "wide"])
+@pytest.mark.parametrize("E,M,K,N", [(3, 2600, 400, 4096), (1, 9700, 400, 4096), (3, 5000, 272, 2016), (2, 9000, 272, 2400),
+                                     (2, 700, 272, 992), (3, 5000, 1168, 736)])
+def test_large_tiles(E, M, K, N, form):
+    """Large products (tiles of 128 and 256 rows, whole last rounds and halved ones) are bit for bit the same rows in calls of
+    50 rows: every sum is added in the order of k, whatever the tile."""
+    o = ops()
+    x, w = rand(M, K, seed=M, spread=False), rand(E, K, N, seed=N, spread=False) * K ** -0.5
+    q, s = o.quant_rows(x)
+    st = o.F8Stack.from_weights(w, halves=1 if form == "store" else 2)
+    counts = R.counts_of(M, E, "skew")
+
+    def product(r, c):
+        c = torch.tensor(c, dtype=torch.int32, device=DEV)
+        if form == "store":
+            return (o.grouped_mm_f8(q[r], s[r], st, c),)
+        act, act_s = o.gate_up_swiglu_f8(q[r], s[r], st, c, wide=form == "wide")
+        return act.view(torch.uint8), act_s.view(torch.uint8)
+
+    whole = product(slice(0, M), counts.tolist())
+    r0 = 0
+    for e, n in enumerate(counts.tolist()):
+        for i in range(r0, r0 + n, 50):
+            r = slice(i, min(i + 50, r0 + n))
+            part = product(r, [(r.stop - r.start) * (j == e) for j in range(E)])
+            assert all(torch.equal(a[r], b) for a, b in zip(whole, part)), (e, i)
+        r0 += n
+
+
 @pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("E,M,d,h,kind", [(1, 1, 16, 16, "even"), (3, 50, 272, 336, "skew"), (4, 600, 400, 144, "skew"),
                                           (2, 600, 128, 272, "one"), (40, 300, 2064, 64, "skew")])

@@ -330,10 +330,16 @@ __global__ __launch_bounds__(C::NT, C::LDS_BYTES > 81920 ? 1 : 2) void f8_gemm_k
   struct Tile {
     int e, nbi, row0, live;
   };
-  // the workgroup's j-th tile: bands of kF8BandM m-tiles of an expert, n-tile by n-tile
+  // The workgroup's j-th tile: bands of kF8BandM m-tiles of an expert, n-tile by n-tile.  Where an XCD's last round has tiles
+  // for at most half of its workgroups, 256-row tiles are halved by rows: waves without rows leave out their products (32768
+  // rows over 16 experts of uneven load, 4096 -> 1536, 3.2 rounds: 205 -> 196 us).
+  constexpr bool kHalve = C::BM == 256 && C::NW == 8;
+  const int wgs = (int)gridDim.x >> 3, whole = kHalve && share % wgs * 2 <= wgs ? share / wgs * wgs : share;
   auto find = [&](int j, Tile& t) __attribute__((always_inline)) {
-    const int v = (int)blockIdx.x + j * (int)gridDim.x, at = v >> 3, tile = (v & 7) * share + at;
-    if (at >= share || tile >= total) return false;
+    const int v = (int)blockIdx.x + j * (int)gridDim.x, at = v >> 3;
+    const bool halved = kHalve && at >= whole;
+    const int mine = halved ? whole + ((at - whole) >> 1) : at, tile = (v & 7) * share + mine;
+    if (mine >= share || tile >= total) return false;
     const int mt = tile / p.nb;
     int e = 0;
     for (int i = 0; i < per; ++i) {
@@ -347,7 +353,12 @@ __global__ __launch_bounds__(C::NT, C::LDS_BYTES > 81920 ? 1 : 2) void f8_gemm_k
     t.nbi = __builtin_amdgcn_readfirstlane(r / mc);
     t.row0 = __builtin_amdgcn_readfirstlane(first + (band + r % mc) * C::BM);
     t.live = __builtin_amdgcn_readfirstlane(min(end - t.row0, C::BM));
-    return true;
+    if (halved) {
+      const int skip = (at - whole) & 1 ? C::BM / 2 : 0;
+      t.row0 += skip;
+      t.live = min(t.live - skip, C::BM / 2);
+    }
+    return t.live > 0;  // (nothing follows the last round's)
   };
   const int nbh = EPI == F8_STORE ? p.nb / p.halves : p.nb;
   // the half a tile lies in, and its first column there (store), or its first column of act (SwiGLU)
@@ -558,7 +569,13 @@ __global__ __launch_bounds__(C::NT, C::LDS_BYTES > 81920 ? 1 : 2) void f8_gemm_k
       stage ^= 1;
     };
     int kt = 0;
-    if constexpr (!WIDE) {
+    if (kHalve && wm * C::TM >= t.live) {  // no rows: this wave copies only
+      for (; kt + 1 < nk; ++kt) {
+        begin_slice(kt);
+        issue(kt + 1, stage ^ 1);
+        end_slice();
+      }
+    } else if constexpr (!WIDE) {
       for (; (kt + 2) * kF8Slice <= K; ++kt) {
         begin_slice(kt);
         products(std::true_type{}, stage, (kt + 1) * kF8Slice);
@@ -739,8 +756,7 @@ static int f8_launch(const F8Params& p, hipStream_t s) {
 // 8 experts of 300 31 instead of 19 us.
 // 8 waves for a tile of 256 x 256: twice the LDS reads per product of 4 waves, but two waves per SIMD, of which one computes
 // while the other waits or is in the epilogue: gate/up 16 x 2048 rows, 1536 -> 8192, 482 -> 440 us, in 16 bits 788 -> 738;
-// plain outputs 510 -> 504 there, 600 rows of 1024 x 768 over 32 experts 41 -> 35.  From K = 4096 on a plain output's epilogue
-// is a small part and 4 waves are ahead (8192^3: 454 -> 440).
+// plain outputs 510 -> 504 there, 600 rows of 1024 x 768 over 32 experts 41 -> 35 (4 waves are 4% ahead where K is 8192).
 template <int EPI, int CDT, bool WIDE = false>
 static int f8_pick(const F8Params& p, hipStream_t s) {
   const int cus = f8_cus();
@@ -763,7 +779,6 @@ static int f8_pick(const F8Params& p, hipStream_t s) {
   if (t32 <= t128 && t32 <= t256) return f8_launch<F8Cfg<32, 256, 1, 4, 2>, EPI, CDT, WIDE>(p, s);
   if constexpr (EPI == F8_STORE) {
     if (t128 <= t256) return f8_launch<F8Cfg<128, 128, 2, 2, 2>, EPI, CDT, WIDE>(p, s);
-    if (p.K >= 4096) return f8_launch<F8Cfg<256, 256, 2, 2, 2>, EPI, CDT, WIDE>(p, s);
   } else {
     if (t128 <= t256) return f8_launch<F8Cfg<128, 256, 2, 4, 2>, EPI, CDT, WIDE>(p, s);
   }
