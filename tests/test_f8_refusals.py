@@ -191,3 +191,9 @@ def test_few_wrappers():
     with pytest.raises(RuntimeError):
         ops.few_experts(x, torch.zeros(2, 1, dtype=torch.int32), torch.ones(2, 1), torch.zeros(1, 64, 32, dtype=torch.bfloat16),
                         torch.zeros(1, 16, 64, dtype=torch.bfloat16))
+
+
+def test_pack_launch_limit(L):
+    """A workgroup per row: 2^25 rows would be 2^33 threads, more than a launch takes."""
+    assert L.hmoe_swiglu_pack(P, 8192, 1 << 25, 4096, P, P, P, BF, None) == SHAPE
+    assert L.hmoe_swiglu_pack_bwd(P, P, P, P, FP, 1 << 25, 4096, P, P, None, P, BF, None) == SHAPE

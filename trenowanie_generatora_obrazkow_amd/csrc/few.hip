@@ -11,6 +11,11 @@
 // instruction, whose 16 columns are the expert's tokens.  The waves' sums meet in LDS, the parts of [g | u] in the second
 // kernel's loads, the parts of the output in the workgroup that finishes a run of columns last: a counter, and no one waits.
 //
+// Measured, whole calls: one token with the router, 2 of 16 bf16 experts (d 1536, h 4096: 75 MB) 28.6 us (17.8 + 11.4); 16
+// tokens over 51 of 64 8-bit experts (d 2048, h 1408: 441 MB) 105 to 109 us (64 + 40; 4.2 TB/s); seven over 9 fp16 experts (d
+// 1000, h 712) 23 us (12 + 12); one over 8 int8 experts (d 2048, h 320) 19.7 us, the host's time (9 + 10).  Small ones are
+// bound by a launch's steps one after another: start, grouping, the weights' latency, the sum over waves and parts.
+//
 // Numerics: fp32 sums throughout and one rounding, that of the output.  The activation enters its product as two bf16 numbers
 // (16 significant bits), fp16 weights there as two as well (their 11 bits); 8-bit experts (F8Stack) take x and the activation
 // quantised as the grouped product does, widened exactly.

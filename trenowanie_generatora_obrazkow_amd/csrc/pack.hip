@@ -8,7 +8,8 @@
 //
 // One pass over the data each, memory-bound (everything in fp32 between one read and one rounding): the forward moves
 // 8.06 M h bytes, the backward 12.06 M h.  Blocks of 32: a scale costs 1/32 byte a value, and a block is four lanes' eight
-// values, so its largest one takes two exchanges.
+// values, so its largest one takes two exchanges.  32768 rows of h 4096 in bf16: 186 us forward, 5.8 TB/s, 236 us backward, 6.9
+// (a copy of 2 GB 5.0).  Non-temporal stores took 181 and 230 us there, but 10.4 instead of 9.3 us for 4096 rows of h 1024.
 #include <algorithm>
 
 #include "f8_common.h"
@@ -159,6 +160,12 @@ static int pack_check(int64_t M, int64_t h, int dtype) {
   if (h % 8 || h > (1 << 28) || M > INT32_MAX) return HMOE_ERR_SHAPE;
   return HMOE_OK;
 }
+// a launch has fewer than 2^32 threads
+static bool pack_fits(int64_t M, int nb) {
+  bool ok = false;
+  pick_tpr(4 * nb, [&](auto tpr) { ok = (M + 256 / decltype(tpr)::value - 1) / (256 / decltype(tpr)::value) < (1 << 24); });
+  return ok;
+}
 static bool mis(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) != 0; }
 
 }  // namespace hmoe
@@ -174,6 +181,7 @@ int hmoe_swiglu_pack(const void* gu, int64_t ldgu, int64_t M, int64_t h, void* a
   if (!gu || !act || !q || !s || ldgu < 2 * h || ldgu % 8 || mis(gu, 16) || mis(act, 16) || mis(q, 8)) return HMOE_ERR_ARG;
   const int nb = (int)((h + kPackBlock - 1) / kPackBlock);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (!pack_fits(M, nb)) return HMOE_ERR_SHAPE;
   pick_tpr(4 * nb, [&](auto tpr) {
     constexpr int TPR = decltype(tpr)::value;
     const dim3 grid((unsigned)((M + 256 / TPR - 1) / (256 / TPR)));
@@ -197,6 +205,7 @@ int hmoe_swiglu_pack_bwd(const void* dh, const void* q, const uint8_t* s, const 
   if (!dh || !q || !s || !dgu || mis(dh, 16) || mis(q, 8) || mis(dgu, 16) || mis(act, 16)) return HMOE_ERR_ARG;
   const int nb = (int)((h + kPackBlock - 1) / kPackBlock);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (!pack_fits(M, nb)) return HMOE_ERR_SHAPE;
   pick_tpr(4 * nb, [&](auto tpr) {
     constexpr int TPR = decltype(tpr)::value;
     const dim3 grid((unsigned)((M + 256 / TPR - 1) / (256 / TPR)));
