@@ -492,11 +492,12 @@ int hmoe_f8_quant_stack(const void* w, int dtype, int64_t E, int64_t K, int64_t 
 /* hmoe_grouped_mm on quantised rows and stacks (aurora/moe_triton.py:22-56 with 8-bit operands): y[y_idx[r] or r] =
  * scale * a[a_idx[r] or r] @ w[e(r)], summed in fp32 and rounded once to y_dtype (bf16, fp16 or fp32).  w (E, N, K) and w_s from
  * hmoe_f8_quant_stack.  scale (M,) fp32, bf16 or fp16 or NULL, by sorted row or, with scale_by_y, by y_idx[r].  Rows that no
- * expert counts are zeros (without y_idx; with it nothing is written for them). */
-int hmoe_f8_grouped_mm(const void* a, int64_t lda, const uint8_t* a_s, int64_t lda_s, const void* w, const uint8_t* w_s,
-                       int64_t E, int64_t K, int64_t N, int halves, const void* counts, int counts_dtype, int64_t M,
-                       const int32_t* a_idx, const int32_t* y_idx, const void* scale, int scale_dtype, int scale_by_y, void* y,
-                       int64_t ldy, int y_dtype, hmoe_stream_t stream);
+ * expert counts are zeros (without y_idx; with it nothing is written for them).  a_rows: rows of a, at least M without a_idx;
+ * with it they span less than 2 GiB (HMOE_ERR_SHAPE). */
+int hmoe_f8_grouped_mm(const void* a, int64_t lda, const uint8_t* a_s, int64_t lda_s, int64_t a_rows, const void* w,
+                       const uint8_t* w_s, int64_t E, int64_t K, int64_t N, int halves, const void* counts, int counts_dtype,
+                       int64_t M, const int32_t* a_idx, const int32_t* y_idx, const void* scale, int scale_dtype,
+                       int scale_by_y, void* y, int64_t ldy, int y_dtype, hmoe_stream_t stream);
 /* Both in one call: x (rows, K) bf16, fp16 or fp32 quantised into the workspace (16-byte aligned), then the product of its rows. */
 size_t hmoe_f8_quant_mm_workspace_size(int64_t rows, int64_t K);
 int hmoe_f8_quant_mm(const void* x, int64_t ldx, int x_dtype, int64_t rows, const void* w, const uint8_t* w_s, int64_t E,
@@ -507,9 +508,9 @@ int hmoe_f8_quant_mm(const void* x, int64_t ldx, int x_dtype, int64_t rows, cons
  * (E, 2h, d) with halves = 2.  The 8-bit matrix instructions drop what lies below 2^-13 of the largest of eight products: some
  * 2^-16 of a sum, which moves about one act in a thousand across a border of its 8 bits.  wide = 1 multiplies the same values
  * as bf16 numbers instead, exactly but for the fp32 sums, at half the rate. */
-int hmoe_f8_gate_up_swiglu(const void* x, int64_t ldx, const uint8_t* x_s, int64_t ldx_s, const int32_t* a_idx, const void* wgu,
-                           const uint8_t* wgu_s, int64_t E, int64_t d, int64_t h, const void* counts, int counts_dtype,
-                           int64_t M, int wide, void* act, uint8_t* act_s, hmoe_stream_t stream);
+int hmoe_f8_gate_up_swiglu(const void* x, int64_t ldx, const uint8_t* x_s, int64_t ldx_s, int64_t x_rows, const int32_t* a_idx,
+                           const void* wgu, const uint8_t* wgu_s, int64_t E, int64_t d, int64_t h, const void* counts,
+                           int counts_dtype, int64_t M, int wide, void* act, uint8_t* act_s, hmoe_stream_t stream);
 /* hmoe_moe_experts with such stacks: x (T, d) bf16 or fp16 is quantised, y (T * k, d) of its type; the routing weights enter
  * as given (not rounded).  fp16: the gate/up products are wide (hmoe_f8_gate_up_swiglu). */
 size_t hmoe_f8_moe_experts_workspace_size(int64_t T, int64_t d, int E, int k, int64_t h);

@@ -52,8 +52,8 @@ def test_quant_stack_codes(L):
 
 def test_grouped_mm_codes(L):
     def f(a=P, lda=64, a_s=P, ld_s=16, w=P, w_s=P, E=2, K=64, N=96, halves=1, c=P, cdt=I32, M=4, ai=None, sc=None, sdt=FP, y=P,
-          ldy=96, ydt=BF):
-        return L.hmoe_f8_grouped_mm(a, lda, a_s, ld_s, w, w_s, E, K, N, halves, c, cdt, M, ai, None, sc, sdt, 0, y, ldy, ydt,
+          ldy=96, ydt=BF, rows=None):
+        return L.hmoe_f8_grouped_mm(a, lda, a_s, ld_s, M if rows is None else rows, w, w_s, E, K, N, halves, c, cdt, M, ai, None, sc, sdt, 0, y, ldy, ydt,
                                     None)
     assert f(M=0) == 0 and f(M=-1) == ARG and f(E=0) == ARG and f(c=None) == ARG and f(cdt=FP) == DTYPE
     assert f(E=1025) == SHAPE and f(M=2 ** 31) == SHAPE and f(ydt=I8) == DTYPE and f(sc=P, sdt=I32) == DTYPE
@@ -62,7 +62,8 @@ def test_grouped_mm_codes(L):
     assert f(lda=48) == ARG and f(lda=72) == ARG and f(ld_s=8) == ARG and f(ldy=88) == ARG and f(ldy=100) == ARG
     assert f(a=P + 8) == ARG and f(a_s=P + 4) == ARG and f(w=P + 8) == ARG and f(w_s=P + 8) == ARG and f(y=P + 8) == ARG
     assert f(K=1 << 16, lda=1 << 16, ld_s=512, N=1 << 15, ldy=1 << 15) == SHAPE  # one expert's weights past 2 GiB
-    assert f(M=1 << 26, ai=P) == SHAPE                                           # gathered rows past 2 GiB
+    assert f(rows=1 << 26, ai=P) == SHAPE                                        # gathered rows past 2 GiB
+    assert f(rows=3) == ARG and f(rows=0, ai=P) == ARG
 
 
 def test_quant_mm_codes(L):
@@ -79,7 +80,7 @@ def test_quant_mm_codes(L):
 
 def test_gate_up_codes(L):
     def f(x=P, M=4, d=64, h=48, act=P, act_s=P, E=2):
-        return L.hmoe_f8_gate_up_swiglu(x, d, P, 16, None, P, P, E, d, h, P, I32, M, 0, act, act_s, None)
+        return L.hmoe_f8_gate_up_swiglu(x, d, P, 16, M, None, P, P, E, d, h, P, I32, M, 0, act, act_s, None)
     assert f(M=0) == 0 and f(h=0) == ARG and f(h=40) == SHAPE and f(act=None) == ARG and f(act_s=None) == ARG and f(act=P + 8) == ARG
 
 

@@ -102,12 +102,12 @@ SIGNATURES = {
     "hmoe_f8_quant_rows": (_I32, [_P, _I64, _I32, _I64, _I64, _P, _I64, _P, _I64, _P]),
     "hmoe_f8_dequant_rows": (_I32, [_P, _I64, _P, _I64, _I64, _I64, _I32, _P, _I64, _I32, _P]),
     "hmoe_f8_quant_stack": (_I32, [_P, _I32, _I64, _I64, _I64, _I64, _I64, _I32, _I32, _P, _P, _P]),
-    "hmoe_f8_grouped_mm": (_I32, [_P, _I64, _P, _I64, _P, _P, _I64, _I64, _I64, _I32, _P, _I32, _I64, _P, _P, _P, _I32,
+    "hmoe_f8_grouped_mm": (_I32, [_P, _I64, _P, _I64, _I64, _P, _P, _I64, _I64, _I64, _I32, _P, _I32, _I64, _P, _P, _P, _I32,
                                   _I32, _P, _I64, _I32, _P]),
     "hmoe_f8_quant_mm_workspace_size": (_SZ, [_I64, _I64]),
     "hmoe_f8_quant_mm": (_I32, [_P, _I64, _I32, _I64, _P, _P, _I64, _I64, _I64, _I32, _P, _I32, _I64, _P, _P, _P, _I32, _I32,
                                 _P, _I64, _I32, _P, _SZ, _P]),
-    "hmoe_f8_gate_up_swiglu": (_I32, [_P, _I64, _P, _I64, _P, _P, _P, _I64, _I64, _I64, _P, _I32, _I64, _I32, _P, _P, _P]),
+    "hmoe_f8_gate_up_swiglu": (_I32, [_P, _I64, _P, _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _P, _I32, _I64, _I32, _P, _P, _P]),
     "hmoe_f8_moe_experts_workspace_size": (_SZ, [_I64, _I64, _I32, _I32, _I64]),
     "hmoe_f8_moe_experts": (_I32, [_P, _I64, _I32, _P, _I32, _P, _I32, _P, _P, _P, _P, _I64, _I64, _I32, _I32, _I64, _P, _P,
                                    _P, _P, _SZ, _P]),

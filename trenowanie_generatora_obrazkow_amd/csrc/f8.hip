@@ -796,8 +796,8 @@ static int f8_pick(const F8Params& p, hipStream_t s) {
 
 static bool al(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
-static int f8_check(const void* a, int64_t lda, const uint8_t* a_s, int64_t lda_s, const int32_t* a_idx, const void* w,
-                    const uint8_t* w_s, int64_t E, int64_t K, int64_t N, int halves, const void* counts, int counts_dtype,
+static int f8_check(const void* a, int64_t lda, const uint8_t* a_s, int64_t lda_s, const int32_t* a_idx, int64_t a_rows,
+                    const void* w, const uint8_t* w_s, int64_t E, int64_t K, int64_t N, int halves, const void* counts, int counts_dtype,
                     int64_t M) {
   if (!counts || E <= 0 || M < 0) return HMOE_ERR_ARG;
   if (E > kMaxEGemm || M > INT32_MAX - 256) return HMOE_ERR_SHAPE;
@@ -807,9 +807,10 @@ static int f8_check(const void* a, int64_t lda, const uint8_t* a_s, int64_t lda_
   if (K % 16 || N / halves % 16) return HMOE_ERR_SHAPE;
   if (lda < K || lda % 16 || lda_s < f8_scale_ld(K) || lda_s % 16 || !al(a, 16) || !al(a_s, 16) || !al(w, 16) || !al(w_s, 16))
     return HMOE_ERR_ARG;
-  // 32-bit copy offsets: one expert's weights, the rows of a tile, all rows where they are gathered
+  // 32-bit copy offsets: one expert's weights, the rows of a tile, all of a where its rows are gathered
   const int64_t lim = ((int64_t)1 << 31) - 32768;
-  if (K > lim / N || lda > lim / 256 || (a_idx && M > lim / lda)) return HMOE_ERR_SHAPE;
+  if (K > lim / N || lda > lim / 256 || (a_idx && a_rows > lim / lda)) return HMOE_ERR_SHAPE;
+  if (a_rows < (a_idx ? 1 : M)) return HMOE_ERR_ARG;
   return HMOE_OK;
 }
 
@@ -920,11 +921,11 @@ int hmoe_f8_quant_stack(const void* w, int dtype, int64_t E, int64_t K, int64_t 
   return HMOE_OK;
 }
 
-int hmoe_f8_grouped_mm(const void* a, int64_t lda, const uint8_t* a_s, int64_t lda_s, const void* w, const uint8_t* w_s,
-                       int64_t E, int64_t K, int64_t N, int halves, const void* counts, int counts_dtype, int64_t M,
-                       const int32_t* a_idx, const int32_t* y_idx, const void* scale, int scale_dtype, int scale_by_y, void* y,
+int hmoe_f8_grouped_mm(const void* a, int64_t lda, const uint8_t* a_s, int64_t lda_s, int64_t a_rows, const void* w,
+                       const uint8_t* w_s, int64_t E, int64_t K, int64_t N, int halves, const void* counts, int counts_dtype,
+                       int64_t M, const int32_t* a_idx, const int32_t* y_idx, const void* scale, int scale_dtype, int scale_by_y, void* y,
                        int64_t ldy, int y_dtype, hmoe_stream_t stream) {
-  int rc = f8_check(a, lda, a_s, lda_s, a_idx, w, w_s, E, K, N, halves, counts, counts_dtype, M);
+  int rc = f8_check(a, lda, a_s, lda_s, a_idx, a_rows, w, w_s, E, K, N, halves, counts, counts_dtype, M);
   if (rc) return rc;
   if (y_dtype != HMOE_DT_BF16 && y_dtype != HMOE_DT_F16 && y_dtype != HMOE_DT_F32) return HMOE_ERR_DTYPE;
   if (scale && scale_dtype != HMOE_DT_BF16 && scale_dtype != HMOE_DT_F16 && scale_dtype != HMOE_DT_F32) return HMOE_ERR_DTYPE;
@@ -958,22 +959,22 @@ int hmoe_f8_quant_mm(const void* x, int64_t ldx, int x_dtype, int64_t rows, cons
   auto* q = static_cast<uint8_t*>(workspace);
   auto* s = q + rows * ((K + 15) / 16 * 16);
   // the product's limits ahead of the first launch, so that a refused call launches nothing
-  int rc = f8_check(q, K, s, f8_scale_ld(K), a_idx, w, w_s, E, K, N, halves, counts, counts_dtype, M);
+  int rc = f8_check(q, K, s, f8_scale_ld(K), a_idx, rows, w, w_s, E, K, N, halves, counts, counts_dtype, M);
   if (rc) return rc;
   if (y_dtype != HMOE_DT_BF16 && y_dtype != HMOE_DT_F16 && y_dtype != HMOE_DT_F32) return HMOE_ERR_DTYPE;
   if (scale && scale_dtype != HMOE_DT_BF16 && scale_dtype != HMOE_DT_F16 && scale_dtype != HMOE_DT_F32) return HMOE_ERR_DTYPE;
-  if (M > 0 && (!y || !al(y, 16) || ldy < N || ldy % 8 || rows < (a_idx ? 1 : M))) return HMOE_ERR_ARG;
+  if (M > 0 && (!y || !al(y, 16) || ldy < N || ldy % 8)) return HMOE_ERR_ARG;
   rc = hmoe_f8_quant_rows(x, ldx, x_dtype, M == 0 ? 0 : rows, K, q, K, s, f8_scale_ld(K), stream);
   if (rc) return rc;
-  return hmoe_f8_grouped_mm(q, K, s, f8_scale_ld(K), w, w_s, E, K, N, halves, counts, counts_dtype, M, a_idx, y_idx, scale,
+  return hmoe_f8_grouped_mm(q, K, s, f8_scale_ld(K), rows, w, w_s, E, K, N, halves, counts, counts_dtype, M, a_idx, y_idx, scale,
                             scale_dtype, scale_by_y, y, ldy, y_dtype, stream);
 }
 
-int hmoe_f8_gate_up_swiglu(const void* x, int64_t ldx, const uint8_t* x_s, int64_t ldx_s, const int32_t* a_idx, const void* wgu,
-                           const uint8_t* wgu_s, int64_t E, int64_t d, int64_t h, const void* counts, int counts_dtype,
+int hmoe_f8_gate_up_swiglu(const void* x, int64_t ldx, const uint8_t* x_s, int64_t ldx_s, int64_t x_rows, const int32_t* a_idx,
+                           const void* wgu, const uint8_t* wgu_s, int64_t E, int64_t d, int64_t h, const void* counts, int counts_dtype,
                            int64_t M, int wide, void* act, uint8_t* act_s, hmoe_stream_t stream) {
   if (h <= 0) return HMOE_ERR_ARG;
-  int rc = f8_check(x, ldx, x_s, ldx_s, a_idx, wgu, wgu_s, E, d, 2 * h, 2, counts, counts_dtype, M);
+  int rc = f8_check(x, ldx, x_s, ldx_s, a_idx, x_rows, wgu, wgu_s, E, d, 2 * h, 2, counts, counts_dtype, M);
   if (rc || M == 0) return rc;
   if (!act || !act_s || !al(act, 16)) return HMOE_ERR_ARG;
   F8Params p = f8_params(x, ldx, x_s, ldx_s, a_idx, wgu, wgu_s, E, d, 2 * h, 2, counts, counts_dtype, M);
@@ -1044,7 +1045,7 @@ int hmoe_f8_moe_experts(const void* x, int64_t ldx, int dtype, const void* topk_
     return HMOE_ERR_ARG;
   const int64_t lim = ((int64_t)1 << 31) - 32768, M = T * k;
   if (d % 16 || h % 16 || E > kMaxEGemm || M > INT32_MAX - 256 || d > lim / (2 * h) || d > lim / 256 || h > lim / 256 ||
-      M > lim / d)
+      T > lim / d)
     return HMOE_ERR_SHAPE;
   char* ws = static_cast<char*>(workspace);
   auto* counts = reinterpret_cast<int32_t*>(ws + L.counts);
@@ -1058,10 +1059,10 @@ int hmoe_f8_moe_experts(const void* x, int64_t ldx, int dtype, const void* topk_
   if (rc != HMOE_OK || M == 0) return rc;
   rc = hmoe_f8_quant_rows(x, ldx, dtype, T, d, ws + L.x8, d, xs, f8_scale_ld(d), stream);
   if (rc != HMOE_OK) return rc;
-  rc = hmoe_f8_gate_up_swiglu(ws + L.x8, d, xs, f8_scale_ld(d), a_idx, wgu, wgu_s, E, d, h, counts, HMOE_DT_I32, M,
+  rc = hmoe_f8_gate_up_swiglu(ws + L.x8, d, xs, f8_scale_ld(d), T, a_idx, wgu, wgu_s, E, d, h, counts, HMOE_DT_I32, M,
                               dtype == HMOE_DT_F16, ws + L.act, act_s, stream);
   if (rc != HMOE_OK) return rc;
-  return hmoe_f8_grouped_mm(ws + L.act, h, act_s, f8_scale_ld(h), wd, wd_s, E, h, d, 1, counts, HMOE_DT_I32, M, nullptr, order,
+  return hmoe_f8_grouped_mm(ws + L.act, h, act_s, f8_scale_ld(h), M, wd, wd_s, E, h, d, 1, counts, HMOE_DT_I32, M, nullptr, order,
                             topk_w, topk_w_dtype, 1, y, d, dtype, stream);
 }
 

@@ -1286,7 +1286,7 @@ def _f8_mm(q, s, wq, ws, E, K, N, halves, counts, M, a_idx, y_idx, scale, dtype,
         raise TypeError(f"dtype {dtype} not in {_FLOATS}")
     counts, scale = _f8_idx(counts, a_idx, y_idx, scale, dev, E, M, rows, ld)
     y = torch.empty(M, N, device=dev, dtype=dtype)
-    _call_on(dev, "hmoe_f8_grouped_mm", L.ptr(q), ld, L.ptr(s), lds, L.ptr(wq), L.ptr(ws), E, K, N, halves, L.ptr(counts),
+    _call_on(dev, "hmoe_f8_grouped_mm", L.ptr(q), ld, L.ptr(s), lds, rows, L.ptr(wq), L.ptr(ws), E, K, N, halves, L.ptr(counts),
              L.dt(counts), M, L.ptr(a_idx), L.ptr(y_idx), L.ptr(scale), L.dt(scale) if scale is not None else 0,
              int(scale_by_y), L.ptr(y), N, L.dt(dtype))
     return y
@@ -1326,7 +1326,7 @@ def gate_up_swiglu_f8(q, s, wgu, counts, M=None, a_idx=None, wide=False):
     counts, _ = _f8_idx(counts, a_idx, None, None, dev, E, M, rows, ld)
     act = torch.empty(M, h, device=dev, dtype=_E4M3)
     act_s = torch.empty(M, _f8_ld(h), device=dev, dtype=_E8M0)
-    _call_on(dev, "hmoe_f8_gate_up_swiglu", L.ptr(q), ld, L.ptr(s), lds, L.ptr(a_idx), L.ptr(wgu.q), L.ptr(wgu.s), E, d, h,
+    _call_on(dev, "hmoe_f8_gate_up_swiglu", L.ptr(q), ld, L.ptr(s), lds, rows, L.ptr(a_idx), L.ptr(wgu.q), L.ptr(wgu.s), E, d, h,
              L.ptr(counts), L.dt(counts), M, int(bool(wide)), L.ptr(act), L.ptr(act_s))
     return act, act_s[:, :-(-h // 128)]
 
