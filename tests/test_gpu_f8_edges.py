@@ -106,3 +106,31 @@ def test_strided_and_shared_gradients():
     y2.backward(dy.contiguous())
     assert torch.equal(y, y2) and torch.equal(wide.grad[:, 32:96], a.grad)
     assert not wide.grad[:, :32].any() and not wide.grad[:, 96:].any()
+
+
+@pytest.mark.parametrize("form", ["store", "gate_up", "wide"])
+@pytest.mark.parametrize("E,M,K,N", [(8, 100, 256, 288), (40, 90, 2048, 96), (1, 1, 128, 32), (3, 70, 640, 544)])
+def test_few_rows_per_expert(E, M, K, N, form):
+    """Few rows per expert (weights copied past the caches), one expert with more than a tile's: the bits of a product of twelve
+    times the rows of each."""
+    o = ops()
+    st = o.F8Stack.from_weights(rand(E, K, N, seed=N) * K ** -0.5, halves=1 if form == "store" else 2)
+    g = torch.Generator().manual_seed(M)
+    counts = torch.bincount(torch.randint(0, E, (M // 2,), generator=g), minlength=E)
+    counts[E // 2] += M - M // 2
+    x = rand(M, K, seed=M)
+
+    def product(x, c):
+        q, s = o.quant_rows(x)
+        if form == "store":
+            return (o.grouped_mm_f8(q, s, st, c.to(DEV)),)
+        act, act_s = o.gate_up_swiglu_f8(q, s, st, c.to(DEV), wide=form == "wide")
+        return act.view(torch.uint8), act_s.view(torch.uint8)
+
+    few = product(x, counts)
+    many = product(torch.cat([t.repeat(12, 1) for t in x.split(counts.tolist())]), counts * 12)
+    r0 = 0
+    for n in counts.tolist():
+        for a, b in zip(few, many):
+            assert torch.equal(a[r0:r0 + n], b[12 * r0:12 * r0 + n])
+        r0 += n

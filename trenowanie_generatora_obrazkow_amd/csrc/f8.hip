@@ -198,8 +198,10 @@ constexpr int kF8BandM = 4;    // m-tiles of an expert that are walked together 
 
 enum F8Epi { F8_STORE = 0, F8_SWIGLU = 1 };
 
-template <int BM_, int BN_, int WM_, int WN_, int NS_>
+// ONCE: each weight is copied once, past the caches (non-temporal)
+template <int BM_, int BN_, int WM_, int WN_, int NS_, bool ONCE_ = false>
 struct F8Cfg {
+  static constexpr bool ONCE = ONCE_;
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NS = NS_;
   static constexpr int NW = WM * WN, NT = 64 * NW, TM = BM / WM, TN = BN / WN, FM = TM / 32, FN = TN / 32;
   static constexpr int A_BYTES = BM * kF8Slice, B_BYTES = BN * kF8Slice, STAGE = A_BYTES + B_BYTES;
@@ -213,6 +215,7 @@ struct F8Cfg {
 __device__ __forceinline__ int f8_swz(int row) { return (row >> 1) & 7; }
 
 // buf2lds (gemm_common.h) by LDS address
+template <bool ONCE = false>
 __device__ __forceinline__ void f8_copy(uint32_t voff, i32x4 rsrc, uint32_t soff, uint32_t lds32) {
   const uint32_t m0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds32);
   rsrc.x = __builtin_amdgcn_readfirstlane(rsrc.x);
@@ -220,8 +223,18 @@ __device__ __forceinline__ void f8_copy(uint32_t voff, i32x4 rsrc, uint32_t soff
   rsrc.z = __builtin_amdgcn_readfirstlane(rsrc.z);
   rsrc.w = __builtin_amdgcn_readfirstlane(rsrc.w);
   soff = (uint32_t)__builtin_amdgcn_readfirstlane((int)soff);
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-               :: "s"(m0), "v"(voff), "s"(rsrc), "s"(soff) : "memory", "m0");
+  if constexpr (ONCE)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen nt lds"
+                 :: "s"(m0), "v"(voff), "s"(rsrc), "s"(soff) : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                 :: "s"(m0), "v"(voff), "s"(rsrc), "s"(soff) : "memory", "m0");
+}
+// and buf2lds_inner, non-temporal
+template <int OFF>
+__device__ __forceinline__ void f8_copy_once(uint32_t voff, const i32x4& rsrc, uint32_t soff, uint32_t lds32) {
+  asm volatile("s_add_u32 m0, %0, %4\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen nt lds"
+               :: "s"(lds32), "v"(voff), "s"(rsrc), "s"(soff), "i"(OFF) : "memory", "m0", "scc");
 }
 
 // The lane's number as a value of this place: what is computed from it is not moved out of the tile loop, where it would be
@@ -266,7 +279,7 @@ __device__ __forceinline__ float row_scale_at(const void* s, int dt, int64_t i) 
 // 8192^3 400 us, 2.75 PFLOP/s; 32768 rows over 16 experts, 1536 -> 8192 367 us, 2.24 (gate/up 364, 2.27), 4096 -> 1536 160 us,
 // 2.58 (a plain library product of 8-bit matrices of these sizes: 360, 354 and 143 us).  With the weights from memory and
 // experts of uneven load 435 and 215 us.  12000 rows over 128 experts, 2048 -> 2 x 320 43 us, 320 -> 2048 31; 288 rows over 64
-// experts, 2048 -> 2 x 1408 70 us, 1408 -> 2048 30, 5.3 and 6.1 TB/s of weights.
+// experts, 2048 -> 2 x 1408 64 us, 1408 -> 2048 30, 5.8 and 6.1 TB/s of weights.
 //
 // The outputs leave with non-temporal stores: a large one would push the rows and weights that the XCD's next tiles share out
 // of its L2.  16 x 2048 rows, 1536 -> 8192: 465 -> 373 us (gate/up, half the columns of one byte, 408 -> 385), one expert 402 ->
@@ -417,7 +430,7 @@ __global__ __launch_bounds__(C::NT, C::LDS_BYTES > 81920 ? 1 : 2) void f8_gemm_k
               slot + (wave * C::PA + i) * 1024);
 #pragma unroll
     for (int i = 0; i < C::PB; ++i)
-      f8_copy(k0 + chunk_of(ln, 8 * (wave * C::PB + i) + (ln >> 3)) * 16 < K ? vB[i] : kOOB, rsB, (uint32_t)k0,
+      f8_copy<C::ONCE>(k0 + chunk_of(ln, 8 * (wave * C::PB + i) + (ln >> 3)) * 16 < K ? vB[i] : kOOB, rsB, (uint32_t)k0,
               slot + C::A_BYTES + (wave * C::PB + i) * 1024);
   };
 
@@ -463,6 +476,8 @@ __global__ __launch_bounds__(C::NT, C::LDS_BYTES > 81920 ? 1 : 2) void f8_gemm_k
           constexpr int c = c0 + decltype(j)::value;
           if constexpr (c < C::PA)
             buf2lds_inner<c * 1024>(vA[c], rsA, so, fa);
+          else if constexpr (C::ONCE)
+            f8_copy_once<(c - C::PA) * 1024>(vB[c - C::PA], rsB, so, fb);
           else
             buf2lds_inner<(c - C::PA) * 1024>(vB[c - C::PA], rsB, so, fb);
         });
@@ -766,6 +781,10 @@ static int f8_launch(const F8Params& p, hipStream_t s) {
 // 8 waves for a tile of 256 x 256: twice the LDS reads per product of 4 waves, but two waves per SIMD, of which one computes
 // while the other waits or is in the epilogue: gate/up 16 x 2048 rows, 1536 -> 8192, 482 -> 440 us, in 16 bits 788 -> 738;
 // plain outputs 510 -> 504 there, 600 rows of 1024 x 768 over 32 experts 41 -> 35 (4 waves are 4% ahead where K is 8192).
+// With at most 32 rows per expert the weights go past the caches, which leaves these to the rows and the outputs: 64 experts of
+// 4 rows, 2048 -> 2 x 1408 70 -> 64 us, 1408 -> 2048 35 -> 32, 16 of 4, 1536 -> 2 x 4096 34 -> 31 (layers whose weights the 256 MB
+// cache holds lose up to 1 us of 16).  Not where further row tiles read them again (128 experts of 96 rows, 2048 -> 2 x 320 64
+// -> 76), nor where a row's end shares its line with the next one's begin (320 -> 2048, 4 rows: 22 -> 27).
 template <int EPI, int CDT, bool WIDE = false>
 static int f8_pick(const F8Params& p, hipStream_t s) {
   const int cus = f8_cus();
@@ -785,7 +804,10 @@ static int f8_pick(const F8Params& p, hipStream_t s) {
   } else {
     t32 = price(32, 256, 2 * cus, 2.5, 1.1), t128 = price(128, 256, cus, 2, 1.3), t256 = price(256, 256, cus, 5, 1.75);
   }
-  if (t32 <= t128 && t32 <= t256) return f8_launch<F8Cfg<32, 256, 1, 4, 2>, EPI, CDT, WIDE>(p, s);
+  if (t32 <= t128 && t32 <= t256) {
+    if (rows <= 32 && p.K % kF8Slice == 0) return f8_launch<F8Cfg<32, 256, 1, 4, 2, true>, EPI, CDT, WIDE>(p, s);
+    return f8_launch<F8Cfg<32, 256, 1, 4, 2>, EPI, CDT, WIDE>(p, s);
+  }
   if constexpr (EPI == F8_STORE) {
     if (t128 <= t256) return f8_launch<F8Cfg<128, 128, 2, 2, 2>, EPI, CDT, WIDE>(p, s);
   } else {
