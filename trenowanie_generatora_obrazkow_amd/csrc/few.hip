@@ -262,6 +262,7 @@ __global__ __launch_bounds__(256, 1) void few_up_kernel(FewParams p) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15, q = lane >> 4;
   const int M = p.M;
+  [[maybe_unused]] int chosen = -1;  // the router's id of flat row tid, as it goes out
   if constexpr (ROUTE) {
 #pragma clang fp contract(off)
     const f32x4 acc = few_router_chain(p.x, p.ldx, p.wr, p.T, p.d, p.E, lane, wave);
@@ -274,6 +275,10 @@ __global__ __launch_bounds__(256, 1) void few_up_kernel(FewParams p) {
     float lg[1] = {__fadd_rn(__fadd_rn(pt[0], pt[256]), __fadd_rn(pt[512], pt[768]))};
     if (p.bias && l16 < p.E) lg[0] = __fadd_rn(lg[0], p.bias[l16]);
     route_select16<1>(lg, 4 * wave, lane, p.T, p.E, p.k, p.renorm, p.scaling, nullptr, g.id, s_w);
+    __syncthreads();
+    // a token of NaN logits has the selection's empty mark in its later slots, which names no expert
+    chosen = g.id[tid];
+    g.id[tid] = chosen >= 0 && chosen < p.E ? chosen : -1;
     __syncthreads();
   } else {
     g.id[tid] = -1;
@@ -298,7 +303,7 @@ __global__ __launch_bounds__(256, 1) void few_up_kernel(FewParams p) {
     }
     if (tid < M) {
       if constexpr (ROUTE) {
-        p.out_ids[tid] = my;
+        p.out_ids[tid] = chosen;
         p.out_w[tid] = s_w[tid];
       }
       h.w[tid] = ROUTE ? s_w[tid] : few_w(p.tw, p.tw_dt, tid);
