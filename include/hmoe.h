@@ -103,8 +103,7 @@ int hmoe_route_sigmoid_group(const void* x, int64_t ldx, const void* wr, const f
  * An expert with the logit or the bias -inf or NaN, or outside the kept groups, is chosen only where no other is left (the
  * lowest such expert first) and has the weight 0; a NaN or +inf logit makes every softmax weight of its row NaN.
  * live (T,) bytes or NULL: a token with live = 0 (padding) gets ids -1 and weights 0 -- it routes nowhere
- * (hmoe_dispatch).  For inference: hmoe_combine_bwd and hmoe_down_dgrad_swiglu_dw take the index arrays of a dispatch in
- * which every slot named an expert (the sorted rows past the valid ones are not written).  E <= 512, k <= 16, k <= E; with groups n_group <= 64, E / n_group >= group_top, k <= topk_group *
+ * (hmoe_dispatch).  E <= 512, k <= 16, k <= E; with groups n_group <= 64, E / n_group >= group_top, k <= topk_group *
  * E / n_group. */
 int hmoe_route_scores(const void* logits, int64_t ld, int dtype, const float* bias, const uint8_t* live, int64_t T,
                       int E, int k, int score, int n_group, int topk_group, int group_top, int renorm, float scaling,
@@ -122,10 +121,11 @@ size_t hmoe_dispatch_workspace_size(int64_t T, int k, int E);
  * n_invalid (1,) int32.  dtype: the 16-bit type of x / xs and of w_sorted (topk_w, fp32, bf16 or fp16, is rounded
  * to it).
  * Expert ids outside [0, E) route nowhere: their flat rows are counted in no expert and get inv_pos = -1, the
- * Sigma counts sorted rows hold the valid ones (the sorted rows past that are not written), and n_invalid receives
- * how many there are (on the device, no host sync: the caller reads it when it chooses).  hmoe_combine with inv_pos
- * then adds zeros for those slots and hmoe_unpermute_bwd skips them, so the layer's output is defined (the slot
- * contributes nothing).  The reference leaves such ids undefined (torch.bincount raises on negative ones and grows
+ * Sigma counts sorted rows hold the valid ones (past them order and a_idx are -1, w_sorted is 0 and xs is not
+ * written), and n_invalid receives how many there are (on the device, no host sync: the caller reads it when it
+ * chooses).  hmoe_combine with inv_pos then adds zeros for those slots, and hmoe_combine_bwd,
+ * hmoe_down_dgrad_swiglu_dw, hmoe_swiglu_pack_bwd and hmoe_unpermute_bwd skip them, so the layer's output and
+ * gradients are defined (the slot contributes nothing).  The reference leaves such ids undefined (torch.bincount raises on negative ones and grows
  * the count array for ids >= E, aurora/hf_compat.py:72).  E <= 1024. */
 int hmoe_dispatch(const void* topk_ids, int ids_dtype, const void* topk_w, int w_dtype, int64_t T, int k, int E,
                   const void* x, int64_t ldx, int64_t d, void* xs, int32_t* counts, int64_t* counts64,
@@ -302,7 +302,8 @@ int hmoe_moe_block(const void* x, int64_t ldx, const void* gate_w, const float* 
 
 /* Backward of :80-82 (weight multiply + combine).  For each sorted row r (token t = a_idx[r], flat f = order[r]):
  * dys[r] = bf16(w_sorted[r] * dout[t]) (M, d) and dtopk_w[f] = <dout[t], yhat[r]> (fp32, fixed order).  yhat NULL:
- * dys only (order and dtopk_w unused; hmoe_down_dgrad_swiglu_dw then gives dtopk_w). */
+ * dys only (order and dtopk_w unused; hmoe_down_dgrad_swiglu_dw then gives dtopk_w).  Rows past the counted ones (a_idx
+ * negative) are left out: dys[r] and the dtopk_w of slots that name no expert are not written. */
 int hmoe_combine_bwd(const void* dout, const void* yhat, const int32_t* order, const int32_t* a_idx,
                      const uint16_t* w_sorted, int64_t M, int k, int64_t d, void* dys, float* dtopk_w,
                      hmoe_stream_t stream);
@@ -320,6 +321,7 @@ int hmoe_down_dgrad_swiglu(const void* dy, const int32_t* a_idx, const uint16_t*
  * act = bf16(bf16(silu(g)) * u) recomputed from gu[r] exactly as the forward rounds it -- <dy[t], act[r] @ wd[e]> in
  * fp32, without a rounded copy of the down projection's output.  Per-(row, column block) partials go to the
  * workspace (hmoe_down_dgrad_dw_workspace_size(M, h) bytes, 16-byte aligned) and are added in column-block order.
+ * Where order[r] is negative (a row past the counted ones) nothing is written, so slots that name no expert keep their dtopk_w.
  * Has no counterpart in the reference (its MoE path has no backward). */
 size_t hmoe_down_dgrad_dw_workspace_size(int64_t M, int64_t h);
 int hmoe_down_dgrad_swiglu_dw(const void* dy, const int32_t* a_idx, const uint16_t* w_sorted, const void* wd,
@@ -529,7 +531,7 @@ int hmoe_swiglu_pack(const void* gu, int64_t ldgu, int64_t M, int64_t h, void* a
                      hmoe_stream_t stream);
 /* Its backward from what it kept, with da = w[r] * dh[r] (w (M,) fp32, bf16 or fp16; NULL = 1): dgu (M, 2h) = [dg | du]; act
  * (M, h), the activation of the kept values (NULL to skip); dw[order[r] or r] = <dh[r], that activation before its rounding>
- * fp32, in a fixed order (NULL to skip). */
+ * fp32, in a fixed order (NULL to skip; nothing is written for a row whose order is negative). */
 int hmoe_swiglu_pack_bwd(const void* dh, const void* q, const uint8_t* s, const void* w, int w_dtype, int64_t M, int64_t h,
                          void* dgu, void* act, const int32_t* order, float* dw, int dtype, hmoe_stream_t stream);
 

@@ -1631,7 +1631,8 @@ size_t hmoe_down_dgrad_dw_workspace_size(int64_t M, int64_t h) {
   return (size_t)(M * dw_partials(h, false) * 4 + 255) / 256 * 256;  // the small tiles' count is the larger
 }
 
-// dtopk_w[order[r]] = sum over q of part[q * M + r], in q order (partial-major: a thread per row, coalesced rows)
+// dtopk_w[order[r]] = sum over q of part[q * M + r], in q order (partial-major: a thread per row, coalesced rows); a row
+// past the counted ones (order negative, as the dispatch leaves it) is left out
 __global__ __launch_bounds__(256) void dw_reduce_kernel(const float* __restrict__ part, int P, int64_t M,
                                                         const int32_t* __restrict__ order, float* __restrict__ dtw) {
   for (int64_t r = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; r < M; r += (int64_t)gridDim.x * blockDim.x) {
@@ -1644,7 +1645,8 @@ __global__ __launch_bounds__(256) void dw_reduce_kernel(const float* __restrict_
       for (int u = 0; u < 8; ++u)
         if (q0 + u < P) s += v[u];
     }
-    dtw[order[r]] = s;
+    const int f = order[r];
+    if (f >= 0) dtw[f] = s;
   }
 }
 

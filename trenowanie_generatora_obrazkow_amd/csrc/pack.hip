@@ -140,7 +140,10 @@ __global__ __launch_bounds__(256) void swiglu_pack_bwd_kernel(const uint16_t* __
 #pragma unroll
     for (int i = 1; i < W; ++i) sum += part[w0 + i];
   }
-  if (threadIdx.x % TPR == 0 && row < M) dw[order ? order[row] : row] = sum;
+  if (threadIdx.x % TPR == 0 && row < M) {
+    const int64_t f = order ? (int64_t)order[row] : row;
+    if (f >= 0) dw[f] = sum;  // (a row past those that a dispatch counted has order -1)
+  }
 }
 
 // threads per row: the least power of two from 8 on that takes a row in one step, at most a workgroup

@@ -878,17 +878,28 @@ __global__ __launch_bounds__(1024) void dispatch_scan_kernel(int32_t* __restrict
   }
 }
 
+// sorted row r belongs to no expert
+__device__ __forceinline__ void mark_uncounted(int64_t r, int32_t* __restrict__ order, int32_t* __restrict__ a_idx,
+                                               uint16_t* __restrict__ w_sorted) {
+  order[r] = -1;
+  if (a_idx) a_idx[r] = -1;
+  if (w_sorted) w_sorted[r] = 0;
+}
+
 // Pass 3 without row copies: the index arrays only, one thread per flat row f (token f / k), so that every row's
 // lookups are in flight together (the per-token pass below visits a token's k rows one after another: at top-8 its
-// lookups are eight dependent round trips per wave).  Same values as the per-token pass.
+// lookups are eight dependent round trips per wave).  Same values as the per-token pass.  The sorted rows past the counted
+// ones (as many as flat rows have ids outside [0, E)) are marked: -1 in order and a_idx, weight 0, in all three forms.
 __global__ __launch_bounds__(256) void dispatch_index_kernel(const void* __restrict__ ids, int ids64,
                                                              const void* __restrict__ tw, int tw_dtype, int ws_f16,
                                                              int64_t M,
                                                              int k, int E, const int32_t* __restrict__ blkoff,
                                                              const int32_t* __restrict__ rank,
+                                                             const int32_t* __restrict__ starts,
                                                              int32_t* __restrict__ order, int32_t* __restrict__ a_idx,
                                                              int32_t* __restrict__ inv_pos,
                                                              uint16_t* __restrict__ w_sorted) {
+  const int counted = starts[E];
   for (int64_t f = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; f < M; f += (int64_t)gridDim.x * blockDim.x) {
     const int e = load_id(ids, ids64, f);
     const int64_t pos = (e >= 0 && e < E) ? (int64_t)blkoff[(f / kFPB) * E + e] + rank[f] : -1;
@@ -898,6 +909,7 @@ __global__ __launch_bounds__(256) void dispatch_index_kernel(const void* __restr
       if (w_sorted) w_sorted[pos] = route_w16(tw, tw_dtype, f, ws_f16);
     }
     if (inv_pos) inv_pos[f] = (int32_t)pos;
+    if (f >= counted) mark_uncounted(f, order, a_idx, w_sorted);
   }
 }
 
@@ -1017,6 +1029,7 @@ __global__ __launch_bounds__(1024) void dispatch_small_kernel(const void* __rest
       if (w_sorted) w_sorted[pos] = route_w16(tw, tw_dtype, f, ws_f16);
     }
     if (inv_pos) inv_pos[f] = (int32_t)pos;
+    if (f >= st[E]) mark_uncounted(f, order, a_idx, w_sorted);
   }
 }
 
@@ -1036,6 +1049,7 @@ __global__ __launch_bounds__(256) void dispatch_scatter_kernel(
   const int lane = threadIdx.x & 63;
   const int nwaves = blockDim.x >> 6;
   const int64_t nvec = d / 8;
+  const int counted = starts[E];
   // rows of up to 2048 elements: the lane's (at most 4) chunks of the token's row are loaded first, since their
   // address needs no lookup, and stay in registers while the positions are looked up
   const bool pre = (xs || xs_tiles) && nvec <= 256;
@@ -1076,6 +1090,7 @@ __global__ __launch_bounds__(256) void dispatch_scatter_kernel(
         if (lane == j && inv_pos) inv_pos[f] = (int32_t)pos[j];
       }
     }
+    if (lane < k && t * k + lane >= counted) mark_uncounted(t * k + lane, order, a_idx, w_sorted);
     if (xs || xs_tiles) {
       auto put = [&](int64_t c, const uint4 v) {
 #pragma unroll
@@ -1221,7 +1236,8 @@ __global__ __launch_bounds__(256) void combine_kernel(const uint16_t* __restrict
 }
 
 // one wave per sorted row: dys[r] = bf16(w_r * dout[t]); dtopk_w[f] = <dout[t], yhat[r]>
-// DW: also dtopk_w[order[r]] = <dout[t], yhat[r]>; without it the scaled rows dys only.
+// DW: also dtopk_w[order[r]] = <dout[t], yhat[r]>; without it the scaled rows dys only.  A row past the counted ones (a_idx
+// negative, as the dispatch leaves it) is left out.
 template <bool DW>
 __global__ __launch_bounds__(256) void combine_bwd_kernel(const uint16_t* __restrict__ dout,
                                                           const uint16_t* __restrict__ yhat,
@@ -1236,6 +1252,7 @@ __global__ __launch_bounds__(256) void combine_bwd_kernel(const uint16_t* __rest
   const int64_t nvec = d / 8;
   for (int64_t r = (int64_t)blockIdx.x * nwaves + (threadIdx.x >> 6); r < M; r += (int64_t)gridDim.x * nwaves) {
     const int64_t t = a_idx[r];
+    if (t < 0) continue;
     const float wr = bf2f(w_sorted[r]);
     const uint4* go = reinterpret_cast<const uint4*>(dout + t * d);
     uint4* dy = reinterpret_cast<uint4*>(dys + r * d);
@@ -1935,7 +1952,7 @@ static int dispatch_impl(const void* topk_ids, int ids_dtype, const void* topk_w
     HMOE_CHECK_LAUNCH();
   } else if (M > 0) {
     hipLaunchKernelGGL(dispatch_index_kernel, dim3(grid_for(M, 256, 8192)), dim3(256), 0, s, topk_ids, ids64, topk_w,
-                       w_dtype, (int)f16, M, k, E, hist, rank, order, a_idx, inv_pos, w_sorted);
+                       w_dtype, (int)f16, M, k, E, hist, rank, starts, order, a_idx, inv_pos, w_sorted);
     HMOE_CHECK_LAUNCH();
   }
   return HMOE_OK;

@@ -306,10 +306,10 @@ class Dispatch:
     counts: torch.Tensor  # (E,) int32
     counts64: torch.Tensor  # (E,) int64 or None
     starts: torch.Tensor  # (E+1,) int32
-    order: torch.Tensor  # (M,) int32  (= y_idx)
-    a_idx: torch.Tensor  # (M,) int32
+    order: torch.Tensor  # (M,) int32  (= y_idx), -1 past the counted rows
+    a_idx: torch.Tensor  # (M,) int32, -1 past the counted rows
     inv_pos: torch.Tensor  # (M,) int32
-    w_sorted: torch.Tensor  # (M,) bf16 or None
+    w_sorted: torch.Tensor  # (M,) bf16 or None, 0 past the counted rows
     xs: torch.Tensor  # (M, d) bf16 or None
     xs_tiles: torch.Tensor = None  # the sorted rows as row-group tiles (bf16 storage) or None
     n_invalid: torch.Tensor = None  # (1,) int32 on the device: flat rows whose expert id lies outside [0, E)
@@ -565,7 +565,8 @@ def combine(y, T, k, add=None, inv_pos=None):
 
 def combine_bwd(dout, yhat, disp: Dispatch, k):
     """(dys (M, d) bf16, dtopk_w (T, k) fp32): the routing-weighted upstream rows in sorted order and, with yhat
-    (the unscaled down-projection rows, sorted), <dout[t], yhat[r]>; yhat None: (dys, None)."""
+    (the unscaled down-projection rows, sorted), <dout[t], yhat[r]>; yhat None: (dys, None).  Rows of dys past the counted
+    ones are not written; dtopk_w is 0 for a slot whose id names no expert."""
     T, d = dout.shape
     M = T * k
     dout = dout.contiguous()
@@ -576,7 +577,7 @@ def combine_bwd(dout, yhat, disp: Dispatch, k):
         _need(t_, n_, (M,), _I32)
     _need(disp.w_sorted, "w_sorted", (M,), _BF16)
     dys = torch.empty(M, d, device=dout.device, dtype=torch.bfloat16)
-    dtw = torch.empty(T, k, device=dout.device, dtype=torch.float32) if yhat is not None else None
+    dtw = torch.zeros(T, k, device=dout.device, dtype=torch.float32) if yhat is not None else None  # (0 for slots without a row)
     with _Probe("combine_bwd"):
         L.call("hmoe_combine_bwd", L.ptr(dout), L.ptr(yhat), L.ptr(disp.order), L.ptr(disp.a_idx), L.ptr(disp.w_sorted),
                M, k, d, L.ptr(dys), L.ptr(dtw), _dev_stream(dout))
@@ -603,7 +604,8 @@ def down_dgrad_swiglu(dy, wd, counts, M, gu, a_idx=None, w_sorted=None):
 
 def down_dgrad_swiglu_dw(dy, wd, counts, M, gu, order, k, a_idx=None, w_sorted=None):
     """(dgu, dtopk_w): down_dgrad_swiglu's dgu and, from the same product, the routing-weight gradient dtopk_w (T, k)
-    fp32 = sum_n (dy[t] @ wd[e]^T)[n] * act[r][n], act recomputed from gu as the forward rounds it."""
+    fp32 = sum_n (dy[t] @ wd[e]^T)[n] * act[r][n], act recomputed from gu as the forward rounds it; 0 for a slot whose id
+    names no expert."""
     _need(wd, "wd", (None, None, None), _BF16)
     E, h, d = wd.shape
     counts = _counts(counts, E)
@@ -618,7 +620,7 @@ def down_dgrad_swiglu_dw(dy, wd, counts, M, gu, order, k, a_idx=None, w_sorted=N
     if M % k:
         raise ValueError(f"M = {M} is not a multiple of k = {k}")
     dgu = torch.empty(M, 2 * h, device=dy.device, dtype=torch.bfloat16)
-    dtw = torch.empty(M // k, k, device=dy.device, dtype=torch.float32)
+    dtw = torch.zeros(M // k, k, device=dy.device, dtype=torch.float32)  # (slots without a row keep it)
     ws_bytes = L.lib().hmoe_down_dgrad_dw_workspace_size(M, h)
     ws = torch.empty(ws_bytes, device=dy.device, dtype=torch.uint8)
     with _Probe("down_dgrad_swiglu"):
@@ -1391,7 +1393,7 @@ def swiglu_pack(gu):
 def swiglu_pack_bwd(dh, kept, w=None, order=None, want_act=True, want_dw=True):
     """The backward of swiglu_pack from what it kept -> (dgu (M, 2h), act (M, h) or None, dw (M,) fp32 or None).  dh (M, h) of
     gu's type; w (M,) multiplies its rows (the routing weight); act is the activation of the kept values and dw[order[r] or r]
-    = <dh[r], act[r]>, w's gradient."""
+    = <dh[r], act[r]>, w's gradient (rows of order -1 have none, places of dw that order does not name are 0)."""
     M, h, ld = _rows(dh, "dh", _H16)
     dev = dh.device
     if ld != h:
@@ -1404,7 +1406,7 @@ def swiglu_pack_bwd(dh, kept, w=None, order=None, want_act=True, want_dw=True):
     order = _on(order, "order", dev, (M,), _I32)
     dgu = torch.empty(M, 2 * h, device=dev, dtype=dh.dtype)
     act = torch.empty(M, h, device=dev, dtype=dh.dtype) if want_act else None
-    dw = torch.empty(M, device=dev, dtype=torch.float32) if want_dw else None
+    dw = (torch.empty if order is None else torch.zeros)(M, device=dev, dtype=torch.float32) if want_dw else None
     _call_on(dev, "hmoe_swiglu_pack_bwd", L.ptr(dh), L.ptr(kept.q), L.ptr(kept.s), L.ptr(w), L.dt(w) if w is not None else 0, M, h,
              L.ptr(dgu), L.ptr(act), L.ptr(order), L.ptr(dw), L.dt(dh))
     return dgu, act, dw
