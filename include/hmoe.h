@@ -538,7 +538,9 @@ int hmoe_swiglu_pack_bwd(const void* dh, const void* q, const uint8_t* s, const 
 /* ---------------------------------------------------------------------------------------------------------------
  * A routed layer for a few tokens, in two kernels (aurora/hf_compat.py:63-82 with T <= 16)
  * out[t] = add[t] + sum over the slots of w[t, s] * (silu(x Wg) * (x Wu)) Wd of expert ids[t, s], everything in fp32 and
- * rounded once (the bits differ from those of hmoe_moe_forward / hmoe_moe_experts, which round on the way).  T <= 16, k <= 16,
+ * rounded once (the bits differ from those of hmoe_moe_forward / hmoe_moe_experts, which round on the way; the activation enters
+ * its product with 16 significant bits, past bf16's largest number as an infinity; fp16 experts make infinities there NaN, and
+ * infinite weights of the down projection always do).  T <= 16, k <= 16,
  * E <= 1024; d and h multiples of 8 (int8 and 8-bit floats: 16).  Experts as hmoe_moe_experts takes them (x's type, or int8
  * with bf16 / fp32 scales), or w_dtype = HMOE_DT_F8: stacks (E, 2h, d) and (E, d, h) of hmoe_f8_quant_stack with their scales.
  * Ids outside [0, E) add nothing, their number goes to n_invalid (1,) (NULL to skip); one expert may come several times.  add (T, d) of x's type or NULL; out (T, d), not over an

@@ -17,7 +17,8 @@
 // bound by a launch's steps one after another: start, grouping, the weights' latency, the sum over waves and parts.
 //
 // Numerics: fp32 sums throughout and one rounding, that of the output.  The activation enters its product as two bf16 numbers
-// (16 significant bits), fp16 weights there as two as well (their 11 bits); 8-bit experts (F8Stack) take x and the activation
+// (16 significant bits; past bf16's largest number an infinity, as where a larger call rounds it), fp16 weights there as two as
+// well (their 11 bits; an infinity, of either side, gives NaN); 8-bit experts (F8Stack) take x and the activation
 // quantised as the grouped product does, widened exactly.
 #include <algorithm>
 
@@ -79,12 +80,15 @@ __device__ __forceinline__ f32x4 few_mfma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// eight floats as bf16 pairs, and what they lose by it as bf16 pairs again
+// eight floats as bf16 pairs, and what they lose by it as bf16 pairs again; with INF, nothing where the first is infinite
+// (so that an infinite number, or one past the largest bf16, stays an infinity instead of inf - inf)
+template <bool INF>
 __device__ __forceinline__ void split8(const float* v, u32x4& hi, u32x4& lo) {
+  auto rest = [](float x, float h) { return !INF || __builtin_fabsf(h) < __builtin_inff() ? x - h : 0.0f; };
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     hi[i] = cvt_bf2(v[2 * i], v[2 * i + 1]);
-    lo[i] = cvt_bf2(v[2 * i] - bf_lo(hi[i]), v[2 * i + 1] - bf_hi(hi[i]));
+    lo[i] = cvt_bf2(rest(v[2 * i], bf_lo(hi[i])), rest(v[2 * i + 1], bf_hi(hi[i])));
   }
 }
 
@@ -499,7 +503,7 @@ __device__ __forceinline__ void few_act(const float* __restrict__ p1, int64_t pa
       const float inv = f8_inv(e);
       a = f8_widen(make_uint2(f8_pack4(v[0], v[1], v[2], v[3], inv), f8_pack4(v[4], v[5], v[6], v[7], inv)), f8_pow(e));
     } else {
-      split8(v, a, b);
+      split8<true>(v, a, b);
       *reinterpret_cast<u32x4*>(lo + r * kFewActLd + c) = b;
     }
     *reinterpret_cast<u32x4*>(hi + r * kFewActLd + c) = a;
@@ -616,7 +620,7 @@ __global__ __launch_bounds__(256, 1) void few_down_kernel(FewParams p) {
                   f[2 * i + 1] = h_hi(v[i]);
                 }
                 u32x4 wh, wl;
-                split8(f, wh, wl);
+                split8<false>(f, wh, wl);
                 acc[j] = few_mfma<false>(wl, hi, acc[j]);
                 acc[j] = few_mfma<false>(wh, lo, acc[j]);
                 acc[j] = few_mfma<false>(wh, hi, acc[j]);
