@@ -21,7 +21,7 @@ import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
 from . import ops
-from .layer import MoESwiGLU, _check_checkpoint, _experts_backward, _experts_forward, _experts_infer, _recorded
+from .layer import MoESwiGLU, _check_checkpoint, _experts_backward, _experts_forward, _experts_infer, _few, _few_infer, _recorded
 
 
 def _flat(x):
@@ -161,19 +161,25 @@ class _MoEResidual(torch.autograd.Function):
 
 def moe_residual(x, router_weight, w_gu, w_d, top_k, pre_weight=None, scale=None, shift=None, post_weight=None, gate=None,
                  post_norm=True, starts=None, eps=1e-6, alpha=1.0, logit_bias=None, renorm=True, router=None,
-                 select_bias=None, checkpoint=None):
+                 select_bias=None, checkpoint=None, few_tokens=0):
     """out (T, d) = alpha * x + gate_b * post_weight * N(moe(N(x) * pre_weight * (1 + scale_b) + shift_b)) of x (T, d), bf16 or
     fp32 (the routed layer runs in bf16), N the RMS norm (post_norm=False: the layer's output itself) -> (out of x's type,
-    topk_ids, topk_weight).  The routed layer and its options are moe_swiglu's (`router` its Gate); the other arguments are
-    norm_modulate's and norm_residual's."""
+    topk_ids, topk_weight).  The routed layer and its options are moe_swiglu's (`router` its Gate; with few_tokens, the layer's
+    output is rounded to bf16 ahead of the norm behind it); the other arguments are norm_modulate's and norm_residual's."""
     if x.dim() != 2 or x.dtype not in (torch.bfloat16, torch.float32):
         raise TypeError(f"x must be a (T, d) matrix in bf16 or fp32 (got {tuple(x.shape)} {x.dtype})")
     _check_checkpoint(checkpoint)
+    few = _few(x.shape[0], top_k, few_tokens)
     if not _recorded(x, router_weight, w_gu, w_d, pre_weight, scale, shift, post_weight, gate):
         x2 = _flat(x)
         h = ops.norm_modulate(x2, _par(pre_weight), _par(scale), _par(shift), starts, eps, torch.bfloat16)
-        y, ids, tw, inv = _experts_infer(h, router_weight, w_gu, w_d, logit_bias, top_k, renorm, router, select_bias)
-        out = ops.norm_residual(y, x2, _par(gate), _par(post_weight), post_norm, starts, eps, alpha, top_k, inv)
+        layer = (h, router_weight, w_gu, w_d, logit_bias, top_k, renorm, router, select_bias)
+        slots, inv = top_k, None
+        if few:
+            (y, ids, tw), slots = _few_infer(*layer), 1
+        else:
+            y, ids, tw, inv = _experts_infer(*layer)
+        out = ops.norm_residual(y, x2, _par(gate), _par(post_weight), post_norm, starts, eps, alpha, slots, inv)
         return out, ids, tw
     cfg = (logit_bias, top_k, renorm, router, select_bias, post_norm, starts, eps, alpha, checkpoint)
     return _MoEResidual.apply(_flat(x), router_weight, w_gu, w_d, pre_weight, scale, shift, post_weight, gate, cfg)
@@ -201,6 +207,6 @@ class MoEResidual(nn.Module):
         m = self.mlp
         out, ids, tw = moe_residual(x.reshape(-1, x.shape[-1]), m.router_weight, m.w_gu, m.w_d, m.top_k, self.norm_weight,
                                     scale, shift, self.post_weight, gate, self.post_norm, starts, self.eps, self.alpha,
-                                    m.logit_bias, m.renorm, m.gate, m.select_bias, m.checkpoint)
+                                    m.logit_bias, m.renorm, m.gate, m.select_bias, m.checkpoint, m.few_tokens)
         m.last_topk_ids, m.last_topk_weight = ids, tw
         return out.view(x.shape)

@@ -116,6 +116,13 @@ def _check_checkpoint(checkpoint):
     return checkpoint is not None
 
 
+def _few(T, top_k, few_tokens):
+    """Whether a call of T tokens without a gradient takes the two kernels for few of them."""
+    if not 0 <= few_tokens <= ops.FEW_TOKENS:
+        raise ValueError(f"few_tokens = {few_tokens}: 0 to {ops.FEW_TOKENS}")
+    return 0 < T <= few_tokens and top_k <= 16
+
+
 def _experts_forward(x, wr, wgu, wd, bias, k, renorm, gate, select_bias, need_grad, checkpoint=None):
     """Routing, dispatch and both projections of x (T, d) bf16 -> (y (T*k, d) in (token, slot) order, ids, weights, state)."""
     _check_layer_args(x, wr, wgu, wd, bias, k)
@@ -235,10 +242,9 @@ def moe_swiglu(x, router_weight, w_gu, w_d, top_k, logit_bias=None, renorm=True,
     (ops.moe_forward; with a gate or a selection bias, the routing and ops.moe_experts): the same kernels and outputs, a
     fraction of the host time."""
     _check_checkpoint(checkpoint)
-    if not 0 <= few_tokens <= ops.FEW_TOKENS:
-        raise ValueError(f"few_tokens = {few_tokens}: 0 to {ops.FEW_TOKENS}")
+    few = _few(x.shape[0], top_k, few_tokens)
     if not _recorded(x, router_weight, w_gu, w_d):
-        if 0 < x.shape[0] <= few_tokens and top_k <= 16:
+        if few:
             return _few_infer(x, router_weight, w_gu, w_d, logit_bias, top_k, renorm, gate, select_bias)
         if gate is None and select_bias is None:
             _check_layer_args(x, router_weight, w_gu, w_d, logit_bias, top_k)
