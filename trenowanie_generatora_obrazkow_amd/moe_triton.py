@@ -11,6 +11,7 @@ from __future__ import annotations
 import torch
 
 from . import ops
+from .block import _dense, _flat
 from .layer import _recorded
 
 BLOCK_M = 64  # aurora/moe_triton.py:13 -- the row granularity of make_schedule's blocks
@@ -69,6 +70,8 @@ def _grouped_mm_f8(a, w, counts, a_idx, y_idx, scale, w_scale):
         raise ValueError("an F8Stack holds its own scales")
     if a.dtype not in (torch.bfloat16, torch.float16, torch.float32):
         raise TypeError(f"a: bf16, fp16 or fp32 expected (got {a.dtype})")
+    if a.dim() == 2:
+        a = _flat(a)
     if _recorded(a, scale):
         if a_idx is not None or y_idx is not None or scale is not None:
             raise ValueError("an 8-bit grouped_mm with a gradient takes sorted rows: no a_idx, y_idx and scale")
@@ -93,7 +96,7 @@ class _GroupedMMF8(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        return ops.grouped_mm_f8_bwd(dy.contiguous(), ctx.w, ctx.saved_tensors[0]), None, None
+        return ops.grouped_mm_f8_bwd(_dense(dy), ctx.w, ctx.saved_tensors[0]), None, None
 
 
 def pad_operands(a, w, w_scale=None):
