@@ -492,7 +492,9 @@ int hmoe_f8_quant_stack(const void* w, int dtype, int64_t E, int64_t K, int64_t 
                         int halves, int transpose, void* q, uint8_t* s, hmoe_stream_t stream);
 
 /* hmoe_grouped_mm on quantised rows and stacks (aurora/moe_triton.py:22-56 with 8-bit operands): y[y_idx[r] or r] =
- * scale * a[a_idx[r] or r] @ w[e(r)], summed in fp32 and rounded once to y_dtype (bf16, fp16 or fp32).  w (E, N, K) and w_s from
+ * scale * a[a_idx[r] or r] @ w[e(r)], rounded once to y_dtype (bf16, fp16 or fp32).  The 8-bit matrix instructions add the
+ * products of eight consecutive k at the exponent of the largest and drop what lies below 2^-13 of it, then add in fp32: some 2^-16
+ * of a sum, which a 16-bit y does not show; of an fp32 y about 16 bits hold.  w (E, N, K) and w_s from
  * hmoe_f8_quant_stack.  scale (M,) fp32, bf16 or fp16 or NULL, by sorted row or, with scale_by_y, by y_idx[r].  Rows that no
  * expert counts are zeros (without y_idx; with it nothing is written for them).  a_rows: rows of a, at least M without a_idx;
  * with it they span less than 2 GiB (HMOE_ERR_SHAPE). */
@@ -537,14 +539,13 @@ int hmoe_swiglu_pack_bwd(const void* dh, const void* q, const uint8_t* s, const 
 
 /* ---------------------------------------------------------------------------------------------------------------
  * A routed layer for a few tokens, in two kernels (aurora/hf_compat.py:63-82 with T <= 16)
- * out[t] = add[t] + sum over the slots of w[t, s] * (silu(x Wg) * (x Wu)) Wd of expert ids[t, s], everything in fp32 and
+ * out[t] = add[t] + sum over the slots of w[t, s] * (silu(x Wg) * (x Wu)) Wd of expert ids[t, s], with fp32 sums and
  * rounded once (the bits differ from those of hmoe_moe_forward / hmoe_moe_experts, which round on the way; the activation enters
  * its product with 16 significant bits, past bf16's largest number as an infinity; fp16 experts make infinities there NaN, and
- * infinite weights of the down projection always do).  T <= 16, k <= 16,
- * E <= 1024; d and h multiples of 8 (int8 and 8-bit floats: 16).  Experts as hmoe_moe_experts takes them (x's type, or int8
+ * infinite weights of the down projection always do).  T <= 16, k <= 16, E <= 1024; d and h multiples of 8 (int8 and 8-bit floats: 16).  Experts as hmoe_moe_experts takes them (x's type, or int8
  * with bf16 / fp32 scales), or w_dtype = HMOE_DT_F8: stacks (E, 2h, d) and (E, d, h) of hmoe_f8_quant_stack with their scales.
- * Ids outside [0, E) add nothing, their number goes to n_invalid (1,) (NULL to skip); one expert may come several times.  add (T, d) of x's type or NULL; out (T, d), not over an
- * input of the call.  workspace: hmoe_few_workspace_size bytes, 256-byte aligned, not shared by calls that may run at once.
+ * Ids outside [0, E) add nothing, their number goes to n_invalid (1,) (NULL to skip); one expert may come several times.
+ * add (T, d) of x's type or NULL; out (T, d), not over an input of the call.  workspace: hmoe_few_workspace_size bytes, 256-byte aligned, not shared by calls that may run at once.
  * ------------------------------------------------------------------------------------------------------------- */
 size_t hmoe_few_workspace_size(int64_t T, int64_t d, int E, int k, int64_t h, int w_dtype, int dtype);
 int hmoe_few_experts(const void* x, int64_t ldx, int dtype, const void* topk_ids, int ids_dtype, const void* topk_w,

@@ -1151,7 +1151,8 @@ def _f8_rows(q, s, block=128):
 
 
 def dequant_rows(q, s, dtype=torch.float32, block=128):
-    """The values of quantised rows (quant_rows; block=32: swiglu_pack's) -> (M, K) of `dtype` (fp32 holds them exactly)."""
+    """The values of quantised rows (quant_rows; block=32: swiglu_pack's) -> (M, K) of `dtype` (fp32 holds them exactly, but
+    for a number of more than 3.29e38, which may have been rounded up to 2^128)."""
     M, K, ld, lds = _f8_rows(q, s, block)
     if dtype not in _FLOATS:
         raise TypeError(f"dtype {dtype} not in {_FLOATS}")
@@ -1296,7 +1297,9 @@ def _f8_mm(q, s, wq, ws, E, K, N, halves, counts, M, a_idx, y_idx, scale, dtype,
 
 def grouped_mm_f8(q, s, w, counts, M=None, a_idx=None, y_idx=None, scale=None, dtype=torch.bfloat16):
     """grouped_mm on rows in 8 bits (quant_rows) and an F8Stack: y[y_idx[r] or r] = scale[r] * a[a_idx[r] or r] @ w[e(r)] ->
-    (M, N) of `dtype` (bf16, fp16 or fp32), summed in fp32 and rounded once.  Index values are trusted, as in grouped_mm.  Rows
+    (M, N) of `dtype` (bf16, fp16 or fp32), rounded once.  The 8-bit matrix instructions drop what lies below 2^-13 of the largest of
+    eight consecutive k's products and add the rest in fp32: some 2^-16 of a sum, which 16-bit outputs do not show; of fp32 outputs
+    about 16 bits hold.  Index values are trusted, as in grouped_mm.  Rows
     that counts name for no expert are zeros; with y_idx they are not written."""
     E, K, N = _f8_stack(w, "w", q.device)
     M = (a_idx.numel() if a_idx is not None else q.shape[0]) if M is None else M
@@ -1460,7 +1463,8 @@ def _few_args(x, k, wgu, wd, wgu_s, wd_s, add):
 
 def few_experts(x, ids, tw, wgu, wd, wgu_s=None, wd_s=None, add=None, want_invalid=False):
     """The experts of a routed layer and the sum over its slots for up to 16 tokens, in two kernels (hmoe_few_experts): moe_experts
-    and combine in fp32 throughout, rounded once -> out (T, d).  x (T, d) bf16 or fp16; ids (T, k) int32 / int64, those outside
+    and combine with fp32 sums throughout, rounded once (the activation enters its product with 16 significant bits, past bf16's
+    largest number as an infinity) -> out (T, d).  x (T, d) bf16 or fp16; ids (T, k) int32 / int64, those outside
     [0, E) add nothing; tw (T, k); wgu (E, d, 2h) and wd (E, h, d) of x's type, int8 with scales, or F8Stacks; add (T, d) of x's
     type (a shared expert's output) joins the sum.  want_invalid: (out, n_invalid (1,) int32), how many ids named no expert."""
     T, k = ids.shape
@@ -1475,7 +1479,7 @@ def few_experts(x, ids, tw, wgu, wd, wgu_s=None, wd_s=None, add=None, want_inval
 
 
 def few_forward(x, wr, wgu, wd, k, bias=None, renorm=True, scaling=1.0, add=None):
-    """moe_forward for up to 16 tokens in two kernels (hmoe_few_forward), in fp32 throughout and rounded once -> (out (T, d),
+    """moe_forward for up to 16 tokens in two kernels (hmoe_few_forward), rounded as few_experts does -> (out (T, d),
     topk_ids (T, k) int32, topk_w (T, k) fp32: those of route_topk).  bf16; add (T, d) joins the sum."""
     _router_args(x, wr)
     T, d, ld, E, h, w, ws, out = _few_args(x, k, wgu, wd, None, None, add)
