@@ -125,8 +125,8 @@ size_t hmoe_dispatch_workspace_size(int64_t T, int k, int E);
  * written), and n_invalid receives how many there are (on the device, no host sync: the caller reads it when it
  * chooses).  hmoe_combine with inv_pos then adds zeros for those slots, and hmoe_combine_bwd,
  * hmoe_down_dgrad_swiglu_dw, hmoe_swiglu_pack_bwd and hmoe_unpermute_bwd skip them, so the layer's output and
- * gradients are defined (the slot contributes nothing).  The reference leaves such ids undefined (torch.bincount raises on negative ones and grows
- * the count array for ids >= E, aurora/hf_compat.py:72).  E <= 1024. */
+ * gradients are defined (the slot contributes nothing).  The reference leaves such ids undefined (torch.bincount raises
+ * on negative ones and grows the count array for ids >= E, aurora/hf_compat.py:72).  E <= 1024. */
 int hmoe_dispatch(const void* topk_ids, int ids_dtype, const void* topk_w, int w_dtype, int64_t T, int k, int E,
                   const void* x, int64_t ldx, int64_t d, void* xs, int32_t* counts, int64_t* counts64,
                   int32_t* starts, int32_t* order, int32_t* a_idx, int32_t* inv_pos, uint16_t* w_sorted,
@@ -542,10 +542,12 @@ int hmoe_swiglu_pack_bwd(const void* dh, const void* q, const uint8_t* s, const 
  * out[t] = add[t] + sum over the slots of w[t, s] * (silu(x Wg) * (x Wu)) Wd of expert ids[t, s], with fp32 sums and
  * rounded once (the bits differ from those of hmoe_moe_forward / hmoe_moe_experts, which round on the way; the activation enters
  * its product with 16 significant bits, past bf16's largest number as an infinity; fp16 experts make infinities there NaN, and
- * infinite weights of the down projection always do).  T <= 16, k <= 16, E <= 1024; d and h multiples of 8 (int8 and 8-bit floats: 16).  Experts as hmoe_moe_experts takes them (x's type, or int8
- * with bf16 / fp32 scales), or w_dtype = HMOE_DT_F8: stacks (E, 2h, d) and (E, d, h) of hmoe_f8_quant_stack with their scales.
+ * infinite weights of the down projection always do).  T <= 16, k <= 16, E <= 1024; d and h multiples of 8 (int8 and
+ * 8-bit floats: 16).  Experts as hmoe_moe_experts takes them (x's type, or int8 with bf16 / fp32 scales), or w_dtype =
+ * HMOE_DT_F8: stacks (E, 2h, d) and (E, d, h) of hmoe_f8_quant_stack with their scales.
  * Ids outside [0, E) add nothing, their number goes to n_invalid (1,) (NULL to skip); one expert may come several times.
- * add (T, d) of x's type or NULL; out (T, d), not over an input of the call.  workspace: hmoe_few_workspace_size bytes, 256-byte aligned, not shared by calls that may run at once.
+ * add (T, d) of x's type or NULL; out (T, d), not over an input of the call.  workspace: hmoe_few_workspace_size bytes,
+ * 256-byte aligned, not shared by calls that may run at once.
  * ------------------------------------------------------------------------------------------------------------- */
 size_t hmoe_few_workspace_size(int64_t T, int64_t d, int E, int k, int64_t h, int w_dtype, int dtype);
 int hmoe_few_experts(const void* x, int64_t ldx, int dtype, const void* topk_ids, int ids_dtype, const void* topk_w,

@@ -5,7 +5,7 @@
 //
 // With so few tokens the layer is its chosen experts' weights read once, plus what a launch costs; the op-by-op form has five
 // to seven dependent launches.  Here a workgroup of either kernel is one piece of one expert: a run of weight columns (one or
-// two lines wide) and a part of the sum, so every CU streams weights however few experts were chosen.  Its four waves take
+// two lines wide) and a part of the sum, so that many CUs stream weights however few experts were chosen.  Its four waves take
 // steps of the sum in turn, weights straight from memory to registers with the next step's loads in flight (nothing is used
 // twice, so nothing goes through the LDS), transposed there by byte permutes into fragments of the 16x16x32 matrix
 // instruction, whose 16 columns are the expert's tokens.  The waves' sums meet in LDS, the parts of [g | u] in the second
@@ -744,6 +744,17 @@ struct FewPlan {
 // each wave).  More parts cost more than they bring: with 512, 256 and 128 workgroups wanted one bf16 token over 2 experts of
 // d 1536, h 4096 took 20.4, 17.6 and 20.4 us (with the router, which every workgroup runs) and 12.2, 11.4 and 11.4, seven fp16
 // tokens over 9 experts of d 1000, h 712 11.4, 12.4 and 12.7 and 19.5, 15.8 and 11.9 (its last workgroups add 18, 12 and 6 parts).
+// The rule counts workgroups and not bytes, and large layers would take more of them.  Whole calls, the weights from memory, with
+// 256 and 128 wanted (these), 256 and 256, 256 and 512, 512 and 128, 128 and 128:
+//   bf16  4 experts of 2304 x 4096, k 2, one token  35.4, 33.3, 37.3, 35.8, 45.8 us;  16 tokens  72.0, 64.2, 71.7, 74.1, 71.9
+//         8 of 4096 x 8192, k 2, one token  104, 89, 88, 101, 104;  8 of 1024 x 2816, k 2, four tokens  36.5, 31.1, 31.0, 34.1, 36.3
+//         16 of 1536 x 4096, k 2, 16 tokens  136, 124, 131, 136, 136;  64 of 1280 x 256, k 8, one and eight tokens  the same but for
+//         34.8 -> 31.2 with 512 and 128 at eight
+//   fp16  the 2304 x 4096 and 1024 x 2816 ones within 5% of bf16;  32 of 1536 x 768, k 4, 16 tokens  57.2, 57.2, 61.1, 56.3, 57.1
+//   int8  32 of 1536 x 768, k 4, two tokens  19.8, 22.6, 22.6, 19.7, 20.0;  8 of 2560 x 6912, k 2, 16 tokens  109, 115, 123, 114,
+//         109;  8 of 4096 x 8192, k 2, one token  65, 57, 60, 63, 82
+//   8-bit floats  8 of 4096 x 8192, k 2, one token  81, 64, 57, 81, 81, eight tokens 170 each;  16 of 2048 x 1024, k 4, one token
+//         18.7, 17.3, 17.2, 19.5, 20.9
 static bool few_plan(int64_t T, int64_t d, int E, int k, int64_t h, int w, FewPlan& P) {
   if (T < 1 || T > kFewT || k < 1 || k > kFewK || E < 1 || d < 1 || h < 1 || d > (1 << 24) || h > (1 << 24)) return false;
   const int cols = w == FW_F8 ? 64 : w == FW_I8 ? 256 : 128, step = w == FW_F8 ? 128 : 32;
