@@ -280,9 +280,9 @@ __device__ __forceinline__ float row_scale_at(const void* s, int dt, int64_t i) 
 // 2.58 (a plain library product of 8-bit matrices of these sizes: 360, 354 and 143 us).  In one run, even and warm, even and
 // from memory, uneven and warm, uneven and from memory (an expert of none, others of twice the rows; loads of a gate in
 // brackets): 1536 -> 8192 386, 434, 400 (415), 454 (463); gate/up 393, 430, 414 (429), 428 (438); 4096 -> 1536 170, 194, 193
-// (192), 221 (228): the weights' and rows' first way costs as much as the load.  6000 rows over 12 experts, 1008 -> 2000: 24 to 25
-// whichever, one round of 240 tiles of eight slices.  12000 rows over 128 experts, 2048 -> 2 x 320 43 us, 320 -> 2048 31; 288 rows over 64
-// experts, 2048 -> 2 x 1408 64 us, 1408 -> 2048 30, 5.8 and 6.1 TB/s of weights.
+// (192), 221 (228): the weights' and rows' first way costs as much as the load.  6000 rows over 12 experts, 1008 -> 2000: 24 to
+// 25 whichever, one round of 240 tiles of eight slices.  12000 rows over 128 experts, 2048 -> 2 x 320 43 us, 320 -> 2048 31;
+// 288 rows over 64 experts, 2048 -> 2 x 1408 64 us, 1408 -> 2048 30, 5.8 and 6.1 TB/s of weights.
 //
 // The outputs leave with non-temporal stores: a large one would push the rows and weights that the XCD's next tiles share out
 // of its L2.  16 x 2048 rows, 1536 -> 8192: 465 -> 373 us (gate/up, half the columns of one byte, 408 -> 385), one expert 402 ->
@@ -785,12 +785,13 @@ static int f8_launch(const F8Params& p, hipStream_t s) {
 // while the other waits or is in the epilogue: gate/up 16 x 2048 rows, 1536 -> 8192, 482 -> 440 us, in 16 bits 788 -> 738;
 // plain outputs 510 -> 504 there, 600 rows of 1024 x 768 over 32 experts 41 -> 35 (4 waves are 4% ahead where K is 8192).
 // With at most 32 rows per expert the weights go past the caches, which leaves these to the rows and the outputs: 64 experts of
-// 4 rows, 2048 -> 2 x 1408 70 -> 64 us, 1408 -> 2048 35 -> 32, 16 of 4, 1536 -> 2 x 4096 34 -> 31 (layers whose weights the 256 MB
-// cache holds lose up to 1 us of 16).  Uneven loads gain as well, though an expert of several row tiles reads its weights several
-// times (14 launches of 8 to 256 experts, 4 to 32 rows an expert on average, the weights from memory; past the caches and through
-// them): loads by 1 / (e + 1), 16 rows on average and 212 at most, 2048 -> 2 x 1408 65.5 and 71.7; 32 and 413 83.4 and 86.5;
-// 1408 -> 2048 44.6 and 47.5; 256 experts, 2048 -> 2 x 256, 16 and 657 56.8 and 61.1; none of the 56 slower.  Not where further row tiles read them again (128 experts of 96 rows, 2048 -> 2 x 320 64
-// -> 76), nor where a row's end shares its line with the next one's begin (320 -> 2048, 4 rows: 22 -> 27).
+// 4 rows, 2048 -> 2 x 1408 70 -> 64 us, 1408 -> 2048 35 -> 32, 16 of 4, 1536 -> 2 x 4096 34 -> 31 (layers whose weights the 256
+// MB cache holds lose up to 1 us of 16).  Uneven loads gain as well, though an expert of several row tiles reads its weights
+// several times (14 launches of 8 to 256 experts, 4 to 32 rows an expert on average, the weights from memory; past the caches
+// and through them): loads by 1 / (e + 1), 16 rows on average and 212 at most, 2048 -> 2 x 1408 65.5 and 71.7; 32 and 413 83.4
+// and 86.5; 1408 -> 2048 44.6 and 47.5; 256 experts, 2048 -> 2 x 256, 16 and 657 56.8 and 61.1; none of the 56 slower.  Not
+// where further row tiles read them again (128 experts of 96 rows, 2048 -> 2 x 320 64 -> 76), nor where a row's end shares its
+// line with the next one's begin (320 -> 2048, 4 rows: 22 -> 27).
 template <int EPI, int CDT, bool WIDE = false>
 static int f8_pick(const F8Params& p, hipStream_t s) {
   const int cus = f8_cus();

@@ -42,8 +42,8 @@ def grouped_mm(a: torch.Tensor, w: torch.Tensor, counts: torch.Tensor, sched=Non
     per-column scale multiplies the fp32 sum, before `scale`.  K and N need not be multiples of the copy granule:
     such operands are zero-padded on the device first (pad_operands).
     w may be an ops.F8Stack: a is quantised to 8 bits (a scale per 128 columns) and the product runs in 8-bit floating point (its
-    sums hold about 16 bits, ops.grouped_mm_f8); K and N are then multiples of 16.  That product is differentiable in a (sorted rows, without a_idx, y_idx and scale; the stack
-    made with grad=True): the gradient is quantised in the same way."""
+    sums hold about 16 bits, ops.grouped_mm_f8); K and N are then multiples of 16.  That product is differentiable in a (sorted
+    rows, without a_idx, y_idx and scale; the stack made with grad=True): the gradient is quantised in the same way."""
     if isinstance(w, ops.F8Stack):
         return _grouped_mm_f8(a, w, counts, a_idx, y_idx, scale, w_scale)
     M = a_idx.numel() if a_idx is not None else a.shape[0]
